@@ -449,6 +449,97 @@ int32_t qwc_op_rope(float* x, uint32_t heads, uint32_t head_dim, const float* co
 /* kernels.siluMul (src/core/qwen3_asr/kernels.zig:233-239). */
 int32_t qwc_op_silu_mul(const float* gate, const float* up, uint32_t n, float* out, void* stream);
 
+/* ---- paged key/value cache and sampling: device-pointer operators ----
+ * For hosts that keep the cache of many streams in one pool of pages rather
+ * than in slots of max_positions rows. A pool holds, for one layer, the same
+ * four planes as a slot (f16 scales and u8 codes of the q8 format, keys and
+ * values apart): row `page * page_size + i` is position i of that page.
+ * One step of a layer is append, then attention; `read` gives rows back as
+ * values; `sample` ends the step where argmax does not. Formats of queries,
+ * rows and logits: f32, f16 and bf16. */
+
+/* One layer's pool. `*_scales`: [pages * page_size][kv_heads * head_dim / 64] f16, 16-byte aligned;
+ * `*_codes`: [pages * page_size][kv_heads * head_dim] u8, 16-byte aligned. */
+typedef struct qwc_paged_cache {
+  void* k_scales;
+  void* k_codes;
+  void* v_scales;
+  void* v_codes;
+  uint32_t pages;
+  uint32_t page_size; /* positions in a page, any number from 1 */
+  uint32_t kv_heads;
+  uint32_t head_dim; /* 64 or 128 */
+} qwc_paged_cache;
+
+/* The tokens of one step. Sequence s owns tokens query_starts[s] .. query_starts[s + 1] - 1 of the
+ * packed rows; they are the last positions of its context, so token i of n is position
+ * context_lens[s] - n + i. Position p lies in page page_table[s][p / page_size]. The three arrays
+ * are in device memory, 4-byte aligned, and may change between calls without a host round trip;
+ * `max_query` and `max_context` are the host's bounds on them (a launch covers no more tokens of a
+ * sequence and no more positions than these). A position below zero (a context shorter than its
+ * tokens) or in a page outside 0 .. pages - 1 counts as not cached: it is not written, attention
+ * does not see it, and its rows read as zero. */
+typedef struct qwc_paged_batch {
+  const int32_t* query_starts; /* [sequences + 1], ascending, the last = tokens */
+  const int32_t* context_lens; /* [sequences], this step's tokens included */
+  const int32_t* page_table;   /* [sequences][table_stride] */
+  uint32_t sequences;
+  uint32_t tokens;
+  uint32_t table_stride;
+  uint32_t max_query;
+  uint32_t max_context;
+  uint32_t reserved;
+} qwc_paged_batch;
+
+/* QK-RMSNorm, rotary positions and the q8 append of a step's rows in one pass (what the decoder does
+ * between the QKV projection and attention, decoder.zig:177-216): q_out = rope(norm(q) * q_norm),
+ * the keys likewise with k_norm, keys and values quantized (quant.zig:197-288) into their pages.
+ * q, k and v are rows of heads * head_dim and kv_heads * head_dim values, `*_stride` elements apart
+ * (views of one joint projection row are fine); q_out may be q. A NULL norm weight leaves that norm
+ * out. cos / sin: [rope_rows][head_dim / 2] f32 (qwc_rope_tables). Row pointers and strides in bytes
+ * are multiples of 16, the tables and norm weights 16-byte aligned (else QWC_INVALID_ARGUMENT).
+ * A token whose position is not cached, or is rope_rows or more, is not written and its q_out
+ * row is zero. */
+int32_t qwc_op_paged_append(const qwc_paged_cache* cache, const qwc_paged_batch* batch, uint32_t format, const void* q,
+                            uint64_t q_stride, const void* k, uint64_t k_stride, const void* v, uint64_t v_stride,
+                            uint32_t heads, const float* q_norm, const float* k_norm, float eps, const float* cos_table,
+                            const float* sin_table, uint32_t rope_rows, void* q_out, uint64_t q_out_stride,
+                            void* stream);
+/* Causal attention of a step's tokens, one or many for each sequence, over the sequences' pages
+ * (kernels.zig:697-767 for one token): query head h reads kv head h / (heads / kv_heads), scores are
+ * scaled by 1 / sqrt(head_dim). Products enter the tensor cores as exact codes against f16 parts of
+ * the queries and weights (two parts, 22 bits, for f32 rows, one for 16-bit rows); sums and the
+ * softmax are f32. A token that sees no position gives a row of zeros. q and out as in append.
+ * `workspace` (16-byte aligned device memory of at least qwc_op_paged_attention_workspace bytes) holds
+ * the partial results of contexts cut into pieces. It must be zero before its first use, is left ready for
+ * the next call, and serves one stream at a time. */
+int32_t qwc_op_paged_attention(const qwc_paged_cache* cache, const qwc_paged_batch* batch, uint32_t format,
+                               const void* q, uint64_t q_stride, uint32_t heads, void* out, uint64_t out_stride,
+                               void* workspace, uint64_t workspace_bytes, void* stream);
+/* Bytes of workspace that qwc_op_paged_attention needs for this pool, batch and head count. Host only. */
+int32_t qwc_op_paged_attention_workspace(const qwc_paged_cache* cache, const qwc_paged_batch* batch, uint32_t format,
+                                         uint32_t heads, uint64_t* bytes);
+/* The cached rows of a step's tokens as values, (code - 128) * scale rounded once to `format`: what append
+ * wrote, or, with as many tokens as positions, whole contexts. k_out / v_out: kv_heads * head_dim values
+ * a row, `*_stride` elements apart; pointers and strides in bytes are multiples of 16. */
+int32_t qwc_op_paged_read(const qwc_paged_cache* cache, const qwc_paged_batch* batch, uint32_t format, void* k_out,
+                          uint64_t k_stride, void* v_out, uint64_t v_stride, void* stream);
+/* One token of each row of logits, drawn with a given number uniforms[row] in [0, 1). With w = exp((x -
+ * max) / temperature), the tokens in order of falling logit (ties: the lowest index first) are cut to the
+ * first top_k (0: all), then to the first whose sum of w reaches top_p of what top_k left (1 or more: all;
+ * the token that reaches it stays), then to those with w >= min_p (0: all); at least one stays. The token is
+ * the first, in index order, whose running sum of the kept w passes uniforms[row] of their total. A
+ * temperature of 0 (or less, or NaN) takes the largest logit, as qwc_op_argmax. NaN logits count as -inf; a row
+ * of nothing else gives token 0 and log-probability -inf. logprobs_out (may be NULL): the token's log-probability under
+ * the row's softmax at its temperature, before the cuts (temperature 1 for a row that takes the
+ * largest). temperature, top_k, top_p, min_p: one value for each row in device memory, or NULL for 1, 0, 1, 0.
+ * Sums are 64-bit integers in units of 2^-42 of the largest w, so the result does not depend on their order.
+ * vocab at most QWC_SAMPLE_MAX_VOCAB; logits aligned to their format's size, rows `row_stride` elements apart. */
+#define QWC_SAMPLE_MAX_VOCAB 1048576u
+int32_t qwc_op_sample(uint32_t format, const void* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
+                      const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                      const float* uniforms, uint32_t* tokens_out, float* logprobs_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

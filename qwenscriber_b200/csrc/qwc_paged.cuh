@@ -1,0 +1,139 @@
+// qwc_paged.cuh -- what the operators on a paged key/value cache share: the
+// pool and the batch as a kernel takes them, and where a token's row lies.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/qwenscriber_cuda.h"
+#include "qwc_internal.h"
+
+namespace qwc {
+
+// qwc_paged_cache and qwc_paged_batch, with the division by the page size as
+// a multiplication and two shifts (Granlund and Montgomery, 1994, figure 4.1,
+// exact for every 32-bit position): with l = ceil(log2 page_size), page_mul
+// is 2^32 (2^l - page_size) / page_size + 1, the shifts min(l, 1) and
+// max(l - 1, 0).
+struct PagedArgs {
+  const uint8_t* k_scales;
+  const uint8_t* k_codes;
+  const uint8_t* v_scales;
+  const uint8_t* v_codes;
+  const int32_t* query_starts;
+  const int32_t* context_lens;
+  const int32_t* page_table;
+  uint32_t pages, page_size, page_mul, page_shift1, page_shift2;
+  uint32_t kv_heads, head_dim;
+  uint32_t code_row;   // kv_heads * head_dim bytes
+  uint32_t scale_row;  // code_row / 64 * 2 bytes
+  uint32_t sequences, tokens, table_stride, max_query, max_context;
+};
+
+// A sequence's tokens in this step: packed rows first .. first + n - 1, which
+// are positions base .. base + n - 1 of its context.
+struct PagedSeq {
+  uint32_t first, n;
+  int32_t base;
+  uint32_t context;
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, uint32_t s) {
+  const int32_t limit = static_cast<int32_t>(a.tokens);
+  const int32_t b = min(max(a.query_starts[s], 0), limit);
+  const int32_t e = min(max(a.query_starts[s + 1], b), limit);
+  const int32_t c = min(max(a.context_lens[s], 0), static_cast<int32_t>(a.max_context));
+  return PagedSeq{static_cast<uint32_t>(b), min(static_cast<uint32_t>(e - b), a.max_query), c - (e - b),
+                  static_cast<uint32_t>(c)};
+}
+
+__device__ __forceinline__ uint32_t page_of(const PagedArgs& a, uint32_t p) {
+  const uint32_t t = __umulhi(p, a.page_mul);
+  return (t + ((p - t) >> a.page_shift1)) >> a.page_shift2;
+}
+
+// Row of the pool that holds position p of sequence s, or -1 if its page
+// is not one of the pool's.
+__device__ __forceinline__ int64_t paged_row(const PagedArgs& a, uint32_t s, uint32_t p) {
+  const uint32_t pg = page_of(a, p);
+  const int32_t id = __ldg(a.page_table + size_t(s) * a.table_stride + pg);
+  if (static_cast<uint32_t>(id) >= a.pages) return -1;
+  return int64_t(id) * a.page_size + (p - pg * a.page_size);
+}
+
+// Rows of f32, f16 or bf16 values, 16 bytes at a time.
+template <typename T>
+struct Vec16 {
+  static constexpr int kCount = 16 / sizeof(T);
+};
+
+__device__ __forceinline__ void unpack16(uint4 w, float (&v)[4]) {
+  v[0] = __uint_as_float(w.x);
+  v[1] = __uint_as_float(w.y);
+  v[2] = __uint_as_float(w.z);
+  v[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void unpack16(uint4 w, float (&v)[8], __half) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack16(uint4 w, float (&v)[8], __nv_bfloat16) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(u[i] << 16);
+    v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack16(uint4 w, float (&v)[4], float) { unpack16(w, v); }
+
+__device__ __forceinline__ uint32_t pair_bits(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pair_bits(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float (&v)[8]) {
+  return make_uint4(pair_bits(v[0], v[1], T()), pair_bits(v[2], v[3], T()), pair_bits(v[4], v[5], T()),
+                    pair_bits(v[6], v[7], T()));
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float (&v)[4]) {
+  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void store_as(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Host side: the checks of the two descriptors, and the kernels' form of
+// them. A refused descriptor is refused before any launch.
+int32_t paged_args(const qwc_paged_cache* cache, const qwc_paged_batch* batch, PagedArgs* out);
+// Rows of `width` values of `format`, `stride` elements apart: 16-byte pointer and stride, no overlap.
+int32_t paged_rows_check(const void* p, uint64_t stride, uint64_t width, uint32_t format);
+int32_t paged_status(cudaError_t e);
+
+constexpr uint32_t kFormatF16 = 1;
+constexpr uint32_t kFormatBF16 = 2;
+constexpr uint32_t kPagedMaxSequences = 65535;  // a grid dimension counts them
+
+inline uint32_t value_bytes(uint32_t format) { return format == kFormatF32 ? 4u : 2u; }
+inline bool value_format_ok(uint32_t format) {
+  return format == kFormatF32 || format == kFormatF16 || format == kFormatBF16;
+}
+
+}  // namespace qwc

@@ -1,0 +1,191 @@
+"""A paged q8 key/value cache on the device: append, attention and read (qwc_op_paged_*).
+
+`PagedCache` names one layer's pool of pages, `PagedBatch` the tokens of one step; both hold
+torch tensors (device memory, nothing is computed by torch) and the descriptors that the C ABI
+takes, so a call is one ABI call on torch's current stream. A refused argument raises `QwcError`
+with the status, as everywhere in this package.
+
+    cache = PagedCache.zeros(pages=512, page_size=64, kv_heads=8, head_dim=128)     # one for each layer
+    batch = PagedBatch(query_starts, context_lens, page_table, tokens=n, max_query=q, max_context=c)
+    q = append(cache, batch, q, k, v, cos, sin, q_norm=qn, k_norm=kn, eps=1e-6)
+    out = attention(cache, batch, q)
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .quant import GROUP
+from .runtime import FORMAT_BF16, FORMAT_F16, FORMAT_F32, STATUS_CODE, PagedBatchDesc, PagedCacheDesc, QwcError, check, lib
+
+FORMATS = {torch.float32: FORMAT_F32, torch.float16: FORMAT_F16, torch.bfloat16: FORMAT_BF16}
+
+
+def refuse(name: str, call: str):
+    raise QwcError(STATUS_CODE[name], call)
+
+
+def current_stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def format_of(t: torch.Tensor, call: str) -> int:
+    fmt = FORMATS.get(t.dtype)
+    if fmt is None:
+        refuse("unsupported", call)
+    return fmt
+
+
+class PagedCache:
+    """One layer's pool: f16 scales [pages * page_size, kv_heads * head_dim / 64] and u8 codes
+    [pages * page_size, kv_heads * head_dim], keys and values."""
+
+    def __init__(self, k_scales: torch.Tensor, k_codes: torch.Tensor, v_scales: torch.Tensor, v_codes: torch.Tensor, *,
+                 page_size: int, kv_heads: int, head_dim: int):
+        width = kv_heads * head_dim
+        rows = k_codes.shape[0] if k_codes.dim() == 2 else -1
+        if page_size < 1 or rows < 0 or rows % page_size or width % GROUP:
+            refuse("shape_mismatch", "PagedCache")
+        for t, cols, dtype in ((k_scales, width // GROUP, torch.float16), (k_codes, width, torch.uint8),
+                               (v_scales, width // GROUP, torch.float16), (v_codes, width, torch.uint8)):
+            if t.dtype != dtype or t.device != k_codes.device or not t.is_contiguous():
+                refuse("invalid_argument", "PagedCache")
+            if t.shape != (rows, cols):
+                refuse("shape_mismatch", "PagedCache")
+        self.k_scales, self.k_codes, self.v_scales, self.v_codes = k_scales, k_codes, v_scales, v_codes
+        self.device = k_codes.device
+        self.pages, self.page_size, self.kv_heads, self.head_dim = rows // page_size, page_size, kv_heads, head_dim
+        self.desc = PagedCacheDesc(k_scales.data_ptr(), k_codes.data_ptr(), v_scales.data_ptr(), v_codes.data_ptr(),
+                                   self.pages, page_size, kv_heads, head_dim)
+        self._ref = ctypes.addressof(self.desc)
+
+    @classmethod
+    def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda") -> "PagedCache":
+        rows, width = pages * page_size, kv_heads * head_dim
+        s = [torch.zeros(rows, width // GROUP, dtype=torch.float16, device=device) for _ in range(2)]
+        c = [torch.zeros(rows, width, dtype=torch.uint8, device=device) for _ in range(2)]
+        return cls(s[0], c[0], s[1], c[1], page_size=page_size, kv_heads=kv_heads, head_dim=head_dim)
+
+
+class PagedBatch:
+    """The tokens of one step: query_starts [sequences + 1], context_lens [sequences] and page_table
+    [sequences, entries], int32 on the device (see qwc_paged_batch). `max_query` and `max_context`
+    bound what they hold; the arrays may change on the device between calls."""
+
+    def __init__(self, query_starts: torch.Tensor, context_lens: torch.Tensor, page_table: torch.Tensor, *, tokens: int,
+                 max_query: int, max_context: int):
+        for t in (query_starts, context_lens, page_table):
+            if t.dtype != torch.int32 or t.device != query_starts.device:
+                refuse("invalid_argument", "PagedBatch")
+        n = context_lens.numel()
+        if (query_starts.shape != (n + 1,) or context_lens.shape != (n,) or page_table.dim() != 2
+                or page_table.shape[0] != n or min(tokens, max_query, max_context) < 0):
+            refuse("shape_mismatch", "PagedBatch")
+        if not (query_starts.is_contiguous() and context_lens.is_contiguous()
+                and (page_table.stride(1) == 1 or page_table.shape[1] <= 1)):
+            refuse("invalid_argument", "PagedBatch")
+        self.query_starts, self.context_lens, self.page_table = query_starts, context_lens, page_table
+        self.device, self.tokens = query_starts.device, tokens
+        entries = page_table.stride(0) if n > 1 else page_table.shape[1]
+        self.desc = PagedBatchDesc(query_starts.data_ptr(), context_lens.data_ptr(), page_table.data_ptr(), n, tokens,
+                                   entries, max_query, max_context, 0)
+        self._ref = ctypes.addressof(self.desc)
+        self._workspace_bytes: dict = {}
+
+
+def _rows(t: torch.Tensor, batch: PagedBatch, heads: int, dim: int, call: str) -> int:
+    """The row stride of a [tokens, heads, dim] tensor whose rows are whole (a view of wider rows is fine)."""
+    if t.shape != (batch.tokens, heads, dim):
+        refuse("shape_mismatch", call)
+    if t.device != batch.device:
+        refuse("invalid_argument", call)
+    stride = t.stride()
+    if (stride[2] != 1 and dim > 1) or (stride[1] != dim and heads > 1):
+        refuse("invalid_argument", call)
+    return stride[0] if batch.tokens > 1 else max(stride[0], heads * dim)
+
+
+# Partial results of attention, one buffer for each (device, stream), zeroed when it is made and
+# kept at the largest size asked for.
+_workspaces: dict = {}
+
+
+def _workspace(cache: PagedCache, batch: PagedBatch, fmt: int, heads: int, stream: int) -> torch.Tensor:
+    key = (cache.pages, cache.page_size, cache.kv_heads, cache.head_dim, fmt, heads)
+    need = batch._workspace_bytes.get(key)
+    if need is None:
+        n = ctypes.c_uint64(0)
+        check(lib().qwc_op_paged_attention_workspace(cache._ref, batch._ref, fmt, heads, ctypes.byref(n)),
+              "qwc_op_paged_attention_workspace")
+        need = batch._workspace_bytes[key] = n.value
+    at = (cache.device, stream)
+    held = _workspaces.get(at)
+    if held is None or held.numel() < need:
+        held = _workspaces[at] = torch.zeros(need, dtype=torch.uint8, device=cache.device)
+    return held
+
+
+def append(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+           sin: torch.Tensor, *, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+           eps: float = 1e-6, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """QK-RMSNorm, rotation and the q8 append of [tokens, heads, head_dim] rows; returns the queries
+    for attention (`q_out`, a new tensor unless given; may be `q`)."""
+    call = "qwc_op_paged_append"
+    fmt = format_of(q, call)
+    if k.dtype != q.dtype or v.dtype != q.dtype or cache.device != batch.device or q.dim() != 3:
+        refuse("invalid_argument", call)
+    heads, dim = q.shape[1], cache.head_dim
+    if q_out is None:
+        q_out = torch.empty(batch.tokens, heads, dim, dtype=q.dtype, device=q.device)
+    elif q_out.dtype != q.dtype:
+        refuse("invalid_argument", call)
+    strides = [_rows(t, batch, n, dim, call) for t, n in ((q, heads), (k, cache.kv_heads), (v, cache.kv_heads), (q_out, heads))]
+    for t, shape in ((cos, (cos.shape[0], dim // 2)), (sin, (cos.shape[0], dim // 2)), (q_norm, (dim,)), (k_norm, (dim,))):
+        if t is None:
+            continue
+        if t.shape != shape:
+            refuse("shape_mismatch", call)
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.device != batch.device:
+            refuse("invalid_argument", call)
+    check(lib().qwc_op_paged_append(
+        cache._ref, batch._ref, fmt, q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(), strides[2], heads,
+        None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps, cos.data_ptr(),
+        sin.data_ptr(), cos.shape[0], q_out.data_ptr(), strides[3], current_stream(cache.device)), call)
+    return q_out
+
+
+def attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the batch's [tokens, heads, head_dim] queries over their sequences' pages."""
+    call = "qwc_op_paged_attention"
+    fmt = format_of(q, call)
+    if cache.device != batch.device or q.dim() != 3:
+        refuse("invalid_argument", call)
+    heads, dim = q.shape[1], cache.head_dim
+    if out is None:
+        out = torch.empty(batch.tokens, heads, dim, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype:
+        refuse("invalid_argument", call)
+    q_stride, out_stride = _rows(q, batch, heads, dim, call), _rows(out, batch, heads, dim, call)
+    stream = current_stream(cache.device)
+    work = _workspace(cache, batch, fmt, heads, stream)
+    check(lib().qwc_op_paged_attention(cache._ref, batch._ref, fmt, q.data_ptr(), q_stride, heads, out.data_ptr(),
+                                       out_stride, work.data_ptr(), work.numel(), stream), call)
+    return out
+
+
+def read(cache: PagedCache, batch: PagedBatch, dtype: torch.dtype = torch.float32, k_out: torch.Tensor | None = None,
+         v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached key and value rows of the batch's tokens as values, [tokens, kv_heads, head_dim]."""
+    call = "qwc_op_paged_read"
+    shape = (batch.tokens, cache.kv_heads, cache.head_dim)
+    k_out = torch.empty(shape, dtype=dtype, device=cache.device) if k_out is None else k_out
+    v_out = torch.empty(shape, dtype=dtype, device=cache.device) if v_out is None else v_out
+    fmt = format_of(k_out, call)
+    if k_out.dtype != v_out.dtype or cache.device != batch.device:
+        refuse("invalid_argument", call)
+    check(lib().qwc_op_paged_read(cache._ref, batch._ref, fmt, k_out.data_ptr(), _rows(k_out, batch, *shape[1:], call),
+                                  v_out.data_ptr(), _rows(v_out, batch, *shape[1:], call),
+                                  current_stream(cache.device)), call)
+    return k_out, v_out

@@ -31,6 +31,8 @@ STATUS = {
 STATUS_CODE = {name: code for code, name in STATUS.items()}
 
 CACHE_F32, CACHE_Q8 = 0, 1
+FORMAT_F32, FORMAT_F16, FORMAT_BF16 = 0, 1, 2
+SAMPLE_MAX_VOCAB = 1048576  # QWC_SAMPLE_MAX_VOCAB
 OPTION_IGNORE_EOS, OPTION_KEEP_LOGITS, OPTION_STEP_CHUNK, OPTION_TRACE, OPTION_PREFILL_SERIAL = 1, 2, 3, 4, 5
 OPTION_EXACT, OPTION_WAIT_LIMIT_US, OPTION_TEST_STALL = 6, 7, 8
 FEATURE_MODEL, FEATURE_DECODE, FEATURE_STREAMS = 1 << 3, 1 << 4, 1 << 8
@@ -94,6 +96,22 @@ SIGNATURES = {
     "qwc_op_rmsnorm": (c_int32, [c_void_p, c_void_p, c_uint32, c_uint32, c_float, c_void_p, c_void_p]),
     "qwc_op_rope": (c_int32, [c_void_p, c_uint32, c_uint32, c_void_p, c_void_p, c_uint32, c_void_p]),
     "qwc_op_silu_mul": (c_int32, [c_void_p, c_void_p, c_uint32, c_void_p, c_void_p]),
+    "qwc_op_paged_append": (
+        c_int32,
+        [c_void_p, c_void_p, c_uint32, c_void_p, c_uint64, c_void_p, c_uint64, c_void_p, c_uint64, c_uint32, c_void_p,
+         c_void_p, c_float, c_void_p, c_void_p, c_uint32, c_void_p, c_uint64, c_void_p],
+    ),
+    "qwc_op_paged_attention": (
+        c_int32,
+        [c_void_p, c_void_p, c_uint32, c_void_p, c_uint64, c_uint32, c_void_p, c_uint64, c_void_p, c_uint64, c_void_p],
+    ),
+    "qwc_op_paged_attention_workspace": (c_int32, [c_void_p, c_void_p, c_uint32, c_uint32, POINTER(c_uint64)]),
+    "qwc_op_paged_read": (c_int32, [c_void_p, c_void_p, c_uint32, c_void_p, c_uint64, c_void_p, c_uint64, c_void_p]),
+    "qwc_op_sample": (
+        c_int32,
+        [c_uint32, c_void_p, c_uint64, c_uint32, c_uint32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p],
+    ),
 }
 
 
@@ -160,6 +178,28 @@ class Requirements(ctypes.Structure):
 
 
 assert ctypes.sizeof(Requirements) == 48
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """qwc_paged_cache: one layer's pool of pages."""
+
+    _fields_ = [
+        ("k_scales", c_void_p), ("k_codes", c_void_p), ("v_scales", c_void_p), ("v_codes", c_void_p),
+        ("pages", c_uint32), ("page_size", c_uint32), ("kv_heads", c_uint32), ("head_dim", c_uint32),
+    ]
+
+
+class PagedBatchDesc(ctypes.Structure):
+    """qwc_paged_batch: the tokens of one step."""
+
+    _fields_ = [
+        ("query_starts", c_void_p), ("context_lens", c_void_p), ("page_table", c_void_p),
+        ("sequences", c_uint32), ("tokens", c_uint32), ("table_stride", c_uint32), ("max_query", c_uint32),
+        ("max_context", c_uint32), ("reserved", c_uint32),
+    ]
+
+
+assert ctypes.sizeof(PagedCacheDesc) == 48 and ctypes.sizeof(PagedBatchDesc) == 48
 
 
 class CudaModel:

@@ -1,0 +1,118 @@
+"""The paged operators' and the sampler's checks, which come before any CUDA call: the addresses here
+are made up, and no GPU is needed."""
+
+import ctypes
+
+import pytest
+
+from qwenscriber_b200 import runtime as rt
+
+A = 1 << 20  # aligned to everything
+
+
+def cache(**kw):
+    d = dict(k_scales=A, k_codes=A, v_scales=A, v_codes=A, pages=10, page_size=16, kv_heads=2, head_dim=128)
+    d.update(kw)
+    return rt.PagedCacheDesc(*d.values())
+
+
+def batch(**kw):
+    d = dict(query_starts=A, context_lens=A, page_table=A, sequences=2, tokens=2, table_stride=5, max_query=1, max_context=80,
+             reserved=0)
+    d.update(kw)
+    return rt.PagedBatchDesc(*d.values())
+
+
+def attention(c, b, fmt=0, q=A, q_stride=512, heads=4, out=A, out_stride=512, work=A, size=1 << 40):
+    return rt.lib().qwc_op_paged_attention(ctypes.addressof(c), ctypes.addressof(b), fmt, q, q_stride, heads, out, out_stride, work,
+                                           size, None)
+
+
+def append(c, b, fmt=0, q=A, q_stride=1024, k=A, k_stride=1024, v=A, v_stride=1024, heads=4, qn=A, kn=A, cos=A, sin=A, out=A,
+           out_stride=1024):
+    return rt.lib().qwc_op_paged_append(ctypes.addressof(c), ctypes.addressof(b), fmt, q, q_stride, k, k_stride, v, v_stride, heads,
+                                        qn, kn, 1e-6, cos, sin, 100, out, out_stride, None)
+
+
+def read(c, b, fmt=0, k=A, k_stride=256, v=A, v_stride=256):
+    return rt.lib().qwc_op_paged_read(ctypes.addressof(c), ctypes.addressof(b), fmt, k, k_stride, v, v_stride, None)
+
+
+INVALID, UNSUPPORTED, SHAPE, LIMIT = (rt.STATUS_CODE[n] for n in ("invalid_argument", "unsupported", "shape_mismatch", "limit_exceeded"))
+
+POOL = [
+    (dict(k_scales=None), {}, INVALID), (dict(v_codes=A + 8), {}, INVALID), (dict(k_codes=A + 1), {}, INVALID),
+    ({}, dict(page_table=None), INVALID), ({}, dict(query_starts=A + 2), INVALID),
+    (dict(head_dim=96), {}, UNSUPPORTED), (dict(head_dim=256), {}, UNSUPPORTED), (dict(head_dim=0), {}, UNSUPPORTED),
+    (dict(kv_heads=0), {}, SHAPE), (dict(page_size=0), {}, SHAPE), (dict(pages=0), {}, SHAPE),
+    ({}, dict(max_context=81), SHAPE), (dict(pages=1 << 31, page_size=16), {}, LIMIT), ({}, dict(sequences=70000), LIMIT),
+]
+
+
+@pytest.mark.parametrize("call", [attention, append, read])
+@pytest.mark.parametrize("c,b,status", POOL)
+def test_descriptors_are_checked(cuda_lib, call, c, b, status):
+    assert call(cache(**c), batch(**b)) == status
+
+
+def test_null_descriptors(cuda_lib):
+    L = rt.lib()
+    c = ctypes.addressof(cache())
+    assert L.qwc_op_paged_read(None, None, 0, A, 256, A, 256, None) == INVALID
+    assert L.qwc_op_paged_read(c, None, 0, A, 256, A, 256, None) == INVALID
+    assert L.qwc_op_paged_attention_workspace(c, None, 0, 4, None) == INVALID
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(fmt=16), UNSUPPORTED), (dict(q=None), INVALID), (dict(q=A + 4), INVALID), (dict(out=A + 8), INVALID),
+    (dict(q_stride=513), INVALID), (dict(fmt=2, q_stride=516), INVALID), (dict(q_stride=256), SHAPE), (dict(out_stride=508), SHAPE),
+    (dict(heads=0), SHAPE), (dict(heads=5), SHAPE), (dict(work=None), INVALID), (dict(work=A + 4), INVALID), (dict(size=0), LIMIT),
+])
+def test_attention_arguments(cuda_lib, kw, status):
+    assert attention(cache(), batch(), **kw) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(fmt=3), UNSUPPORTED), (dict(k=None), INVALID), (dict(v=A + 4), INVALID), (dict(cos=None), INVALID), (dict(sin=A + 4), INVALID),
+    (dict(qn=A + 4), INVALID), (dict(kn=A + 8), INVALID), (dict(k_stride=252), SHAPE), (dict(v_stride=1022), INVALID),
+    (dict(heads=3), SHAPE), (dict(out=None), INVALID),
+])
+def test_append_arguments(cuda_lib, kw, status):
+    assert append(cache(), batch(), **kw) == status
+
+
+@pytest.mark.parametrize("kw,status", [(dict(fmt=18), UNSUPPORTED), (dict(k=None), INVALID), (dict(v=A + 2), INVALID),
+                                       (dict(k_stride=128), SHAPE), (dict(fmt=1, v_stride=260), INVALID)])
+def test_read_arguments(cuda_lib, kw, status):
+    assert read(cache(), batch(), **kw) == status
+
+
+def test_nothing_to_do_launches_nothing(cuda_lib):
+    # No tokens, or no sequences: ok without a device.
+    for b in (batch(tokens=0), batch(max_query=0), batch(sequences=0)):
+        assert attention(cache(), b) == 0 and append(cache(), b) == 0 and read(cache(), b) == 0
+
+
+def test_workspace_is_bounded_by_the_batch(cuda_lib):
+    def need(b, fmt=0, heads=4):
+        n = ctypes.c_uint64(0)
+        assert rt.lib().qwc_op_paged_attention_workspace(ctypes.addressof(cache()), ctypes.addressof(b), fmt, heads, ctypes.byref(n)) == 0
+        return n.value
+
+    assert 0 < need(batch()) <= need(batch(sequences=64, tokens=64))
+    assert need(batch(sequences=64, tokens=64 * 512, max_query=512, max_context=80)) < 1 << 30
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(fmt=16), UNSUPPORTED), (dict(logits=None), INVALID), (dict(uniforms=None), INVALID), (dict(out=None), INVALID),
+    (dict(vocab=0), INVALID), (dict(logits=A + 2), INVALID), (dict(fmt=1, logits=A + 1), INVALID), (dict(top_k=A + 2), INVALID),
+    (dict(stride=99), SHAPE), (dict(vocab=rt.SAMPLE_MAX_VOCAB + 1, stride=1 << 21), LIMIT),
+])
+def test_sample_arguments(cuda_lib, kw, status):
+    d = dict(fmt=0, logits=A, stride=100, rows=2, vocab=100, temperature=A, top_k=A, top_p=A, min_p=A, uniforms=A, out=A, logprobs=A)
+    d.update(kw)
+    assert rt.lib().qwc_op_sample(*d.values(), None) == status
+
+
+def test_sample_of_no_rows(cuda_lib):
+    assert rt.lib().qwc_op_sample(0, A, 100, 0, 100, None, None, None, None, A, A, None, None) == 0

@@ -58,14 +58,632 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attention_kernel(const Page
   }
 }
 
+// ---- few query rows ----
+//
+// A sequence whose tokens give at most kRows rows to a kv head (a row is one
+// token's query head) is bound by its cache: every code byte is read once and
+// used by a handful of rows. The products run on mma.sync m16n8k16 (f16
+// operands, f32 sums), whose rate is ample here; tcgen05's 128-row tiles
+// would be nearly empty.
+//
+// Work is dealt evenly whatever the lengths: the steps of all (sequence, group
+// of kv heads) pairs, 16 * PB positions each, stand in one line and each CTA
+// takes an equal stretch of it. In a step warp (pb, h) takes head h's 16
+// positions number pb. A (sequence, group) that lies in one stretch is finished there; one that is
+// cut leaves a partial result (maximum, sum, unnormalised output) for each stretch, and the CTA that
+// comes last adds them up in the order of the stretches, so the result does
+// not depend on who was last.
+//
+// Scores: A rows are query rows (f32: rows 0-7 the f16 parts hi, rows 8-15 the parts lo of the
+// same eight, so a score is the sum of two accumulator rows), B columns are
+// positions, codes entering as exact f16 integers; a group of 64 dims has its
+// own accumulator, which the key scale multiplies afterwards. Values: the
+// accumulator layout of the weights is the A layout of the second product; the
+// weight times the value scale of each group, again as one or two f16 parts,
+// times exact codes. The weights carry a factor 2^(28 - e) with e the largest exponent of a value
+// scale so far, which keeps them in f16's normal range whatever the scales.
+
+constexpr int kFewWarps = 8;
+constexpr int kFewThreads = 32 * kFewWarps;
+constexpr int kFewBlock = 16;   // positions a warp takes at a time
+constexpr int kFewStages = 2;   // blocks of codes in a warp's ring
+constexpr int kMaxFewCtas = 1024;
+
+template <int DIM>
+struct FewTile {
+  uint8_t k[kFewBlock][DIM];
+  uint8_t v[kFewBlock][DIM];
+};
+
+struct AttnArgs {
+  uint64_t q_stride, out_stride;
+  const void* q;
+  void* out;
+  float* partials;     // [2 * grid][group heads][rows][DIM + 4]
+  uint32_t* counters;  // [kMaxFewCtas], zero between calls
+  uint32_t heads, share;
+  uint32_t group;      // kv heads of a CTA
+  uint32_t pb;         // position blocks of a step
+  uint32_t rows;       // most rows of a kv head: max_query * share
+  float scaling;
+};
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
+  const uint32_t h = __byte_perm(w, 0x64646464u, SEL);
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));  // (1024 + u) - (1024 + 128)
+  return r;
+}
+
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 f16x2_f32(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The power of two that brings a row of queries near 1: their f16 parts then
+// hold 11 (or 22) bits of every value that matters beside the largest.
+__device__ __forceinline__ int row_exponent(float amax) {
+  const int e = static_cast<int>((__float_as_uint(amax) >> 23) & 0xFFu) - 127;
+  return min(max(e, -126), 126);
+}
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(const PagedArgs a, const AttnArgs p) {
+  constexpr bool SPLIT = sizeof(T) == 4;  // f32 rows enter as two f16 parts
+  constexpr int G = DIM / 64;             // scale groups of a head
+  constexpr int CHUNKS = DIM / 16;        // 16-byte chunks of a row of codes
+  constexpr int NT = DIM / 8;             // 8-column tiles of the output
+  constexpr uint32_t kValueSwizzle = DIM == 128 ? 6u : 2u;  // chunks of the rows that a half warp reads at once: apart
+  constexpr int STATE = DIM + 4;          // a row's state in shared memory or a partial: output, maximum, sum
+  extern __shared__ __align__(128) uint8_t few_smem[];
+  FewTile<DIM>* ring = reinterpret_cast<FewTile<DIM>*>(few_smem);                                  // [warp][stage]
+  uint32_t* scales = reinterpret_cast<uint32_t*>(few_smem + sizeof(FewTile<DIM>) * kFewWarps * kFewStages);  // [warp][2][16]
+  float* states = reinterpret_cast<float*>(scales + kFewWarps * 32);                                 // [warp][rows][STATE]
+  __shared__ uint64_t sums[kFewWarps];
+  __shared__ uint64_t found_base;
+  __shared__ uint32_t found_s, last_flag;
+
+  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t r = lane >> 2, c = lane & 3u;
+  const uint32_t ngroups = a.kv_heads / p.group;
+  const uint32_t span = kFewBlock * p.pb;
+  const uint32_t wh = warp % p.group, wpb = warp / p.group;
+  const bool works = warp < p.group * p.pb;
+
+  // ---- this CTA's stretch of the line of steps ----
+  auto steps_of = [&](const PagedSeq& q) -> uint32_t { return q.n ? max(1u, (q.context + span - 1) / span) : 0u; };
+  uint64_t part = 0;
+  for (uint32_t s = tid; s < a.sequences; s += kFewThreads) part += uint64_t(steps_of(paged_seq(a, s))) * ngroups;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+  if (lane == 0) sums[warp] = part;
+  __syncthreads();
+  uint64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kFewWarps; ++w) total += sums[w];
+  const uint64_t grid = total < gridDim.x ? total : gridDim.x;
+  if (blockIdx.x >= grid) return;
+  const uint64_t u0 = total * blockIdx.x / grid, u1 = total * (blockIdx.x + 1) / grid;
+  uint64_t running = 0;
+  for (uint32_t base = 0; base < a.sequences; base += kFewThreads) {
+    const uint32_t s = base + tid;
+    const uint64_t v = s < a.sequences ? uint64_t(steps_of(paged_seq(a, s))) * ngroups : 0;
+    uint64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= static_cast<uint32_t>(o)) inc += t;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = inc;
+    __syncthreads();
+    uint64_t before = running, all = running;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      if (w < static_cast<int>(warp)) before += sums[w];
+      all += sums[w];
+    }
+    if (v && before + inc - v <= u0 && u0 < before + inc) {
+      found_s = s;
+      found_base = before + inc - v;
+    }
+    running = all;
+    if (running > u0) break;
+  }
+  __syncthreads();
+  uint32_t s = found_s;
+  uint64_t seq_base = found_base;
+  PagedSeq seq = paged_seq(a, s);
+  uint32_t sp = steps_of(seq);
+
+  FewTile<DIM>* my_ring = ring + warp * kFewStages;
+  uint32_t* my_scales = scales + warp * 32;  // [0..15] keys, [16..31] values of the block in hand
+
+  for (uint64_t cur = u0; cur < u1;) {
+    while (cur >= seq_base + uint64_t(sp) * ngroups) {
+      seq_base += uint64_t(sp) * ngroups;
+      seq = paged_seq(a, ++s);
+      sp = steps_of(seq);
+    }
+    const uint32_t gi = static_cast<uint32_t>((cur - seq_base) / sp);
+    const uint64_t seg0 = seq_base + uint64_t(gi) * sp, seg1 = seg0 + sp;
+    const uint64_t stop = u1 < seg1 ? u1 : seg1;
+    const uint32_t j0 = static_cast<uint32_t>(cur - seg0), j1 = static_cast<uint32_t>(stop - seg0);
+    const uint32_t h = gi * p.group + wh;
+    const uint32_t rows = min(seq.n * p.share, p.rows);
+
+    if (works) {
+      // ---- queries ----
+      // Lane (r, c) holds, of rows r and r + 8, dims 64 g + 16 c + 4 t + 0..3 for every (g, t).
+      uint32_t qa[G * 4][4];
+      float factor[2];  // log2(e) / sqrt(d) * 2^e: from a sum to a score in powers of two
+      int32_t limit[2];  // last position that the row sees
+#pragma unroll
+      for (int half = 0; half < (SPLIT ? 1 : 2); ++half) {
+        const uint32_t row = r + 8 * half;
+        const bool in = row < rows;
+        const uint32_t tok = in ? row / p.share : 0, hq = h * p.share + (in ? row % p.share : 0);
+        const T* src = static_cast<const T*>(p.q) + size_t(seq.first + tok) * p.q_stride + size_t(hq) * DIM;
+        float x[G * 4][4];
+        float amax = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < G * 4; ++kk) {
+          const uint32_t d = 64u * (kk / 4) + 16u * c + 4u * (kk % 4);
+          if constexpr (SPLIT) {
+            const float4 f = in ? *reinterpret_cast<const float4*>(src + d) : make_float4(0, 0, 0, 0);
+            x[kk][0] = f.x, x[kk][1] = f.y, x[kk][2] = f.z, x[kk][3] = f.w;
+          } else {
+            const uint2 f = in ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
+            float y[8];
+            unpack16(make_uint4(f.x, f.y, 0, 0), y, T());
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[kk][e] = y[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[kk][e]));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int e2 = row_exponent(amax);
+        const float down = pow2i(-e2);
+        factor[half] = p.scaling * 1.4426950408889634f * pow2i(e2);
+        limit[half] = in ? seq.base + static_cast<int32_t>(tok) : -1;
+#pragma unroll
+        for (int kk = 0; kk < G * 4; ++kk) {
+          float y[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = fmaf(x[kk][e], down, x[kk][e] - x[kk][e]);  // an infinity is NaN from here on
+          const uint32_t h01 = f16x2(y[0], y[1]), h23 = f16x2(y[2], y[3]);
+          qa[kk][half] = h01;
+          qa[kk][2 + half] = h23;
+          if constexpr (SPLIT) {
+            const float2 f01 = f16x2_f32(h01), f23 = f16x2_f32(h23);
+            lo[0] = y[0] - f01.x, lo[1] = y[1] - f01.y, lo[2] = y[2] - f23.x, lo[3] = y[3] - f23.y;
+            qa[kk][1] = f16x2(lo[0], lo[1]);
+            qa[kk][3] = f16x2(lo[2], lo[3]);
+          }
+        }
+      }
+
+      // ---- the loads: positions of block j, one row for each lane of a half warp ----
+      const uint32_t context = seq.context;
+      auto position = [&](uint32_t j) { return j * span + wpb * kFewBlock + (lane & 15u); };
+      auto page_id = [&](uint32_t j) -> int32_t {
+        const uint32_t pos = position(j);
+        return j < j1 && pos < context ? __ldg(a.page_table + size_t(s) * a.table_stride + page_of(a, pos)) : -1;
+      };
+      auto row_of = [&](uint32_t j, int32_t id) -> int32_t {
+        const uint32_t pos = position(j);
+        return static_cast<uint32_t>(id) < a.pages ? id * static_cast<int32_t>(a.page_size) +
+                                                         static_cast<int32_t>(pos - page_of(a, pos) * a.page_size)
+                                                   : -1;
+      };
+      uint32_t scale_next = 0, valid_next = 0;
+      auto load = [&](uint32_t j, int32_t id) {  // block j's codes into its stage; its scales into a register
+        const int32_t row = row_of(j, id);
+        valid_next = __ballot_sync(0xffffffffu, row >= 0) & 0xFFFFu;
+        FewTile<DIM>* t = my_ring + j % kFewStages;
+#pragma unroll
+        for (int i = 0; i < CHUNKS / 2; ++i) {
+          const uint32_t tr = lane / CHUNKS + i * (32 / CHUNKS), ch = lane % CHUNKS;
+          const int32_t src = __shfl_sync(0xffffffffu, row, tr);
+          const size_t at = size_t(src < 0 ? 0 : src) * a.code_row + size_t(h) * DIM + 16u * ch;
+          cp_async16(&t->k[tr][16u * (ch ^ ((tr & 1u) * (CHUNKS / 2)))], a.k_codes + at, src >= 0);
+          cp_async16(&t->v[tr][16u * (ch ^ (tr & kValueSwizzle))], a.v_codes + at, src >= 0);
+        }
+        cp_async_commit();
+        const uint8_t* plane = lane < 16 ? a.k_scales : a.v_scales;
+        scale_next = 0;
+        if (row >= 0) {
+          const uint8_t* at = plane + size_t(row) * a.scale_row + size_t(h) * (2 * G);
+          scale_next = G == 2 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
+        }
+      };
+
+      float acc[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+      uint32_t vexp = 0;  // the largest exponent field of a value scale so far
+
+      int32_t id = page_id(j0);
+      load(j0, id);
+      id = page_id(j0 + 1);
+      for (uint32_t j = j0; j < j1; ++j) {
+        const uint32_t valid = valid_next;
+        __syncwarp();  // the last block's reads of the scales are done
+        my_scales[lane] = scale_next;
+        if (j + 1 < j1) {
+          load(j + 1, id);
+          id = page_id(j + 2);
+          cp_async_wait<1>();
+        } else {
+          cp_async_wait<0>();
+        }
+        __syncwarp();
+        const FewTile<DIM>* t = my_ring + j % kFewStages;
+
+        // ---- scores of positions 2 c, 2 c + 1 (tile 0) and 8 + those (tile 1), rows r and r + 8 ----
+        float sc[2][2][2];  // [row half][tile][column]
+        uint32_t vs[4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const uint32_t kr = 8u * nt + r;
+          float d[G][4];
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            d[g][0] = d[g][1] = d[g][2] = d[g][3] = 0.0f;
+            const uint4 kw = *reinterpret_cast<const uint4*>(&t->k[kr][16u * ((4u * g + c) ^ ((kr & 1u) * (CHUNKS / 2)))]);
+            const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              mma16816(d[g], qa[4 * g + e][0], qa[4 * g + e][1], qa[4 * g + e][2], qa[4 * g + e][3],
+                       codes_f16x2<0x4140>(w[e]), codes_f16x2<0x4342>(w[e]));
+            }
+          }
+#pragma unroll
+          for (int col = 0; col < 2; ++col) {
+            const uint32_t key = 8u * nt + 2u * c + col;
+            const uint32_t ks = my_scales[key];
+            vs[2 * nt + col] = my_scales[16 + key];
+            const float k0 = f16_bits_to_f32(ks & 0xFFFFu), k1 = G == 2 ? f16_bits_to_f32(ks >> 16) : 0.0f;
+            if constexpr (SPLIT) {
+              float x = (d[0][col] + d[0][2 + col]) * k0;
+              if constexpr (G == 2) x = fmaf(d[G - 1][col] + d[G - 1][2 + col], k1, x);
+              sc[0][nt][col] = x;
+            } else {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                float x = d[0][2 * half + col] * k0;
+                if constexpr (G == 2) x = fmaf(d[G - 1][2 * half + col], k1, x);
+                sc[half][nt][col] = x;
+              }
+            }
+          }
+        }
+        const int32_t pos0 = static_cast<int32_t>(j * span + wpb * kFewBlock);
+        constexpr int HALVES = SPLIT ? 1 : 2;
+        float rescale[2] = {1.0f, 1.0f};
+        bool grew = false;
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+            for (int col = 0; col < 2; ++col) {
+              const uint32_t key = 8u * nt + 2u * c + col;
+              const bool seen = ((valid >> key) & 1u) && pos0 + static_cast<int32_t>(key) <= limit[half];
+              const float x = seen ? sc[half][nt][col] * factor[half] : -INFINITY;
+              sc[half][nt][col] = x;
+              mx = fmaxf(mx, x);
+            }
+          }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (mx > m[half]) {
+            rescale[half] = m[half] == -INFINITY ? 0.0f : ex2(m[half] - mx);
+            m[half] = mx;
+            grew = true;
+          }
+          const float base = m[half] == -INFINITY ? 0.0f : m[half];
+          float sum = 0.0f;
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+            for (int col = 0; col < 2; ++col) {
+              sc[half][nt][col] = ex2(sc[half][nt][col] - base);
+              sum += sc[half][nt][col];
+            }
+          }
+          l[half] = fmaf(l[half], rescale[half], sum);
+        }
+        // Value scales: a position nobody sees (or that is not cached) counts as zero.
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t key = 8u * (i / 2) + 2u * c + (i % 2);
+          if (!((valid >> key) & 1u)) vs[i] = 0;
+          top = max(top, max((vs[i] >> 10) & 31u, (vs[i] >> 26) & 31u));
+        }
+        top = min(__reduce_max_sync(0xffffffffu, top), 30u);
+        float down = 1.0f;
+        if (top > vexp) {
+          down = pow2i(static_cast<int>(vexp) - static_cast<int>(top));
+          vexp = top;
+          grew = true;
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+          const float f0 = rescale[0] * down, f1 = SPLIT ? f0 : rescale[1] * down;
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            acc[i][0] *= f0;
+            acc[i][1] *= f0;
+            acc[i][2] *= f1;
+            acc[i][3] *= f1;
+          }
+        }
+        const float up = pow2i(28 - static_cast<int>(vexp));
+        // ---- weights: A fragments for each group ----
+        uint32_t wa[G][4];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            const float v0 = f16_bits_to_f32((vs[2 * nt] >> (16 * g)) & 0xFFFFu) * up;
+            const float v1 = f16_bits_to_f32((vs[2 * nt + 1] >> (16 * g)) & 0xFFFFu) * up;
+            const float w0 = sc[0][nt][0] * v0, w1 = sc[0][nt][1] * v1;
+            const uint32_t hi = f16x2(w0, w1);
+            wa[g][2 * nt] = hi;
+            if constexpr (SPLIT) {
+              const float2 f = f16x2_f32(hi);
+              wa[g][2 * nt + 1] = f16x2(w0 - f.x, w1 - f.y);
+            } else {
+              wa[g][2 * nt + 1] = f16x2(sc[1][nt][0] * v0, sc[1][nt][1] * v1);
+            }
+          }
+        }
+        // ---- values: output tile 8 g + i has column n at dim 64 g + 8 n + i ----
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          uint2 vw[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t vr = 8u * (i / 2) + 2u * c + (i % 2);
+            const uint32_t ch = (4u * g + r / 2) ^ (vr & kValueSwizzle);
+            vw[i] = *reinterpret_cast<const uint2*>(&t->v[vr][16u * ch + 8u * (r & 1u)]);
+          }
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t x0 = w ? vw[0].y : vw[0].x, x1 = w ? vw[1].y : vw[1].x;
+            const uint32_t x2 = w ? vw[2].y : vw[2].x, x3 = w ? vw[3].y : vw[3].x;
+            const uint32_t a01 = __byte_perm(x0, x1, 0x5140), a23 = __byte_perm(x0, x1, 0x7362);
+            const uint32_t b01 = __byte_perm(x2, x3, 0x5140), b23 = __byte_perm(x2, x3, 0x7362);
+            float(*o)[4] = &acc[8 * g + 4 * w];
+            mma16816(o[0], wa[g][0], wa[g][1], wa[g][2], wa[g][3], codes_f16x2<0x4140>(a01), codes_f16x2<0x4140>(b01));
+            mma16816(o[1], wa[g][0], wa[g][1], wa[g][2], wa[g][3], codes_f16x2<0x4342>(a01), codes_f16x2<0x4342>(b01));
+            mma16816(o[2], wa[g][0], wa[g][1], wa[g][2], wa[g][3], codes_f16x2<0x4140>(a23), codes_f16x2<0x4140>(b23));
+            mma16816(o[3], wa[g][0], wa[g][1], wa[g][2], wa[g][3], codes_f16x2<0x4342>(a23), codes_f16x2<0x4342>(b23));
+          }
+        }
+      }
+
+      // ---- this warp's state: lane (r, c) has dims 64 g + 16 c + 0..15 of its rows ----
+      const float back = pow2i(static_cast<int>(vexp) - 28);
+#pragma unroll
+      for (int half = 0; half < (SPLIT ? 1 : 2); ++half) {
+        const uint32_t row = r + 8 * half;
+        float lsum = l[half] + __shfl_xor_sync(0xffffffffu, l[half], 1);
+        lsum += __shfl_xor_sync(0xffffffffu, lsum, 2);
+        if (row < rows) {
+          float* st = states + (size_t(warp) * p.rows + row) * STATE;
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+#pragma unroll
+            for (int col = 0; col < 2; ++col) {
+              float o[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                o[i] = (SPLIT ? acc[8 * g + i][col] + acc[8 * g + i][2 + col] : acc[8 * g + i][2 * half + col]) * back;
+              }
+              float* dst = st + 64 * g + 16 * c + 8 * col;
+              *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<float4*>(dst + 4) = make_float4(o[4], o[5], o[6], o[7]);
+            }
+          }
+          if (c == 0) {
+            st[DIM] = m[half];
+            st[DIM + 1] = lsum;
+          }
+        }
+      }
+    }
+    __syncthreads();
+
+    // ---- the segment's rows: merge the position blocks, then finish or leave a partial ----
+    const bool whole = j0 == 0 && j1 == sp;
+    const uint32_t tasks = p.group * rows;
+    constexpr int PER = DIM / 32;
+    const uint32_t slot = 2 * blockIdx.x + (seg0 > u0 ? 1u : 0u);
+    auto finish = [&](uint32_t hh, uint32_t row, const float (&o)[PER], float lsum) {
+      T* dst = static_cast<T*>(p.out) + size_t(seq.first + row / p.share) * p.out_stride +
+               size_t((gi * p.group + hh) * p.share + row % p.share) * DIM + PER * lane;
+      const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) store_as(dst + e, o[e] * inv);
+    };
+    for (uint32_t task = warp; task < tasks; task += kFewWarps) {
+      const uint32_t hh = task / rows, row = task % rows;
+      float mx = -INFINITY;
+      for (uint32_t b = 0; b < p.pb; ++b) {
+        const float* st = states + (size_t(b * p.group + hh) * p.rows + row) * STATE;
+        mx = fmaxf(mx, st[DIM]);
+      }
+      float o[PER], lsum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] = 0.0f;
+      for (uint32_t b = 0; b < p.pb; ++b) {
+        const float* st = states + (size_t(b * p.group + hh) * p.rows + row) * STATE;
+        const float f = mx == -INFINITY ? 1.0f : ex2(st[DIM] - mx);
+        lsum = fmaf(st[DIM + 1], f, lsum);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[e] = fmaf(st[PER * lane + e], f, o[e]);
+      }
+      if (whole) {
+        finish(hh, row, o, lsum);
+      } else {
+        float* dst = p.partials + (size_t(slot * p.group + hh) * p.rows + row) * STATE;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) dst[PER * lane + e] = o[e];
+        if (lane == 0) {
+          dst[DIM] = mx;
+          dst[DIM + 1] = lsum;
+        }
+      }
+    }
+    if (!whole) {
+      // The stretches that hold this segment: c0 .. c1 (stretch x starts at floor(x * total / grid)).
+      const uint32_t c0 = static_cast<uint32_t>(((seg0 + 1) * grid - 1) / total);
+      const uint32_t c1 = static_cast<uint32_t>((seg1 * grid - 1) / total);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const uint32_t before = atomicAdd(&p.counters[c0], 1u);
+        last_flag = before == c1 - c0;
+        if (before == c1 - c0) p.counters[c0] = 0;
+      }
+      __syncthreads();
+      if (last_flag) {
+        __threadfence();
+        for (uint32_t task = warp; task < tasks; task += kFewWarps) {
+          const uint32_t hh = task / rows, row = task % rows;
+          auto piece = [&](uint32_t x) {
+            const uint32_t sl = 2 * x + (seg0 > total * x / grid ? 1u : 0u);
+            return p.partials + (size_t(sl * p.group + hh) * p.rows + row) * STATE;
+          };
+          float mx = -INFINITY;
+          for (uint32_t x = c0 + lane; x <= c1; x += 32) mx = fmaxf(mx, __ldcg(piece(x) + DIM));
+          mx = warp_max(mx);
+          float o[PER], lsum = 0.0f;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) o[e] = 0.0f;
+          for (uint32_t x0 = c0; x0 <= c1; x0 += 8) {
+            float v[8][PER], pm[8], pl[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const bool in = x0 + i <= c1;
+              const float* src = piece(in ? x0 + i : c1);
+              pm[i] = in ? __ldcg(src + DIM) : -INFINITY;
+              pl[i] = in ? __ldcg(src + DIM + 1) : 0.0f;
+              if constexpr (PER == 4) {
+                const float4 f = __ldcg(reinterpret_cast<const float4*>(src) + lane);
+                v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
+              } else {
+                const float2 f = __ldcg(reinterpret_cast<const float2*>(src) + lane);
+                v[i][0] = f.x, v[i][1] = f.y;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (x0 + i > c1) break;
+              const float f = mx == -INFINITY ? 1.0f : ex2(pm[i] - mx);
+              lsum = fmaf(pl[i], f, lsum);
+#pragma unroll
+              for (int e = 0; e < PER; ++e) o[e] = fmaf(v[i][e], f, o[e]);
+            }
+          }
+          finish(hh, row, o, lsum);
+        }
+      }
+    }
+    __syncthreads();  // the states are free again
+    cur = stop;
+  }
+}
+
+template <typename T, int DIM>
+size_t few_smem_bytes(uint32_t rows) {
+  return sizeof(FewTile<DIM>) * kFewWarps * kFewStages + kFewWarps * 32 * 4 + size_t(kFewWarps) * rows * (DIM + 4) * 4;
+}
+
+// How a call is run: which kernel, its grid, and its part of the workspace.
+struct AttnPlan {
+  bool few;
+  uint32_t grid, group, pb, rows;
+  uint64_t partial_bytes;
+};
+
+AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
+  AttnPlan p = {};
+  const uint64_t rows = uint64_t(a.max_query) * (heads / a.kv_heads);
+  p.few = rows <= (format == kFormatF32 ? 8u : 16u);
+  if (!p.few) return p;
+  p.rows = static_cast<uint32_t>(rows);
+  const uint64_t sms = 148;
+  p.group = 1;
+  if (uint64_t(a.sequences) * a.kv_heads * a.max_context >= 8ull * 2 * sms * 512) {
+    for (uint32_t g = 2; g <= 8; ++g) {
+      if (a.kv_heads % g == 0) p.group = g;
+    }
+  }
+  p.pb = kFewWarps / p.group;
+  const uint64_t span = uint64_t(kFewBlock) * p.pb;
+  const uint64_t steps = uint64_t(a.sequences) * (a.kv_heads / p.group) * (a.max_context ? (a.max_context + span - 1) / span : 1);
+  p.grid = static_cast<uint32_t>(steps < 2 * sms ? steps : 2 * sms);
+  p.partial_bytes = uint64_t(2) * p.grid * p.group * p.rows * (a.head_dim + 4) * 4;
+  return p;
+}
+
+constexpr uint64_t kCounterBytes = kMaxFewCtas * 4;
+
+template <typename T, int DIM>
+int32_t launch_few(const PagedArgs& a, AttnArgs p, const AttnPlan& plan, cudaStream_t stream) {
+  const size_t smem = few_smem_bytes<T, DIM>(plan.rows);
+  cudaError_t e = cudaFuncSetAttribute(paged_attention_few_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(smem));
+  if (e != cudaSuccess) return paged_status(e);
+  p.group = plan.group;
+  p.pb = plan.pb;
+  p.rows = plan.rows;
+  paged_attention_few_kernel<T, DIM><<<plan.grid, kFewThreads, smem, stream>>>(a, p);
+  return paged_status(cudaGetLastError());
+}
+
 template <typename T>
-int32_t attention_as(const PagedArgs& a, const void* q, uint64_t q_stride, uint32_t heads, void* out, uint64_t out_stride,
-                     cudaStream_t stream) {
-  const float scaling = 1.0f / sqrtf(static_cast<float>(a.head_dim));
-  const dim3 grid(static_cast<uint32_t>((uint64_t(a.max_query) * heads + kWarps - 1) / kWarps), a.sequences);
+int32_t attention_as(const PagedArgs& a, AttnArgs p, const AttnPlan& plan, cudaStream_t stream) {
+  if (plan.few) return a.head_dim == 128 ? launch_few<T, 128>(a, p, plan, stream) : launch_few<T, 64>(a, p, plan, stream);
+  const dim3 grid(static_cast<uint32_t>((uint64_t(a.max_query) * p.heads + kWarps - 1) / kWarps), a.sequences);
   auto kernel = a.head_dim == 128 ? paged_attention_kernel<T, 128> : paged_attention_kernel<T, 64>;
-  kernel<<<grid, 32 * kWarps, 0, stream>>>(a, static_cast<const T*>(q), q_stride, heads, static_cast<T*>(out), out_stride,
-                                           scaling);
+  kernel<<<grid, 32 * kWarps, 0, stream>>>(a, static_cast<const T*>(p.q), p.q_stride, p.heads, static_cast<T*>(p.out),
+                                           p.out_stride, p.scaling);
   return paged_status(cudaGetLastError());
 }
 
@@ -84,7 +702,7 @@ int32_t qwc_op_paged_attention_workspace(const qwc_paged_cache* cache, const qwc
   const int32_t st = paged_args(cache, batch, &a);
   if (st != QWC_OK) return st;
   if (heads == 0 || heads % a.kv_heads != 0) return QWC_SHAPE_MISMATCH;
-  *bytes = 16;
+  *bytes = kCounterBytes + attention_plan(a, format, heads).partial_bytes;
   return QWC_OK;
 }
 
@@ -102,12 +720,22 @@ int32_t qwc_op_paged_attention(const qwc_paged_cache* cache, const qwc_paged_bat
   if ((st = paged_rows_check(q, q_stride, qw, format)) != QWC_OK) return st;
   if ((st = paged_rows_check(out, out_stride, qw, format)) != QWC_OK) return st;
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return QWC_INVALID_ARGUMENT;
-  uint64_t need = 0;
-  qwc_op_paged_attention_workspace(cache, batch, format, heads, &need);
-  if (workspace_bytes < need) return QWC_LIMIT_EXCEEDED;
+  const AttnPlan plan = attention_plan(a, format, heads);
+  if (workspace_bytes < kCounterBytes + plan.partial_bytes) return QWC_LIMIT_EXCEEDED;
+  AttnArgs p = {};
+  p.q = q;
+  p.q_stride = q_stride;
+  p.out = out;
+  p.out_stride = out_stride;
+  p.counters = static_cast<uint32_t*>(workspace);
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+  p.heads = heads;
+  p.share = heads / a.kv_heads;
+  p.scaling = 1.0f / sqrtf(static_cast<float>(a.head_dim));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto run = format == kFormatF32 ? attention_as<float> : format == kFormatF16 ? attention_as<__half> : attention_as<__nv_bfloat16>;
-  return run(a, q, q_stride, heads, out, out_stride, s);
+  return format == kFormatF32   ? attention_as<float>(a, p, plan, s)
+         : format == kFormatF16 ? attention_as<__half>(a, p, plan, s)
+                                : attention_as<__nv_bfloat16>(a, p, plan, s);
 }
 
 }  // extern "C"

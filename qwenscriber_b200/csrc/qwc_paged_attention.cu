@@ -74,14 +74,16 @@ __global__ void __launch_bounds__(32 * kWarps) paged_attention_kernel(const Page
 // comes last adds them up in the order of the stretches, so the result does
 // not depend on who was last.
 //
-// Scores: A rows are query rows (f32: rows 0-7 the f16 parts hi, rows 8-15 the parts lo of the
-// same eight, so a score is the sum of two accumulator rows), B columns are
-// positions, codes entering as exact f16 integers; a group of 64 dims has its
-// own accumulator, which the key scale multiplies afterwards. Values: the
-// accumulator layout of the weights is the A layout of the second product; the
-// weight times the value scale of each group, again as one or two f16 parts,
-// times exact codes. The weights carry a factor 2^(28 - e) with e the largest exponent of a value
+// Scores: A rows are 16 positions, the codes as exact f16 integers; B columns are query rows, an f32
+// row as two columns (its f16 parts hi and lo, 22 bits), a 16-bit row as one, so NCT column tiles of 8
+// hold 4 NCT or 8 NCT rows. Each group of 64 dims has its own sum, which the key scale multiplies. Values:
+// A rows are 16 dims, the codes transposed between registers, B the weights times the value scale of
+// the group, again in one or two f16 parts; movmatrix turns the score layout
+// into that operand. The weights carry a factor 2^(28 - e) with e the largest exponent field of a value
 // scale so far, which keeps them in f16's normal range whatever the scales.
+//
+// Both products have the cache on the 16-row side: with the query rows there instead, twice as many
+// MMAs and twice the output registers were spent on mostly empty rows (64 x 1 over 4096, f32: 95 us).
 
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = 32 * kFewWarps;
@@ -155,18 +157,26 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return min(max(e, -126), 126);
 }
 
-template <typename T, int DIM>
+// The transpose of an 8 x 8 matrix of f16 held two to a lane (row lane / 4, columns 2 (lane % 4) + 0, 1).
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <typename T, int DIM, int NCT>
 __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(const PagedArgs a, const AttnArgs p) {
   constexpr bool SPLIT = sizeof(T) == 4;  // f32 rows enter as two f16 parts
   constexpr int G = DIM / 64;             // scale groups of a head
   constexpr int CHUNKS = DIM / 16;        // 16-byte chunks of a row of codes
-  constexpr int NT = DIM / 8;             // 8-column tiles of the output
+  constexpr int PARTS = SPLIT ? 2 : 1;    // columns of a query row
+  constexpr int RPL = SPLIT ? 1 : 2;      // rows of a column tile whose scores a lane holds
   constexpr uint32_t kValueSwizzle = DIM == 128 ? 6u : 2u;  // chunks of the rows that a half warp reads at once: apart
   constexpr int STATE = DIM + 4;          // a row's state in shared memory or a partial: output, maximum, sum
   extern __shared__ __align__(128) uint8_t few_smem[];
   FewTile<DIM>* ring = reinterpret_cast<FewTile<DIM>*>(few_smem);                                  // [warp][stage]
-  uint32_t* scales = reinterpret_cast<uint32_t*>(few_smem + sizeof(FewTile<DIM>) * kFewWarps * kFewStages);  // [warp][2][16]
-  float* states = reinterpret_cast<float*>(scales + kFewWarps * 32);                                 // [warp][rows][STATE]
+  float2* scales = reinterpret_cast<float2*>(few_smem + sizeof(FewTile<DIM>) * kFewWarps * kFewStages);  // [warp][keys, values][16]
+  float* states = reinterpret_cast<float*>(scales + kFewWarps * 32);  // [warp][rows][STATE]
   __shared__ uint64_t sums[kFewWarps];
   __shared__ uint64_t found_base;
   __shared__ uint32_t found_s, last_flag;
@@ -225,7 +235,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
   uint32_t sp = steps_of(seq);
 
   FewTile<DIM>* my_ring = ring + warp * kFewStages;
-  uint32_t* my_scales = scales + warp * 32;  // [0..15] keys, [16..31] values of the block in hand
+  float2* my_scales = scales + warp * 32;  // both groups' scales of the block in hand: [0..15] keys, [16..31] values times `up`
 
   for (uint64_t cur = u0; cur < u1;) {
     while (cur >= seq_base + uint64_t(sp) * ngroups) {
@@ -242,13 +252,14 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
 
     if (works) {
       // ---- queries ----
-      // Lane (r, c) holds, of rows r and r + 8, dims 64 g + 16 c + 4 t + 0..3 for every (g, t).
-      uint32_t qa[G * 4][4];
-      float factor[2];  // log2(e) / sqrt(d) * 2^e: from a sum to a score in powers of two
-      int32_t limit[2];  // last position that the row sees
+      // Lane (r, c) holds column r of each tile: dims 64 g + 16 c + 4 t + 0..3 of its row, for every (g, t).
+      // Of the scores it holds rows (tile, c) or (tile, 2 c), (tile, 2 c + 1).
+      uint32_t qb[NCT][G * 4][2];
+      float factor[NCT][RPL];   // log2(e) / sqrt(d) * 2^e: from a difference of sums to a power of two
+      int32_t limit[NCT][RPL];  // last position that the row sees
 #pragma unroll
-      for (int half = 0; half < (SPLIT ? 1 : 2); ++half) {
-        const uint32_t row = r + 8 * half;
+      for (int ct = 0; ct < NCT; ++ct) {
+        const uint32_t row = ct * (8 / PARTS) + r / PARTS;
         const bool in = row < rows;
         const uint32_t tok = in ? row / p.share : 0, hq = h * p.share + (in ? row % p.share : 0);
         const T* src = static_cast<const T*>(p.q) + size_t(seq.first + tok) * p.q_stride + size_t(hq) * DIM;
@@ -274,76 +285,106 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const int e2 = row_exponent(amax);
         const float down = pow2i(-e2);
-        factor[half] = p.scaling * 1.4426950408889634f * pow2i(e2);
-        limit[half] = in ? seq.base + static_cast<int32_t>(tok) : -1;
+        const float my_factor = p.scaling * 1.4426950408889634f * pow2i(e2);
+        const int32_t my_limit = in ? seq.base + static_cast<int32_t>(tok) : -1;
+#pragma unroll
+        for (int e = 0; e < RPL; ++e) {
+          const int from = static_cast<int>((SPLIT ? 2 * c : 2 * c + e) * 4);
+          factor[ct][e] = __shfl_sync(0xffffffffu, my_factor, from);
+          limit[ct][e] = __shfl_sync(0xffffffffu, my_limit, from);
+        }
 #pragma unroll
         for (int kk = 0; kk < G * 4; ++kk) {
-          float y[4], lo[4];
+          float y[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[e] = fmaf(x[kk][e], down, x[kk][e] - x[kk][e]);  // an infinity is NaN from here on
-          const uint32_t h01 = f16x2(y[0], y[1]), h23 = f16x2(y[2], y[3]);
-          qa[kk][half] = h01;
-          qa[kk][2 + half] = h23;
-          if constexpr (SPLIT) {
+          uint32_t h01 = f16x2(y[0], y[1]), h23 = f16x2(y[2], y[3]);
+          if (SPLIT && (r & 1u)) {
             const float2 f01 = f16x2_f32(h01), f23 = f16x2_f32(h23);
-            lo[0] = y[0] - f01.x, lo[1] = y[1] - f01.y, lo[2] = y[2] - f23.x, lo[3] = y[3] - f23.y;
-            qa[kk][1] = f16x2(lo[0], lo[1]);
-            qa[kk][3] = f16x2(lo[2], lo[3]);
+            h01 = f16x2(y[0] - f01.x, y[1] - f01.y);
+            h23 = f16x2(y[2] - f23.x, y[3] - f23.y);
           }
+          qb[ct][kk][0] = h01;
+          qb[ct][kk][1] = h23;
         }
       }
 
       // ---- the loads: positions of block j, one row for each lane of a half warp ----
       const uint32_t context = seq.context;
-      auto position = [&](uint32_t j) { return j * span + wpb * kFewBlock + (lane & 15u); };
-      auto page_id = [&](uint32_t j) -> int32_t {
-        const uint32_t pos = position(j);
-        return j < j1 && pos < context ? __ldg(a.page_table + size_t(s) * a.table_stride + page_of(a, pos)) : -1;
+      const int32_t* table = a.page_table + size_t(s) * a.table_stride;
+      struct Place {
+        int32_t page, at;  // a position's page, and its row there
       };
-      auto row_of = [&](uint32_t j, int32_t id) -> int32_t {
-        const uint32_t pos = position(j);
-        return static_cast<uint32_t>(id) < a.pages ? id * static_cast<int32_t>(a.page_size) +
-                                                         static_cast<int32_t>(pos - page_of(a, pos) * a.page_size)
-                                                   : -1;
+      auto place_of = [&](uint32_t j) -> Place {
+        const uint32_t pos = j * span + wpb * kFewBlock + (lane & 15u);
+        if (j >= j1 || pos >= context) return Place{-1, 0};
+        const uint32_t pg = page_of(a, pos);
+        return Place{__ldg(table + pg), static_cast<int32_t>(pos - pg * a.page_size)};
       };
+      const uint32_t lane_row = lane / CHUNKS, lane_chunk = lane % CHUNKS;
+      const uint8_t* k_src = a.k_codes + size_t(h) * DIM + 16u * lane_chunk;
+      const uint8_t* v_src = a.v_codes + size_t(h) * DIM + 16u * lane_chunk;
+      const uint8_t* s_src = (lane < 16 ? a.k_scales : a.v_scales) + size_t(h) * (2 * G);
       uint32_t scale_next = 0, valid_next = 0;
-      auto load = [&](uint32_t j, int32_t id) {  // block j's codes into its stage; its scales into a register
-        const int32_t row = row_of(j, id);
+      auto load = [&](uint32_t j, Place at) {  // block j's codes into its stage; its scales into a register
+        const int32_t row = static_cast<uint32_t>(at.page) < a.pages ? at.page * static_cast<int32_t>(a.page_size) + at.at : -1;
         valid_next = __ballot_sync(0xffffffffu, row >= 0) & 0xFFFFu;
         FewTile<DIM>* t = my_ring + j % kFewStages;
 #pragma unroll
         for (int i = 0; i < CHUNKS / 2; ++i) {
-          const uint32_t tr = lane / CHUNKS + i * (32 / CHUNKS), ch = lane % CHUNKS;
+          const uint32_t tr = lane_row + i * (32 / CHUNKS);
           const int32_t src = __shfl_sync(0xffffffffu, row, tr);
-          const size_t at = size_t(src < 0 ? 0 : src) * a.code_row + size_t(h) * DIM + 16u * ch;
-          cp_async16(&t->k[tr][16u * (ch ^ ((tr & 1u) * (CHUNKS / 2)))], a.k_codes + at, src >= 0);
-          cp_async16(&t->v[tr][16u * (ch ^ (tr & kValueSwizzle))], a.v_codes + at, src >= 0);
+          const uint64_t off = uint64_t(static_cast<uint32_t>(max(src, 0))) * a.code_row;
+          cp_async16(&t->k[tr][16u * (lane_chunk ^ ((tr & 1u) * (CHUNKS / 2)))], k_src + off, src >= 0);
+          cp_async16(&t->v[tr][16u * (lane_chunk ^ (tr & kValueSwizzle))], v_src + off, src >= 0);
         }
         cp_async_commit();
-        const uint8_t* plane = lane < 16 ? a.k_scales : a.v_scales;
         scale_next = 0;
         if (row >= 0) {
-          const uint8_t* at = plane + size_t(row) * a.scale_row + size_t(h) * (2 * G);
-          scale_next = G == 2 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
+          const uint8_t* from = s_src + uint64_t(static_cast<uint32_t>(row)) * a.scale_row;
+          scale_next = G == 2 ? *reinterpret_cast<const uint32_t*>(from) : *reinterpret_cast<const uint16_t*>(from);
         }
       };
 
-      float acc[NT][4];
+      // Output tile (g, i) has row n at dim 64 g + 8 n + 2 i and row n + 8 at the next dim.
+      float acc[NCT][G * 4][4];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+      for (int ct = 0; ct < NCT; ++ct) {
+#pragma unroll
+        for (int i = 0; i < G * 4; ++i) acc[ct][i][0] = acc[ct][i][1] = acc[ct][i][2] = acc[ct][i][3] = 0.0f;
+      }
+      // Maxima are of the bare sums; `factor` (positive) turns a difference into a power of two.
+      float m[NCT][RPL], l[NCT][RPL];
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+#pragma unroll
+        for (int e = 0; e < RPL; ++e) m[ct][e] = -INFINITY, l[ct][e] = 0.0f;
+      }
       uint32_t vexp = 0;  // the largest exponent field of a value scale so far
 
-      int32_t id = page_id(j0);
-      load(j0, id);
-      id = page_id(j0 + 1);
+      load(j0, place_of(j0));
+      Place ahead = place_of(j0 + 1);
       for (uint32_t j = j0; j < j1; ++j) {
         const uint32_t valid = valid_next;
-        __syncwarp();  // the last block's reads of the scales are done
-        my_scales[lane] = scale_next;
+        // Value scales: the largest exponent so far decides the weights' factor.
+        bool grew = false;
+        float down = 1.0f;
+        {
+          const uint32_t f = scale_next;
+          const uint32_t e = lane < 16 ? 0u : max((f >> 10) & 31u, (f >> 26) & 31u);
+          const uint32_t top = min(__reduce_max_sync(0xffffffffu, e), 30u);
+          if (top > vexp) {
+            down = pow2i(static_cast<int>(vexp) - static_cast<int>(top));
+            vexp = top;
+            grew = true;
+          }
+          const float up = lane < 16 ? 1.0f : pow2i(28 - static_cast<int>(vexp));
+          const float2 both = f16x2_f32(f);
+          my_scales[lane] = make_float2(both.x * up, both.y * up);  // (the last block's reads lie before the loop's end)
+        }
         if (j + 1 < j1) {
-          load(j + 1, id);
-          id = page_id(j + 2);
+          load(j + 1, ahead);
+          ahead = place_of(j + 2);
           cp_async_wait<1>();
         } else {
           cp_async_wait<0>();
@@ -351,127 +392,113 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
         __syncwarp();
         const FewTile<DIM>* t = my_ring + j % kFewStages;
 
-        // ---- scores of positions 2 c, 2 c + 1 (tile 0) and 8 + those (tile 1), rows r and r + 8 ----
-        float sc[2][2][2];  // [row half][tile][column]
-        uint32_t vs[4];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const uint32_t kr = 8u * nt + r;
-          float d[G][4];
+        // ---- sums of positions r and r + 8 ----
+        float sc[NCT][2][RPL];  // [tile][position half][row]
+        {
+          float d[NCT][G][4];
 #pragma unroll
           for (int g = 0; g < G; ++g) {
-            d[g][0] = d[g][1] = d[g][2] = d[g][3] = 0.0f;
-            const uint4 kw = *reinterpret_cast<const uint4*>(&t->k[kr][16u * ((4u * g + c) ^ ((kr & 1u) * (CHUNKS / 2)))]);
-            const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+            const uint32_t at = 16u * ((4u * g + c) ^ ((r & 1u) * (CHUNKS / 2)));
+            const uint4 k0 = *reinterpret_cast<const uint4*>(&t->k[r][at]);
+            const uint4 k1 = *reinterpret_cast<const uint4*>(&t->k[r + 8][at]);
+            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) d[ct][g][0] = d[ct][g][1] = d[ct][g][2] = d[ct][g][3] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              mma16816(d[g], qa[4 * g + e][0], qa[4 * g + e][1], qa[4 * g + e][2], qa[4 * g + e][3],
-                       codes_f16x2<0x4140>(w[e]), codes_f16x2<0x4342>(w[e]));
+              const uint32_t a0 = codes_f16x2<0x4140>(w0[e]), a1 = codes_f16x2<0x4140>(w1[e]);
+              const uint32_t a2 = codes_f16x2<0x4342>(w0[e]), a3 = codes_f16x2<0x4342>(w1[e]);
+#pragma unroll
+              for (int ct = 0; ct < NCT; ++ct) mma16816(d[ct][g], a0, a1, a2, a3, qb[ct][4 * g + e][0], qb[ct][4 * g + e][1]);
             }
           }
+          const float2 ks[2] = {my_scales[r], my_scales[r + 8]};
 #pragma unroll
-          for (int col = 0; col < 2; ++col) {
-            const uint32_t key = 8u * nt + 2u * c + col;
-            const uint32_t ks = my_scales[key];
-            vs[2 * nt + col] = my_scales[16 + key];
-            const float k0 = f16_bits_to_f32(ks & 0xFFFFu), k1 = G == 2 ? f16_bits_to_f32(ks >> 16) : 0.0f;
-            if constexpr (SPLIT) {
-              float x = (d[0][col] + d[0][2 + col]) * k0;
-              if constexpr (G == 2) x = fmaf(d[G - 1][col] + d[G - 1][2 + col], k1, x);
-              sc[0][nt][col] = x;
-            } else {
+          for (int ct = 0; ct < NCT; ++ct) {
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                float x = d[0][2 * half + col] * k0;
-                if constexpr (G == 2) x = fmaf(d[G - 1][2 * half + col], k1, x);
-                sc[half][nt][col] = x;
+            for (int hp = 0; hp < 2; ++hp) {
+#pragma unroll
+              for (int e = 0; e < RPL; ++e) {
+                float x[G];
+#pragma unroll
+                for (int g = 0; g < G; ++g) x[g] = SPLIT ? d[ct][g][2 * hp] + d[ct][g][2 * hp + 1] : d[ct][g][2 * hp + e];
+                float v = x[0] * ks[hp].x;
+                if constexpr (G == 2) v = fmaf(x[G - 1], ks[hp].y, v);
+                sc[ct][hp][e] = v;
               }
             }
           }
         }
+        // ---- what a row does not see: only in the blocks at the end of the context, or with rows missing ----
         const int32_t pos0 = static_cast<int32_t>(j * span + wpb * kFewBlock);
-        constexpr int HALVES = SPLIT ? 1 : 2;
-        float rescale[2] = {1.0f, 1.0f};
-        bool grew = false;
+        if (valid != 0xFFFFu || pos0 + kFewBlock - 1 > seq.base) {
 #pragma unroll
-        for (int half = 0; half < HALVES; ++half) {
-          float mx = -INFINITY;
+          for (int ct = 0; ct < NCT; ++ct) {
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
+            for (int hp = 0; hp < 2; ++hp) {
+              const uint32_t key = r + 8u * hp;
 #pragma unroll
-            for (int col = 0; col < 2; ++col) {
-              const uint32_t key = 8u * nt + 2u * c + col;
-              const bool seen = ((valid >> key) & 1u) && pos0 + static_cast<int32_t>(key) <= limit[half];
-              const float x = seen ? sc[half][nt][col] * factor[half] : -INFINITY;
-              sc[half][nt][col] = x;
-              mx = fmaxf(mx, x);
+              for (int e = 0; e < RPL; ++e) {
+                if (!((valid >> key) & 1u) || pos0 + static_cast<int32_t>(key) > limit[ct][e]) sc[ct][hp][e] = -INFINITY;
+              }
             }
           }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          if (mx > m[half]) {
-            rescale[half] = m[half] == -INFINITY ? 0.0f : ex2(m[half] - mx);
-            m[half] = mx;
-            grew = true;
-          }
-          const float base = m[half] == -INFINITY ? 0.0f : m[half];
-          float sum = 0.0f;
+        }
+        float rescale[NCT][RPL];
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
+        for (int ct = 0; ct < NCT; ++ct) {
 #pragma unroll
-            for (int col = 0; col < 2; ++col) {
-              sc[half][nt][col] = ex2(sc[half][nt][col] - base);
-              sum += sc[half][nt][col];
+          for (int e = 0; e < RPL; ++e) {
+            float mx = fmaxf(sc[ct][0][e], sc[ct][1][e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            rescale[ct][e] = 1.0f;
+            if (mx > m[ct][e]) {
+              rescale[ct][e] = m[ct][e] == -INFINITY ? 0.0f : ex2((m[ct][e] - mx) * factor[ct][e]);
+              m[ct][e] = mx;
+              grew = true;
             }
+            const float base = m[ct][e] == -INFINITY ? 0.0f : m[ct][e];
+            sc[ct][0][e] = ex2((sc[ct][0][e] - base) * factor[ct][e]);
+            sc[ct][1][e] = ex2((sc[ct][1][e] - base) * factor[ct][e]);
+            l[ct][e] = fmaf(l[ct][e], rescale[ct][e], sc[ct][0][e] + sc[ct][1][e]);
           }
-          l[half] = fmaf(l[half], rescale[half], sum);
-        }
-        // Value scales: a position nobody sees (or that is not cached) counts as zero.
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t key = 8u * (i / 2) + 2u * c + (i % 2);
-          if (!((valid >> key) & 1u)) vs[i] = 0;
-          top = max(top, max((vs[i] >> 10) & 31u, (vs[i] >> 26) & 31u));
-        }
-        top = min(__reduce_max_sync(0xffffffffu, top), 30u);
-        float down = 1.0f;
-        if (top > vexp) {
-          down = pow2i(static_cast<int>(vexp) - static_cast<int>(top));
-          vexp = top;
-          grew = true;
         }
         if (__any_sync(0xffffffffu, grew)) {
-          const float f0 = rescale[0] * down, f1 = SPLIT ? f0 : rescale[1] * down;
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            acc[i][0] *= f0;
-            acc[i][1] *= f0;
-            acc[i][2] *= f1;
-            acc[i][3] *= f1;
-          }
-        }
-        const float up = pow2i(28 - static_cast<int>(vexp));
-        // ---- weights: A fragments for each group ----
-        uint32_t wa[G][4];
+          for (int ct = 0; ct < NCT; ++ct) {
+            const float f0 = rescale[ct][0] * down, f1 = rescale[ct][RPL - 1] * down;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const float v0 = f16_bits_to_f32((vs[2 * nt] >> (16 * g)) & 0xFFFFu) * up;
-            const float v1 = f16_bits_to_f32((vs[2 * nt + 1] >> (16 * g)) & 0xFFFFu) * up;
-            const float w0 = sc[0][nt][0] * v0, w1 = sc[0][nt][1] * v1;
-            const uint32_t hi = f16x2(w0, w1);
-            wa[g][2 * nt] = hi;
-            if constexpr (SPLIT) {
-              const float2 f = f16x2_f32(hi);
-              wa[g][2 * nt + 1] = f16x2(w0 - f.x, w1 - f.y);
-            } else {
-              wa[g][2 * nt + 1] = f16x2(sc[1][nt][0] * v0, sc[1][nt][1] * v1);
+            for (int i = 0; i < G * 4; ++i) {
+              acc[ct][i][0] *= f0;
+              acc[ct][i][1] *= f1;
+              acc[ct][i][2] *= f0;
+              acc[ct][i][3] *= f1;
             }
           }
         }
-        // ---- values: output tile 8 g + i has column n at dim 64 g + 8 n + i ----
+        // ---- weights: B fragments for each group ----
+        uint32_t wb[NCT][G][2];
+#pragma unroll
+        for (int hp = 0; hp < 2; ++hp) {
+          const float2 vs = my_scales[16 + r + 8 * hp];
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const float v = g ? vs.y : vs.x;
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) {
+              if constexpr (SPLIT) {
+                const float w = sc[ct][hp][0] * v;
+                const float hi = __half2float(__float2half_rn(w));
+                wb[ct][g][hp] = transpose8x8(f16x2(hi, w - hi));
+              } else {
+                wb[ct][g][hp] = transpose8x8(f16x2(sc[ct][hp][0] * v, sc[ct][hp][RPL - 1] * v));
+              }
+            }
+          }
+        }
+        // ---- values ----
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           uint2 vw[4];
@@ -487,41 +514,49 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
             const uint32_t x2 = w ? vw[2].y : vw[2].x, x3 = w ? vw[3].y : vw[3].x;
             const uint32_t a01 = __byte_perm(x0, x1, 0x5140), a23 = __byte_perm(x0, x1, 0x7362);
             const uint32_t b01 = __byte_perm(x2, x3, 0x5140), b23 = __byte_perm(x2, x3, 0x7362);
-            float(*o)[4] = &acc[8 * g + 4 * w];
-            mma16816(o[0], wa[g][0], wa[g][1], wa[g][2], wa[g][3], codes_f16x2<0x4140>(a01), codes_f16x2<0x4140>(b01));
-            mma16816(o[1], wa[g][0], wa[g][1], wa[g][2], wa[g][3], codes_f16x2<0x4342>(a01), codes_f16x2<0x4342>(b01));
-            mma16816(o[2], wa[g][0], wa[g][1], wa[g][2], wa[g][3], codes_f16x2<0x4140>(a23), codes_f16x2<0x4140>(b23));
-            mma16816(o[3], wa[g][0], wa[g][1], wa[g][2], wa[g][3], codes_f16x2<0x4342>(a23), codes_f16x2<0x4342>(b23));
-          }
-        }
-      }
-
-      // ---- this warp's state: lane (r, c) has dims 64 g + 16 c + 0..15 of its rows ----
-      const float back = pow2i(static_cast<int>(vexp) - 28);
+            const uint32_t e0 = codes_f16x2<0x4140>(a01), e1 = codes_f16x2<0x4342>(a01);
+            const uint32_t e2 = codes_f16x2<0x4140>(b01), e3 = codes_f16x2<0x4342>(b01);
+            const uint32_t o0 = codes_f16x2<0x4140>(a23), o1 = codes_f16x2<0x4342>(a23);
+            const uint32_t o2 = codes_f16x2<0x4140>(b23), o3 = codes_f16x2<0x4342>(b23);
 #pragma unroll
-      for (int half = 0; half < (SPLIT ? 1 : 2); ++half) {
-        const uint32_t row = r + 8 * half;
-        float lsum = l[half] + __shfl_xor_sync(0xffffffffu, l[half], 1);
-        lsum += __shfl_xor_sync(0xffffffffu, lsum, 2);
-        if (row < rows) {
-          float* st = states + (size_t(warp) * p.rows + row) * STATE;
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-#pragma unroll
-            for (int col = 0; col < 2; ++col) {
-              float o[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                o[i] = (SPLIT ? acc[8 * g + i][col] + acc[8 * g + i][2 + col] : acc[8 * g + i][2 * half + col]) * back;
-              }
-              float* dst = st + 64 * g + 16 * c + 8 * col;
-              *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
-              *reinterpret_cast<float4*>(dst + 4) = make_float4(o[4], o[5], o[6], o[7]);
+            for (int ct = 0; ct < NCT; ++ct) {
+              mma16816(acc[ct][4 * g + 2 * w], e0, e1, e2, e3, wb[ct][g][0], wb[ct][g][1]);
+              mma16816(acc[ct][4 * g + 2 * w + 1], o0, o1, o2, o3, wb[ct][g][0], wb[ct][g][1]);
             }
           }
-          if (c == 0) {
-            st[DIM] = m[half];
-            st[DIM + 1] = lsum;
+        }
+        __syncwarp();  // the block's stage and scales are free
+      }
+
+      // ---- this warp's state: lane (r, c) has dims 64 g + 8 r + 0..7 of its rows ----
+      const float back = pow2i(static_cast<int>(vexp) - 28);
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+#pragma unroll
+        for (int e = 0; e < RPL; ++e) {
+          const uint32_t row = ct * (8 / PARTS) + RPL * c + e;
+          float lsum = l[ct][e];
+          lsum += __shfl_xor_sync(0xffffffffu, lsum, 4);
+          lsum += __shfl_xor_sync(0xffffffffu, lsum, 8);
+          lsum += __shfl_xor_sync(0xffffffffu, lsum, 16);
+          if (row < rows) {
+            float* st = states + (size_t(warp) * p.rows + row) * STATE;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              float o[8];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float(&f)[4] = acc[ct][4 * g + i];
+                o[2 * i] = (SPLIT ? f[0] + f[1] : f[e]) * back;
+                o[2 * i + 1] = (SPLIT ? f[2] + f[3] : f[2 + e]) * back;
+              }
+              *reinterpret_cast<float4*>(st + 64 * g + 8 * r) = make_float4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<float4*>(st + 64 * g + 8 * r + 4) = make_float4(o[4], o[5], o[6], o[7]);
+            }
+            if (r == 0) {
+              st[DIM] = m[ct][e] * factor[ct][e];
+              st[DIM + 1] = lsum;
+            }
           }
         }
       }
@@ -629,9 +664,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
   }
 }
 
-template <typename T, int DIM>
+template <int DIM>
 size_t few_smem_bytes(uint32_t rows) {
-  return sizeof(FewTile<DIM>) * kFewWarps * kFewStages + kFewWarps * 32 * 4 + size_t(kFewWarps) * rows * (DIM + 4) * 4;
+  return sizeof(FewTile<DIM>) * kFewWarps * kFewStages + kFewWarps * 32 * 8 + size_t(kFewWarps) * rows * (DIM + 4) * 4;
 }
 
 // How a call is run: which kernel, its grid, and its part of the workspace.
@@ -650,7 +685,7 @@ AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
   const uint64_t sms = 148;
   p.group = 1;
   if (uint64_t(a.sequences) * a.kv_heads * a.max_context >= 8ull * 2 * sms * 512) {
-    for (uint32_t g = 2; g <= 8; ++g) {
+    for (uint32_t g = 2; g <= 4; ++g) {
       if (a.kv_heads % g == 0) p.group = g;
     }
   }
@@ -664,22 +699,26 @@ AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
 
 constexpr uint64_t kCounterBytes = kMaxFewCtas * 4;
 
-template <typename T, int DIM>
+template <typename T, int DIM, int NCT>
 int32_t launch_few(const PagedArgs& a, AttnArgs p, const AttnPlan& plan, cudaStream_t stream) {
-  const size_t smem = few_smem_bytes<T, DIM>(plan.rows);
-  cudaError_t e = cudaFuncSetAttribute(paged_attention_few_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  const size_t smem = few_smem_bytes<DIM>(plan.rows);
+  cudaError_t e = cudaFuncSetAttribute(paged_attention_few_kernel<T, DIM, NCT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(smem));
   if (e != cudaSuccess) return paged_status(e);
   p.group = plan.group;
   p.pb = plan.pb;
   p.rows = plan.rows;
-  paged_attention_few_kernel<T, DIM><<<plan.grid, kFewThreads, smem, stream>>>(a, p);
+  paged_attention_few_kernel<T, DIM, NCT><<<plan.grid, kFewThreads, smem, stream>>>(a, p);
   return paged_status(cudaGetLastError());
 }
 
 template <typename T>
 int32_t attention_as(const PagedArgs& a, AttnArgs p, const AttnPlan& plan, cudaStream_t stream) {
-  if (plan.few) return a.head_dim == 128 ? launch_few<T, 128>(a, p, plan, stream) : launch_few<T, 64>(a, p, plan, stream);
+  if (plan.few) {
+    const bool one = plan.rows <= (sizeof(T) == 4 ? 4u : 8u);  // column tiles
+    if (a.head_dim == 128) return one ? launch_few<T, 128, 1>(a, p, plan, stream) : launch_few<T, 128, 2>(a, p, plan, stream);
+    return one ? launch_few<T, 64, 1>(a, p, plan, stream) : launch_few<T, 64, 2>(a, p, plan, stream);
+  }
   const dim3 grid(static_cast<uint32_t>((uint64_t(a.max_query) * p.heads + kWarps - 1) / kWarps), a.sequences);
   auto kernel = a.head_dim == 128 ? paged_attention_kernel<T, 128> : paged_attention_kernel<T, 64>;
   kernel<<<grid, 32 * kWarps, 0, stream>>>(a, static_cast<const T*>(p.q), p.q_stride, p.heads, static_cast<T*>(p.out),

@@ -120,6 +120,62 @@ __device__ __forceinline__ void store_as(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// One attention call, as its kernels take it.
+struct AttnArgs {
+  uint64_t q_stride, out_stride;
+  const void* q;
+  void* out;
+  float* partials;     // results of stretches that are not a whole segment, two for each CTA
+  uint32_t* counters;  // [kAttnCounters], zero between calls
+  int32_t* error;      // set when a bounded wait gave up
+  uint64_t timeout_ns;
+  uint32_t heads, share;
+  uint32_t group;      // few rows: kv heads of a CTA
+  uint32_t pb;         // few rows: position blocks of a step
+  uint32_t rows;       // few rows: most rows of a kv head, max_query * share
+  float scaling;
+};
+
+constexpr uint32_t kMaxAttnCtas = 1024;
+constexpr uint32_t kAttnCounters = 4 * kMaxAttnCtas;
+constexpr uint64_t kAttnHeadBytes = 256 + kAttnCounters * 4;  // of the workspace: the error word, the counters
+
+// Many rows (qwc_paged_tile.cu).
+uint32_t paged_tile_grid(const PagedArgs& a, uint32_t heads, uint32_t sms);
+uint64_t paged_tile_partial_bytes(const PagedArgs& a, uint32_t grid);
+int32_t paged_tile_launch(const PagedArgs& a, const AttnArgs& p, uint32_t format, uint32_t grid, cudaStream_t stream);
+
+// ---- arithmetic of the attention kernels ----
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
+  const uint32_t h = __byte_perm(w, 0x64646464u, SEL);
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));  // (1024 + u) - (1024 + 128)
+  return r;
+}
+
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 f16x2_f32(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+
+// The power of two that brings a row of queries near 1: their f16 parts then
+// hold 11 (or 22) bits of every value that matters beside the largest.
+__device__ __forceinline__ int row_exponent(float amax) {
+  const int e = static_cast<int>((__float_as_uint(amax) >> 23) & 0xFFu) - 127;
+  return min(max(e, -126), 126);
+}
+
 // Host side: the checks of the two descriptors, and the kernels' form of
 // them. A refused descriptor is refused before any launch.
 int32_t paged_args(const qwc_paged_cache* cache, const qwc_paged_batch* batch, PagedArgs* out);

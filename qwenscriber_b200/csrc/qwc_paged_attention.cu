@@ -3,60 +3,13 @@
 
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "qwc_device.cuh"
 #include "qwc_paged.cuh"
 
 namespace qwc {
 namespace {
-
-constexpr int kWarps = 4;
-
-// One warp for each (token, query head): lane l holds DIM / 32 values of the
-// query and of the output and walks the positions with a running maximum and
-// sum.
-template <typename T, int DIM>
-__global__ void __launch_bounds__(32 * kWarps) paged_attention_kernel(const PagedArgs a, const T* q, uint64_t q_stride,
-                                                                      uint32_t heads, T* out, uint64_t out_stride,
-                                                                      float scaling) {
-  constexpr int V = DIM / 32;
-  const PagedSeq seq = paged_seq(a, blockIdx.y);
-  const uint32_t unit = blockIdx.x * kWarps + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t i = unit / heads, h = unit % heads;
-  if (i >= seq.n) return;
-  const uint32_t token = seq.first + i;
-  const uint32_t kvh = h / (heads / a.kv_heads);
-  const int32_t last = seq.base + static_cast<int32_t>(i);
-  float x[V], o[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    x[e] = to_f32(q[size_t(token) * q_stride + size_t(h) * DIM + lane * V + e]);
-    o[e] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  const uint32_t d = kvh * DIM + lane * V;
-  for (int32_t p = 0; p <= last; ++p) {
-    const int64_t row = paged_row(a, blockIdx.y, static_cast<uint32_t>(p));
-    if (row < 0) continue;
-    const uint8_t* kc = a.k_codes + size_t(row) * a.code_row + d;
-    const uint8_t* vc = a.v_codes + size_t(row) * a.code_row + d;
-    const float ks = f16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.k_scales + size_t(row) * a.scale_row)[d / kGroup]);
-    const float vs = f16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.v_scales + size_t(row) * a.scale_row)[d / kGroup]);
-    float t = 0.0f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) t = fmaf(x[e], static_cast<float>(static_cast<int>(kc[e]) - 128) * ks, t);
-    const float s = warp_sum(t) * scaling;
-    const float nm = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.0f : expf(m - nm), w = s == -INFINITY ? 0.0f : expf(s - nm);
-    l = l * keep + w;
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = o[e] * keep + w * (static_cast<float>(static_cast<int>(vc[e]) - 128) * vs);
-    m = nm;
-  }
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    store_as(&out[size_t(token) * out_stride + size_t(h) * DIM + lane * V + e], last < 0 || l == 0.0f ? 0.0f : o[e] / l);
-  }
-}
 
 // ---- few query rows ----
 //
@@ -89,25 +42,11 @@ constexpr int kFewWarps = 8;
 constexpr int kFewThreads = 32 * kFewWarps;
 constexpr int kFewBlock = 16;   // positions a warp takes at a time
 constexpr int kFewStages = 2;   // blocks of codes in a warp's ring
-constexpr int kMaxFewCtas = 1024;
 
 template <int DIM>
 struct FewTile {
   uint8_t k[kFewBlock][DIM];
   uint8_t v[kFewBlock][DIM];
-};
-
-struct AttnArgs {
-  uint64_t q_stride, out_stride;
-  const void* q;
-  void* out;
-  float* partials;     // [2 * grid][group heads][rows][DIM + 4]
-  uint32_t* counters;  // [kMaxFewCtas], zero between calls
-  uint32_t heads, share;
-  uint32_t group;      // kv heads of a CTA
-  uint32_t pb;         // position blocks of a step
-  uint32_t rows;       // most rows of a kv head: max_query * share
-  float scaling;
 };
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool in) {
@@ -119,28 +58,6 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
-  const uint32_t h = __byte_perm(w, 0x64646464u, SEL);
-  uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));  // (1024 + u) - (1024 + 128)
-  return r;
-}
-
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 f16x2_f32(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
@@ -148,13 +65,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// The power of two that brings a row of queries near 1: their f16 parts then
-// hold 11 (or 22) bits of every value that matters beside the largest.
-__device__ __forceinline__ int row_exponent(float amax) {
-  const int e = static_cast<int>((__float_as_uint(amax) >> 23) & 0xFFu) - 127;
-  return min(max(e, -126), 126);
 }
 
 // The transpose of an 8 x 8 matrix of f16 held two to a lane (row lane / 4, columns 2 (lane % 4) + 0, 1).
@@ -669,6 +579,8 @@ size_t few_smem_bytes(uint32_t rows) {
   return sizeof(FewTile<DIM>) * kFewWarps * kFewStages + kFewWarps * 32 * 8 + size_t(kFewWarps) * rows * (DIM + 4) * 4;
 }
 
+constexpr uint64_t kTimeoutNs = 2000000000ull;
+
 // How a call is run: which kernel, its grid, and its part of the workspace.
 struct AttnPlan {
   bool few;
@@ -679,10 +591,14 @@ struct AttnPlan {
 AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
   AttnPlan p = {};
   const uint64_t rows = uint64_t(a.max_query) * (heads / a.kv_heads);
-  p.few = rows <= (format == kFormatF32 ? 8u : 16u);
-  if (!p.few) return p;
-  p.rows = static_cast<uint32_t>(rows);
   const uint64_t sms = 148;
+  p.few = rows <= (format == kFormatF32 ? 8u : 16u);
+  if (!p.few) {
+    p.grid = paged_tile_grid(a, heads, sms);
+    p.partial_bytes = paged_tile_partial_bytes(a, p.grid);
+    return p;
+  }
+  p.rows = static_cast<uint32_t>(rows);
   p.group = 1;
   if (uint64_t(a.sequences) * a.kv_heads * a.max_context >= 8ull * 2 * sms * 512) {
     for (uint32_t g = 2; g <= 4; ++g) {
@@ -696,8 +612,6 @@ AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
   p.partial_bytes = uint64_t(2) * p.grid * p.group * p.rows * (a.head_dim + 4) * 4;
   return p;
 }
-
-constexpr uint64_t kCounterBytes = kMaxFewCtas * 4;
 
 template <typename T, int DIM, int NCT>
 int32_t launch_few(const PagedArgs& a, AttnArgs p, const AttnPlan& plan, cudaStream_t stream) {
@@ -719,11 +633,8 @@ int32_t attention_as(const PagedArgs& a, AttnArgs p, const AttnPlan& plan, cudaS
     if (a.head_dim == 128) return one ? launch_few<T, 128, 1>(a, p, plan, stream) : launch_few<T, 128, 2>(a, p, plan, stream);
     return one ? launch_few<T, 64, 1>(a, p, plan, stream) : launch_few<T, 64, 2>(a, p, plan, stream);
   }
-  const dim3 grid(static_cast<uint32_t>((uint64_t(a.max_query) * p.heads + kWarps - 1) / kWarps), a.sequences);
-  auto kernel = a.head_dim == 128 ? paged_attention_kernel<T, 128> : paged_attention_kernel<T, 64>;
-  kernel<<<grid, 32 * kWarps, 0, stream>>>(a, static_cast<const T*>(p.q), p.q_stride, p.heads, static_cast<T*>(p.out),
-                                           p.out_stride, p.scaling);
-  return paged_status(cudaGetLastError());
+  return paged_tile_launch(a, p, sizeof(T) == 4 ? kFormatF32 : std::is_same<T, __half>::value ? kFormatF16 : kFormatBF16,
+                           plan.grid, stream);
 }
 
 }  // namespace
@@ -741,7 +652,7 @@ int32_t qwc_op_paged_attention_workspace(const qwc_paged_cache* cache, const qwc
   const int32_t st = paged_args(cache, batch, &a);
   if (st != QWC_OK) return st;
   if (heads == 0 || heads % a.kv_heads != 0) return QWC_SHAPE_MISMATCH;
-  *bytes = kCounterBytes + attention_plan(a, format, heads).partial_bytes;
+  *bytes = kAttnHeadBytes + attention_plan(a, format, heads).partial_bytes;
   return QWC_OK;
 }
 
@@ -760,14 +671,16 @@ int32_t qwc_op_paged_attention(const qwc_paged_cache* cache, const qwc_paged_bat
   if ((st = paged_rows_check(out, out_stride, qw, format)) != QWC_OK) return st;
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return QWC_INVALID_ARGUMENT;
   const AttnPlan plan = attention_plan(a, format, heads);
-  if (workspace_bytes < kCounterBytes + plan.partial_bytes) return QWC_LIMIT_EXCEEDED;
+  if (workspace_bytes < kAttnHeadBytes + plan.partial_bytes) return QWC_LIMIT_EXCEEDED;
   AttnArgs p = {};
   p.q = q;
   p.q_stride = q_stride;
   p.out = out;
   p.out_stride = out_stride;
-  p.counters = static_cast<uint32_t*>(workspace);
-  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+  p.error = static_cast<int32_t*>(workspace);
+  p.timeout_ns = kTimeoutNs;
+  p.counters = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + 256);
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kAttnHeadBytes);
   p.heads = heads;
   p.share = heads / a.kv_heads;
   p.scaling = 1.0f / sqrtf(static_cast<float>(a.head_dim));

@@ -126,7 +126,7 @@ struct AttnArgs {
   const void* q;
   void* out;
   float* partials;     // results of stretches that are not a whole segment, two for each CTA
-  uint32_t* counters;  // [kAttnCounters], zero between calls
+  uint32_t* counters;  // [kMaxAttnCtas][kAttnCounterStride], zero between calls
   int32_t* error;      // set when a bounded wait gave up
   uint64_t timeout_ns;
   uint32_t heads, share;
@@ -137,13 +137,17 @@ struct AttnArgs {
 };
 
 constexpr uint32_t kMaxAttnCtas = 1024;
-constexpr uint32_t kAttnCounters = 4 * kMaxAttnCtas;
+constexpr uint32_t kAttnCounterStride = 8;  // a CTA's counters: one for each softmax warp
+constexpr uint32_t kAttnCounters = kAttnCounterStride * kMaxAttnCtas;
 constexpr uint64_t kAttnHeadBytes = 256 + kAttnCounters * 4;  // of the workspace: the error word, the counters
 
-// Many rows (qwc_paged_tile.cu).
-uint32_t paged_tile_grid(const PagedArgs& a, uint32_t heads, uint32_t sms);
-uint64_t paged_tile_partial_bytes(const PagedArgs& a, uint32_t grid);
-int32_t paged_tile_launch(const PagedArgs& a, const AttnArgs& p, uint32_t format, uint32_t grid, cudaStream_t stream);
+// Many rows (qwc_paged_tile.cu): 128-row tiles that a CTA takes at once, its grid, its part of the workspace.
+struct TilePlan {
+  uint32_t tiles, grid;
+  uint64_t partial_bytes;
+};
+TilePlan paged_tile_plan(const PagedArgs& a, uint32_t heads, uint32_t sms);
+int32_t paged_tile_launch(const PagedArgs& a, const AttnArgs& p, uint32_t format, const TilePlan& plan, cudaStream_t stream);
 
 // ---- arithmetic of the attention kernels ----
 

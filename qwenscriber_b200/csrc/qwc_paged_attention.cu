@@ -521,9 +521,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
       __threadfence();
       __syncthreads();
       if (tid == 0) {
-        const uint32_t before = atomicAdd(&p.counters[c0], 1u);
+        const uint32_t before = atomicAdd(&p.counters[kAttnCounterStride * c0], 1u);
         last_flag = before == c1 - c0;
-        if (before == c1 - c0) p.counters[c0] = 0;
+        if (before == c1 - c0) p.counters[kAttnCounterStride * c0] = 0;
       }
       __syncthreads();
       if (last_flag) {
@@ -585,6 +585,7 @@ constexpr uint64_t kTimeoutNs = 2000000000ull;
 struct AttnPlan {
   bool few;
   uint32_t grid, group, pb, rows;
+  TilePlan tile;
   uint64_t partial_bytes;
 };
 
@@ -594,8 +595,8 @@ AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
   const uint64_t sms = 148;
   p.few = rows <= (format == kFormatF32 ? 8u : 16u);
   if (!p.few) {
-    p.grid = paged_tile_grid(a, heads, sms);
-    p.partial_bytes = paged_tile_partial_bytes(a, p.grid);
+    p.tile = paged_tile_plan(a, heads, sms);
+    p.partial_bytes = p.tile.partial_bytes;
     return p;
   }
   p.rows = static_cast<uint32_t>(rows);
@@ -634,7 +635,7 @@ int32_t attention_as(const PagedArgs& a, AttnArgs p, const AttnPlan& plan, cudaS
     return one ? launch_few<T, 64, 1>(a, p, plan, stream) : launch_few<T, 64, 2>(a, p, plan, stream);
   }
   return paged_tile_launch(a, p, sizeof(T) == 4 ? kFormatF32 : std::is_same<T, __half>::value ? kFormatF16 : kFormatBF16,
-                           plan.grid, stream);
+                           plan.tile, stream);
 }
 
 }  // namespace

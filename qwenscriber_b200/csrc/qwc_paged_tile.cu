@@ -3,32 +3,43 @@
 // 5th-generation tensor cores.
 //
 // A tile is 128 rows of one (sequence, kv head): row i is token i / share,
-// query head i % share of the kv head's. It walks the positions that its last
-// token sees, 64 at a time:
+// query head i % share of the kv head's. A CTA walks one or two tiles (TILES)
+// over the positions that their last token sees, 64 at a time:
 //
-//   warps 0-3  softmax: one row to a thread. Scores from tensor memory, the
-//              key scales, the causal limit, the running maximum and sum;
-//              the weights go back to tensor memory in place of the scores.
-//   warps 4-7  convert: the step's code rows, fetched through the page table
-//              into registers a step ahead, become f16 integers in shared memory
-//              (keys and values alike, 128-byte swizzled rows of 64 dims).
-//   warp 8     issues the MMAs: scores S_g = Q_g K_g^T for each group g of 64
-//              dims (its own accumulator, as each position has a scale for each
-//              group), output O_g += (P . vs_g) V_g with the weights read from tensor memory.
+//   softmax  four warps a tile, one row to a thread: scores from tensor
+//            memory, the causal limit, the running maximum and sum; the weights
+//            go back to tensor memory in place of the scores.
+//   convert  four warps: the step's code rows, fetched through the page table
+//            into registers a step ahead, become f16 in shared memory (keys and
+//            values alike, 128-byte swizzled rows of 64 dims).
+//   MMA      one thread: scores S = Q K^T, output O += P V with the weights
+//            read from tensor memory.
 //
-// Codes are exact in f16. A query row enters as f16 at its own power of two
-// (f32 rows as two parts, hi and lo), a weight times its value scale likewise;
-// everything else is f32. Tensor memory: 256 columns a CTA (scores 128, output
-// 128), so two CTAs share an SM and one's softmax covers the other's MMAs.
+// How the scales enter depends on the rows' type.
+// f32 and f16 rows (exact): the codes are f16 integers. Each group of 64 dims has
+// its own scores, which the softmax threads multiply by the key scales, and its
+// own weights, the softmax weight times the group's value scale. f32 queries and
+// weights enter as two f16 parts, hi and lo (22 bits), f16 rows as one.
+// bf16 rows (scaled): code times scale is rounded to f16 as it is converted, at a
+// power of two of the step. That adds a relative 2^-12 to each factor of a sum that
+// is rounded to 2^-9 in the end, and leaves the softmax threads a third of the work.
 //
-// The output is rescaled only when a row's maximum has grown by more than
-// 2^8: until then the old maximum serves, and the weights stay below 2^8.
+// Each row of queries has its own power of two, so f16 holds its values whatever
+// their size; sums, maxima and the output are f32. The output is rescaled only when a
+// row's maximum has grown by more than 2^8: until then the old maximum serves,
+// and the weights stay below 2^8.
+//
+// Tensor memory: G x 64 columns of scores and DIM of output for a tile. With one
+// tile two CTAs share an SM, with two one CTA has it: either way one tile's
+// softmax covers the other's MMAs. Two tiles convert each step once for 256 rows.
 //
 // Work is dealt as in qwc_paged_attention.cu: the steps of all tiles stand in
 // one line, each CTA takes an equal stretch, a tile that is cut is joined by
 // the CTA that comes last, in the order of the stretches.
 
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "qwc_device.cuh"
 #include "qwc_paged.cuh"
@@ -39,29 +50,45 @@ namespace {
 
 constexpr uint32_t kRows = 128;   // rows of a tile
 constexpr uint32_t kStep = 64;    // positions of a step
-constexpr uint32_t kTileThreads = 288;
 constexpr uint32_t kGrowth = 8;   // log2 of how far a maximum may run ahead of the one in use
 
-template <int DIM, bool SPLIT>
-struct __align__(1024) TileSmem {
+template <typename T, int DIM_, int TILES_>
+struct TileConfig {
+  static constexpr int DIM = DIM_, TILES = TILES_;
+  static constexpr bool SPLIT = sizeof(T) == 4;
+  static constexpr bool SCALED = std::is_same<T, __nv_bfloat16>::value;
   static constexpr int G = DIM / 64;
   static constexpr int PARTS = SPLIT ? 2 : 1;
-  uint8_t q[PARTS][G][kRows * 128];  // f16, 128-byte swizzled rows of 64 dims
-  uint8_t k[G][kStep * 128];
-  uint8_t v[G][kStep * 128];
-  float ks[2][G][kStep];  // the step's key scales; by the step's parity
-  float vs[2][G][kStep];  // its value scales, times 2^(21 - vexp)
-  uint32_t valid[2][2];   // one bit for each position that is cached
-  uint32_t vexp[2];
-  uint64_t q_full, k_full, k_empty, s_full, p_full, v_full, v_empty, o_full;
-  uint64_t scales_full[2];  // by the step's parity, like the scales
-  uint64_t sums[9];
+  static constexpr int SCORES = SCALED ? 1 : G;              // accumulators of 64 columns
+  static constexpr int STAGES = TILES == 2 || !SPLIT ? 2 : 1;  // steps of converted keys and values
+  static constexpr int WARPS = 4 * TILES + 5;
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr uint32_t TMEM_TILE = G * kStep + DIM;     // columns of a tile: scores, output
+  // The weights' power of two, 2^(UP - vexp): weight times value scale below 2^15 (exact), value below 2^7 (scaled).
+  static constexpr int UP = SCALED ? 14 : 21;
+};
+
+template <typename C>
+struct __align__(1024) TileSmem {
+  uint8_t q[C::TILES][C::PARTS][C::G][kRows * 128];  // f16, 128-byte swizzled rows of 64 dims
+  uint8_t k[C::STAGES][C::G][kStep * 128];
+  uint8_t v[C::STAGES][C::G][kStep * 128];
+  // What the softmax needs to know of a step, for the three steps that may be in hand at once (step n + 3
+  // is converted only after step n's output).
+  float ks[4][C::G][kStep];  // exact: the key scales
+  float vs[4][C::G][kStep];  // and the value scales, times 2^(UP - vexp)
+  uint32_t valid[4][2];      // one bit for each position that is cached
+  uint32_t kexp[4], vexp[4];
+  uint64_t q_full[C::TILES], s_full[C::TILES], p_full[C::TILES], o_full[C::TILES];
+  uint64_t k_full[C::STAGES], k_empty[C::STAGES], v_full[C::STAGES], v_empty[C::STAGES];
+  uint64_t scales_full[4];
+  uint64_t sums[C::WARPS];
   uint64_t found_base;
   uint32_t found_s;
   uint32_t tmem;
 };
 
-// A tile of the line, and the tiles after it.
+// A tile of the line (`height` rows: all of a CTA's tiles), and the tiles after it.
 struct TileWalk {
   uint32_t s, h, qt;
   uint32_t tiles, steps;  // of the sequence's kv head; of this tile
@@ -69,21 +96,25 @@ struct TileWalk {
   PagedSeq seq;
 };
 
+template <uint32_t HEIGHT>
 __device__ __forceinline__ uint32_t tiles_of(const PagedSeq& q, uint32_t share) {
-  return (q.n * share + kRows - 1) / kRows;
+  return (q.n * share + HEIGHT - 1) / HEIGHT;
 }
+template <uint32_t HEIGHT>
 __device__ __forceinline__ uint32_t tile_steps(const PagedSeq& q, uint32_t share, uint32_t qt) {
-  const uint32_t last = min((qt * kRows + kRows - 1) / share, q.n - 1);
+  const uint32_t last = min((qt * HEIGHT + HEIGHT - 1) / share, q.n - 1);
   const int32_t seen = min(q.base + static_cast<int32_t>(last) + 1, static_cast<int32_t>(q.context));
   return seen > 0 ? (static_cast<uint32_t>(seen) + kStep - 1) / kStep : 1u;
 }
+template <uint32_t HEIGHT>
 __device__ __forceinline__ uint64_t head_steps(const PagedSeq& q, uint32_t share) {
-  const uint32_t t = tiles_of(q, share);
+  const uint32_t t = tiles_of<HEIGHT>(q, share);
   uint64_t sum = 0;
-  for (uint32_t i = 0; i < t; ++i) sum += tile_steps(q, share, i);
+  for (uint32_t i = 0; i < t; ++i) sum += tile_steps<HEIGHT>(q, share, i);
   return sum;
 }
 
+template <uint32_t HEIGHT>
 __device__ __forceinline__ void next_tile(const PagedArgs& a, uint32_t share, TileWalk& w) {
   w.first += w.steps;
   if (++w.qt == w.tiles) {
@@ -93,10 +124,10 @@ __device__ __forceinline__ void next_tile(const PagedArgs& a, uint32_t share, Ti
       do {
         w.seq = paged_seq(a, ++w.s);
       } while (w.seq.n == 0 && w.s + 1 < a.sequences);
-      w.tiles = tiles_of(w.seq, share);
+      w.tiles = tiles_of<HEIGHT>(w.seq, share);
     }
   }
-  w.steps = tile_steps(w.seq, share, w.qt);
+  w.steps = tile_steps<HEIGHT>(w.seq, share, w.qt);
 }
 
 // 16 columns of each of two places in tensor memory (lane quarter of this warp).
@@ -142,13 +173,34 @@ __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence
 constexpr uint32_t kIdescScores = (1u << 4) | ((kStep >> 3) << 17) | ((kRows >> 4) << 24);
 constexpr uint32_t kIdescOutput = (1u << 4) | (1u << 16) | ((64u >> 3) << 17) | ((kRows >> 4) << 24);
 
-template <typename T, int DIM>
-__global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(const PagedArgs a, const AttnArgs p) {
-  constexpr bool SPLIT = sizeof(T) == 4;
-  constexpr int G = DIM / 64;
-  constexpr int PARTS = SPLIT ? 2 : 1;
-  constexpr uint32_t kTmemScores = 0, kTmemOutput = G * kStep, kTmemCols = G * kStep + DIM;
-  using Smem = TileSmem<DIM, SPLIT>;
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 32 columns (16 pairs) of tensor memory, or 16 columns at each of two places.
+__device__ __forceinline__ void tmem_ld_pairs(uint32_t t0, uint32_t t1, uint64_t (&x)[8], uint64_t (&y)[8]) {
+  float f0[16], f1[16];
+  tmem_ld16x2(t0, t1, f0, f1);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = pack2(f0[2 * i], f0[2 * i + 1]);
+    y[i] = pack2(f1[2 * i], f1[2 * i + 1]);
+  }
+}
+
+template <typename T, int DIM, int TILES>
+__global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1 ? 2 : 1)
+    paged_attention_tile_kernel(const PagedArgs a, const AttnArgs p) {
+  using C = TileConfig<T, DIM, TILES>;
+  constexpr bool SPLIT = C::SPLIT, SCALED = C::SCALED;
+  constexpr int G = C::G, PARTS = C::PARTS, STAGES = C::STAGES, WARPS = C::WARPS;
+  constexpr uint32_t HEIGHT = kRows * TILES;
+  constexpr uint32_t kOutput = G * kStep;  // columns of a tile: scores, then output
+  constexpr uint32_t kTmemCols = C::TMEM_TILE * TILES;
+  constexpr uint32_t CONVERT = 4 * TILES;  // first convert warp
+  using Smem = TileSmem<C>;
   extern __shared__ __align__(1024) uint8_t tile_smem_raw[];
   const uint32_t pad = (1024u - (smem_addr(tile_smem_raw) & 1023u)) & 1023u;
   Smem* sm = reinterpret_cast<Smem*>(tile_smem_raw + pad);
@@ -156,20 +208,20 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
 
   // ---- this CTA's stretch of the line ----
   uint64_t part = 0;
-  for (uint32_t s = tid; s < a.sequences; s += kTileThreads) part += head_steps(paged_seq(a, s), p.share) * a.kv_heads;
+  for (uint32_t s = tid; s < a.sequences; s += C::THREADS) part += head_steps<HEIGHT>(paged_seq(a, s), p.share) * a.kv_heads;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
   if (lane == 0) sm->sums[warp] = part;
   __syncthreads();
   uint64_t total = 0;
-  for (int w = 0; w < 9; ++w) total += sm->sums[w];
+  for (int w = 0; w < WARPS; ++w) total += sm->sums[w];
   const uint64_t grid = total < gridDim.x ? total : gridDim.x;
   if (blockIdx.x >= grid) return;
   const uint64_t u0 = total * blockIdx.x / grid, u1 = total * (blockIdx.x + 1) / grid;
   uint64_t running = 0;
-  for (uint32_t base = 0; base < a.sequences; base += kTileThreads) {
+  for (uint32_t base = 0; base < a.sequences; base += C::THREADS) {
     const uint32_t s = base + tid;
-    const uint64_t v = s < a.sequences ? head_steps(paged_seq(a, s), p.share) * a.kv_heads : 0;
+    const uint64_t v = s < a.sequences ? head_steps<HEIGHT>(paged_seq(a, s), p.share) * a.kv_heads : 0;
     uint64_t inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -180,7 +232,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
     if (lane == 31) sm->sums[warp] = inc;
     __syncthreads();
     uint64_t before = running, all = running;
-    for (uint32_t w = 0; w < 9; ++w) {
+    for (uint32_t w = 0; w < WARPS; ++w) {
       if (w < warp) before += sm->sums[w];
       all += sm->sums[w];
     }
@@ -192,19 +244,22 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
     if (running > u0) break;
   }
   if (tid == 0) {
-    mbar_init(&sm->q_full, 4);
-    mbar_init(&sm->k_full, 4);
-    mbar_init(&sm->k_empty, 1);
-    mbar_init(&sm->s_full, 1);
-    mbar_init(&sm->p_full, 4);
-    mbar_init(&sm->v_full, 4);
-    mbar_init(&sm->v_empty, 1);
-    mbar_init(&sm->o_full, 1);
-    mbar_init(&sm->scales_full[0], 4);
-    mbar_init(&sm->scales_full[1], 4);
+    for (int t = 0; t < TILES; ++t) {
+      mbar_init(&sm->q_full[t], 4);
+      mbar_init(&sm->s_full[t], 1);
+      mbar_init(&sm->p_full[t], 4);
+      mbar_init(&sm->o_full[t], 1);
+    }
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&sm->k_full[i], 4);
+      mbar_init(&sm->k_empty[i], 1);
+      mbar_init(&sm->v_full[i], 4);
+      mbar_init(&sm->v_empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&sm->scales_full[i], 4);
     fence_mbar_init();
   }
-  if (warp == 8) tmem_alloc(&sm->tmem, kTmemCols);
+  if (warp == WARPS - 1) tmem_alloc(&sm->tmem, kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -213,18 +268,18 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
   {
     walk.s = sm->found_s;
     walk.seq = paged_seq(a, walk.s);
-    walk.tiles = tiles_of(walk.seq, p.share);
-    const uint64_t per_head = head_steps(walk.seq, p.share);
+    walk.tiles = tiles_of<HEIGHT>(walk.seq, p.share);
+    const uint64_t per_head = head_steps<HEIGHT>(walk.seq, p.share);
     uint64_t off = u0 - sm->found_base;
     walk.h = static_cast<uint32_t>(off / per_head);
     off -= walk.h * per_head;
     walk.first = u0 - off;
     walk.qt = 0;
-    walk.steps = tile_steps(walk.seq, p.share, 0);
+    walk.steps = tile_steps<HEIGHT>(walk.seq, p.share, 0);
     while (off >= walk.steps) {
       off -= walk.steps;
       walk.first += walk.steps;
-      walk.steps = tile_steps(walk.seq, p.share, ++walk.qt);
+      walk.steps = tile_steps<HEIGHT>(walk.seq, p.share, ++walk.qt);
     }
   }
   bool ok = true;
@@ -232,14 +287,15 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
     return mbar_wait_bounded(bar, n & 1u, p.error, p.timeout_ns, code);
   };
 
-  if (warp < 4) {
-    // ---- softmax: row tid of the tile ----
-    const uint32_t taddr = tmem + ((warp * 32u) << 16);
+  if (warp < CONVERT) {
+    // ---- softmax: row tid of the CTA's tiles ----
+    const uint32_t t = warp / 4, trow = tid % kRows;
+    const uint32_t taddr = tmem + ((warp % 4 * 32u) << 16) + t * C::TMEM_TILE;
     uint32_t it = 0, seg = 0;
     for (uint64_t cur = u0; cur < u1 && ok; ++seg) {
       const uint32_t j0 = static_cast<uint32_t>(cur - walk.first);
       const uint32_t j1 = static_cast<uint32_t>((u1 < walk.first + walk.steps ? u1 : walk.first + walk.steps) - walk.first);
-      const uint32_t row = walk.qt * kRows + tid;
+      const uint32_t row = walk.qt * HEIGHT + tid;
       const bool in = row < walk.seq.n * p.share;
       const uint32_t tok = in ? row / p.share : 0u, head = walk.h * p.share + (in ? row % p.share : 0u);
       // The row's queries: its largest value gives the power of two, then the f16 parts.
@@ -280,40 +336,42 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
           const float2 f = f16x2_f32(hi[e]);
           lo[e] = f16x2(y0 - f.x, y1 - f.y);
         }
-        const uint32_t at = tid * 128u + ((((d % 64) / 8) ^ (tid & 7u)) << 4);
-        *reinterpret_cast<uint4*>(&sm->q[0][d / 64][at]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (SPLIT) *reinterpret_cast<uint4*>(&sm->q[PARTS - 1][d / 64][at]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        const uint32_t at = trow * 128u + ((((d % 64) / 8) ^ (trow & 7u)) << 4);
+        *reinterpret_cast<uint4*>(&sm->q[t][0][d / 64][at]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (SPLIT) *reinterpret_cast<uint4*>(&sm->q[t][PARTS - 1][d / 64][at]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       fence_proxy_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm->q_full);
+      if (lane == 0) mbar_arrive(&sm->q_full[t]);
 
+      // Maxima and sums are those of scores in powers of two.
       float m = -INFINITY, l = 0.0f;
       uint32_t vexp = 0;
       for (uint32_t j = j0; j < j1; ++j, ++it) {
-        const uint32_t b = it & 1u;
-        ok = __all_sync(0xffffffffu, wait(&sm->scales_full[b], it >> 1, 210) && wait(&sm->s_full, it, 201));
+        const uint32_t b = it & 3u;
+        ok = __all_sync(0xffffffffu, wait(&sm->scales_full[b], it >> 2, 210) && wait(&sm->s_full[t], it, 201));
         if (!ok) break;
         tc_fence_after();
-        float x[kStep];
-        float mx = -INFINITY;
+        uint64_t x[kStep / 2];
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(kStep); i += 32 / G) {
-          // Both groups' sums of 16 positions, or the one group's of 32.
-          float s0[16], s1[16];
-          tmem_ld16x2(taddr + kTmemScores + i, taddr + kTmemScores + i + (G == 2 ? kStep : 16u), s0, s1);
+        for (int i = 0; i < static_cast<int>(kStep); i += 32 / C::SCORES) {
+          // Both groups' sums of 16 positions, or the one sum of 32.
+          uint64_t s0[8], s1[8];
+          tmem_ld_pairs(taddr + i, taddr + i + (C::SCORES == 2 ? kStep : 16u), s0, s1);
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const float4 k0 = *reinterpret_cast<const float4*>(&sm->ks[b][0][i + e]);
-            const float4 k1 = *reinterpret_cast<const float4*>(G == 2 ? &sm->ks[b][G - 1][i + e] : &sm->ks[b][0][i + 16 + e]);
-            const float f0[4] = {k0.x, k0.y, k0.z, k0.w}, f1[4] = {k1.x, k1.y, k1.z, k1.w};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
+          for (int e = 0; e < 8; e += 2) {
+            if constexpr (SCALED) {
+              x[i / 2 + e] = s0[e], x[i / 2 + e + 1] = s0[e + 1];
+              x[i / 2 + 8 + e] = s1[e], x[i / 2 + 8 + e + 1] = s1[e + 1];
+            } else {
+              const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(&sm->ks[b][0][i + 2 * e]);
+              const ulonglong2 k1 = *reinterpret_cast<const ulonglong2*>(G == 2 ? &sm->ks[b][G - 1][i + 2 * e] : &sm->ks[b][0][i + 16 + 2 * e]);
               if constexpr (G == 2) {
-                x[i + e + q] = fmaf(s1[e + q], f1[q], s0[e + q] * f0[q]);
+                x[i / 2 + e] = fma2(s1[e], k1.x, mul2(s0[e], k0.x));
+                x[i / 2 + e + 1] = fma2(s1[e + 1], k1.y, mul2(s0[e + 1], k0.y));
               } else {
-                x[i + e + q] = s0[e + q] * f0[q];
-                x[i + 16 + e + q] = s1[e + q] * f1[q];
+                x[i / 2 + e] = mul2(s0[e], k0.x), x[i / 2 + e + 1] = mul2(s0[e + 1], k0.y);
+                x[i / 2 + 8 + e] = mul2(s1[e], k1.x), x[i / 2 + 8 + e + 1] = mul2(s1[e + 1], k1.y);
               }
             }
           }
@@ -322,16 +380,27 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         const uint32_t v0 = sm->valid[b][0], v1 = sm->valid[b][1];
         if (pos0 + static_cast<int32_t>(kStep) - 1 > limit || (v0 & v1) != 0xFFFFFFFFu) {
 #pragma unroll
-          for (int i = 0; i < static_cast<int>(kStep); ++i) {
-            if (pos0 + i > limit || !(((i < 32 ? v0 : v1) >> (i % 32)) & 1u)) x[i] = -INFINITY;
+          for (int i = 0; i < static_cast<int>(kStep); i += 2) {
+            float2 f = unpack2(x[i / 2]);
+            const uint32_t bits = (i < 32 ? v0 : v1) >> (i % 32);
+            if (pos0 + i > limit || !(bits & 1u)) f.x = -INFINITY;
+            if (pos0 + i + 1 > limit || !(bits & 2u)) f.y = -INFINITY;
+            x[i / 2] = pack2(f.x, f.y);
           }
         }
+        float mx = -INFINITY, my = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(kStep); ++i) mx = fmaxf(mx, x[i]);
+        for (int i = 0; i < static_cast<int>(kStep) / 2; i += 2) {
+          const float2 f0 = unpack2(x[i]), f1 = unpack2(x[i + 1]);
+          mx = fmaxf(mx, fmaxf(f0.x, f0.y));
+          my = fmaxf(my, fmaxf(f1.x, f1.y));
+        }
+        const float step_factor = SCALED ? factor * pow2i(static_cast<int>(sm->kexp[b]) - 14) : factor;
+        mx = fmaxf(mx, my) * step_factor;
         float rescale = 1.0f;
         bool grew = false;
-        if ((mx - m) * factor > static_cast<float>(kGrowth) || (m == -INFINITY && mx > m)) {
-          rescale = m == -INFINITY ? 0.0f : ex2((m - mx) * factor);
+        if (mx - m > static_cast<float>(kGrowth) || (m == -INFINITY && mx > m)) {
+          rescale = m == -INFINITY ? 0.0f : ex2(m - mx);
           l *= rescale;
           m = mx;
           grew = true;
@@ -347,70 +416,82 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
 #pragma unroll
           for (int i = 0; i < DIM; i += 32) {
             float o0[16], o1[16];
-            tmem_ld16x2(taddr + kTmemOutput + i, taddr + kTmemOutput + i + 16, o0, o1);
+            tmem_ld16x2(taddr + kOutput + i, taddr + kOutput + i + 16, o0, o1);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               o0[e] *= rescale;
               o1[e] *= rescale;
             }
-            tmem_st16f(taddr + kTmemOutput + i, o0);
-            tmem_st16f(taddr + kTmemOutput + i + 16, o1);
+            tmem_st16f(taddr + kOutput + i, o0);
+            tmem_st16f(taddr + kOutput + i + 16, o1);
           }
         }
-        const float mf = m == -INFINITY ? 0.0f : m * factor;
+        const float base = m == -INFINITY ? 0.0f : -m;
+        const uint64_t f2 = pack2(step_factor, step_factor), b2 = pack2(base, base);
+        uint64_t l0 = 0, l1 = 0;
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(kStep); ++i) {
-          x[i] = ex2(fmaf(x[i], factor, -mf));
-          l += x[i];
+        for (int i = 0; i < static_cast<int>(kStep) / 2; i += 2) {
+          const float2 e0 = unpack2(fma2(x[i], f2, b2)), e1 = unpack2(fma2(x[i + 1], f2, b2));
+          x[i] = pack2(ex2(e0.x), ex2(e0.y));
+          x[i + 1] = pack2(ex2(e1.x), ex2(e1.y));
+          l0 = add2(l0, x[i]);
+          l1 = add2(l1, x[i + 1]);
         }
+        const float2 lf = unpack2(add2(l0, l1));
+        l += lf.x + lf.y;
         // Weights over the scores' columns: part q of group g at columns 32 (q G + g).
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int g = 0; g < C::SCORES; ++g) {
 #pragma unroll
           for (int i = 0; i < static_cast<int>(kStep); i += 32) {
             uint32_t hi[16], lo[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(&sm->vs[b][g][i + e]);
-              const float w0 = x[i + e] * f.x, w1 = x[i + e + 1] * f.y, w2 = x[i + e + 2] * f.z, w3 = x[i + e + 3] * f.w;
-              hi[e / 2] = f16x2(w0, w1);
-              hi[e / 2 + 1] = f16x2(w2, w3);
+              uint64_t w0 = x[(i + e) / 2], w1 = x[(i + e) / 2 + 1];
+              if constexpr (!SCALED) {
+                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sm->vs[b][g][i + e]);
+                w0 = mul2(w0, f.x);
+                w1 = mul2(w1, f.y);
+              }
+              const float2 a0 = unpack2(w0), a1 = unpack2(w1);
+              hi[e / 2] = f16x2(a0.x, a0.y);
+              hi[e / 2 + 1] = f16x2(a1.x, a1.y);
               if constexpr (SPLIT) {
                 const float2 r0 = f16x2_f32(hi[e / 2]), r1 = f16x2_f32(hi[e / 2 + 1]);
-                lo[e / 2] = f16x2(w0 - r0.x, w1 - r0.y);
-                lo[e / 2 + 1] = f16x2(w2 - r1.x, w3 - r1.y);
+                lo[e / 2] = f16x2(a0.x - r0.x, a0.y - r0.y);
+                lo[e / 2 + 1] = f16x2(a1.x - r1.x, a1.y - r1.y);
               }
             }
-            tmem_st16(taddr + kTmemScores + 32 * g + i / 2, hi);
-            if constexpr (SPLIT) tmem_st16(taddr + kTmemScores + 32 * (G + g) + i / 2, lo);
+            tmem_st16(taddr + 32 * g + i / 2, hi);
+            if constexpr (SPLIT) tmem_st16(taddr + 32 * (G + g) + i / 2, lo);
           }
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm->p_full);
+        if (lane == 0) mbar_arrive(&sm->p_full[t]);
       }
       if (!ok) break;
 
       // ---- the tile's output, or this stretch's part of it ----
-      ok = __all_sync(0xffffffffu, wait(&sm->o_full, seg, 202));
+      ok = __all_sync(0xffffffffu, wait(&sm->o_full[t], seg, 202));
       if (!ok) break;
       tc_fence_after();
-      const float back = pow2i(static_cast<int>(vexp) - 21);
+      const float back = pow2i(static_cast<int>(vexp) - C::UP);
       T* dst = static_cast<T*>(p.out) + size_t(walk.seq.first + tok) * p.out_stride + size_t(head) * DIM;
       const bool whole = j0 == 0 && j1 == walk.steps;
       const uint32_t slot = 2 * blockIdx.x + (walk.first > u0 ? 1u : 0u);
-      float* mine = p.partials + size_t(slot) * (DIM + 2) * kRows + tid;
+      float* mine = p.partials + size_t(slot) * (DIM + 2) * HEIGHT + tid;
       const float inv = whole ? (l == 0.0f ? 0.0f : back / l) : back;
 #pragma unroll
       for (int i = 0; i < DIM; i += 32) {
         float o[32];
-        tmem_ld32(taddr + kTmemOutput + i, o);
+        tmem_ld32(taddr + kOutput + i, o);
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * inv;
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mine[size_t(i + e) * kRows] = o[e];
+          for (int e = 0; e < 32; ++e) mine[size_t(i + e) * HEIGHT] = o[e];
         } else if (in) {
           constexpr int W = Vec16<T>::kCount;
 #pragma unroll
@@ -423,8 +504,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         }
       }
       if (!whole) {
-        mine[size_t(DIM) * kRows] = m == -INFINITY ? m : m * factor;
-        mine[size_t(DIM + 1) * kRows] = l;
+        mine[size_t(DIM) * HEIGHT] = m;
+        mine[size_t(DIM + 1) * HEIGHT] = l;
         // The stretches that hold this tile: c0 .. c1 (stretch x starts at
         // floor(x * total / grid)). Each warp joins its 32 rows by itself.
         const uint64_t seg0 = walk.first, seg1 = walk.first + walk.steps;
@@ -434,7 +515,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         __syncwarp();
         uint32_t last = 0;
         if (lane == 0) {
-          uint32_t* counter = &p.counters[4 * c0 + warp];
+          uint32_t* counter = &p.counters[kAttnCounterStride * c0 + warp];
           const uint32_t before = atomicAdd(counter, 1u);
           last = before == c1 - c0;
           if (last) *counter = 0;
@@ -444,13 +525,13 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
           __threadfence();
           auto piece = [&](uint32_t x) {
             const uint32_t sl = 2 * x + (seg0 > total * x / grid ? 1u : 0u);
-            return p.partials + size_t(sl) * (DIM + 2) * kRows + tid;
+            return p.partials + size_t(sl) * (DIM + 2) * HEIGHT + tid;
           };
           float best = -INFINITY, sum = 0.0f;
-          for (uint32_t x = c0; x <= c1; ++x) best = fmaxf(best, __ldcg(piece(x) + size_t(DIM) * kRows));
+          for (uint32_t x = c0; x <= c1; ++x) best = fmaxf(best, __ldcg(piece(x) + size_t(DIM) * HEIGHT));
           for (uint32_t x = c0; x <= c1; ++x) {
-            const float pm = __ldcg(piece(x) + size_t(DIM) * kRows);
-            sum = fmaf(__ldcg(piece(x) + size_t(DIM + 1) * kRows), best == -INFINITY ? 1.0f : ex2(pm - best), sum);
+            const float pm = __ldcg(piece(x) + size_t(DIM) * HEIGHT);
+            sum = fmaf(__ldcg(piece(x) + size_t(DIM + 1) * HEIGHT), best == -INFINITY ? 1.0f : ex2(pm - best), sum);
           }
           const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
@@ -460,10 +541,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             for (int e = 0; e < 16; ++e) o[e] = 0.0f;
             for (uint32_t x = c0; x <= c1; ++x) {
               const float* from = piece(x);
-              const float pm = __ldcg(from + size_t(DIM) * kRows);
+              const float pm = __ldcg(from + size_t(DIM) * HEIGHT);
               const float f = (best == -INFINITY ? 1.0f : ex2(pm - best)) * norm;
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = fmaf(__ldcg(from + size_t(i + e) * kRows), f, o[e]);
+              for (int e = 0; e < 16; ++e) o[e] = fmaf(__ldcg(from + size_t(i + e) * HEIGHT), f, o[e]);
             }
             if (in) {
               constexpr int W = Vec16<T>::kCount;
@@ -480,18 +561,18 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
       }
       tc_fence_before();  // the output's columns may be written again once the next weights arrive
       cur = walk.first + j1;
-      if (cur < u1) next_tile(a, p.share, walk);
+      if (cur < u1) next_tile<HEIGHT>(a, p.share, walk);
     }
-  } else if (warp < 8) {
+  } else if (warp < CONVERT + 4) {
     // ---- convert: keys, then values, of each step ----
-    const uint32_t ct = tid - 128;
+    const uint32_t cw = warp - CONVERT, ct = tid - 32 * CONVERT;
     constexpr uint32_t CH = DIM / 16;              // 16-byte chunks of a row of codes
     constexpr uint32_t ROWS_PASS = 128 / CH;       // rows that the 128 threads fetch at once
     constexpr uint32_t PASSES = kStep / ROWS_PASS;
     const uint32_t ch = ct % CH, r0 = ct / CH;
     uint32_t it = 0;
     uint32_t vexp = 0;
-    // A step ahead: its code chunks, and its scales (lane l: positions 2 l and 2 l + 1).
+    // A step ahead: its code chunks, and its scales (lane l: positions l and 32 + l).
     uint4 kraw[PASSES], vraw[PASSES];
     TileWalk ahead = walk;
     uint32_t aj = static_cast<uint32_t>(u0 - walk.first);
@@ -507,7 +588,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
                           : make_uint4(0, 0, 0, 0);
       }
     };
-    uint32_t scale_raw[2][2];  // [key, value][position 2 lane + e]: both groups
+    uint32_t scale_raw[2][2];  // [key, value][position 32 e + lane]: both groups
     uint32_t valid_bits[2];
     auto fetch_scales = [&]() {
 #pragma unroll
@@ -524,49 +605,76 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
         }
       }
     };
-    auto put = [&](uint8_t* tile, const uint4 (&raw)[PASSES]) {
+    auto put = [&](uint8_t* tile, const uint4 (&raw)[PASSES], const uint32_t (&mul)[PASSES]) {
       // Chunk ch is dims 16 ch .. + 15: two 16-byte chunks of f16 in group ch / 4's tile.
       uint8_t* base = tile + (ch / 4) * (kStep * 128);
+      const uint32_t c2 = 2 * (ch % 4), flip = ch / 4;  // the two groups' lanes on different banks
 #pragma unroll
       for (uint32_t i = 0; i < PASSES; ++i) {
         const uint32_t r = r0 + i * ROWS_PASS;
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        uint4 o[2];
-        o[0] = make_uint4(codes_f16x2<0x4140>(w[0]), codes_f16x2<0x4342>(w[0]), codes_f16x2<0x4140>(w[1]), codes_f16x2<0x4342>(w[1]));
-        o[1] = make_uint4(codes_f16x2<0x4140>(w[2]), codes_f16x2<0x4342>(w[2]), codes_f16x2<0x4140>(w[3]), codes_f16x2<0x4342>(w[3]));
-        const uint32_t c2 = 2 * (ch % 4), flip = ch / 4;  // the two groups' lanes on different banks
-        *reinterpret_cast<uint4*>(base + r * 128u + (((c2 + flip) ^ (r & 7u)) << 4)) = flip ? o[1] : o[0];
-        *reinterpret_cast<uint4*>(base + r * 128u + (((c2 + 1 - flip) ^ (r & 7u)) << 4)) = flip ? o[0] : o[1];
+        uint32_t h[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          h[2 * e] = codes_f16x2<0x4140>(w[e]);
+          h[2 * e + 1] = codes_f16x2<0x4342>(w[e]);
+        }
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(mul[i]));
+        }
+        const uint4 o0 = make_uint4(h[0], h[1], h[2], h[3]), o1 = make_uint4(h[4], h[5], h[6], h[7]);
+        *reinterpret_cast<uint4*>(base + r * 128u + (((c2 + flip) ^ (r & 7u)) << 4)) = flip ? o1 : o0;
+        *reinterpret_cast<uint4*>(base + r * 128u + (((c2 + 1 - flip) ^ (r & 7u)) << 4)) = flip ? o0 : o1;
       }
+    };
+    // Scaled: the scales of this thread's rows, times 2^up, as f16 pairs.
+    auto row_scales = [&](uint32_t (&mul)[PASSES], const uint32_t (&raw)[2], int up) {
+#pragma unroll
+      for (uint32_t i = 0; i < PASSES; ++i) {
+        mul[i] = 0;
+        if constexpr (SCALED) {
+          const uint32_t both = __shfl_sync(0xffffffffu, raw[i * ROWS_PASS / 32], (r0 + i * ROWS_PASS) % 32);
+          const float f = f16_bits_to_f32(ch >= 4 ? both >> 16 : both & 0xFFFFu) * pow2i(up);
+          mul[i] = f16x2(f, f);
+        }
+      }
+    };
+    auto top_exponent = [&](const uint32_t (&raw)[2]) {
+      uint32_t e = 0;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) e = max(e, max((raw[n] >> 10) & 31u, (raw[n] >> 26) & 31u));
+      return min(__reduce_max_sync(0xffffffffu, e), 30u);
     };
     fetch(kraw, a.k_codes);
     fetch_scales();
     fetch(vraw, a.v_codes);
     for (uint64_t cur = u0; cur < u1; ++cur, ++it) {
-      const uint32_t b = it & 1u;
-      if (cur >= walk.first + walk.steps) next_tile(a, p.share, walk);
-      if (cur == walk.first || it == 0) vexp = 0;
+      const uint32_t b = it & 3u, st = it % STAGES, use = it / STAGES;
+      if (cur >= walk.first + walk.steps) next_tile<HEIGHT>(a, p.share, walk);
+      if (cur == walk.first) vexp = 0;
       // The place of the step after this one.
       const bool more = cur + 1 < u1;
       if (more) {
         if (++aj == ahead.steps) {
-          next_tile(a, p.share, ahead);
+          next_tile<HEIGHT>(a, p.share, ahead);
           aj = 0;
         }
       }
-      if (it > 0) ok = __all_sync(0xffffffffu, wait(&sm->k_empty, it - 1, 203));
+      if (it >= STAGES) ok = __all_sync(0xffffffffu, wait(&sm->k_empty[st], use - 1, 203));
       if (!ok) break;
-      put(&sm->k[0][0], kraw);
-      {
-        // Every warp finds the largest exponent of the step's value scales; each writes 16 positions' scales.
-        uint32_t e = 0;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) e = max(e, max((scale_raw[1][n] >> 10) & 31u, (scale_raw[1][n] >> 26) & 31u));
-        vexp = max(vexp, min(__reduce_max_sync(0xffffffffu, e), 30u));
-        const float up = pow2i(21 - static_cast<int>(vexp));
-        const uint32_t half = (warp - 4) / 2;
-        if (lane / 16 == (warp & 1u)) {
-          const float2 kf = f16x2_f32(scale_raw[0][half]), vf = f16x2_f32(scale_raw[1][half]);
+      uint32_t mul[PASSES];
+      const uint32_t kexp = SCALED ? top_exponent(scale_raw[0]) : 14u;
+      row_scales(mul, scale_raw[0], 14 - static_cast<int>(kexp));
+      put(&sm->k[st][0][0], kraw, mul);
+      // Every warp finds the largest exponent of the value scales; each writes 16 positions' scales.
+      vexp = max(vexp, top_exponent(scale_raw[1]));
+      row_scales(mul, scale_raw[1], C::UP - static_cast<int>(vexp));
+      if constexpr (!SCALED) {
+        const float up = pow2i(C::UP - static_cast<int>(vexp));
+        const uint32_t half = cw / 2;
+        if (lane / 16 == (cw & 1u)) {
+          const float2 kf = f16x2_f32(half ? scale_raw[0][1] : scale_raw[0][0]), vf = f16x2_f32(half ? scale_raw[1][1] : scale_raw[1][0]);
           const uint32_t at = 32u * half + lane;
           sm->ks[b][0][at] = kf.x;
           sm->vs[b][0][at] = vf.x * up;
@@ -575,124 +683,150 @@ __global__ void __launch_bounds__(kTileThreads, 2) paged_attention_tile_kernel(c
             sm->vs[b][G - 1][at] = vf.y * up;
           }
         }
-        if (warp == 4 && lane == 0) {
-          sm->valid[b][0] = valid_bits[0];
-          sm->valid[b][1] = valid_bits[1];
-          sm->vexp[b] = vexp;
-        }
+      }
+      if (cw == 0 && lane == 0) {
+        sm->valid[b][0] = valid_bits[0];
+        sm->valid[b][1] = valid_bits[1];
+        sm->vexp[b] = vexp;
+        sm->kexp[b] = kexp;
       }
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&sm->k_full);
+        mbar_arrive(&sm->k_full[st]);
         mbar_arrive(&sm->scales_full[b]);
       }
       if (more) {
         fetch(kraw, a.k_codes);
         fetch_scales();
       }
-      if (it > 0) ok = __all_sync(0xffffffffu, wait(&sm->v_empty, it - 1, 204));
+      if (it >= STAGES) ok = __all_sync(0xffffffffu, wait(&sm->v_empty[st], use - 1, 204));
       if (!ok) break;
-      put(&sm->v[0][0], vraw);
+      put(&sm->v[st][0][0], vraw, mul);
       fence_proxy_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm->v_full);
+      if (lane == 0) mbar_arrive(&sm->v_full[st]);
       if (more) fetch(vraw, a.v_codes);
     }
   } else if (lane == 0) {
     // ---- MMAs ----
     uint32_t it = 0, seg = 0;
-    bool waiting = false;  // a commit to o_full is due before this thread may leave
+    bool waiting = false;  // MMAs may be in flight
+    auto scores = [&](uint32_t t, uint32_t st) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint64_t kd = umma_desc(smem_addr(sm->k[st][g]), 16, 1024, kLayoutSw128);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+          const uint64_t qd = umma_desc(smem_addr(sm->q[t][q][g]), 16, 1024, kLayoutSw128);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {  // 16 dims: 32 bytes of each row
+            umma_f16_ss(tmem + t * C::TMEM_TILE + (SCALED ? 0 : g * kStep), qd + 2 * kk, kd + 2 * kk, kIdescScores,
+                        (SCALED && g > 0) || q > 0 || kk > 0);
+          }
+        }
+      }
+    };
+    auto output = [&](uint32_t t, uint32_t st, bool first) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {  // 16 positions: 16 rows of 128 bytes
+            const uint64_t vd = umma_desc(smem_addr(sm->v[st][g]) + kk * 2048u, 16, 1024, kLayoutSw128);
+            umma_f16_ts(tmem + t * C::TMEM_TILE + kOutput + 64 * g,
+                        tmem + t * C::TMEM_TILE + (SCALED ? 0 : 32 * (q * G + g)) + 8 * kk, vd, kIdescOutput,
+                        !first || q > 0 || kk > 0);
+          }
+        }
+      }
+    };
     for (uint64_t cur = u0; cur < u1 && ok; ++seg) {
       const uint32_t j0 = static_cast<uint32_t>(cur - walk.first);
       const uint32_t j1 = static_cast<uint32_t>((u1 < walk.first + walk.steps ? u1 : walk.first + walk.steps) - walk.first);
-      ok = wait(&sm->q_full, seg, 205);
-      for (uint32_t j = j0; j < j1 && ok; ++j, ++it) {
-        ok = wait(&sm->k_full, it, 206);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const uint64_t kd = umma_desc(smem_addr(sm->k[g]), 16, 1024, kLayoutSw128);
-#pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
-            const uint64_t qd = umma_desc(smem_addr(sm->q[q][g]), 16, 1024, kLayoutSw128);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {  // 16 dims: 32 bytes of each row
-              umma_f16_ss(tmem + kTmemScores + g * kStep, qd + 2 * kk, kd + 2 * kk, kIdescScores, q > 0 || kk > 0);
-            }
+      for (int t = 0; t < TILES && ok; ++t) ok = wait(&sm->q_full[t], seg, 205);
+      // Step j's scores are issued behind step j - 1's output, tile by tile: the weights lie in the
+      // scores' columns. MMAs of one thread run in order.
+      for (uint32_t j = j0; j <= j1 && ok; ++j) {
+        const uint32_t st = it % STAGES, prev = (it + STAGES - 1) % STAGES;
+        if (j < j1) ok = wait(&sm->k_full[st], it / STAGES, 206);
+        if (ok && j > j0) ok = wait(&sm->v_full[prev], (it - 1) / STAGES, 207);
+        for (int t = 0; t < TILES && ok; ++t) {
+          if (j > j0) {
+            ok = wait(&sm->p_full[t], it - 1, 208);
+            if (!ok) break;
+            tc_fence_after();
+            output(t, prev, j == j0 + 1);
+            if (t == TILES - 1) umma_commit(&sm->v_empty[prev]);
+            if (j == j1) umma_commit(&sm->o_full[t]);
+          }
+          if (j < j1) {
+            tc_fence_after();
+            scores(t, st);
+            umma_commit(&sm->s_full[t]);
+            waiting = true;
+            if (t == TILES - 1) umma_commit(&sm->k_empty[st]);
           }
         }
-        umma_commit(&sm->k_empty);
-        umma_commit(&sm->s_full);
-        waiting = true;
-        ok = wait(&sm->v_full, it, 207) && wait(&sm->p_full, it, 208);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-#pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {  // 16 positions: 16 rows of 128 bytes
-              const uint64_t vd = umma_desc(smem_addr(sm->v[g]) + kk * 2048u, 16, 1024, kLayoutSw128);
-              umma_f16_ts(tmem + kTmemOutput + 64 * g, tmem + kTmemScores + 32 * (q * G + g) + 8 * kk, vd, kIdescOutput,
-                          j > j0 || q > 0 || kk > 0);
-            }
-          }
-        }
-        umma_commit(&sm->v_empty);
+        if (j < j1) ++it;
       }
       if (ok) {
-        umma_commit(&sm->o_full);
         cur = walk.first + j1;
-        if (cur < u1) next_tile(a, p.share, walk);
+        if (cur < u1) next_tile<HEIGHT>(a, p.share, walk);
       }
     }
     if (!ok && waiting) {  // MMAs in flight end before tensor memory is freed
-      umma_commit(&sm->o_full);
-      mbar_wait_bounded(&sm->o_full, seg & 1u, p.error, p.timeout_ns, 209);
+      umma_commit(&sm->o_full[0]);
+      mbar_wait_bounded(&sm->o_full[0], seg & 1u, p.error, p.timeout_ns, 209);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == WARPS - 1) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, int TILES>
 int32_t launch_tile(const PagedArgs& a, const AttnArgs& p, uint32_t grid, cudaStream_t stream) {
-  const size_t smem = sizeof(TileSmem<DIM, sizeof(T) == 4>) + 1024;  // + alignment of the dynamic window
-  const cudaError_t e = cudaFuncSetAttribute(paged_attention_tile_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
+  using C = TileConfig<T, DIM, TILES>;
+  const size_t smem = sizeof(TileSmem<C>) + 1024;  // + alignment of the dynamic window
+  const cudaError_t e = cudaFuncSetAttribute(paged_attention_tile_kernel<T, DIM, TILES>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return paged_status(e);
-  paged_attention_tile_kernel<T, DIM><<<grid, kTileThreads, smem, stream>>>(a, p);
+  paged_attention_tile_kernel<T, DIM, TILES><<<grid, C::THREADS, smem, stream>>>(a, p);
   return paged_status(cudaGetLastError());
+}
+
+template <typename T>
+int32_t launch_tile_as(const PagedArgs& a, const AttnArgs& p, const TilePlan& plan, cudaStream_t stream) {
+  if (a.head_dim == 128) {
+    return plan.tiles == 2 ? launch_tile<T, 128, 2>(a, p, plan.grid, stream) : launch_tile<T, 128, 1>(a, p, plan.grid, stream);
+  }
+  return plan.tiles == 2 ? launch_tile<T, 64, 2>(a, p, plan.grid, stream) : launch_tile<T, 64, 1>(a, p, plan.grid, stream);
 }
 
 }  // namespace
 
-uint32_t paged_tile_grid(const PagedArgs& a, uint32_t heads, uint32_t sms) {
-  const uint64_t tiles = (uint64_t(a.max_query) * (heads / a.kv_heads) + kRows - 1) / kRows;
-  const uint64_t steps = uint64_t(a.sequences) * a.kv_heads * tiles * (a.max_context ? (a.max_context + kStep - 1) / kStep : 1);
-  return static_cast<uint32_t>(steps < 2 * sms ? steps : 2 * sms);
+TilePlan paged_tile_plan(const PagedArgs& a, uint32_t heads, uint32_t sms) {
+  TilePlan plan;
+  const uint64_t rows = uint64_t(a.max_query) * (heads / a.kv_heads);
+  plan.tiles = rows > kRows ? 2 : 1;
+  const uint64_t height = uint64_t(kRows) * plan.tiles;
+  const uint64_t steps = uint64_t(a.sequences) * a.kv_heads * ((rows + height - 1) / height) *
+                         (a.max_context ? (a.max_context + kStep - 1) / kStep : 1);
+  const uint64_t most = plan.tiles == 2 ? sms : 2 * sms;  // what is resident at once
+  plan.grid = static_cast<uint32_t>(steps < most ? steps : most);
+  plan.partial_bytes = uint64_t(2) * plan.grid * (a.head_dim + 2) * height * 4;
+  return plan;
 }
 
-uint64_t paged_tile_partial_bytes(const PagedArgs& a, uint32_t grid) {
-  return uint64_t(2) * grid * (a.head_dim + 2) * kRows * 4;
-}
-
-int32_t paged_tile_launch(const PagedArgs& a, const AttnArgs& p, uint32_t format, uint32_t grid, cudaStream_t stream) {
-  if (a.head_dim == 128) {
-    return format == kFormatF32   ? launch_tile<float, 128>(a, p, grid, stream)
-           : format == kFormatF16 ? launch_tile<__half, 128>(a, p, grid, stream)
-                                  : launch_tile<__nv_bfloat16, 128>(a, p, grid, stream);
-  }
-  return format == kFormatF32   ? launch_tile<float, 64>(a, p, grid, stream)
-         : format == kFormatF16 ? launch_tile<__half, 64>(a, p, grid, stream)
-                                : launch_tile<__nv_bfloat16, 64>(a, p, grid, stream);
+int32_t paged_tile_launch(const PagedArgs& a, const AttnArgs& p, uint32_t format, const TilePlan& plan, cudaStream_t stream) {
+  return format == kFormatF32   ? launch_tile_as<float>(a, p, plan, stream)
+         : format == kFormatF16 ? launch_tile_as<__half>(a, p, plan, stream)
+                                : launch_tile_as<__nv_bfloat16>(a, p, plan, stream);
 }
 
 }  // namespace qwc

@@ -64,6 +64,12 @@ struct TileConfig {
   static constexpr int WARPS = 4 * TILES + 5;
   static constexpr int THREADS = 32 * WARPS;
   static constexpr uint32_t TMEM_TILE = G * kStep + DIM;     // columns of a tile: scores, output
+  // Registers a thread: at launch what fits (65,536 over the resident warps, by quarters of an SM), then the
+  // softmax warps take what the convert warps give back.
+  static constexpr int LAUNCH_REGS = TILES == 2 ? 128 : 96;
+  static constexpr int SOFTMAX_REGS = TILES == 2 ? 152 : 128;
+  static constexpr int CONVERT_REGS = TILES == 2 ? 80 : 64;
+  static_assert(4 * TILES * SOFTMAX_REGS + 4 * CONVERT_REGS + LAUNCH_REGS <= WARPS * LAUNCH_REGS, "a split cannot exceed the launch");
   // The weights' power of two, 2^(UP - vexp): weight times value scale below 2^15 (exact), value below 2^7 (scaled).
   static constexpr int UP = SCALED ? 14 : 21;
 };
@@ -166,6 +172,29 @@ __device__ __forceinline__ void tmem_st16f(uint32_t t, const float (&f)[16]) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The MMAs and commits of a warp whose lanes all come here: one elected lane (always the same one)
+// issues. The operands then stay warp-uniform, which the instruction wants.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
+      : "memory");
+}
+
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // D = f32, A and B f16, M = 128, N = 64; B with the dims along its rows (keys)
@@ -188,6 +217,31 @@ __device__ __forceinline__ void tmem_ld_pairs(uint32_t t0, uint32_t t1, uint64_t
     x[i] = pack2(f0[2 * i], f0[2 * i + 1]);
     y[i] = pack2(f1[2 * i], f1[2 * i + 1]);
   }
+}
+
+// PER (2 or 4) values of a row, as one load.
+template <int PER>
+__device__ __forceinline__ void load_values(const float* src, float (&x)[PER]) {
+  if constexpr (PER == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(src);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  } else {
+    const float2 f = *reinterpret_cast<const float2*>(src);
+    x[0] = f.x, x[1] = f.y;
+  }
+}
+template <int PER, typename T>
+__device__ __forceinline__ void load_values(const T* src, float (&x)[PER]) {
+  uint2 w = make_uint2(0, 0);
+  if constexpr (PER == 4) {
+    w = *reinterpret_cast<const uint2*>(src);
+  } else {
+    w.x = *reinterpret_cast<const uint32_t*>(src);
+  }
+  float y[8];
+  unpack16(make_uint4(w.x, w.y, 0, 0), y, T());
+#pragma unroll
+  for (int e = 0; e < PER; ++e) x[e] = y[e];
 }
 
 template <typename T, int DIM, int TILES>
@@ -288,6 +342,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
   };
 
   if (warp < CONVERT) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
     // ---- softmax: row tid of the CTA's tiles ----
     const uint32_t t = warp / 4, trow = tid % kRows;
     const uint32_t taddr = tmem + ((warp % 4 * 32u) << 16) + t * C::TMEM_TILE;
@@ -295,50 +350,57 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     for (uint64_t cur = u0; cur < u1 && ok; ++seg) {
       const uint32_t j0 = static_cast<uint32_t>(cur - walk.first);
       const uint32_t j1 = static_cast<uint32_t>((u1 < walk.first + walk.steps ? u1 : walk.first + walk.steps) - walk.first);
+      const uint32_t rows = walk.seq.n * p.share;
       const uint32_t row = walk.qt * HEIGHT + tid;
-      const bool in = row < walk.seq.n * p.share;
+      const bool in = row < rows;
       const uint32_t tok = in ? row / p.share : 0u, head = walk.h * p.share + (in ? row % p.share : 0u);
-      // The row's queries: its largest value gives the power of two, then the f16 parts.
-      const T* src = static_cast<const T*>(p.q) + size_t(walk.seq.first + tok) * p.q_stride + size_t(head) * DIM;
-      constexpr int V = Vec16<T>::kCount;
-      float amax = 0.0f;
-      if (in) {
-#pragma unroll 4
-        for (int d = 0; d < DIM; d += V) {
-          float x[V];
-          unpack16(*reinterpret_cast<const uint4*>(src + d), x, T());
-#pragma unroll
-          for (int e = 0; e < V; ++e) amax = fmaxf(amax, fabsf(x[e]));
-        }
-      }
-      const int e2 = row_exponent(amax);
-      const float down = pow2i(-e2);
-      const float factor = p.scaling * 1.4426950408889634f * pow2i(e2);
       const int32_t limit = in ? walk.seq.base + static_cast<int32_t>(tok) : -1;
-#pragma unroll 2
-      for (int d = 0; d < DIM; d += 8) {
-        float x[8];
-        if (!in) {
+      // The warp's 32 rows of queries, a whole row at a time (lane l: dims PER l .. + PER - 1): the largest
+      // value gives the row's power of two, then the f16 parts go to shared memory.
+      constexpr int PER = DIM / 32;
+      constexpr int BATCH = 8;  // rows in flight
+      float factor = 0.0f;
+#pragma unroll 1
+      for (uint32_t r0 = 0; r0 < 32; r0 += BATCH) {
+        float x[BATCH][PER];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-        } else if constexpr (SPLIT) {
-          const float4 f0 = *reinterpret_cast<const float4*>(src + d), f1 = *reinterpret_cast<const float4*>(src + d + 4);
-          x[0] = f0.x, x[1] = f0.y, x[2] = f0.z, x[3] = f0.w, x[4] = f1.x, x[5] = f1.y, x[6] = f1.z, x[7] = f1.w;
-        } else {
-          unpack16(*reinterpret_cast<const uint4*>(src + d), x, T());
-        }
-        uint32_t hi[4], lo[4];
+        for (int i = 0; i < BATCH; ++i) {
+          const uint32_t rr = row - lane + r0 + i;  // (row - lane: the warp's first row)
+          const T* src = static_cast<const T*>(p.q) + size_t(walk.seq.first + rr / p.share) * p.q_stride +
+                         size_t(walk.h * p.share + rr % p.share) * DIM + PER * lane;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y0 = fmaf(x[2 * e], down, x[2 * e] - x[2 * e]);  // an infinity is NaN from here on
-          const float y1 = fmaf(x[2 * e + 1], down, x[2 * e + 1] - x[2 * e + 1]);
-          hi[e] = f16x2(y0, y1);
-          const float2 f = f16x2_f32(hi[e]);
-          lo[e] = f16x2(y0 - f.x, y1 - f.y);
+          for (int e = 0; e < PER; ++e) x[i][e] = 0.0f;
+          if (rr < rows) load_values<PER>(src, x[i]);
         }
-        const uint32_t at = trow * 128u + ((((d % 64) / 8) ^ (trow & 7u)) << 4);
-        *reinterpret_cast<uint4*>(&sm->q[t][0][d / 64][at]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (SPLIT) *reinterpret_cast<uint4*>(&sm->q[t][PARTS - 1][d / 64][at]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
+          const int e2 = row_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
+          const float down = pow2i(-e2);
+          if (lane == r0 + i) factor = p.scaling * 1.4426950408889634f * pow2i(e2);
+          uint32_t hi[PER / 2], lo[PER / 2];
+#pragma unroll
+          for (int e = 0; e < PER / 2; ++e) {
+            const float y0 = fmaf(x[i][2 * e], down, x[i][2 * e] - x[i][2 * e]);  // an infinity is NaN from here on
+            const float y1 = fmaf(x[i][2 * e + 1], down, x[i][2 * e + 1] - x[i][2 * e + 1]);
+            hi[e] = f16x2(y0, y1);
+            const float2 f = f16x2_f32(hi[e]);
+            lo[e] = f16x2(y0 - f.x, y1 - f.y);
+          }
+          const uint32_t r = trow - lane + r0 + i, d = PER * lane;
+          const uint32_t at = r * 128u + ((((d % 64) / 8) ^ (r & 7u)) << 4) + (d % 8) * 2;
+          uint8_t* dst = &sm->q[t][0][d / 64][at];
+          uint8_t* dst_lo = &sm->q[t][PARTS - 1][d / 64][at];
+          if constexpr (PER == 4) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+            if constexpr (SPLIT) *reinterpret_cast<uint2*>(dst_lo) = make_uint2(lo[0], lo[1]);
+          } else {
+            *reinterpret_cast<uint32_t*>(dst) = hi[0];
+            if constexpr (SPLIT) *reinterpret_cast<uint32_t*>(dst_lo) = lo[0];
+          }
+        }
       }
       fence_proxy_async_shared();
       __syncwarp();
@@ -481,7 +543,8 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       T* dst = static_cast<T*>(p.out) + size_t(walk.seq.first + tok) * p.out_stride + size_t(head) * DIM;
       const bool whole = j0 == 0 && j1 == walk.steps;
       const uint32_t slot = 2 * blockIdx.x + (walk.first > u0 ? 1u : 0u);
-      float* mine = p.partials + size_t(slot) * (DIM + 2) * HEIGHT + tid;
+      // A partial: [DIM / 4][HEIGHT] of four dims, then maxima and sums.
+      float* mine = p.partials + size_t(slot) * (DIM + 2) * HEIGHT;
       const float inv = whole ? (l == 0.0f ? 0.0f : back / l) : back;
 #pragma unroll
       for (int i = 0; i < DIM; i += 32) {
@@ -491,7 +554,9 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * inv;
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mine[size_t(i + e) * HEIGHT] = o[e];
+          for (int e = 0; e < 32; e += 4) {
+            reinterpret_cast<float4*>(mine)[size_t((i + e) / 4) * HEIGHT + tid] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
         } else if (in) {
           constexpr int W = Vec16<T>::kCount;
 #pragma unroll
@@ -504,8 +569,8 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         }
       }
       if (!whole) {
-        mine[size_t(DIM) * HEIGHT] = m;
-        mine[size_t(DIM + 1) * HEIGHT] = l;
+        mine[size_t(DIM) * HEIGHT + tid] = m;
+        mine[size_t(DIM + 1) * HEIGHT + tid] = l;
         // The stretches that hold this tile: c0 .. c1 (stretch x starts at
         // floor(x * total / grid)). Each warp joins its 32 rows by itself.
         const uint64_t seg0 = walk.first, seg1 = walk.first + walk.steps;
@@ -525,31 +590,40 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           __threadfence();
           auto piece = [&](uint32_t x) {
             const uint32_t sl = 2 * x + (seg0 > total * x / grid ? 1u : 0u);
-            return p.partials + size_t(sl) * (DIM + 2) * HEIGHT + tid;
+            return p.partials + size_t(sl) * (DIM + 2) * HEIGHT;
           };
           float best = -INFINITY, sum = 0.0f;
-          for (uint32_t x = c0; x <= c1; ++x) best = fmaxf(best, __ldcg(piece(x) + size_t(DIM) * HEIGHT));
+          for (uint32_t x = c0; x <= c1; ++x) best = fmaxf(best, __ldcg(piece(x) + size_t(DIM) * HEIGHT + tid));
           for (uint32_t x = c0; x <= c1; ++x) {
-            const float pm = __ldcg(piece(x) + size_t(DIM) * HEIGHT);
-            sum = fmaf(__ldcg(piece(x) + size_t(DIM + 1) * HEIGHT), best == -INFINITY ? 1.0f : ex2(pm - best), sum);
+            const float pm = __ldcg(piece(x) + size_t(DIM) * HEIGHT + tid);
+            sum = fmaf(__ldcg(piece(x) + size_t(DIM + 1) * HEIGHT + tid), best == -INFINITY ? 1.0f : ex2(pm - best), sum);
           }
           const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
-          for (int i = 0; i < DIM; i += 16) {
-            float o[16];
+          for (int i = 0; i < DIM; i += 32) {
+            float o[32];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+#pragma unroll 1
             for (uint32_t x = c0; x <= c1; ++x) {
               const float* from = piece(x);
-              const float pm = __ldcg(from + size_t(DIM) * HEIGHT);
+              const float pm = __ldcg(from + size_t(DIM) * HEIGHT + tid);
+              float4 v[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = __ldcg(reinterpret_cast<const float4*>(from) + size_t(i / 4 + e) * HEIGHT + tid);
               const float f = (best == -INFINITY ? 1.0f : ex2(pm - best)) * norm;
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = fmaf(__ldcg(from + size_t(i + e) * HEIGHT), f, o[e]);
+              for (int e = 0; e < 8; ++e) {
+                o[4 * e] = fmaf(v[e].x, f, o[4 * e]);
+                o[4 * e + 1] = fmaf(v[e].y, f, o[4 * e + 1]);
+                o[4 * e + 2] = fmaf(v[e].z, f, o[4 * e + 2]);
+                o[4 * e + 3] = fmaf(v[e].w, f, o[4 * e + 3]);
+              }
             }
             if (in) {
               constexpr int W = Vec16<T>::kCount;
 #pragma unroll
-              for (int e = 0; e < 16; e += W) {
+              for (int e = 0; e < 32; e += W) {
                 float y[W];
 #pragma unroll
                 for (int q = 0; q < W; ++q) y[q] = o[e + q];
@@ -564,6 +638,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       if (cur < u1) next_tile<HEIGHT>(a, p.share, walk);
     }
   } else if (warp < CONVERT + 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::CONVERT_REGS));
     // ---- convert: keys, then values, of each step ----
     const uint32_t cw = warp - CONVERT, ct = tid - 32 * CONVERT;
     constexpr uint32_t CH = DIM / 16;              // 16-byte chunks of a row of codes
@@ -576,16 +651,30 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     uint4 kraw[PASSES], vraw[PASSES];
     TileWalk ahead = walk;
     uint32_t aj = static_cast<uint32_t>(u0 - walk.first);
-    auto row_at = [&](uint32_t pos) -> int32_t {
-      if (pos >= ahead.seq.context) return -1;
-      return static_cast<int32_t>(paged_row(a, ahead.s, pos));
+    // Rows of the pool of that step's positions 32 e + lane (-1: not cached): the page table is read
+    // before the step in hand is converted, its answers are used after.
+    int32_t page_id[2], page_at[2], rows[2];
+    auto look_up = [&]() {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t pos = aj * kStep + 32u * e + lane;
+        const uint32_t pg = page_of(a, pos);
+        page_at[e] = static_cast<int32_t>(pos - pg * a.page_size);
+        page_id[e] = pos < ahead.seq.context ? __ldg(a.page_table + size_t(ahead.s) * a.table_stride + pg) : -1;
+      }
+    };
+    auto found = [&]() {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        rows[e] = static_cast<uint32_t>(page_id[e]) < a.pages ? page_id[e] * static_cast<int32_t>(a.page_size) + page_at[e] : -1;
+      }
     };
     auto fetch = [&](uint4 (&raw)[PASSES], const uint8_t* plane) {
+      const uint8_t* from = plane + ahead.h * DIM + 16u * ch;
 #pragma unroll
       for (uint32_t i = 0; i < PASSES; ++i) {
-        const int32_t row = row_at(aj * kStep + r0 + i * ROWS_PASS);
-        raw[i] = row >= 0 ? ld_nc4(plane + uint64_t(static_cast<uint32_t>(row)) * a.code_row + ahead.h * DIM + 16u * ch)
-                          : make_uint4(0, 0, 0, 0);
+        const int32_t row = __shfl_sync(0xffffffffu, rows[i * ROWS_PASS / 32], (r0 + i * ROWS_PASS) % 32);
+        raw[i] = row >= 0 ? ld_nc4(from + uint64_t(static_cast<uint32_t>(row)) * a.code_row) : make_uint4(0, 0, 0, 0);
       }
     };
     uint32_t scale_raw[2][2];  // [key, value][position 32 e + lane]: both groups
@@ -593,13 +682,12 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     auto fetch_scales = [&]() {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int32_t row = row_at(aj * kStep + 32u * e + lane);
-        valid_bits[e] = __ballot_sync(0xffffffffu, row >= 0);
+        valid_bits[e] = __ballot_sync(0xffffffffu, rows[e] >= 0);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           scale_raw[n][e] = 0;
-          if (row >= 0) {
-            const uint8_t* from = (n ? a.v_scales : a.k_scales) + uint64_t(static_cast<uint32_t>(row)) * a.scale_row + ahead.h * (2 * G);
+          if (rows[e] >= 0) {
+            const uint8_t* from = (n ? a.v_scales : a.k_scales) + uint64_t(static_cast<uint32_t>(rows[e])) * a.scale_row + ahead.h * (2 * G);
             scale_raw[n][e] = G == 2 ? *reinterpret_cast<const uint32_t*>(from) : *reinterpret_cast<const uint16_t*>(from);
           }
         }
@@ -646,6 +734,8 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       for (int n = 0; n < 2; ++n) e = max(e, max((raw[n] >> 10) & 31u, (raw[n] >> 26) & 31u));
       return min(__reduce_max_sync(0xffffffffu, e), 30u);
     };
+    look_up();
+    found();
     fetch(kraw, a.k_codes);
     fetch_scales();
     fetch(vraw, a.v_codes);
@@ -660,6 +750,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           next_tile<HEIGHT>(a, p.share, ahead);
           aj = 0;
         }
+        look_up();
       }
       if (it >= STAGES) ok = __all_sync(0xffffffffu, wait(&sm->k_empty[st], use - 1, 203));
       if (!ok) break;
@@ -697,6 +788,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         mbar_arrive(&sm->scales_full[b]);
       }
       if (more) {
+        found();
         fetch(kraw, a.k_codes);
         fetch_scales();
       }
@@ -708,21 +800,27 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       if (lane == 0) mbar_arrive(&sm->v_full[st]);
       if (more) fetch(vraw, a.v_codes);
     }
-  } else if (lane == 0) {
-    // ---- MMAs ----
+  } else {
+    // ---- MMAs: the whole warp walks, one lane issues ----
     uint32_t it = 0, seg = 0;
     bool waiting = false;  // MMAs may be in flight
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t q0 = umma_desc(smem_addr(sm->q[0][0][0]), 16, 1024, kLayoutSw128);
+    const uint64_t k0 = umma_desc(smem_addr(sm->k[0][0]), 16, 1024, kLayoutSw128);
+    const uint64_t v0 = umma_desc(smem_addr(sm->v[0][0]), 16, 1024, kLayoutSw128);
+    constexpr uint32_t kQTile = kRows * 128 / 16, kKvTile = kStep * 128 / 16;  // in a descriptor's units
+    auto wait_all = [&](uint64_t* bar, uint32_t n, int32_t code) { return __all_sync(0xffffffffu, wait(bar, n, code)) != 0; };
     auto scores = [&](uint32_t t, uint32_t st) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const uint64_t kd = umma_desc(smem_addr(sm->k[st][g]), 16, 1024, kLayoutSw128);
+        const uint64_t kd = k0 + (st * G + g) * kKvTile;
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
-          const uint64_t qd = umma_desc(smem_addr(sm->q[t][q][g]), 16, 1024, kLayoutSw128);
+          const uint64_t qd = q0 + ((t * PARTS + q) * G + g) * kQTile;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // 16 dims: 32 bytes of each row
-            umma_f16_ss(tmem + t * C::TMEM_TILE + (SCALED ? 0 : g * kStep), qd + 2 * kk, kd + 2 * kk, kIdescScores,
-                        (SCALED && g > 0) || q > 0 || kk > 0);
+            mma_ss(base + t * C::TMEM_TILE + (SCALED ? 0 : g * kStep), qd + 2 * kk, kd + 2 * kk, kIdescScores,
+                   (SCALED && g > 0) || q > 0 || kk > 0);
           }
         }
       }
@@ -730,14 +828,14 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     auto output = [&](uint32_t t, uint32_t st, bool first) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
+        const uint64_t vd = v0 + (st * G + g) * kKvTile;
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // 16 positions: 16 rows of 128 bytes
-            const uint64_t vd = umma_desc(smem_addr(sm->v[st][g]) + kk * 2048u, 16, 1024, kLayoutSw128);
-            umma_f16_ts(tmem + t * C::TMEM_TILE + kOutput + 64 * g,
-                        tmem + t * C::TMEM_TILE + (SCALED ? 0 : 32 * (q * G + g)) + 8 * kk, vd, kIdescOutput,
-                        !first || q > 0 || kk > 0);
+            mma_ts(base + t * C::TMEM_TILE + kOutput + 64 * g,
+                   base + t * C::TMEM_TILE + (SCALED ? 0 : 32 * (q * G + g)) + 8 * kk, vd + 128 * kk, kIdescOutput,
+                   !first || q > 0 || kk > 0);
           }
         }
       }
@@ -745,28 +843,28 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     for (uint64_t cur = u0; cur < u1 && ok; ++seg) {
       const uint32_t j0 = static_cast<uint32_t>(cur - walk.first);
       const uint32_t j1 = static_cast<uint32_t>((u1 < walk.first + walk.steps ? u1 : walk.first + walk.steps) - walk.first);
-      for (int t = 0; t < TILES && ok; ++t) ok = wait(&sm->q_full[t], seg, 205);
+      for (int t = 0; t < TILES && ok; ++t) ok = wait_all(&sm->q_full[t], seg, 205);
       // Step j's scores are issued behind step j - 1's output, tile by tile: the weights lie in the
       // scores' columns. MMAs of one thread run in order.
       for (uint32_t j = j0; j <= j1 && ok; ++j) {
         const uint32_t st = it % STAGES, prev = (it + STAGES - 1) % STAGES;
-        if (j < j1) ok = wait(&sm->k_full[st], it / STAGES, 206);
-        if (ok && j > j0) ok = wait(&sm->v_full[prev], (it - 1) / STAGES, 207);
+        if (j < j1) ok = wait_all(&sm->k_full[st], it / STAGES, 206);
+        if (ok && j > j0) ok = wait_all(&sm->v_full[prev], (it - 1) / STAGES, 207);
         for (int t = 0; t < TILES && ok; ++t) {
           if (j > j0) {
-            ok = wait(&sm->p_full[t], it - 1, 208);
+            ok = wait_all(&sm->p_full[t], it - 1, 208);
             if (!ok) break;
             tc_fence_after();
             output(t, prev, j == j0 + 1);
-            if (t == TILES - 1) umma_commit(&sm->v_empty[prev]);
-            if (j == j1) umma_commit(&sm->o_full[t]);
+            if (t == TILES - 1) mma_commit(&sm->v_empty[prev]);
+            if (j == j1) mma_commit(&sm->o_full[t]);
           }
           if (j < j1) {
             tc_fence_after();
             scores(t, st);
-            umma_commit(&sm->s_full[t]);
+            mma_commit(&sm->s_full[t]);
             waiting = true;
-            if (t == TILES - 1) umma_commit(&sm->k_empty[st]);
+            if (t == TILES - 1) mma_commit(&sm->k_empty[st]);
           }
         }
         if (j < j1) ++it;
@@ -777,7 +875,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       }
     }
     if (!ok && waiting) {  // MMAs in flight end before tensor memory is freed
-      umma_commit(&sm->o_full[0]);
+      mma_commit(&sm->o_full[0]);
       mbar_wait_bounded(&sm->o_full[0], seg & 1u, p.error, p.timeout_ns, 209);
     }
   }

@@ -193,11 +193,7 @@ int32_t paged_args(const qwc_paged_cache* c, const qwc_paged_batch* b, PagedArgs
   a.page_table = b->page_table;
   a.pages = c->pages;
   a.page_size = c->page_size;
-  uint32_t shift = 0;
-  while ((uint64_t(1) << shift) < c->page_size) ++shift;
-  a.page_mul = static_cast<uint32_t>(((((uint64_t(1) << shift) - c->page_size) << 32) / c->page_size) + 1);
-  a.page_shift1 = shift > 0 ? 1 : 0;
-  a.page_shift2 = shift > 0 ? shift - 1 : 0;
+  a.by_page = divisor(c->page_size);
   a.kv_heads = c->kv_heads;
   a.head_dim = c->head_dim;
   a.code_row = c->kv_heads * c->head_dim;

@@ -13,11 +13,26 @@
 
 namespace qwc {
 
-// qwc_paged_cache and qwc_paged_batch, with the division by the page size as
-// a multiplication and two shifts (Granlund and Montgomery, 1994, figure 4.1,
-// exact for every 32-bit position): with l = ceil(log2 page_size), page_mul
-// is 2^32 (2^l - page_size) / page_size + 1, the shifts min(l, 1) and
+// Division of a 32-bit number by one known at the launch, as a multiplication
+// and two shifts (Granlund and Montgomery, 1994, figure 4.1, exact for all):
+// with l = ceil(log2 d), mul is 2^32 (2^l - d) / d + 1, the shifts min(l, 1) and
 // max(l - 1, 0).
+struct Divisor {
+  uint32_t mul, shift1, shift2;
+#ifdef __CUDACC__
+  __device__ __forceinline__ uint32_t of(uint32_t x) const {
+    const uint32_t t = __umulhi(x, mul);
+    return (t + ((x - t) >> shift1)) >> shift2;
+  }
+#endif
+};
+inline Divisor divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < d) ++l;
+  return Divisor{static_cast<uint32_t>(((((uint64_t(1) << l) - d) << 32) / d) + 1), l > 0 ? 1u : 0u, l > 0 ? l - 1 : 0u};
+}
+
+// qwc_paged_cache and qwc_paged_batch as the kernels take them.
 struct PagedArgs {
   const uint8_t* k_scales;
   const uint8_t* k_codes;
@@ -26,7 +41,8 @@ struct PagedArgs {
   const int32_t* query_starts;
   const int32_t* context_lens;
   const int32_t* page_table;
-  uint32_t pages, page_size, page_mul, page_shift1, page_shift2;
+  uint32_t pages, page_size;
+  Divisor by_page;
   uint32_t kv_heads, head_dim;
   uint32_t code_row;   // kv_heads * head_dim bytes
   uint32_t scale_row;  // code_row / 64 * 2 bytes
@@ -50,10 +66,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, uint32_t s) {
                   static_cast<uint32_t>(c)};
 }
 
-__device__ __forceinline__ uint32_t page_of(const PagedArgs& a, uint32_t p) {
-  const uint32_t t = __umulhi(p, a.page_mul);
-  return (t + ((p - t) >> a.page_shift1)) >> a.page_shift2;
-}
+__device__ __forceinline__ uint32_t page_of(const PagedArgs& a, uint32_t p) { return a.by_page.of(p); }
 
 // Row of the pool that holds position p of sequence s, or -1 if its page
 // is not one of the pool's.
@@ -128,8 +141,9 @@ struct AttnArgs {
   float* partials;     // results of stretches that are not a whole segment, two for each CTA
   uint32_t* counters;  // [kMaxAttnCtas][kAttnCounterStride], zero between calls
   int32_t* error;      // set when a bounded wait gave up
-  uint64_t timeout_ns;
-  uint32_t heads, share;
+  uint32_t wait_tries;  // its bound
+  uint32_t heads, share;  // query heads, and those of a kv head
+  Divisor by_share;
   uint32_t group;      // few rows: kv heads of a CTA
   uint32_t pb;         // few rows: position blocks of a step
   uint32_t rows;       // few rows: most rows of a kv head, max_query * share
@@ -144,6 +158,7 @@ constexpr uint64_t kAttnHeadBytes = 256 + kAttnCounters * 4;  // of the workspac
 // Many rows (qwc_paged_tile.cu): 128-row tiles that a CTA takes at once, its grid, its part of the workspace.
 struct TilePlan {
   uint32_t tiles, grid;
+  bool too_long;
   uint64_t partial_bytes;
 };
 TilePlan paged_tile_plan(const PagedArgs& a, uint32_t heads, uint32_t sms);

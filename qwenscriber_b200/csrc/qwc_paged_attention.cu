@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
       for (int ct = 0; ct < NCT; ++ct) {
         const uint32_t row = ct * (8 / PARTS) + r / PARTS;
         const bool in = row < rows;
-        const uint32_t tok = in ? row / p.share : 0, hq = h * p.share + (in ? row % p.share : 0);
+        const uint32_t tok = in ? p.by_share.of(row) : 0, hq = h * p.share + (in ? row - tok * p.share : 0);
         const T* src = static_cast<const T*>(p.q) + size_t(seq.first + tok) * p.q_stride + size_t(hq) * DIM;
         float x[G * 4][4];
         float amax = 0.0f;
@@ -579,7 +579,7 @@ size_t few_smem_bytes(uint32_t rows) {
   return sizeof(FewTile<DIM>) * kFewWarps * kFewStages + kFewWarps * 32 * 8 + size_t(kFewWarps) * rows * (DIM + 4) * 4;
 }
 
-constexpr uint64_t kTimeoutNs = 2000000000ull;
+constexpr uint32_t kWaitTries = 100000;  // tries that sleep up to 20 us each: at most 2 s
 
 // How a call is run: which kernel, its grid, and its part of the workspace.
 struct AttnPlan {
@@ -672,6 +672,7 @@ int32_t qwc_op_paged_attention(const qwc_paged_cache* cache, const qwc_paged_bat
   if ((st = paged_rows_check(out, out_stride, qw, format)) != QWC_OK) return st;
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return QWC_INVALID_ARGUMENT;
   const AttnPlan plan = attention_plan(a, format, heads);
+  if (!plan.few && plan.tile.too_long) return QWC_LIMIT_EXCEEDED;
   if (workspace_bytes < kAttnHeadBytes + plan.partial_bytes) return QWC_LIMIT_EXCEEDED;
   AttnArgs p = {};
   p.q = q;
@@ -679,11 +680,12 @@ int32_t qwc_op_paged_attention(const qwc_paged_cache* cache, const qwc_paged_bat
   p.out = out;
   p.out_stride = out_stride;
   p.error = static_cast<int32_t*>(workspace);
-  p.timeout_ns = kTimeoutNs;
+  p.wait_tries = kWaitTries;
   p.counters = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + 256);
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kAttnHeadBytes);
   p.heads = heads;
   p.share = heads / a.kv_heads;
+  p.by_share = divisor(p.share);
   p.scaling = 1.0f / sqrtf(static_cast<float>(a.head_dim));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return format == kFormatF32   ? attention_as<float>(a, p, plan, s)

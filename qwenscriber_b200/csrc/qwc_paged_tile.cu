@@ -9,9 +9,9 @@
 //   softmax  four warps a tile, one row to a thread: scores from tensor
 //            memory, the causal limit, the running maximum and sum; the weights
 //            go back to tensor memory in place of the scores.
-//   convert  four warps: the step's code rows, fetched through the page table
-//            into registers a step ahead, become f16 in shared memory (keys and
-//            values alike, 128-byte swizzled rows of 64 dims).
+//   convert  the step's code rows, fetched through the page table into registers
+//            a step ahead, become f16 in shared memory (128-byte swizzled rows of
+//            64 dims); half of these warps take the keys, half the values.
 //   MMA      one thread: scores S = Q K^T, output O += P V with the weights
 //            read from tensor memory.
 //
@@ -61,15 +61,19 @@ struct TileConfig {
   static constexpr int PARTS = SPLIT ? 2 : 1;
   static constexpr int SCORES = SCALED ? 1 : G;              // accumulators of 64 columns
   static constexpr int STAGES = TILES == 2 || !SPLIT ? 2 : 1;  // steps of converted keys and values
-  static constexpr int WARPS = 4 * TILES + 5;
+  static constexpr int CONVERT_WARPS = 2 * TILES;            // for the keys, and as many for the values
+  static constexpr int WARPS = 4 * TILES + 2 * CONVERT_WARPS + 1;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr uint32_t TMEM_TILE = G * kStep + DIM;     // columns of a tile: scores, output
+  static constexpr uint32_t SCORE_COLS = SCALED ? 2 * kStep : G * kStep;  // scaled: two steps' scores in turn
+  static constexpr uint32_t TMEM_TILE = SCORE_COLS + DIM;    // columns of a tile: scores, output
+  static constexpr uint32_t TMEM_COLS = TMEM_TILE * TILES <= 128 ? 128 : TMEM_TILE * TILES <= 256 ? 256 : 512;
   // Registers a thread: at launch what fits (65,536 over the resident warps, by quarters of an SM), then the
   // softmax warps take what the convert warps give back.
-  static constexpr int LAUNCH_REGS = TILES == 2 ? 128 : 96;
-  static constexpr int SOFTMAX_REGS = TILES == 2 ? 152 : 128;
-  static constexpr int CONVERT_REGS = TILES == 2 ? 80 : 64;
-  static_assert(4 * TILES * SOFTMAX_REGS + 4 * CONVERT_REGS + LAUNCH_REGS <= WARPS * LAUNCH_REGS, "a split cannot exceed the launch");
+  static constexpr int LAUNCH_REGS = 96;
+  static constexpr int SOFTMAX_REGS = 128;
+  static constexpr int CONVERT_REGS = 64;
+  static_assert(4 * TILES * SOFTMAX_REGS + 2 * CONVERT_WARPS * CONVERT_REGS + LAUNCH_REGS <= WARPS * LAUNCH_REGS,
+                "a split cannot exceed the launch");
   // The weights' power of two, 2^(UP - vexp): weight times value scale below 2^15 (exact), value below 2^7 (scaled).
   static constexpr int UP = SCALED ? 14 : 21;
 };
@@ -79,15 +83,18 @@ struct __align__(1024) TileSmem {
   uint8_t q[C::TILES][C::PARTS][C::G][kRows * 128];  // f16, 128-byte swizzled rows of 64 dims
   uint8_t k[C::STAGES][C::G][kStep * 128];
   uint8_t v[C::STAGES][C::G][kStep * 128];
-  // What the softmax needs to know of a step, for the three steps that may be in hand at once (step n + 3
-  // is converted only after step n's output).
+  // What the softmax needs to know of a step, for the four steps that may be in hand at once (step n + 4's
+  // keys are converted only after step n's weights are made).
   float ks[4][C::G][kStep];  // exact: the key scales
   float vs[4][C::G][kStep];  // and the value scales, times 2^(UP - vexp)
-  uint32_t valid[4][2];      // one bit for each position that is cached
+  uint64_t valid[4];         // one bit for each position that is cached
   uint32_t kexp[4], vexp[4];
-  uint64_t q_full[C::TILES], s_full[C::TILES], p_full[C::TILES], o_full[C::TILES];
+  // Scores and weights by the step's parity: with scores a step ahead, a barrier of one phase could pass two
+  // phases before a late warp looks.
+  uint64_t s_full[2][C::TILES], p_full[2][C::TILES];
+  uint64_t q_full[C::TILES], pv_done[C::TILES], o_full[C::TILES];
   uint64_t k_full[C::STAGES], k_empty[C::STAGES], v_full[C::STAGES], v_empty[C::STAGES];
-  uint64_t scales_full[4];
+  uint64_t ks_full[4], vs_full[4];
   uint64_t sums[C::WARPS];
   uint64_t found_base;
   uint32_t found_s;
@@ -98,31 +105,31 @@ struct __align__(1024) TileSmem {
 struct TileWalk {
   uint32_t s, h, qt;
   uint32_t tiles, steps;  // of the sequence's kv head; of this tile
-  uint64_t first;         // its first step in the line
+  int32_t first;          // its first step, counted from the start of the CTA's stretch
   PagedSeq seq;
 };
 
 template <uint32_t HEIGHT>
-__device__ __forceinline__ uint32_t tiles_of(const PagedSeq& q, uint32_t share) {
-  return (q.n * share + HEIGHT - 1) / HEIGHT;
+__device__ __forceinline__ uint32_t tiles_of(const PagedSeq& q, const AttnArgs& p) {
+  return (q.n * p.share + HEIGHT - 1) / HEIGHT;
 }
 template <uint32_t HEIGHT>
-__device__ __forceinline__ uint32_t tile_steps(const PagedSeq& q, uint32_t share, uint32_t qt) {
-  const uint32_t last = min((qt * HEIGHT + HEIGHT - 1) / share, q.n - 1);
+__device__ __forceinline__ uint32_t tile_steps(const PagedSeq& q, const AttnArgs& p, uint32_t qt) {
+  const uint32_t last = min(p.by_share.of(qt * HEIGHT + HEIGHT - 1), q.n - 1);
   const int32_t seen = min(q.base + static_cast<int32_t>(last) + 1, static_cast<int32_t>(q.context));
   return seen > 0 ? (static_cast<uint32_t>(seen) + kStep - 1) / kStep : 1u;
 }
 template <uint32_t HEIGHT>
-__device__ __forceinline__ uint64_t head_steps(const PagedSeq& q, uint32_t share) {
-  const uint32_t t = tiles_of<HEIGHT>(q, share);
+__device__ __forceinline__ uint64_t head_steps(const PagedSeq& q, const AttnArgs& p) {
+  const uint32_t t = tiles_of<HEIGHT>(q, p);
   uint64_t sum = 0;
-  for (uint32_t i = 0; i < t; ++i) sum += tile_steps<HEIGHT>(q, share, i);
+  for (uint32_t i = 0; i < t; ++i) sum += tile_steps<HEIGHT>(q, p, i);
   return sum;
 }
 
 template <uint32_t HEIGHT>
-__device__ __forceinline__ void next_tile(const PagedArgs& a, uint32_t share, TileWalk& w) {
-  w.first += w.steps;
+__device__ __forceinline__ void next_tile(const PagedArgs& a, const AttnArgs& p, TileWalk& w) {
+  w.first += static_cast<int32_t>(w.steps);
   if (++w.qt == w.tiles) {
     w.qt = 0;
     if (++w.h == a.kv_heads) {
@@ -130,10 +137,10 @@ __device__ __forceinline__ void next_tile(const PagedArgs& a, uint32_t share, Ti
       do {
         w.seq = paged_seq(a, ++w.s);
       } while (w.seq.n == 0 && w.s + 1 < a.sequences);
-      w.tiles = tiles_of<HEIGHT>(w.seq, share);
+      w.tiles = tiles_of<HEIGHT>(w.seq, p);
     }
   }
-  w.steps = tile_steps<HEIGHT>(w.seq, share, w.qt);
+  w.steps = tile_steps<HEIGHT>(w.seq, p, w.qt);
 }
 
 // 16 columns of each of two places in tensor memory (lane quarter of this warp).
@@ -219,31 +226,6 @@ __device__ __forceinline__ void tmem_ld_pairs(uint32_t t0, uint32_t t1, uint64_t
   }
 }
 
-// PER (2 or 4) values of a row, as one load.
-template <int PER>
-__device__ __forceinline__ void load_values(const float* src, float (&x)[PER]) {
-  if constexpr (PER == 4) {
-    const float4 f = *reinterpret_cast<const float4*>(src);
-    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-  } else {
-    const float2 f = *reinterpret_cast<const float2*>(src);
-    x[0] = f.x, x[1] = f.y;
-  }
-}
-template <int PER, typename T>
-__device__ __forceinline__ void load_values(const T* src, float (&x)[PER]) {
-  uint2 w = make_uint2(0, 0);
-  if constexpr (PER == 4) {
-    w = *reinterpret_cast<const uint2*>(src);
-  } else {
-    w.x = *reinterpret_cast<const uint32_t*>(src);
-  }
-  float y[8];
-  unpack16(make_uint4(w.x, w.y, 0, 0), y, T());
-#pragma unroll
-  for (int e = 0; e < PER; ++e) x[e] = y[e];
-}
-
 template <typename T, int DIM, int TILES>
 __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1 ? 2 : 1)
     paged_attention_tile_kernel(const PagedArgs a, const AttnArgs p) {
@@ -251,8 +233,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
   constexpr bool SPLIT = C::SPLIT, SCALED = C::SCALED;
   constexpr int G = C::G, PARTS = C::PARTS, STAGES = C::STAGES, WARPS = C::WARPS;
   constexpr uint32_t HEIGHT = kRows * TILES;
-  constexpr uint32_t kOutput = G * kStep;  // columns of a tile: scores, then output
-  constexpr uint32_t kTmemCols = C::TMEM_TILE * TILES;
+  constexpr uint32_t kOutput = C::SCORE_COLS;  // columns of a tile: scores, then output
   constexpr uint32_t CONVERT = 4 * TILES;  // first convert warp
   using Smem = TileSmem<C>;
   extern __shared__ __align__(1024) uint8_t tile_smem_raw[];
@@ -261,8 +242,12 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
 
   // ---- this CTA's stretch of the line ----
-  uint64_t part = 0;
-  for (uint32_t s = tid; s < a.sequences; s += C::THREADS) part += head_steps<HEIGHT>(paged_seq(a, s), p.share) * a.kv_heads;
+  uint64_t part = 0, mine_steps = 0;  // (of sequence tid: all there is to look up in a batch of fewer sequences than threads)
+  for (uint32_t s = tid; s < a.sequences; s += C::THREADS) {
+    const uint64_t v = head_steps<HEIGHT>(paged_seq(a, s), p) * a.kv_heads;
+    if (s == tid) mine_steps = v;
+    part += v;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
   if (lane == 0) sm->sums[warp] = part;
@@ -275,7 +260,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
   uint64_t running = 0;
   for (uint32_t base = 0; base < a.sequences; base += C::THREADS) {
     const uint32_t s = base + tid;
-    const uint64_t v = s < a.sequences ? head_steps<HEIGHT>(paged_seq(a, s), p.share) * a.kv_heads : 0;
+    const uint64_t v = base == 0 ? mine_steps : s < a.sequences ? head_steps<HEIGHT>(paged_seq(a, s), p) * a.kv_heads : 0;
     uint64_t inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -300,20 +285,26 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
   if (tid == 0) {
     for (int t = 0; t < TILES; ++t) {
       mbar_init(&sm->q_full[t], 4);
-      mbar_init(&sm->s_full[t], 1);
-      mbar_init(&sm->p_full[t], 4);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm->s_full[i][t], 1);
+        mbar_init(&sm->p_full[i][t], 4);
+      }
+      mbar_init(&sm->pv_done[t], 1);
       mbar_init(&sm->o_full[t], 1);
     }
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&sm->k_full[i], 4);
+      mbar_init(&sm->k_full[i], C::CONVERT_WARPS);
       mbar_init(&sm->k_empty[i], 1);
-      mbar_init(&sm->v_full[i], 4);
+      mbar_init(&sm->v_full[i], C::CONVERT_WARPS);
       mbar_init(&sm->v_empty[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&sm->scales_full[i], 4);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sm->ks_full[i], C::CONVERT_WARPS);
+      mbar_init(&sm->vs_full[i], C::CONVERT_WARPS);
+    }
     fence_mbar_init();
   }
-  if (warp == WARPS - 1) tmem_alloc(&sm->tmem, kTmemCols);
+  if (warp == WARPS - 1) tmem_alloc(&sm->tmem, C::TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -322,23 +313,33 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
   {
     walk.s = sm->found_s;
     walk.seq = paged_seq(a, walk.s);
-    walk.tiles = tiles_of<HEIGHT>(walk.seq, p.share);
-    const uint64_t per_head = head_steps<HEIGHT>(walk.seq, p.share);
+    walk.tiles = tiles_of<HEIGHT>(walk.seq, p);
+    const uint64_t per_head = head_steps<HEIGHT>(walk.seq, p);
     uint64_t off = u0 - sm->found_base;
     walk.h = static_cast<uint32_t>(off / per_head);
     off -= walk.h * per_head;
-    walk.first = u0 - off;
     walk.qt = 0;
-    walk.steps = tile_steps<HEIGHT>(walk.seq, p.share, 0);
+    walk.steps = tile_steps<HEIGHT>(walk.seq, p, 0);
     while (off >= walk.steps) {
       off -= walk.steps;
-      walk.first += walk.steps;
-      walk.steps = tile_steps<HEIGHT>(walk.seq, p.share, ++walk.qt);
+      walk.steps = tile_steps<HEIGHT>(walk.seq, p, ++walk.qt);
     }
+    walk.first = -static_cast<int32_t>(off);
   }
+  const uint32_t len = static_cast<uint32_t>(u1 - u0);  // steps of the stretch
   bool ok = true;
-  auto wait = [&](uint64_t* bar, uint32_t n, int32_t code) {  // phase n of a barrier
-    return mbar_wait_bounded(bar, n & 1u, p.error, p.timeout_ns, code);
+  // Phase n of a barrier, bounded: each try sleeps up to 20 us, so the limit of tries is also one of time. (Few
+  // instructions on purpose: there are twenty such waits, and the loops around them have to stay in the
+  // instruction cache.)
+  auto wait = [&](uint64_t* bar, uint32_t n, int32_t code) {
+    uint32_t left = p.wait_tries;
+    while (!mbar_try_wait_sleep(bar, n & 1u, 20000u)) {
+      if (--left == 0) {
+        atomicCAS(p.error, 0, code);
+        return false;
+      }
+    }
+    return true;
   };
 
   if (warp < CONVERT) {
@@ -347,58 +348,71 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     const uint32_t t = warp / 4, trow = tid % kRows;
     const uint32_t taddr = tmem + ((warp % 4 * 32u) << 16) + t * C::TMEM_TILE;
     uint32_t it = 0, seg = 0;
-    for (uint64_t cur = u0; cur < u1 && ok; ++seg) {
-      const uint32_t j0 = static_cast<uint32_t>(cur - walk.first);
-      const uint32_t j1 = static_cast<uint32_t>((u1 < walk.first + walk.steps ? u1 : walk.first + walk.steps) - walk.first);
+    for (uint32_t cur = 0; cur < len && ok; ++seg) {
+      const uint32_t j0 = static_cast<uint32_t>(static_cast<int32_t>(cur) - walk.first);
+      const uint32_t j1 = min(walk.steps, j0 + len - cur);
       const uint32_t rows = walk.seq.n * p.share;
       const uint32_t row = walk.qt * HEIGHT + tid;
       const bool in = row < rows;
-      const uint32_t tok = in ? row / p.share : 0u, head = walk.h * p.share + (in ? row % p.share : 0u);
+      const uint32_t tok = in ? p.by_share.of(row) : 0u;
       const int32_t limit = in ? walk.seq.base + static_cast<int32_t>(tok) : -1;
-      // The warp's 32 rows of queries, a whole row at a time (lane l: dims PER l .. + PER - 1): the largest
-      // value gives the row's power of two, then the f16 parts go to shared memory.
-      constexpr int PER = DIM / 32;
-      constexpr int BATCH = 8;  // rows in flight
+      auto row_at = [&](uint32_t rr) -> size_t {  // of a tensor of rows: the token (times a stride) and the head
+        return walk.seq.first + p.by_share.of(rr);
+      };
+      auto head_at = [&](uint32_t rr) { return walk.h * p.share + (rr - p.by_share.of(rr) * p.share); };
+      // The warp's 32 rows of queries, eight lanes to a row: the largest value gives the row's power of two,
+      // then the f16 parts go to shared memory.
+      constexpr int PER = DIM / 8;                      // values of a lane
+      constexpr int LOADS = PER / Vec16<T>::kCount;     // 16-byte loads of a lane
+      constexpr int AHEAD = 16 / LOADS < 4 ? 16 / LOADS : 4;  // rows of eight lanes in flight
       float factor = 0.0f;
 #pragma unroll 1
-      for (uint32_t r0 = 0; r0 < 32; r0 += BATCH) {
-        float x[BATCH][PER];
+      for (uint32_t r0 = 0; r0 < 32; r0 += 4 * AHEAD) {
+        uint4 raw[AHEAD][LOADS];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const uint32_t rr = row - lane + r0 + i;  // (row - lane: the warp's first row)
-          const T* src = static_cast<const T*>(p.q) + size_t(walk.seq.first + rr / p.share) * p.q_stride +
-                         size_t(walk.h * p.share + rr % p.share) * DIM + PER * lane;
+        for (int i = 0; i < AHEAD; ++i) {
+          const uint32_t rr = row - lane + r0 + 4 * i + lane / 8;  // (row - lane: the warp's first row)
+          const T* src = static_cast<const T*>(p.q) + row_at(rr) * p.q_stride + size_t(head_at(rr)) * DIM + PER * (lane % 8);
 #pragma unroll
-          for (int e = 0; e < PER; ++e) x[i][e] = 0.0f;
-          if (rr < rows) load_values<PER>(src, x[i]);
+          for (int e = 0; e < LOADS; ++e) {
+            raw[i][e] = rr < rows ? reinterpret_cast<const uint4*>(src)[e] : make_uint4(0, 0, 0, 0);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          uint32_t top = 0;
+        for (int i = 0; i < AHEAD; ++i) {
+          float x[LOADS][Vec16<T>::kCount];
+          float top = 0.0f;
 #pragma unroll
-          for (int e = 0; e < PER; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
-          const int e2 = row_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
-          const float down = pow2i(-e2);
-          if (lane == r0 + i) factor = p.scaling * 1.4426950408889634f * pow2i(e2);
-          uint32_t hi[PER / 2], lo[PER / 2];
+          for (int e = 0; e < LOADS; ++e) {
+            unpack16(raw[i][e], x[e], T());
 #pragma unroll
-          for (int e = 0; e < PER / 2; ++e) {
-            const float y0 = fmaf(x[i][2 * e], down, x[i][2 * e] - x[i][2 * e]);  // an infinity is NaN from here on
-            const float y1 = fmaf(x[i][2 * e + 1], down, x[i][2 * e + 1] - x[i][2 * e + 1]);
-            hi[e] = f16x2(y0, y1);
-            const float2 f = f16x2_f32(hi[e]);
-            lo[e] = f16x2(y0 - f.x, y1 - f.y);
+            for (int k = 0; k < Vec16<T>::kCount; ++k) top = fmaxf(top, fabsf(x[e][k]));
           }
-          const uint32_t r = trow - lane + r0 + i, d = PER * lane;
-          const uint32_t at = r * 128u + ((((d % 64) / 8) ^ (r & 7u)) << 4) + (d % 8) * 2;
-          uint8_t* dst = &sm->q[t][0][d / 64][at];
-          uint8_t* dst_lo = &sm->q[t][PARTS - 1][d / 64][at];
-          if constexpr (PER == 4) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-            if constexpr (SPLIT) *reinterpret_cast<uint2*>(dst_lo) = make_uint2(lo[0], lo[1]);
-          } else {
-            *reinterpret_cast<uint32_t*>(dst) = hi[0];
-            if constexpr (SPLIT) *reinterpret_cast<uint32_t*>(dst_lo) = lo[0];
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          const int e2 = row_exponent(top);
+          const float down = pow2i(-e2);
+          // The thread that owns the row takes its factor.
+          const float f = __shfl_sync(0xffffffffu, p.scaling * 1.4426950408889634f * pow2i(e2), (lane % 4) * 8);
+          if (lane / 4 == r0 / 4 + i) factor = f;
+          const uint32_t r = trow - lane + r0 + 4 * i + lane / 8, d = PER * (lane % 8);
+          uint8_t* dst = &sm->q[t][0][d / 64][r * 128u];
+          uint8_t* dst_lo = &sm->q[t][PARTS - 1][d / 64][r * 128u];
+#pragma unroll
+          for (int e = 0; e < PER; e += 8) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float a0 = (&x[0][0])[e + 2 * k], a1 = (&x[0][0])[e + 2 * k + 1];
+              const float y0 = fmaf(a0, down, a0 - a0), y1 = fmaf(a1, down, a1 - a1);  // an infinity is NaN from here on
+              hi[k] = f16x2(y0, y1);
+              const float2 h = f16x2_f32(hi[k]);
+              lo[k] = f16x2(y0 - h.x, y1 - h.y);
+            }
+            const uint32_t at = (((d % 64 + e) / 8) ^ (r & 7u)) << 4;
+            *reinterpret_cast<uint4*>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (SPLIT) *reinterpret_cast<uint4*>(dst_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
         }
       }
@@ -411,15 +425,17 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       uint32_t vexp = 0;
       for (uint32_t j = j0; j < j1; ++j, ++it) {
         const uint32_t b = it & 3u;
-        ok = __all_sync(0xffffffffu, wait(&sm->scales_full[b], it >> 2, 210) && wait(&sm->s_full[t], it, 201));
+        ok = __all_sync(0xffffffffu, wait(&sm->ks_full[b], it >> 2, 210) && wait(&sm->s_full[it & 1u][t], it >> 1, 201) &&
+                                            wait(&sm->vs_full[b], it >> 2, 211));
         if (!ok) break;
         tc_fence_after();
+        const uint32_t scol = taddr + (SCALED ? (it & 1u) * kStep : 0u);
         uint64_t x[kStep / 2];
 #pragma unroll
         for (int i = 0; i < static_cast<int>(kStep); i += 32 / C::SCORES) {
           // Both groups' sums of 16 positions, or the one sum of 32.
           uint64_t s0[8], s1[8];
-          tmem_ld_pairs(taddr + i, taddr + i + (C::SCORES == 2 ? kStep : 16u), s0, s1);
+          tmem_ld_pairs(scol + i, scol + i + (C::SCORES == 2 ? kStep : 16u), s0, s1);
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             if constexpr (SCALED) {
@@ -439,26 +455,24 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           }
         }
         const int32_t pos0 = static_cast<int32_t>(j * kStep);
-        const uint32_t v0 = sm->valid[b][0], v1 = sm->valid[b][1];
-        if (pos0 + static_cast<int32_t>(kStep) - 1 > limit || (v0 & v1) != 0xFFFFFFFFu) {
+        uint64_t seen = sm->valid[b];
+        if (pos0 + static_cast<int32_t>(kStep) - 1 > limit) seen &= limit < pos0 ? 0ull : (2ull << (limit - pos0)) - 1;
+        if (seen != ~0ull) {
 #pragma unroll
           for (int i = 0; i < static_cast<int>(kStep); i += 2) {
-            float2 f = unpack2(x[i / 2]);
-            const uint32_t bits = (i < 32 ? v0 : v1) >> (i % 32);
-            if (pos0 + i > limit || !(bits & 1u)) f.x = -INFINITY;
-            if (pos0 + i + 1 > limit || !(bits & 2u)) f.y = -INFINITY;
-            x[i / 2] = pack2(f.x, f.y);
+            const uint32_t bits = static_cast<uint32_t>(i < 32 ? seen : seen >> 32);
+            const float2 f = unpack2(x[i / 2]);
+            x[i / 2] = pack2((bits & (1u << (i % 32))) ? f.x : -INFINITY, (bits & (2u << (i % 32))) ? f.y : -INFINITY);
           }
         }
-        float mx = -INFINITY, my = -INFINITY;
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(kStep) / 2; i += 2) {
-          const float2 f0 = unpack2(x[i]), f1 = unpack2(x[i + 1]);
-          mx = fmaxf(mx, fmaxf(f0.x, f0.y));
-          my = fmaxf(my, fmaxf(f1.x, f1.y));
+        for (int i = 0; i < static_cast<int>(kStep) / 2; ++i) {
+          const float2 f = unpack2(x[i]);
+          mx4[i % 4] = fmaxf(fmaxf(mx4[i % 4], f.x), f.y);
         }
         const float step_factor = SCALED ? factor * pow2i(static_cast<int>(sm->kexp[b]) - 14) : factor;
-        mx = fmaxf(mx, my) * step_factor;
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * step_factor;
         float rescale = 1.0f;
         bool grew = false;
         if (mx - m > static_cast<float>(kGrowth) || (m == -INFINITY && mx > m)) {
@@ -474,8 +488,11 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           grew = true;
         }
         if (j > j0 && __any_sync(0xffffffffu, grew)) {
-          // The MMAs behind s_full are the last step's too: its output is complete.
-#pragma unroll
+          // The last step's output must be complete. (The one before it is: its MMAs came before this step's scores.)
+          ok = __all_sync(0xffffffffu, wait(&sm->pv_done[t], it - 1, 212));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
           for (int i = 0; i < DIM; i += 32) {
             float o0[16], o1[16];
             tmem_ld16x2(taddr + kOutput + i, taddr + kOutput + i + 16, o0, o1);
@@ -524,14 +541,14 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
                 lo[e / 2 + 1] = f16x2(a1.x - r1.x, a1.y - r1.y);
               }
             }
-            tmem_st16(taddr + 32 * g + i / 2, hi);
-            if constexpr (SPLIT) tmem_st16(taddr + 32 * (G + g) + i / 2, lo);
+            tmem_st16(scol + 32 * g + i / 2, hi);
+            if constexpr (SPLIT) tmem_st16(scol + 32 * (G + g) + i / 2, lo);
           }
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm->p_full[t]);
+        if (lane == 0) mbar_arrive(&sm->p_full[it & 1u][t]);
       }
       if (!ok) break;
 
@@ -540,40 +557,68 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       if (!ok) break;
       tc_fence_after();
       const float back = pow2i(static_cast<int>(vexp) - C::UP);
-      T* dst = static_cast<T*>(p.out) + size_t(walk.seq.first + tok) * p.out_stride + size_t(head) * DIM;
       const bool whole = j0 == 0 && j1 == walk.steps;
-      const uint32_t slot = 2 * blockIdx.x + (walk.first > u0 ? 1u : 0u);
-      // A partial: [DIM / 4][HEIGHT] of four dims, then maxima and sums.
-      float* mine = p.partials + size_t(slot) * (DIM + 2) * HEIGHT;
-      const float inv = whole ? (l == 0.0f ? 0.0f : back / l) : back;
+      // Finished rows go through shared memory (the tile's queries are done with) and leave a row at a time.
+      constexpr int W = Vec16<T>::kCount;
+      constexpr int ROW_CHUNKS = DIM / W;
+      uint8_t* const stage = &sm->q[t][0][0][0];
+      static_assert(sizeof(sm->q[0]) == size_t(kRows) * DIM * sizeof(T), "the queries' room holds the tile's output");
+      auto put_row = [&](int i, const float (&o)[32]) {
 #pragma unroll
-      for (int i = 0; i < DIM; i += 32) {
-        float o[32];
-        tmem_ld32(taddr + kOutput + i, o);
+        for (int e = 0; e < 32; e += W) {
+          float y[W];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * inv;
-        if (!whole) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            reinterpret_cast<float4*>(mine)[size_t((i + e) / 4) * HEIGHT + tid] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-        } else if (in) {
-          constexpr int W = Vec16<T>::kCount;
-#pragma unroll
-          for (int e = 0; e < 32; e += W) {
-            float y[W];
-#pragma unroll
-            for (int q = 0; q < W; ++q) y[q] = o[e + q];
-            *reinterpret_cast<uint4*>(dst + i + e) = pack16<T>(y);
+          for (int q = 0; q < W; ++q) y[q] = o[e + q];
+          const uint32_t chunk = (i + e) / W;
+          *reinterpret_cast<uint4*>(stage + (chunk / 8) * (kRows * 128) + trow * 128u + (((chunk % 8) ^ (trow & 7u)) << 4)) = pack16<T>(y);
+        }
+      };
+      auto write_rows = [&]() {
+        __syncwarp();
+        constexpr uint32_t AT_ONCE = 32 / ROW_CHUNKS;  // rows of an instruction
+#pragma unroll 4
+        for (uint32_t r0 = 0; r0 < 32; r0 += AT_ONCE) {
+          const uint32_t r = r0 + lane / ROW_CHUNKS, chunk = lane % ROW_CHUNKS;
+          const uint32_t rr = row - lane + r, tr = trow - lane + r;
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + (chunk / 8) * (kRows * 128) + tr * 128u + (((chunk % 8) ^ (tr & 7u)) << 4));
+          if (rr < rows) {
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row_at(rr) * p.out_stride + size_t(head_at(rr)) * DIM + W * chunk) = v;
           }
         }
-      }
-      if (!whole) {
+        __syncwarp();
+      };
+      if (whole) {
+        const float inv = l == 0.0f ? 0.0f : back / l;
+#pragma unroll 1
+        for (int i = 0; i < DIM; i += 32) {
+          float o[32];
+          tmem_ld32(taddr + kOutput + i, o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * inv;
+          put_row(i, o);
+        }
+        write_rows();
+      } else {
+        // A partial: [DIM / 4][HEIGHT] of four dims, then maxima and sums. In the slots of stretch x: 2 x for the tile
+        // that the stretch begins with, 2 x + 1 for the one that it ends with.
+        auto slot = [&](uint32_t i) { return p.partials + size_t(i) * (DIM + 2) * HEIGHT; };
+        float* mine = slot(2 * blockIdx.x + (walk.first > 0 ? 1u : 0u));
+#pragma unroll 1
+        for (int i = 0; i < DIM; i += 32) {
+          float o[32];
+          tmem_ld32(taddr + kOutput + i, o);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float k = l == 0.0f ? 0.0f : 1.0f;  // (l == 0: nothing seen, and the columns may hold anything)
+            reinterpret_cast<float4*>(mine)[size_t((i + e) / 4) * HEIGHT + tid] =
+                k == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o[e] * back, o[e + 1] * back, o[e + 2] * back, o[e + 3] * back);
+          }
+        }
         mine[size_t(DIM) * HEIGHT + tid] = m;
         mine[size_t(DIM + 1) * HEIGHT + tid] = l;
         // The stretches that hold this tile: c0 .. c1 (stretch x starts at
         // floor(x * total / grid)). Each warp joins its 32 rows by itself.
-        const uint64_t seg0 = walk.first, seg1 = walk.first + walk.steps;
+        const uint64_t seg0 = u0 + static_cast<int64_t>(walk.first), seg1 = seg0 + walk.steps;
         const uint32_t c0 = static_cast<uint32_t>(((seg0 + 1) * grid - 1) / total);
         const uint32_t c1 = static_cast<uint32_t>((seg1 * grid - 1) / total);
         __threadfence();
@@ -588,15 +633,13 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         last = __shfl_sync(0xffffffffu, last, 0);
         if (last) {
           __threadfence();
-          auto piece = [&](uint32_t x) {
-            const uint32_t sl = 2 * x + (seg0 > total * x / grid ? 1u : 0u);
-            return p.partials + size_t(sl) * (DIM + 2) * HEIGHT;
-          };
+          const float* first = slot(2 * c0 + (seg0 > total * c0 / grid ? 1u : 0u));
+          auto piece = [&](uint32_t x) -> const float* { return x == c0 ? first : slot(2 * x); };
+          constexpr uint32_t kMax = DIM * HEIGHT, kSum = (DIM + 1) * HEIGHT;
           float best = -INFINITY, sum = 0.0f;
-          for (uint32_t x = c0; x <= c1; ++x) best = fmaxf(best, __ldcg(piece(x) + size_t(DIM) * HEIGHT + tid));
+          for (uint32_t x = c0; x <= c1; ++x) best = fmaxf(best, __ldcg(piece(x) + kMax + tid));
           for (uint32_t x = c0; x <= c1; ++x) {
-            const float pm = __ldcg(piece(x) + size_t(DIM) * HEIGHT + tid);
-            sum = fmaf(__ldcg(piece(x) + size_t(DIM + 1) * HEIGHT + tid), best == -INFINITY ? 1.0f : ex2(pm - best), sum);
+            sum = fmaf(__ldcg(piece(x) + kSum + tid), best == -INFINITY ? 1.0f : ex2(__ldcg(piece(x) + kMax + tid) - best), sum);
           }
           const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
@@ -604,201 +647,180 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
             float o[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+            // Two pieces' loads in flight.
 #pragma unroll 1
-            for (uint32_t x = c0; x <= c1; ++x) {
-              const float* from = piece(x);
-              const float pm = __ldcg(from + size_t(DIM) * HEIGHT + tid);
-              float4 v[8];
+            for (uint32_t x0 = c0; x0 <= c1; x0 += 2) {
+              float4 v[2][8];
+              float f[2];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = __ldcg(reinterpret_cast<const float4*>(from) + size_t(i / 4 + e) * HEIGHT + tid);
-              const float f = (best == -INFINITY ? 1.0f : ex2(pm - best)) * norm;
+              for (int w = 0; w < 2; ++w) {
+                const float* from = piece(min(x0 + w, c1));
+                f[w] = __ldcg(from + kMax + tid);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                o[4 * e] = fmaf(v[e].x, f, o[4 * e]);
-                o[4 * e + 1] = fmaf(v[e].y, f, o[4 * e + 1]);
-                o[4 * e + 2] = fmaf(v[e].z, f, o[4 * e + 2]);
-                o[4 * e + 3] = fmaf(v[e].w, f, o[4 * e + 3]);
+                for (int e = 0; e < 8; ++e) v[w][e] = __ldcg(reinterpret_cast<const float4*>(from) + size_t(i / 4 + e) * HEIGHT + tid);
+              }
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                if (x0 + w > c1) break;
+                const float k = (best == -INFINITY ? 1.0f : ex2(f[w] - best)) * norm;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  o[4 * e] = fmaf(v[w][e].x, k, o[4 * e]);
+                  o[4 * e + 1] = fmaf(v[w][e].y, k, o[4 * e + 1]);
+                  o[4 * e + 2] = fmaf(v[w][e].z, k, o[4 * e + 2]);
+                  o[4 * e + 3] = fmaf(v[w][e].w, k, o[4 * e + 3]);
+                }
               }
             }
-            if (in) {
-              constexpr int W = Vec16<T>::kCount;
-#pragma unroll
-              for (int e = 0; e < 32; e += W) {
-                float y[W];
-#pragma unroll
-                for (int q = 0; q < W; ++q) y[q] = o[e + q];
-                *reinterpret_cast<uint4*>(dst + i + e) = pack16<T>(y);
-              }
-            }
+            put_row(i, o);
           }
+          write_rows();
         }
       }
       tc_fence_before();  // the output's columns may be written again once the next weights arrive
-      cur = walk.first + j1;
-      if (cur < u1) next_tile<HEIGHT>(a, p.share, walk);
+      cur += j1 - j0;
+      if (cur < len) next_tile<HEIGHT>(a, p, walk);
     }
-  } else if (warp < CONVERT + 4) {
+  } else if (warp < WARPS - 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::CONVERT_REGS));
-    // ---- convert: keys, then values, of each step ----
-    const uint32_t cw = warp - CONVERT, ct = tid - 32 * CONVERT;
-    constexpr uint32_t CH = DIM / 16;              // 16-byte chunks of a row of codes
-    constexpr uint32_t ROWS_PASS = 128 / CH;       // rows that the 128 threads fetch at once
-    constexpr uint32_t PASSES = kStep / ROWS_PASS;
-    const uint32_t ch = ct % CH, r0 = ct / CH;
-    uint32_t it = 0;
-    uint32_t vexp = 0;
-    // A step ahead: its code chunks, and its scales (lane l: positions l and 32 + l).
-    uint4 kraw[PASSES], vraw[PASSES];
-    TileWalk ahead = walk;
-    uint32_t aj = static_cast<uint32_t>(u0 - walk.first);
-    // Rows of the pool of that step's positions 32 e + lane (-1: not cached): the page table is read
-    // before the step in hand is converted, its answers are used after.
-    int32_t page_id[2], page_at[2], rows[2];
-    auto look_up = [&]() {
+    // ---- convert: half of these warps the keys of each step, half the values ----
+    auto convert = [&](auto is_v) {
+      constexpr bool VALUES = decltype(is_v)::value;
+      constexpr uint32_t CW = C::CONVERT_WARPS;
+      const uint32_t cw = (warp - CONVERT) % CW, ct = cw * 32 + lane;
+      constexpr uint32_t CH = DIM / 16;              // 16-byte chunks of a row of codes
+      constexpr uint32_t ROWS_PASS = 32 * CW / CH;   // rows that the warps fetch at once
+      constexpr uint32_t PASSES = kStep / ROWS_PASS;
+      const uint32_t ch = ct % CH, r0 = ct / CH;
+      const uint8_t* code_plane = VALUES ? a.v_codes : a.k_codes;
+      const uint8_t* scale_plane = VALUES ? a.v_scales : a.k_scales;
+      uint64_t* full = VALUES ? sm->v_full : sm->k_full;
+      uint64_t* empty = VALUES ? sm->v_empty : sm->k_empty;
+      uint8_t* tiles = VALUES ? &sm->v[0][0][0] : &sm->k[0][0][0];
+      // A step ahead: its code chunks and its scales.
+      uint4 raw[PASSES];
+      TileWalk ahead = walk;
+      uint32_t aj = static_cast<uint32_t>(-walk.first);
+      // Rows of the pool of that step's positions 32 e + lane (-1: not cached): the page table is read
+      // before the step in hand is converted, its answers are used after.
+      int32_t page_id[2], page_at[2], rows[2];
+      auto look_up = [&]() {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t pos = aj * kStep + 32u * e + lane;
-        const uint32_t pg = page_of(a, pos);
-        page_at[e] = static_cast<int32_t>(pos - pg * a.page_size);
-        page_id[e] = pos < ahead.seq.context ? __ldg(a.page_table + size_t(ahead.s) * a.table_stride + pg) : -1;
-      }
-    };
-    auto found = [&]() {
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t pos = aj * kStep + 32u * e + lane;
+          const uint32_t pg = page_of(a, pos);
+          page_at[e] = static_cast<int32_t>(pos - pg * a.page_size);
+          page_id[e] = pos < ahead.seq.context ? __ldg(a.page_table + size_t(ahead.s) * a.table_stride + pg) : -1;
+        }
+      };
+      uint32_t scale_raw[2];  // position 32 e + lane: both groups
+      uint32_t valid_bits[2];
+      auto fetch = [&]() {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        rows[e] = static_cast<uint32_t>(page_id[e]) < a.pages ? page_id[e] * static_cast<int32_t>(a.page_size) + page_at[e] : -1;
-      }
-    };
-    auto fetch = [&](uint4 (&raw)[PASSES], const uint8_t* plane) {
-      const uint8_t* from = plane + ahead.h * DIM + 16u * ch;
+        for (int e = 0; e < 2; ++e) {
+          rows[e] = static_cast<uint32_t>(page_id[e]) < a.pages ? page_id[e] * static_cast<int32_t>(a.page_size) + page_at[e] : -1;
+        }
+        const uint8_t* from = code_plane + ahead.h * DIM + 16u * ch;
 #pragma unroll
-      for (uint32_t i = 0; i < PASSES; ++i) {
-        const int32_t row = __shfl_sync(0xffffffffu, rows[i * ROWS_PASS / 32], (r0 + i * ROWS_PASS) % 32);
-        raw[i] = row >= 0 ? ld_nc4(from + uint64_t(static_cast<uint32_t>(row)) * a.code_row) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    uint32_t scale_raw[2][2];  // [key, value][position 32 e + lane]: both groups
-    uint32_t valid_bits[2];
-    auto fetch_scales = [&]() {
+        for (uint32_t i = 0; i < PASSES; ++i) {
+          const int32_t row = __shfl_sync(0xffffffffu, rows[i * ROWS_PASS / 32], (r0 + i * ROWS_PASS) % 32);
+          raw[i] = row >= 0 ? ld_nc4(from + uint64_t(static_cast<uint32_t>(row)) * a.code_row) : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        valid_bits[e] = __ballot_sync(0xffffffffu, rows[e] >= 0);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          scale_raw[n][e] = 0;
+        for (int e = 0; e < 2; ++e) {
+          valid_bits[e] = __ballot_sync(0xffffffffu, rows[e] >= 0);
+          scale_raw[e] = 0;
           if (rows[e] >= 0) {
-            const uint8_t* from = (n ? a.v_scales : a.k_scales) + uint64_t(static_cast<uint32_t>(rows[e])) * a.scale_row + ahead.h * (2 * G);
-            scale_raw[n][e] = G == 2 ? *reinterpret_cast<const uint32_t*>(from) : *reinterpret_cast<const uint16_t*>(from);
+            const uint8_t* at = scale_plane + uint64_t(static_cast<uint32_t>(rows[e])) * a.scale_row + ahead.h * (2 * G);
+            scale_raw[e] = G == 2 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
           }
         }
-      }
-    };
-    auto put = [&](uint8_t* tile, const uint4 (&raw)[PASSES], const uint32_t (&mul)[PASSES]) {
-      // Chunk ch is dims 16 ch .. + 15: two 16-byte chunks of f16 in group ch / 4's tile.
-      uint8_t* base = tile + (ch / 4) * (kStep * 128);
-      const uint32_t c2 = 2 * (ch % 4), flip = ch / 4;  // the two groups' lanes on different banks
-#pragma unroll
-      for (uint32_t i = 0; i < PASSES; ++i) {
-        const uint32_t r = r0 + i * ROWS_PASS;
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        uint32_t h[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[2 * e] = codes_f16x2<0x4140>(w[e]);
-          h[2 * e + 1] = codes_f16x2<0x4342>(w[e]);
+      };
+      look_up();
+      fetch();
+      uint32_t top = 0;  // values: the largest exponent field of a scale of the tile so far; keys: of the step
+      uint32_t it = 0;
+      for (; it < len; ++it) {
+        const uint32_t b = it & 3u, st = it % STAGES, use = it / STAGES;
+        if (!VALUES || aj == 0) top = 0;  // (aj: still the step in hand)
+        // The place of the step after this one.
+        const bool more = it + 1 < len;
+        if (more) {
+          if (++aj == ahead.steps) {
+            next_tile<HEIGHT>(a, p, ahead);
+            aj = 0;
+          }
+          look_up();
         }
-        if constexpr (SCALED) {
+        if (it >= STAGES) ok = __all_sync(0xffffffffu, wait(&empty[st], use - 1, VALUES ? 204 : 203));
+        if (!ok) break;
+        // Every warp finds the largest exponent for itself.
+        int up = 0;
+        if (VALUES || SCALED) {
+          uint32_t e = 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(mul[i]));
+          for (int n = 0; n < 2; ++n) e = max(e, max((scale_raw[n] >> 10) & 31u, (scale_raw[n] >> 26) & 31u));
+          top = max(top, min(__reduce_max_sync(0xffffffffu, e), 30u));
+          up = (VALUES ? C::UP : 14) - static_cast<int>(top);
         }
-        const uint4 o0 = make_uint4(h[0], h[1], h[2], h[3]), o1 = make_uint4(h[4], h[5], h[6], h[7]);
-        *reinterpret_cast<uint4*>(base + r * 128u + (((c2 + flip) ^ (r & 7u)) << 4)) = flip ? o1 : o0;
-        *reinterpret_cast<uint4*>(base + r * 128u + (((c2 + 1 - flip) ^ (r & 7u)) << 4)) = flip ? o0 : o1;
-      }
-    };
-    // Scaled: the scales of this thread's rows, times 2^up, as f16 pairs.
-    auto row_scales = [&](uint32_t (&mul)[PASSES], const uint32_t (&raw)[2], int up) {
+        const float up2 = pow2i(up);
+        // Chunk ch is dims 16 ch .. + 15: two 16-byte chunks of f16 in group ch / 4's tile.
+        uint8_t* base = tiles + (st * G + ch / 4) * (kStep * 128);
+        const uint32_t c2 = 2 * (ch % 4), flip = ch / 4;  // the two groups' lanes on different banks
 #pragma unroll
-      for (uint32_t i = 0; i < PASSES; ++i) {
-        mul[i] = 0;
-        if constexpr (SCALED) {
-          const uint32_t both = __shfl_sync(0xffffffffu, raw[i * ROWS_PASS / 32], (r0 + i * ROWS_PASS) % 32);
-          const float f = f16_bits_to_f32(ch >= 4 ? both >> 16 : both & 0xFFFFu) * pow2i(up);
-          mul[i] = f16x2(f, f);
-        }
-      }
-    };
-    auto top_exponent = [&](const uint32_t (&raw)[2]) {
-      uint32_t e = 0;
+        for (uint32_t i = 0; i < PASSES; ++i) {
+          const uint32_t r = r0 + i * ROWS_PASS;
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t h[8];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) e = max(e, max((raw[n] >> 10) & 31u, (raw[n] >> 26) & 31u));
-      return min(__reduce_max_sync(0xffffffffu, e), 30u);
-    };
-    look_up();
-    found();
-    fetch(kraw, a.k_codes);
-    fetch_scales();
-    fetch(vraw, a.v_codes);
-    for (uint64_t cur = u0; cur < u1; ++cur, ++it) {
-      const uint32_t b = it & 3u, st = it % STAGES, use = it / STAGES;
-      if (cur >= walk.first + walk.steps) next_tile<HEIGHT>(a, p.share, walk);
-      if (cur == walk.first) vexp = 0;
-      // The place of the step after this one.
-      const bool more = cur + 1 < u1;
-      if (more) {
-        if (++aj == ahead.steps) {
-          next_tile<HEIGHT>(a, p.share, ahead);
-          aj = 0;
+          for (int e = 0; e < 4; ++e) {
+            h[2 * e] = codes_f16x2<0x4140>(w[e]);
+            h[2 * e + 1] = codes_f16x2<0x4342>(w[e]);
+          }
+          if constexpr (SCALED) {
+            const uint32_t both = __shfl_sync(0xffffffffu, scale_raw[i * ROWS_PASS / 32], r % 32);
+            const float f = f16_bits_to_f32(ch >= 4 ? both >> 16 : both & 0xFFFFu) * up2;
+            const uint32_t f2 = f16x2(f, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(f2));
+          }
+          const uint4 o0 = make_uint4(h[0], h[1], h[2], h[3]), o1 = make_uint4(h[4], h[5], h[6], h[7]);
+          *reinterpret_cast<uint4*>(base + r * 128u + (((c2 + flip) ^ (r & 7u)) << 4)) = flip ? o1 : o0;
+          *reinterpret_cast<uint4*>(base + r * 128u + (((c2 + 1 - flip) ^ (r & 7u)) << 4)) = flip ? o0 : o1;
         }
-        look_up();
-      }
-      if (it >= STAGES) ok = __all_sync(0xffffffffu, wait(&sm->k_empty[st], use - 1, 203));
-      if (!ok) break;
-      uint32_t mul[PASSES];
-      const uint32_t kexp = SCALED ? top_exponent(scale_raw[0]) : 14u;
-      row_scales(mul, scale_raw[0], 14 - static_cast<int>(kexp));
-      put(&sm->k[st][0][0], kraw, mul);
-      // Every warp finds the largest exponent of the value scales; each writes 16 positions' scales.
-      vexp = max(vexp, top_exponent(scale_raw[1]));
-      row_scales(mul, scale_raw[1], C::UP - static_cast<int>(vexp));
-      if constexpr (!SCALED) {
-        const float up = pow2i(C::UP - static_cast<int>(vexp));
-        const uint32_t half = cw / 2;
-        if (lane / 16 == (cw & 1u)) {
-          const float2 kf = f16x2_f32(half ? scale_raw[0][1] : scale_raw[0][0]), vf = f16x2_f32(half ? scale_raw[1][1] : scale_raw[1][0]);
-          const uint32_t at = 32u * half + lane;
-          sm->ks[b][0][at] = kf.x;
-          sm->vs[b][0][at] = vf.x * up;
-          if constexpr (G == 2) {
-            sm->ks[b][G - 1][at] = kf.y;
-            sm->vs[b][G - 1][at] = vf.y * up;
+        if constexpr (!SCALED) {
+          // Each warp writes its share of the positions' scales.
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t pos = 32u * e + lane;
+            if (pos / (kStep / CW) != cw) continue;
+            const float2 f = f16x2_f32(scale_raw[e]);
+            float* dst = VALUES ? &sm->vs[b][0][pos] : &sm->ks[b][0][pos];
+            dst[0] = f.x * up2;
+            if constexpr (G == 2) dst[kStep] = f.y * up2;
           }
         }
+        if (cw == 0 && lane == 0) {
+          if constexpr (VALUES) {
+            sm->vexp[b] = top;
+          } else {
+            sm->valid[b] = valid_bits[0] | uint64_t(valid_bits[1]) << 32;
+            sm->kexp[b] = top;
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&full[st]);
+          mbar_arrive(VALUES ? &sm->vs_full[b] : &sm->ks_full[b]);
+        }
+        if (more) fetch();
       }
-      if (cw == 0 && lane == 0) {
-        sm->valid[b][0] = valid_bits[0];
-        sm->valid[b][1] = valid_bits[1];
-        sm->vexp[b] = vexp;
-        sm->kexp[b] = kexp;
-      }
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm->k_full[st]);
-        mbar_arrive(&sm->scales_full[b]);
-      }
-      if (more) {
-        found();
-        fetch(kraw, a.k_codes);
-        fetch_scales();
-      }
-      if (it >= STAGES) ok = __all_sync(0xffffffffu, wait(&sm->v_empty[st], use - 1, 204));
-      if (!ok) break;
-      put(&sm->v[st][0][0], vraw, mul);
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm->v_full[st]);
-      if (more) fetch(vraw, a.v_codes);
+    };
+    if (warp < CONVERT + C::CONVERT_WARPS) {
+      convert(std::false_type());
+    } else {
+      convert(std::true_type());
     }
   } else {
     // ---- MMAs: the whole warp walks, one lane issues ----
@@ -810,7 +832,8 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     const uint64_t v0 = umma_desc(smem_addr(sm->v[0][0]), 16, 1024, kLayoutSw128);
     constexpr uint32_t kQTile = kRows * 128 / 16, kKvTile = kStep * 128 / 16;  // in a descriptor's units
     auto wait_all = [&](uint64_t* bar, uint32_t n, int32_t code) { return __all_sync(0xffffffffu, wait(bar, n, code)) != 0; };
-    auto scores = [&](uint32_t t, uint32_t st) {
+    auto scores = [&](uint32_t t, uint32_t n) {  // of step n
+      const uint32_t st = n % STAGES;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const uint64_t kd = k0 + (st * G + g) * kKvTile;
@@ -819,13 +842,14 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           const uint64_t qd = q0 + ((t * PARTS + q) * G + g) * kQTile;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // 16 dims: 32 bytes of each row
-            mma_ss(base + t * C::TMEM_TILE + (SCALED ? 0 : g * kStep), qd + 2 * kk, kd + 2 * kk, kIdescScores,
+            mma_ss(base + t * C::TMEM_TILE + (SCALED ? (n & 1u) * kStep : g * kStep), qd + 2 * kk, kd + 2 * kk, kIdescScores,
                    (SCALED && g > 0) || q > 0 || kk > 0);
           }
         }
       }
     };
-    auto output = [&](uint32_t t, uint32_t st, bool first) {
+    auto output = [&](uint32_t t, uint32_t n, bool first) {
+      const uint32_t st = n % STAGES;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const uint64_t vd = v0 + (st * G + g) * kKvTile;
@@ -834,56 +858,61 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // 16 positions: 16 rows of 128 bytes
             mma_ts(base + t * C::TMEM_TILE + kOutput + 64 * g,
-                   base + t * C::TMEM_TILE + (SCALED ? 0 : 32 * (q * G + g)) + 8 * kk, vd + 128 * kk, kIdescOutput,
+                   base + t * C::TMEM_TILE + (SCALED ? (n & 1u) * kStep : 32 * (q * G + g)) + 8 * kk, vd + 128 * kk, kIdescOutput,
                    !first || q > 0 || kk > 0);
           }
         }
       }
     };
-    for (uint64_t cur = u0; cur < u1 && ok; ++seg) {
-      const uint32_t j0 = static_cast<uint32_t>(cur - walk.first);
-      const uint32_t j1 = static_cast<uint32_t>((u1 < walk.first + walk.steps ? u1 : walk.first + walk.steps) - walk.first);
+    for (uint32_t cur = 0; cur < len && ok; ++seg) {
+      const uint32_t j0 = static_cast<uint32_t>(static_cast<int32_t>(cur) - walk.first);
+      const uint32_t j1 = min(walk.steps, j0 + len - cur);
       for (int t = 0; t < TILES && ok; ++t) ok = wait_all(&sm->q_full[t], seg, 205);
-      // Step j's scores are issued behind step j - 1's output, tile by tile: the weights lie in the
-      // scores' columns. MMAs of one thread run in order.
-      for (uint32_t j = j0; j <= j1 && ok; ++j) {
-        const uint32_t st = it % STAGES, prev = (it + STAGES - 1) % STAGES;
-        if (j < j1) ok = wait_all(&sm->k_full[st], it / STAGES, 206);
-        if (ok && j > j0) ok = wait_all(&sm->v_full[prev], (it - 1) / STAGES, 207);
-        for (int t = 0; t < TILES && ok; ++t) {
-          if (j > j0) {
-            ok = wait_all(&sm->p_full[t], it - 1, 208);
-            if (!ok) break;
-            tc_fence_after();
-            output(t, prev, j == j0 + 1);
-            if (t == TILES - 1) mma_commit(&sm->v_empty[prev]);
-            if (j == j1) mma_commit(&sm->o_full[t]);
-          }
-          if (j < j1) {
-            tc_fence_after();
-            scores(t, st);
-            mma_commit(&sm->s_full[t]);
-            waiting = true;
-            if (t == TILES - 1) mma_commit(&sm->k_empty[st]);
-          }
+      // Exact: step n's scores are issued behind step n - 1's output, tile by tile, as the weights lie in the
+      // scores' columns. Scaled: they have columns of their own, and are issued before step n - 1's
+      // weights are made. MMAs of one thread run in order.
+      auto issue_scores = [&](uint32_t t, uint32_t n) {
+        tc_fence_after();
+        scores(t, n);
+        mma_commit(&sm->s_full[n & 1u][t]);
+        waiting = true;
+        if (t == TILES - 1) mma_commit(&sm->k_empty[n % STAGES]);
+      };
+      ok = ok && wait_all(&sm->k_full[it % STAGES], it / STAGES, 206);
+      for (int t = 0; t < TILES && ok; ++t) issue_scores(t, it);
+      for (uint32_t j = j0; j < j1 && ok; ++j, ++it) {
+        const bool more = j + 1 < j1;
+        if (more) ok = wait_all(&sm->k_full[(it + 1) % STAGES], (it + 1) / STAGES, 206);
+        if (SCALED && more && ok) {
+          for (int t = 0; t < TILES; ++t) issue_scores(t, it + 1);
         }
-        if (j < j1) ++it;
+        if (ok) ok = wait_all(&sm->v_full[it % STAGES], it / STAGES, 207);
+        for (int t = 0; t < TILES && ok; ++t) {
+          ok = wait_all(&sm->p_full[it & 1u][t], it >> 1, 208);
+          if (!ok) break;
+          tc_fence_after();
+          output(t, it, j == j0);
+          mma_commit(&sm->pv_done[t]);
+          if (!more) mma_commit(&sm->o_full[t]);
+          if (t == TILES - 1) mma_commit(&sm->v_empty[it % STAGES]);
+          if (!SCALED && more) issue_scores(t, it + 1);
+        }
       }
       if (ok) {
-        cur = walk.first + j1;
-        if (cur < u1) next_tile<HEIGHT>(a, p.share, walk);
+        cur += j1 - j0;
+        if (cur < len) next_tile<HEIGHT>(a, p, walk);
       }
     }
     if (!ok && waiting) {  // MMAs in flight end before tensor memory is freed
       mma_commit(&sm->o_full[0]);
-      mbar_wait_bounded(&sm->o_full[0], seg & 1u, p.error, p.timeout_ns, 209);
+      wait(&sm->o_full[0], seg, 209);
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == WARPS - 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    tmem_dealloc(tmem, C::TMEM_COLS);
   }
 }
 
@@ -916,6 +945,7 @@ TilePlan paged_tile_plan(const PagedArgs& a, uint32_t heads, uint32_t sms) {
   const uint64_t steps = uint64_t(a.sequences) * a.kv_heads * ((rows + height - 1) / height) *
                          (a.max_context ? (a.max_context + kStep - 1) / kStep : 1);
   const uint64_t most = plan.tiles == 2 ? sms : 2 * sms;  // what is resident at once
+  plan.too_long = steps / most >= 0x7FFFFFFFu;            // a stretch's steps are counted in 31 bits
   plan.grid = static_cast<uint32_t>(steps < most ? steps : most);
   plan.partial_bytes = uint64_t(2) * plan.grid * (a.head_dim + 2) * height * 4;
   return plan;

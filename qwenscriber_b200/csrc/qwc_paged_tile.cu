@@ -51,6 +51,9 @@ namespace {
 constexpr uint32_t kRows = 128;   // rows of a tile
 constexpr uint32_t kStep = 64;    // positions of a step
 constexpr uint32_t kGrowth = 8;   // log2 of how far a maximum may run ahead of the one in use
+// What setting up and finishing a tile takes, in steps, when the work is dealt: these places of the line are
+// paid for but empty. Measured as COST_MEASURED.
+constexpr uint32_t kTileCost = 3;
 
 template <typename T, int DIM_, int TILES_>
 struct TileConfig {
@@ -101,11 +104,12 @@ struct __align__(1024) TileSmem {
   uint32_t tmem;
 };
 
-// A tile of the line (`height` rows: all of a CTA's tiles), and the tiles after it.
+// A tile of the line (HEIGHT rows: all of a CTA's tiles), and the tiles after it. It takes kTileCost places,
+// then one for each step.
 struct TileWalk {
   uint32_t s, h, qt;
   uint32_t tiles, steps;  // of the sequence's kv head; of this tile
-  int32_t first;          // its first step, counted from the start of the CTA's stretch
+  int32_t first;          // its first place, counted from the start of the CTA's stretch
   PagedSeq seq;
 };
 
@@ -120,16 +124,16 @@ __device__ __forceinline__ uint32_t tile_steps(const PagedSeq& q, const AttnArgs
   return seen > 0 ? (static_cast<uint32_t>(seen) + kStep - 1) / kStep : 1u;
 }
 template <uint32_t HEIGHT>
-__device__ __forceinline__ uint64_t head_steps(const PagedSeq& q, const AttnArgs& p) {
+__device__ __forceinline__ uint64_t head_places(const PagedSeq& q, const AttnArgs& p) {
   const uint32_t t = tiles_of<HEIGHT>(q, p);
   uint64_t sum = 0;
-  for (uint32_t i = 0; i < t; ++i) sum += tile_steps<HEIGHT>(q, p, i);
+  for (uint32_t i = 0; i < t; ++i) sum += kTileCost + tile_steps<HEIGHT>(q, p, i);
   return sum;
 }
 
 template <uint32_t HEIGHT>
 __device__ __forceinline__ void next_tile(const PagedArgs& a, const AttnArgs& p, TileWalk& w) {
-  w.first += static_cast<int32_t>(w.steps);
+  w.first += static_cast<int32_t>(kTileCost + w.steps);
   if (++w.qt == w.tiles) {
     w.qt = 0;
     if (++w.h == a.kv_heads) {
@@ -141,6 +145,22 @@ __device__ __forceinline__ void next_tile(const PagedArgs& a, const AttnArgs& p,
     }
   }
   w.steps = tile_steps<HEIGHT>(w.seq, p, w.qt);
+}
+
+// The steps j0 .. j1 - 1 of a tile that a stretch of `len` places holds; false if none.
+__device__ __forceinline__ bool piece_of(const TileWalk& w, int32_t len, uint32_t& j0, uint32_t& j1) {
+  const int32_t f = w.first + static_cast<int32_t>(kTileCost);
+  j0 = static_cast<uint32_t>(max(0, -f));
+  j1 = static_cast<uint32_t>(max(0, min(static_cast<int32_t>(w.steps), len - f)));
+  return j1 > j0;
+}
+template <uint32_t HEIGHT>
+__device__ __forceinline__ bool next_piece(const PagedArgs& a, const AttnArgs& p, TileWalk& w, int32_t len, uint32_t& j0, uint32_t& j1) {
+  do {
+    if (w.first + static_cast<int32_t>(kTileCost + w.steps) >= len) return false;
+    next_tile<HEIGHT>(a, p, w);
+  } while (!piece_of(w, len, j0, j1));
+  return true;
 }
 
 // 16 columns of each of two places in tensor memory (lane quarter of this warp).
@@ -244,7 +264,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
   // ---- this CTA's stretch of the line ----
   uint64_t part = 0, mine_steps = 0;  // (of sequence tid: all there is to look up in a batch of fewer sequences than threads)
   for (uint32_t s = tid; s < a.sequences; s += C::THREADS) {
-    const uint64_t v = head_steps<HEIGHT>(paged_seq(a, s), p) * a.kv_heads;
+    const uint64_t v = head_places<HEIGHT>(paged_seq(a, s), p) * a.kv_heads;
     if (s == tid) mine_steps = v;
     part += v;
   }
@@ -260,7 +280,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
   uint64_t running = 0;
   for (uint32_t base = 0; base < a.sequences; base += C::THREADS) {
     const uint32_t s = base + tid;
-    const uint64_t v = base == 0 ? mine_steps : s < a.sequences ? head_steps<HEIGHT>(paged_seq(a, s), p) * a.kv_heads : 0;
+    const uint64_t v = base == 0 ? mine_steps : s < a.sequences ? head_places<HEIGHT>(paged_seq(a, s), p) * a.kv_heads : 0;
     uint64_t inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -314,19 +334,21 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     walk.s = sm->found_s;
     walk.seq = paged_seq(a, walk.s);
     walk.tiles = tiles_of<HEIGHT>(walk.seq, p);
-    const uint64_t per_head = head_steps<HEIGHT>(walk.seq, p);
+    const uint64_t per_head = head_places<HEIGHT>(walk.seq, p);
     uint64_t off = u0 - sm->found_base;
     walk.h = static_cast<uint32_t>(off / per_head);
     off -= walk.h * per_head;
     walk.qt = 0;
     walk.steps = tile_steps<HEIGHT>(walk.seq, p, 0);
-    while (off >= walk.steps) {
-      off -= walk.steps;
+    while (off >= kTileCost + walk.steps) {
+      off -= kTileCost + walk.steps;
       walk.steps = tile_steps<HEIGHT>(walk.seq, p, ++walk.qt);
     }
     walk.first = -static_cast<int32_t>(off);
   }
-  const uint32_t len = static_cast<uint32_t>(u1 - u0);  // steps of the stretch
+  const int32_t len = static_cast<int32_t>(u1 - u0);  // places of the stretch
+  uint32_t first_j0, first_j1;
+  const bool any = piece_of(walk, len, first_j0, first_j1) || next_piece<HEIGHT>(a, p, walk, len, first_j0, first_j1);
   bool ok = true;
   // Phase n of a barrier, bounded: each try sleeps up to 20 us, so the limit of tries is also one of time. (Few
   // instructions on purpose: there are twenty such waits, and the loops around them have to stay in the
@@ -348,9 +370,8 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
     const uint32_t t = warp / 4, trow = tid % kRows;
     const uint32_t taddr = tmem + ((warp % 4 * 32u) << 16) + t * C::TMEM_TILE;
     uint32_t it = 0, seg = 0;
-    for (uint32_t cur = 0; cur < len && ok; ++seg) {
-      const uint32_t j0 = static_cast<uint32_t>(static_cast<int32_t>(cur) - walk.first);
-      const uint32_t j1 = min(walk.steps, j0 + len - cur);
+    uint32_t j0 = first_j0, j1 = first_j1;
+    for (bool more_pieces = any; more_pieces && ok; more_pieces = next_piece<HEIGHT>(a, p, walk, len, j0, j1), ++seg) {
       const uint32_t rows = walk.seq.n * p.share;
       const uint32_t row = walk.qt * HEIGHT + tid;
       const bool in = row < rows;
@@ -430,6 +451,9 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         if (!ok) break;
         tc_fence_after();
         const uint32_t scol = taddr + (SCALED ? (it & 1u) * kStep : 0u);
+        uint64_t seen = sm->valid[b];
+        const uint32_t top = sm->vexp[b];
+        const float step_factor = SCALED ? factor * pow2i(static_cast<int>(sm->kexp[b]) - 14) : factor;
         uint64_t x[kStep / 2];
 #pragma unroll
         for (int i = 0; i < static_cast<int>(kStep); i += 32 / C::SCORES) {
@@ -455,7 +479,6 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           }
         }
         const int32_t pos0 = static_cast<int32_t>(j * kStep);
-        uint64_t seen = sm->valid[b];
         if (pos0 + static_cast<int32_t>(kStep) - 1 > limit) seen &= limit < pos0 ? 0ull : (2ull << (limit - pos0)) - 1;
         if (seen != ~0ull) {
 #pragma unroll
@@ -471,7 +494,6 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           const float2 f = unpack2(x[i]);
           mx4[i % 4] = fmaxf(fmaxf(mx4[i % 4], f.x), f.y);
         }
-        const float step_factor = SCALED ? factor * pow2i(static_cast<int>(sm->kexp[b]) - 14) : factor;
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * step_factor;
         float rescale = 1.0f;
         bool grew = false;
@@ -481,7 +503,6 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           m = mx;
           grew = true;
         }
-        const uint32_t top = sm->vexp[b];
         if (top > vexp) {
           rescale *= pow2i(static_cast<int>(vexp) - static_cast<int>(top));
           vexp = top;
@@ -602,7 +623,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         // A partial: [DIM / 4][HEIGHT] of four dims, then maxima and sums. In the slots of stretch x: 2 x for the tile
         // that the stretch begins with, 2 x + 1 for the one that it ends with.
         auto slot = [&](uint32_t i) { return p.partials + size_t(i) * (DIM + 2) * HEIGHT; };
-        float* mine = slot(2 * blockIdx.x + (walk.first > 0 ? 1u : 0u));
+        float* mine = slot(2 * blockIdx.x + (walk.first + static_cast<int32_t>(kTileCost) > 0 ? 1u : 0u));
 #pragma unroll 1
         for (int i = 0; i < DIM; i += 32) {
           float o[32];
@@ -618,7 +639,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         mine[size_t(DIM + 1) * HEIGHT + tid] = l;
         // The stretches that hold this tile: c0 .. c1 (stretch x starts at
         // floor(x * total / grid)). Each warp joins its 32 rows by itself.
-        const uint64_t seg0 = u0 + static_cast<int64_t>(walk.first), seg1 = seg0 + walk.steps;
+        const uint64_t seg0 = u0 + static_cast<int64_t>(walk.first) + kTileCost, seg1 = seg0 + walk.steps;
         const uint32_t c0 = static_cast<uint32_t>(((seg0 + 1) * grid - 1) / total);
         const uint32_t c1 = static_cast<uint32_t>((seg1 * grid - 1) / total);
         __threadfence();
@@ -678,8 +699,6 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         }
       }
       tc_fence_before();  // the output's columns may be written again once the next weights arrive
-      cur += j1 - j0;
-      if (cur < len) next_tile<HEIGHT>(a, p, walk);
     }
   } else if (warp < WARPS - 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::CONVERT_REGS));
@@ -700,7 +719,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       // A step ahead: its code chunks and its scales.
       uint4 raw[PASSES];
       TileWalk ahead = walk;
-      uint32_t aj = static_cast<uint32_t>(-walk.first);
+      uint32_t aj = first_j0, aj1 = first_j1;
       // Rows of the pool of that step's positions 32 e + lane (-1: not cached): the page table is read
       // before the step in hand is converted, its answers are used after.
       int32_t page_id[2], page_at[2], rows[2];
@@ -736,22 +755,19 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           }
         }
       };
-      look_up();
-      fetch();
+      bool have = any;
+      if (have) {
+        look_up();
+        fetch();
+      }
       uint32_t top = 0;  // values: the largest exponent field of a scale of the tile so far; keys: of the step
       uint32_t it = 0;
-      for (; it < len; ++it) {
+      for (; have; ++it) {
         const uint32_t b = it & 3u, st = it % STAGES, use = it / STAGES;
         if (!VALUES || aj == 0) top = 0;  // (aj: still the step in hand)
         // The place of the step after this one.
-        const bool more = it + 1 < len;
-        if (more) {
-          if (++aj == ahead.steps) {
-            next_tile<HEIGHT>(a, p, ahead);
-            aj = 0;
-          }
-          look_up();
-        }
+        if (++aj == aj1) have = next_piece<HEIGHT>(a, p, ahead, len, aj, aj1);
+        if (have) look_up();
         if (it >= STAGES) ok = __all_sync(0xffffffffu, wait(&empty[st], use - 1, VALUES ? 204 : 203));
         if (!ok) break;
         // Every warp finds the largest exponent for itself.
@@ -814,7 +830,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           mbar_arrive(&full[st]);
           mbar_arrive(VALUES ? &sm->vs_full[b] : &sm->ks_full[b]);
         }
-        if (more) fetch();
+        if (have) fetch();
       }
     };
     if (warp < CONVERT + C::CONVERT_WARPS) {
@@ -864,9 +880,8 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         }
       }
     };
-    for (uint32_t cur = 0; cur < len && ok; ++seg) {
-      const uint32_t j0 = static_cast<uint32_t>(static_cast<int32_t>(cur) - walk.first);
-      const uint32_t j1 = min(walk.steps, j0 + len - cur);
+    uint32_t j0 = first_j0, j1 = first_j1;
+    for (bool more_pieces = any; more_pieces && ok; more_pieces = next_piece<HEIGHT>(a, p, walk, len, j0, j1), ++seg) {
       for (int t = 0; t < TILES && ok; ++t) ok = wait_all(&sm->q_full[t], seg, 205);
       // Exact: step n's scores are issued behind step n - 1's output, tile by tile, as the weights lie in the
       // scores' columns. Scaled: they have columns of their own, and are issued before step n - 1's
@@ -897,10 +912,6 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           if (t == TILES - 1) mma_commit(&sm->v_empty[it % STAGES]);
           if (!SCALED && more) issue_scores(t, it + 1);
         }
-      }
-      if (ok) {
-        cur += j1 - j0;
-        if (cur < len) next_tile<HEIGHT>(a, p, walk);
       }
     }
     if (!ok && waiting) {  // MMAs in flight end before tensor memory is freed

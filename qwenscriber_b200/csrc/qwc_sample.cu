@@ -3,16 +3,23 @@
 // With x the row, m its maximum and T the temperature, w_i = exp((x_i - m) / T).
 // The tokens kept are a prefix of the order (falling logit, rising index):
 // top_k cuts it by count, top_p by the sum of w, min_p by w itself. So the
-// kept set is one threshold logit t and a number of tokens that equal it:
-// everything above t, and the first of those at t. The threshold comes from a
-// radix selection on the logits' order-preserving bits; no sort. The token is
-// the first in index order whose running sum of the kept w passes u times their
-// total.
+// kept set is one threshold logit and a number of tokens that equal it:
+// everything above, and the first of those at it. No sort: the threshold is
+// found by narrowing. A histogram over (m - x) / T in steps of 1/32 gives the
+// bin that holds it, histograms over the logits' order-preserving bits within
+// that bin the rest, ten bits at a time. The token is the first in index order
+// whose running sum of the kept w passes u times their total.
 //
 // Sums are of integers, w in units of 2^-42: they are exact, so neither the
 // order of the atomics nor the split over threads changes a result.
+//
+// A cluster of CTAs takes a row, each CTA a slice that it reads once and keeps in
+// shared memory; histograms and totals meet in the first CTA's.
 
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "qwc_device.cuh"
 #include "qwc_paged.cuh"
@@ -20,15 +27,21 @@
 namespace qwc {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kBins = 2048;
+constexpr uint32_t kBins = kSampleThreads;  // a scan takes one bin for each thread
+constexpr uint32_t kBinBits = 10;
+constexpr float kBinScale = 32.0f;      // coarse bins in a nat; the last bin takes all below e^-32, whose units are 0
 constexpr float kUnits = 4398046511104.0f;  // 2^42: 2^20 tokens of weight 1 stay below 2^63
 
 struct SampleArgs {
   const void* logits;
   uint64_t row_stride;
   uint32_t vocab;
+  uint32_t run;   // values of a warp, a multiple of 32
+  uint32_t held;  // values of a slice that fit shared memory; the others are read again from global memory
   const float* temperature;
   const int32_t* top_k;
   const float* top_p;
@@ -39,22 +52,36 @@ struct SampleArgs {
 };
 
 // A logit as the operator sees it: NaN is -inf, and -0 is 0 so that the two tie.
+__device__ __forceinline__ float logit(float x) { return x != x ? -INFINITY : x + 0.0f; }
+
+// Bits in the order of the values, without those that a value of type T leaves the same.
 template <typename T>
-__device__ __forceinline__ float logit(const T* row, uint32_t i) {
-  const float x = to_f32(row[i]);
-  return x != x ? -INFINITY : x + 0.0f;
-}
-
-// Bits in the order of the values.
 __device__ __forceinline__ uint32_t order_key(float x) {
+  constexpr int kIdle = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 13 : 16;
   const uint32_t b = __float_as_uint(x);
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  return ((b & 0x80000000u) ? ~b : b | 0x80000000u) >> kIdle;
+}
+template <typename T>
+__device__ __forceinline__ float key_value(uint32_t key) {
+  constexpr int kIdle = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 13 : 16;
+  const uint32_t k = key << kIdle;
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~(k | ((1u << kIdle) - 1u)));
 }
 
-__device__ __forceinline__ float weight_of(float x, float best, float heat) {
-  return x == best ? 1.0f : expf((x - best) / heat);
-}
+// (best - x) / heat, correctly rounded save for the rarest cases: one step of Newton's on the product with
+// the reciprocal.
+struct Heat {
+  float heat, inverse;
+  __device__ __forceinline__ float fall(float best, float x) const {
+    const float d = best - x;
+    const float q = d * inverse;
+    const float r = fmaf(-q, heat, d);
+    const float f = fmaf(r, inverse, q);
+    return f == f ? f : q;  // (d infinite)
+  }
+};
 
+__device__ __forceinline__ float weight_of(float fall) { return expf(-fall); }
 __device__ __forceinline__ uint64_t units_of(float w) { return __float2ull_rn(w * kUnits); }
 
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
@@ -72,240 +99,364 @@ __device__ __forceinline__ uint64_t warp_scan_u64(uint64_t v) {
   return v;
 }
 
-struct SampleSmem {
+struct Histogram {
   uint64_t mass[kBins];
   uint32_t count[kBins];
-  uint64_t sums[kSampleWarps];
-  uint32_t keys[kSampleWarps];
-  uint64_t above;
+};
+
+// Where a prefix of the order ends: at the tokens whose key is `key`, with `count` tokens and `mass` above
+// them and `here` tokens (of mass `here_mass`) at it.
+struct Cut {
+  uint64_t mass, here_mass;
+  uint32_t count, here;
   uint32_t bin;
 };
 
-__device__ __forceinline__ uint64_t block_sum(SampleSmem* s, uint64_t v) {
-  v = warp_sum_u64(v);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) s->sums[threadIdx.x / 32] = v;
-  __syncthreads();
-  uint64_t t = 0;
-  for (int i = 0; i < kSampleWarps; ++i) t += s->sums[i];
-  return t;
+struct SampleSmem {
+  Histogram coarse, fine;  // the first CTA's are the row's
+  uint64_t sums[kSampleWarps];
+  uint64_t scan[kSampleWarps];
+  uint32_t scan_count[kSampleWarps];
+  uint64_t total;      // the row's (first CTA) sum of all units
+  uint64_t slice_sum;  // this slice's sum of kept units
+  uint32_t slice_ties;
+  float best;
+  uint32_t best_at;
+  Cut cut;
+  float values[];
+};
+
+__device__ __forceinline__ void clear(Histogram& h) {
+  h.mass[threadIdx.x] = 0;
+  h.count[threadIdx.x] = 0;
 }
 
-// The key where the prefix of (falling key) reaches `target`, counted in
-// tokens (by_mass false) or in units of w, and what lies above that key.
-template <typename T>
-__device__ void select(SampleSmem* s, const T* row, uint32_t vocab, float best, float heat, bool by_mass, uint64_t target,
-                       uint32_t* key, uint64_t* above_out) {
-  uint32_t prefix = 0, mask = 0;
-  uint64_t above = 0;
-  const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
-  for (int d = 0; d < 3; ++d) {
-    const uint32_t bins = 1u << bits[d];
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kSampleThreads) {
-      s->mass[i] = 0;
-      s->count[i] = 0;
+__device__ __forceinline__ void add_to(Histogram* h, uint32_t bin, uint32_t count, uint64_t mass) {
+  atomicAdd(&h->count[bin], count);
+  if (mass) atomicAdd(reinterpret_cast<unsigned long long*>(&h->mass[bin]), static_cast<unsigned long long>(mass));
+}
+
+// The bin of `h` (bin 0 on top) where what lies above it, added to `from`, reaches the target: `target` tokens, or
+// units if by_mass. One thread for each bin of the first CTA.
+__device__ void find_bin(SampleSmem* s, const Histogram& h, bool by_mass, uint64_t target, uint32_t from_count, uint64_t from_mass) {
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint64_t m = h.mass[threadIdx.x];
+  const uint32_t n = h.count[threadIdx.x];
+  uint64_t im = m;
+  uint32_t in = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t um = __shfl_up_sync(0xffffffffu, im, o);
+    const uint32_t un = __shfl_up_sync(0xffffffffu, in, o);
+    if (lane >= static_cast<uint32_t>(o)) {
+      im += um;
+      in += un;
     }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < vocab; i += kSampleThreads) {
-      const float x = logit(row, i);
-      const uint32_t k = order_key(x);
-      if ((k & mask) != prefix) continue;
-      const uint32_t b = (k >> shifts[d]) & (bins - 1);
-      if (by_mass) {
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s->mass[b]),
-                  static_cast<unsigned long long>(units_of(weight_of(x, best, heat))));
-      } else {
-        atomicAdd(&s->count[b], 1u);
-      }
-    }
-    __syncthreads();
-    // Bins from the top, two for each thread.
-    const int b1 = static_cast<int>(bins) - 1 - 2 * static_cast<int>(threadIdx.x), b0 = b1 - 1;
-    const uint64_t v1 = b1 >= 0 ? (by_mass ? s->mass[b1] : s->count[b1]) : 0;
-    const uint64_t v0 = b0 >= 0 ? (by_mass ? s->mass[b0] : s->count[b0]) : 0;
-    const uint64_t inc = warp_scan_u64(v0 + v1);
-    if (threadIdx.x % 32 == 31) s->sums[threadIdx.x / 32] = inc;
-    __syncthreads();
-    uint64_t base = above;
-    for (uint32_t w = 0; w < threadIdx.x / 32; ++w) base += s->sums[w];
-    const uint64_t before1 = base + inc - v0 - v1, before0 = base + inc - v0;
-    if (before1 < target && target <= before1 + v1) {
-      s->bin = static_cast<uint32_t>(b1);
-      s->above = before1;
-    }
-    if (before0 < target && target <= before0 + v0) {
-      s->bin = static_cast<uint32_t>(b0);
-      s->above = before0;
-    }
-    __syncthreads();
-    prefix |= s->bin << shifts[d];
-    mask |= (bins - 1) << shifts[d];
-    above = s->above;
   }
-  *key = prefix;
-  *above_out = above;
+  if (lane == 31) {
+    s->scan[warp] = im;
+    s->scan_count[warp] = in;
+  }
+  __syncthreads();
+  const uint64_t wm = s->scan[lane];
+  const uint32_t wn = s->scan_count[lane];
+  const uint64_t bm = warp_sum_u64(lane < warp ? wm : 0);
+  const uint32_t bn = __reduce_add_sync(0xffffffffu, lane < warp ? wn : 0u);
+  const uint64_t above_mass = from_mass + bm + im - m;
+  const uint32_t above_count = from_count + bn + in - n;
+  const uint64_t above = by_mass ? above_mass : above_count, here = by_mass ? m : n;
+  if (above < target && target <= above + here) s->cut = Cut{above_mass, m, above_count, n, threadIdx.x};
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t sample_smem[];
   SampleSmem* s = reinterpret_cast<SampleSmem*>(sample_smem);
-  const uint32_t r = blockIdx.x;
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t size = cluster.num_blocks(), rank = cluster.block_rank();
+  SampleSmem* s0 = cluster.map_shared_rank(s, 0);
+  const uint32_t r = blockIdx.x / size;
   const T* row = static_cast<const T*>(a.logits) + size_t(r) * a.row_stride;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const float heat_given = a.temperature ? a.temperature[r] : 1.0f;
   const bool greedy = !(heat_given > 0.0f);
-  const float heat = greedy ? 1.0f : heat_given;
-  const int32_t k = a.top_k ? a.top_k[r] : 0;
-  const float top_p = a.top_p ? a.top_p[r] : 1.0f;
+  const Heat heat{greedy ? 1.0f : heat_given, 1.0f / (greedy ? 1.0f : heat_given)};
+  const int32_t k_given = a.top_k ? a.top_k[r] : 0;
+  const float p_given = a.top_p ? a.top_p[r] : 1.0f;
   const float least = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
+  const bool by_count = !greedy && k_given > 0 && static_cast<uint32_t>(k_given) < a.vocab;
+  const bool by_mass = !greedy && p_given < 1.0f;
 
+  // This CTA's slice, and this warp's run of it.
+  const uint32_t slice0 = min(rank * a.run * kSampleWarps, a.vocab), slice1 = min(slice0 + a.run * kSampleWarps, a.vocab);
+  const uint32_t i0 = min(slice0 + warp * a.run, slice1), i1 = min(i0 + a.run, slice1);
+  auto value = [&](uint32_t i) {
+    return i - slice0 < a.held ? s->values[i - slice0] : logit(to_f32(row[i]));
+  };
   // The largest logit, and its first index.
   float best = -INFINITY;
   uint32_t at = 0xFFFFFFFFu;
-  for (uint32_t i = threadIdx.x; i < a.vocab; i += kSampleThreads) {
-    const float x = logit(row, i);
+  auto take = [&](uint32_t i, float x) {
+    x = logit(x);
+    if (i - slice0 < a.held) s->values[i - slice0] = x;
     if (x > best) {
       best = x;
       at = i;
     }
-  }
+  };
+  constexpr uint32_t V = 16 / sizeof(T);
+  // 16-byte loads between the first and the last aligned value of the slice.
+  const uint32_t skew = static_cast<uint32_t>((reinterpret_cast<uintptr_t>(row + slice0) % 16) / sizeof(T));
+  const uint32_t v0 = min(slice0 + (skew ? V - skew : 0u), slice1), nv = (slice1 - v0) / V;
+  if (threadIdx.x < v0 - slice0) take(slice0 + threadIdx.x, to_f32(row[slice0 + threadIdx.x]));
+  for (uint32_t c = threadIdx.x; c < nv; c += 4 * kSampleThreads) {
+    uint4 w[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float ob = __shfl_xor_sync(0xffffffffu, best, o);
-    const uint32_t oa = __shfl_xor_sync(0xffffffffu, at, o);
+    for (int j = 0; j < 4; ++j) {
+      if (c + j * kSampleThreads < nv) w[j] = ld_nc4(row + v0 + (c + j * kSampleThreads) * V);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c + j * kSampleThreads < nv) {
+        float x[V];
+        unpack16(w[j], x, T());
+#pragma unroll
+        for (uint32_t e = 0; e < V; ++e) take(v0 + (c + j * kSampleThreads) * V + e, x[e]);
+      }
+    }
+  }
+  if (threadIdx.x < slice1 - v0 - nv * V) take(v0 + nv * V + threadIdx.x, to_f32(row[v0 + nv * V + threadIdx.x]));
+  auto better = [&](float ob, uint32_t oa) {
     if (ob > best || (ob == best && oa < at)) {
       best = ob;
       at = oa;
     }
-  }
-  if (lane == 0) {
-    s->sums[warp] = at;
-    s->keys[warp] = __float_as_uint(best);
-  }
+  };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
+  if (lane == 0) s->sums[warp] = uint64_t(__float_as_uint(best)) << 32 | at;
+  clear(s->coarse);
+  clear(s->fine);
+  if (threadIdx.x == 0) s->total = 0;
   __syncthreads();
-  for (int w = 0; w < kSampleWarps; ++w) {
-    const float ob = __uint_as_float(s->keys[w]);
-    const uint32_t oa = static_cast<uint32_t>(s->sums[w]);
-    if (ob > best || (ob == best && oa < at)) {
-      best = ob;
-      at = oa;
-    }
+  better(__uint_as_float(static_cast<uint32_t>(s->sums[lane] >> 32)), static_cast<uint32_t>(s->sums[lane]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
+  if (threadIdx.x == 0) {
+    s->best = best;
+    s->best_at = at;
   }
+  cluster.sync();
+  if (lane < size) better(cluster.map_shared_rank(s, lane)->best, cluster.map_shared_rank(s, lane)->best_at);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
   if (best == -INFINITY) {
-    if (threadIdx.x == 0) {
+    if (rank == 0 && threadIdx.x == 0) {
       a.tokens[r] = 0;
       if (a.logprobs) a.logprobs[r] = -INFINITY;
     }
+    cluster.sync();  // (the others may still be reading this CTA's maximum)
     return;
   }
-  uint64_t part = 0;
-  for (uint32_t i = threadIdx.x; i < a.vocab; i += kSampleThreads) part += units_of(weight_of(logit(row, i), best, heat));
-  const uint64_t all = block_sum(s, part);
+
+  // All units, and the coarse histogram.
+  auto fall_of = [&](float x) { return x == best ? 0.0f : heat.fall(best, x); };
+  auto coarse_bin = [&](float fall) { return static_cast<uint32_t>(fminf(fall * kBinScale, static_cast<float>(kBins - 1))); };
+  const bool cuts = by_count || by_mass;
+  uint64_t run_sum = 0;
+  for (uint32_t i = i0 + lane; i < i1; i += 32) {
+    const float fall = fall_of(value(i));
+    const uint64_t u = units_of(weight_of(fall));
+    run_sum += u;
+    if (cuts) {
+      const uint32_t bin = coarse_bin(fall);
+      // The last bin's units are 0, and it can hold most of a row: one count for all its lanes.
+      const uint32_t low = __match_any_sync(__activemask(), bin == kBins - 1);
+      if (bin != kBins - 1) {
+        add_to(&s->coarse, bin, 1, u);
+      } else if (lane == static_cast<uint32_t>(__ffs(low)) - 1) {
+        atomicAdd(&s->coarse.count[bin], static_cast<uint32_t>(__popc(low)));
+      }
+    }
+  }
+  run_sum = warp_sum_u64(run_sum);
+  if (lane == 0) {
+    s->sums[warp] = run_sum;
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s0->total), static_cast<unsigned long long>(run_sum));
+  }
+  __syncthreads();
+  if (cuts && rank != 0 && s->coarse.count[threadIdx.x]) {
+    add_to(&s0->coarse, threadIdx.x, s->coarse.count[threadIdx.x], s->coarse.mass[threadIdx.x]);
+  }
+  cluster.sync();
+  const uint64_t all = s0->total;
   const float log_all = logf(static_cast<float>(all) / kUnits);
   if (greedy) {
-    if (threadIdx.x == 0) {
+    if (rank == 0 && threadIdx.x == 0) {
       a.tokens[r] = at;
       if (a.logprobs) a.logprobs[r] = -log_all;
     }
+    cluster.sync();
     return;
   }
 
-  // The kept set: keys above `cut`, and the first `ties` of those at it.
-  uint32_t cut = 0, ties = 0xFFFFFFFFu;
-  uint64_t mass = all;
-  if (k > 0 && static_cast<uint32_t>(k) < a.vocab) {
-    uint64_t above;
-    select(s, row, a.vocab, best, heat, false, static_cast<uint64_t>(k), &cut, &above);
-    ties = static_cast<uint32_t>(k - above);
-    part = 0;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += kSampleThreads) {
-      const float x = logit(row, i);
-      if (order_key(x) > cut) part += units_of(weight_of(x, best, heat));
+  // The key at which a prefix reaches the target. Every CTA comes here or none.
+  auto find_cut = [&](bool mass, uint64_t target, uint32_t& key, Cut& cut) {
+    if (rank == 0) find_bin(s, s->coarse, mass, target, 0, 0);
+    cluster.sync();
+    cut = s0->cut;
+    const uint32_t bin = cut.bin;
+    // The bin's keys: its ends in logits, a little wider for their rounding.
+    const float slack = 4e-7f * (fabsf(best) + heat.heat * (bin + 2) / kBinScale);
+    uint32_t hi = order_key<T>(best - heat.heat * bin / kBinScale + slack);
+    uint32_t lo = bin == kBins - 1 ? 0u : order_key<T>(best - heat.heat * (bin + 1) / kBinScale - slack);
+    if (!(best < INFINITY) || !(hi >= lo)) lo = 0, hi = 0xFFFFFFFFu;
+    for (;;) {
+      const uint32_t span = hi - lo;
+      const uint32_t bits = 32 - __clz(span | 1u);
+      const uint32_t shift = bits > kBinBits ? bits - kBinBits : 0u;
+      for (uint32_t i = i0 + lane; i < i1; i += 32) {
+        const float x = value(i);
+        const uint32_t k = order_key<T>(x);
+        if (k > hi || k < lo) continue;
+        const float fall = fall_of(x);
+        if (coarse_bin(fall) != bin) continue;
+        add_to(&s0->fine, (hi - k) >> shift, 1, units_of(weight_of(fall)));
+      }
+      cluster.sync();
+      if (rank == 0) {
+        const uint32_t from_count = s->cut.count;
+        const uint64_t from_mass = s->cut.mass;
+        __syncthreads();
+        find_bin(s, s->fine, mass, target, from_count, from_mass);
+        __syncthreads();
+        clear(s->fine);
+      }
+      cluster.sync();
+      cut = s0->cut;
+      hi -= cut.bin << shift;
+      if (shift == 0) break;
+      lo = hi - min(hi - lo, (1u << shift) - 1u);
     }
-    mass = block_sum(s, part);
-    const uint32_t bits = (cut & 0x80000000u) ? cut ^ 0x80000000u : ~cut;
-    mass += ties * units_of(weight_of(__uint_as_float(bits), best, heat));
+    key = hi;
+  };
+
+  // The kept set: keys above `cut`, and the first `ties` of the `here` at it.
+  uint32_t key = 0, ties = 0xFFFFFFFFu, here = 0;
+  uint64_t mass = all;
+  if (by_count) {
+    Cut cut;
+    find_cut(false, static_cast<uint64_t>(k_given), key, cut);
+    ties = static_cast<uint32_t>(k_given) - cut.count;
+    here = cut.here;
+    mass = cut.mass + cut.here_mass / cut.here * ties;
   }
-  if (top_p < 1.0f) {
-    const double want = ceil(static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(mass));
-    uint64_t target = static_cast<uint64_t>(want);
-    if (target < 1) target = 1;
+  if (by_mass) {
+    uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
+    if (!(p_given > 0.0f) || target < 1) target = 1;
     if (target > mass) target = mass;
-    uint64_t above;
-    select(s, row, a.vocab, best, heat, true, target, &cut, &above);
-    const uint32_t bits = (cut & 0x80000000u) ? cut ^ 0x80000000u : ~cut;
-    const uint64_t each = units_of(weight_of(__uint_as_float(bits), best, heat));
-    ties = each ? static_cast<uint32_t>((target - above + each - 1) / each) : 0xFFFFFFFFu;
+    Cut cut;
+    find_cut(true, target, key, cut);
+    const uint64_t each = cut.here_mass / cut.here;
+    ties = static_cast<uint32_t>((target - cut.mass + each - 1) / each);
+    here = cut.here;
   }
 
-  // Each warp takes a run of the row. Tokens at the cut in its run, then the
-  // mass that it keeps, then the walk of the one run that holds the token.
-  const uint32_t run = (a.vocab + kSampleThreads - 1) / kSampleThreads * 32;
-  const uint32_t i0 = min(warp * run, a.vocab), i1 = min(i0 + run, a.vocab);
+  // Tokens at the cut in the runs before this one, where not all of them stay.
   uint32_t tie_base = 0;
-  if (ties != 0xFFFFFFFFu) {
+  const bool rank_ties = ties < here;
+  if (rank_ties) {
     uint32_t n = 0;
-    for (uint32_t i = i0 + lane; i < i1; i += 32) n += order_key(logit(row, i)) == cut ? 1u : 0u;
-    const uint64_t sum = warp_sum_u64(n);
+    for (uint32_t i = i0 + lane; i < i1; i += 32) n += order_key<T>(value(i)) == key ? 1u : 0u;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) s->scan_count[warp] = n;
     __syncthreads();
-    if (lane == 0) s->sums[warp] = sum;
-    __syncthreads();
-    for (uint32_t w = 0; w < warp; ++w) tie_base += static_cast<uint32_t>(s->sums[w]);
-    __syncthreads();
+    const uint32_t mine = s->scan_count[lane];
+    tie_base = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0u);
+    const uint32_t sum = __reduce_add_sync(0xffffffffu, mine);
+    if (threadIdx.x == 0) s->slice_ties = sum;
+    cluster.sync();
+    tie_base += __reduce_add_sync(0xffffffffu, lane < rank ? cluster.map_shared_rank(s, lane)->slice_ties : 0u);
   }
   auto kept_units = [&](uint32_t i, uint32_t& tie_at) -> uint64_t {
     const bool in = i < i1;
-    const float x = in ? logit(row, i) : -INFINITY;
-    const uint32_t key = order_key(x);
-    const bool tie = in && key == cut;
-    const uint32_t votes = __ballot_sync(0xffffffffu, tie);
-    const uint32_t rank = tie_at + __popc(votes & ((1u << lane) - 1u));
-    tie_at += __popc(votes);
-    const float w = weight_of(x, best, heat);
-    const bool keep = in && w >= least && (key > cut || (tie && rank < ties));
-    return keep ? units_of(w) : 0;
+    const float x = in ? value(i) : -INFINITY;
+    const uint32_t k = order_key<T>(x);
+    bool keep = in && k >= key;
+    if (rank_ties) {
+      const bool tie = in && k == key;
+      const uint32_t votes = __ballot_sync(0xffffffffu, tie);
+      if (tie && tie_at + __popc(votes & ((1u << lane) - 1u)) >= ties) keep = false;
+      tie_at += __popc(votes);
+    }
+    if (!keep) return 0;
+    const float w = weight_of(fall_of(x));
+    return w >= least ? units_of(w) : 0;
   };
-  part = 0;
-  uint32_t tie_at = tie_base;
-  for (uint32_t i = i0; i < i1; i += 32) part += kept_units(i + lane, tie_at);
-  part = warp_sum_u64(part);
-  __syncthreads();
-  if (lane == 0) s->sums[warp] = part;
-  __syncthreads();
-  uint64_t total = 0, before = 0;
-  for (uint32_t w = 0; w < kSampleWarps; ++w) {
-    if (w == warp) before = total;
-    total += s->sums[w];
+  // The sum of each run, then the walk of the one that holds the token.
+  const bool every = !cuts && !(least > 0.0f);
+  if (!every) {
+    uint32_t tie_at = tie_base;
+    run_sum = 0;
+    for (uint32_t i = i0; i < i1; i += 32) run_sum += kept_units(i + lane, tie_at);
+    run_sum = warp_sum_u64(run_sum);
+    if (lane == 0) s->sums[warp] = run_sum;
+    __syncthreads();
   }
+  const uint64_t other = s->sums[lane];
+  uint64_t before = warp_sum_u64(lane < warp ? other : 0);
+  if (warp == 0) {
+    const uint64_t sum = warp_sum_u64(other);
+    if (lane == 0) s->slice_sum = sum;
+  }
+  cluster.sync();
+  const uint64_t slice = lane < size ? cluster.map_shared_rank(s, lane)->slice_sum : 0;
+  before += warp_sum_u64(lane < rank ? slice : 0);
+  const uint64_t kept = warp_sum_u64(slice);
   const float u = fminf(fmaxf(a.uniforms[r], 0.0f), 1.0f);
-  uint64_t goal = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total));
-  if (goal >= total) goal = total - 1;
-  if (before <= goal && goal < before + part) {
+  uint64_t goal = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(kept));
+  if (goal >= kept) goal = kept - 1;
+  if (before <= goal && goal < before + run_sum) {
     uint64_t sum = before;
-    tie_at = tie_base;
+    uint32_t tie_at = tie_base;
     for (uint32_t i = i0; i < i1; i += 32) {
-      const uint64_t v = kept_units(i + lane, tie_at);
-      const uint64_t inc = sum + warp_scan_u64(v);
+      const uint64_t inc = sum + warp_scan_u64(kept_units(i + lane, tie_at));
       const uint32_t past = __ballot_sync(0xffffffffu, inc > goal);
       if (past) {
         if (lane == static_cast<uint32_t>(__ffs(past)) - 1) {
-          const float x = logit(row, i + lane);
           a.tokens[r] = i + lane;
-          if (a.logprobs) a.logprobs[r] = (x == best ? 0.0f : (x - best) / heat) - log_all;
+          if (a.logprobs) a.logprobs[r] = -fall_of(value(i + lane)) - log_all;
         }
         break;
       }
       sum = __shfl_sync(0xffffffffu, inc, 31);
     }
   }
+  cluster.sync();  // no CTA leaves while another reads its sums
 }
 
 template <typename T>
-int32_t sample_as(const SampleArgs& a, uint32_t rows, cudaStream_t stream) {
-  sample_kernel<T><<<rows, kSampleThreads, sizeof(SampleSmem), stream>>>(a);
-  return paged_status(cudaGetLastError());
+int32_t sample_as(SampleArgs a, uint32_t rows, cudaStream_t stream) {
+  const uint32_t size = 8;
+  a.run = ((a.vocab + size * kSampleWarps - 1) / (size * kSampleWarps) + 31) / 32 * 32;
+  const uint32_t most = (227 * 1024 - 1024 - static_cast<uint32_t>(sizeof(SampleSmem))) / 4;
+  a.held = a.run * kSampleWarps < most ? a.run * kSampleWarps : most;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows * size);
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = sizeof(SampleSmem) + size_t(a.held) * 4;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(cfg.dynamicSmemBytes));
+  if (e != cudaSuccess) return paged_status(e);
+  return paged_status(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
 }
 
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -328,8 +479,8 @@ int32_t qwc_op_sample(uint32_t format, const void* logits, uint64_t row_stride, 
     return QWC_INVALID_ARGUMENT;
   }
   if (rows > 1 && row_stride < vocab) return QWC_SHAPE_MISMATCH;
-  if (vocab > QWC_SAMPLE_MAX_VOCAB || rows > 0x7FFFFFFFu || row_stride > (uint64_t(1) << 31)) return QWC_LIMIT_EXCEEDED;
-  const SampleArgs a{logits, row_stride, vocab, temperature, top_k, top_p, min_p, uniforms, tokens_out, logprobs_out};
+  if (vocab > QWC_SAMPLE_MAX_VOCAB || rows > (1u << 24) || row_stride > (uint64_t(1) << 31)) return QWC_LIMIT_EXCEEDED;
+  const SampleArgs a{logits, row_stride, vocab, 0, 0, temperature, top_k, top_p, min_p, uniforms, tokens_out, logprobs_out};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return format == kFormatF32 ? sample_as<float>(a, rows, s)
          : format == kFormatF16 ? sample_as<__half>(a, rows, s)

@@ -6,8 +6,8 @@
 // kept set is one threshold logit and a number of tokens that equal it:
 // everything above, and the first of those at it. No sort: the threshold is
 // found by narrowing. A histogram over (m - x) / T in steps of 1/32 gives the
-// bin that holds it, histograms over the logits' order-preserving bits within
-// that bin the rest, ten bits at a time. The token is the first in index order
+// bin that holds it; the tokens of that bin, a few hundred as a rule, go to the first CTA, which finds the rest
+// by histograms over the logits' order-preserving bits, eight at a time (all CTAs do so where a bin has too many). The token is the first in index order
 // whose running sum of the kept w passes u times their total.
 //
 // Sums are of integers, w in units of 2^-42: they are exact, so neither the
@@ -32,7 +32,9 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr uint32_t kBins = kSampleThreads;  // a scan takes one bin for each thread
-constexpr uint32_t kBinBits = 10;
+constexpr uint32_t kFineBits = 8, kFineBins = 1u << kFineBits;
+constexpr uint32_t kListed = 512;           // tokens of one coarse bin that the first CTA can take by themselves
+constexpr uint32_t kLimbBits = 14;          // 2^17 tokens of a slice times 2^14 stay below 2^32
 constexpr float kBinScale = 32.0f;      // coarse bins in a nat; the last bin takes all below e^-32, whose units are 0
 constexpr float kUnits = 4398046511104.0f;  // 2^42: 2^20 tokens of weight 1 stay below 2^63
 
@@ -99,9 +101,10 @@ __device__ __forceinline__ uint64_t warp_scan_u64(uint64_t v) {
   return v;
 }
 
+template <uint32_t BINS>
 struct Histogram {
-  uint64_t mass[kBins];
-  uint32_t count[kBins];
+  uint64_t mass[BINS];
+  uint32_t count[BINS];
 };
 
 // Where a prefix of the order ends: at the tokens whose key is `key`, with `count` tokens and `mass` above
@@ -113,7 +116,17 @@ struct Cut {
 };
 
 struct SampleSmem {
-  Histogram coarse, fine;  // the first CTA's are the row's
+  // The first CTA's are the row's.
+  Histogram<kBins> coarse;
+  Histogram<kFineBins> fine;
+  union {
+    uint32_t limb[3][kBins];  // the slice's masses by bin, in limbs: 32-bit additions are native, 64-bit ones are not
+    struct {
+      uint64_t units[kListed];
+      uint32_t key[kListed];
+    } list;
+  };
+  uint32_t listed;
   uint64_t sums[kSampleWarps];
   uint64_t scan[kSampleWarps];
   uint32_t scan_count[kSampleWarps];
@@ -126,22 +139,27 @@ struct SampleSmem {
   float values[];
 };
 
-__device__ __forceinline__ void clear(Histogram& h) {
-  h.mass[threadIdx.x] = 0;
-  h.count[threadIdx.x] = 0;
+template <uint32_t BINS>
+__device__ __forceinline__ void clear(Histogram<BINS>& h) {
+  if (threadIdx.x < BINS) {
+    h.mass[threadIdx.x] = 0;
+    h.count[threadIdx.x] = 0;
+  }
 }
 
-__device__ __forceinline__ void add_to(Histogram* h, uint32_t bin, uint32_t count, uint64_t mass) {
+template <uint32_t BINS>
+__device__ __forceinline__ void add_to(Histogram<BINS>* h, uint32_t bin, uint32_t count, uint64_t mass) {
   atomicAdd(&h->count[bin], count);
   if (mass) atomicAdd(reinterpret_cast<unsigned long long*>(&h->mass[bin]), static_cast<unsigned long long>(mass));
 }
 
 // The bin of `h` (bin 0 on top) where what lies above it, added to `from`, reaches the target: `target` tokens, or
-// units if by_mass. One thread for each bin of the first CTA.
-__device__ void find_bin(SampleSmem* s, const Histogram& h, bool by_mass, uint64_t target, uint32_t from_count, uint64_t from_mass) {
+// units if by_mass. All threads of the first CTA, one for each bin.
+template <uint32_t BINS>
+__device__ void find_bin(SampleSmem* s, const Histogram<BINS>& h, bool by_mass, uint64_t target, uint32_t from_count, uint64_t from_mass) {
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint64_t m = h.mass[threadIdx.x];
-  const uint32_t n = h.count[threadIdx.x];
+  const uint64_t m = threadIdx.x < BINS ? h.mass[threadIdx.x] : 0;
+  const uint32_t n = threadIdx.x < BINS ? h.count[threadIdx.x] : 0;
   uint64_t im = m;
   uint32_t in = n;
 #pragma unroll
@@ -168,7 +186,7 @@ __device__ void find_bin(SampleSmem* s, const Histogram& h, bool by_mass, uint64
   if (above < target && target <= above + here) s->cut = Cut{above_mass, m, above_count, n, threadIdx.x};
 }
 
-template <typename T>
+template <typename T, bool HELD>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t sample_smem[];
   SampleSmem* s = reinterpret_cast<SampleSmem*>(sample_smem);
@@ -191,14 +209,14 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   const uint32_t slice0 = min(rank * a.run * kSampleWarps, a.vocab), slice1 = min(slice0 + a.run * kSampleWarps, a.vocab);
   const uint32_t i0 = min(slice0 + warp * a.run, slice1), i1 = min(i0 + a.run, slice1);
   auto value = [&](uint32_t i) {
-    return i - slice0 < a.held ? s->values[i - slice0] : logit(to_f32(row[i]));
+    return HELD || i - slice0 < a.held ? s->values[i - slice0] : logit(to_f32(row[i]));
   };
   // The largest logit, and its first index.
   float best = -INFINITY;
   uint32_t at = 0xFFFFFFFFu;
   auto take = [&](uint32_t i, float x) {
     x = logit(x);
-    if (i - slice0 < a.held) s->values[i - slice0] = x;
+    if (HELD || i - slice0 < a.held) s->values[i - slice0] = x;
     if (x > best) {
       best = x;
       at = i;
@@ -237,7 +255,9 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   if (lane == 0) s->sums[warp] = uint64_t(__float_as_uint(best)) << 32 | at;
   clear(s->coarse);
   clear(s->fine);
-  if (threadIdx.x == 0) s->total = 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) s->limb[i][threadIdx.x] = 0;
+  if (threadIdx.x == 0) s->total = 0, s->listed = 0;
   __syncthreads();
   better(__uint_as_float(static_cast<uint32_t>(s->sums[lane] >> 32)), static_cast<uint32_t>(s->sums[lane]));
 #pragma unroll
@@ -264,18 +284,25 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   auto coarse_bin = [&](float fall) { return static_cast<uint32_t>(fminf(fall * kBinScale, static_cast<float>(kBins - 1))); };
   const bool cuts = by_count || by_mass;
   uint64_t run_sum = 0;
-  for (uint32_t i = i0 + lane; i < i1; i += 32) {
-    const float fall = fall_of(value(i));
+#pragma unroll 4
+  for (uint32_t i = i0; i < i1; i += 32) {
+    const bool in = i + lane < i1;
+    const float fall = in ? fall_of(value(i + lane)) : INFINITY;
     const uint64_t u = units_of(weight_of(fall));
     run_sum += u;
     if (cuts) {
       const uint32_t bin = coarse_bin(fall);
       // The last bin's units are 0, and it can hold most of a row: one count for all its lanes.
-      const uint32_t low = __match_any_sync(__activemask(), bin == kBins - 1);
-      if (bin != kBins - 1) {
-        add_to(&s->coarse, bin, 1, u);
-      } else if (lane == static_cast<uint32_t>(__ffs(low)) - 1) {
-        atomicAdd(&s->coarse.count[bin], static_cast<uint32_t>(__popc(low)));
+      const uint32_t last = __ballot_sync(0xffffffffu, in && bin == kBins - 1);
+      if (last && lane == 0) atomicAdd(&s->coarse.count[kBins - 1], static_cast<uint32_t>(__popc(last)));
+      if (in && bin != kBins - 1) {
+        constexpr uint32_t kLimb = (1u << kLimbBits) - 1u;
+        const uint32_t l0 = static_cast<uint32_t>(u) & kLimb, l1 = static_cast<uint32_t>(u >> kLimbBits) & kLimb;
+        const uint32_t l2 = static_cast<uint32_t>(u >> (2 * kLimbBits));
+        atomicAdd(&s->coarse.count[bin], 1u);
+        atomicAdd(&s->limb[0][bin], l0);
+        if (l1) atomicAdd(&s->limb[1][bin], l1);
+        if (l2) atomicAdd(&s->limb[2][bin], l2);
       }
     }
   }
@@ -285,8 +312,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     atomicAdd(reinterpret_cast<unsigned long long*>(&s0->total), static_cast<unsigned long long>(run_sum));
   }
   __syncthreads();
-  if (cuts && rank != 0 && s->coarse.count[threadIdx.x]) {
-    add_to(&s0->coarse, threadIdx.x, s->coarse.count[threadIdx.x], s->coarse.mass[threadIdx.x]);
+  if (cuts) {
+    const uint32_t n = s->coarse.count[threadIdx.x];
+    const uint64_t u = s->limb[0][threadIdx.x] + (uint64_t(s->limb[1][threadIdx.x]) << kLimbBits) +
+                       (uint64_t(s->limb[2][threadIdx.x]) << (2 * kLimbBits));
+    if (n) add_to(&s0->coarse, threadIdx.x, rank ? n : 0u, u);
   }
   cluster.sync();
   const uint64_t all = s0->total;
@@ -311,32 +341,70 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     uint32_t hi = order_key<T>(best - heat.heat * bin / kBinScale + slack);
     uint32_t lo = bin == kBins - 1 ? 0u : order_key<T>(best - heat.heat * (bin + 1) / kBinScale - slack);
     if (!(best < INFINITY) || !(hi >= lo)) lo = 0, hi = 0xFFFFFFFFu;
-    for (;;) {
-      const uint32_t span = hi - lo;
-      const uint32_t bits = 32 - __clz(span | 1u);
-      const uint32_t shift = bits > kBinBits ? bits - kBinBits : 0u;
-      for (uint32_t i = i0 + lane; i < i1; i += 32) {
-        const float x = value(i);
+    const bool by_list = cut.here <= kListed;
+    auto each_of_bin = [&](auto use) {  // the bin's tokens of this slice, those with keys lo .. hi
+#pragma unroll 4
+      for (uint32_t i = i0; i < i1; i += 32) {
+        const bool in = i + lane < i1;
+        const float x = in ? value(i + lane) : 0.0f;
         const uint32_t k = order_key<T>(x);
-        if (k > hi || k < lo) continue;
+        bool mine = in && k <= hi && k >= lo;
+        if (!__any_sync(0xffffffffu, mine)) continue;
         const float fall = fall_of(x);
-        if (coarse_bin(fall) != bin) continue;
-        add_to(&s0->fine, (hi - k) >> shift, 1, units_of(weight_of(fall)));
+        mine = mine && coarse_bin(fall) == bin;
+        use(mine, k, units_of(weight_of(fall)));
       }
+    };
+    if (by_list) {
+      each_of_bin([&](bool mine, uint32_t k, uint64_t u) {
+        const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+        if (!votes) return;
+        uint32_t at0 = 0;
+        if (lane == 0) at0 = atomicAdd(&s0->listed, static_cast<uint32_t>(__popc(votes)));
+        at0 = __shfl_sync(0xffffffffu, at0, 0) + __popc(votes & ((1u << lane) - 1u));
+        if (mine && at0 < kListed) {
+          s0->list.key[at0] = k;
+          s0->list.units[at0] = u;
+        }
+      });
       cluster.sync();
+    }
+    const bool have = by_list && rank == 0 && threadIdx.x < min(cut.here, s->listed);
+    const uint32_t my_key = have ? s->list.key[threadIdx.x] : 0u;
+    const uint64_t my_units = have ? s->list.units[threadIdx.x] : 0u;
+    while (!by_list || rank == 0) {
+      const uint32_t bits = 32 - __clz((hi - lo) | 1u);
+      const uint32_t shift = bits > kFineBits ? bits - kFineBits : 0u;
+      if (by_list) {
+        if (have && my_key <= hi && my_key >= lo) add_to(&s->fine, (hi - my_key) >> shift, 1, my_units);
+      } else {
+        each_of_bin([&](bool mine, uint32_t k, uint64_t u) {
+          if (mine) add_to(&s0->fine, (hi - k) >> shift, 1, u);
+        });
+        cluster.sync();
+      }
       if (rank == 0) {
-        const uint32_t from_count = s->cut.count;
-        const uint64_t from_mass = s->cut.mass;
         __syncthreads();
-        find_bin(s, s->fine, mass, target, from_count, from_mass);
+        find_bin(s, s->fine, mass, target, cut.count, cut.mass);
         __syncthreads();
         clear(s->fine);
+        if (threadIdx.x == 0) s->listed = 0;
+        __syncthreads();
       }
-      cluster.sync();
+      if (!by_list) cluster.sync();
       cut = s0->cut;
       hi -= cut.bin << shift;
       if (shift == 0) break;
       lo = hi - min(hi - lo, (1u << shift) - 1u);
+      if (!by_list) cluster.sync();  // (the first CTA does not write its cut again before all have read it)
+      if (by_list) __syncthreads();
+    }
+    if (by_list) {
+      __syncthreads();
+      if (rank == 0 && threadIdx.x == 0) s->cut.bin = hi;  // now the key
+      cluster.sync();
+      cut = s0->cut;
+      hi = cut.bin;
     }
     key = hi;
   };
@@ -352,6 +420,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     mass = cut.mass + cut.here_mass / cut.here * ties;
   }
   if (by_mass) {
+    if (by_count) cluster.sync();  // (all have read the first cut)
     uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
     if (!(p_given > 0.0f) || target < 1) target = 1;
     if (target > mass) target = mass;
@@ -367,6 +436,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   const bool rank_ties = ties < here;
   if (rank_ties) {
     uint32_t n = 0;
+#pragma unroll 4
     for (uint32_t i = i0 + lane; i < i1; i += 32) n += order_key<T>(value(i)) == key ? 1u : 0u;
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) s->scan_count[warp] = n;
@@ -389,6 +459,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       if (tie && tie_at + __popc(votes & ((1u << lane) - 1u)) >= ties) keep = false;
       tie_at += __popc(votes);
     }
+    if (!__any_sync(0xffffffffu, keep)) return 0;
     if (!keep) return 0;
     const float w = weight_of(fall_of(x));
     return w >= least ? units_of(w) : 0;
@@ -398,6 +469,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   if (!every) {
     uint32_t tie_at = tie_base;
     run_sum = 0;
+#pragma unroll 4
     for (uint32_t i = i0; i < i1; i += 32) run_sum += kept_units(i + lane, tie_at);
     run_sum = warp_sum_u64(run_sum);
     if (lane == 0) s->sums[warp] = run_sum;
@@ -453,10 +525,10 @@ int32_t sample_as(SampleArgs a, uint32_t rows, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(cfg.dynamicSmemBytes));
+  auto kernel = a.run * kSampleWarps <= most ? sample_kernel<T, true> : sample_kernel<T, false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cfg.dynamicSmemBytes));
   if (e != cudaSuccess) return paged_status(e);
-  return paged_status(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
+  return paged_status(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }

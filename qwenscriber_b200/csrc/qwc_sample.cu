@@ -5,10 +5,13 @@
 // top_k cuts it by count, top_p by the sum of w, min_p by w itself. So the
 // kept set is one threshold logit and a number of tokens that equal it:
 // everything above, and the first of those at it. No sort: the threshold is
-// found by narrowing. A histogram over (m - x) / T in steps of 1/32 gives the
-// bin that holds it; the tokens of that bin, a few hundred as a rule, go to the first CTA, which finds the rest
-// by histograms over the logits' order-preserving bits, eight at a time (all CTAs do so where a bin has too many). The token is the first in index order
-// whose running sum of the kept w passes u times their total.
+// found by narrowing, ten bits at a time. A histogram of (m - x) / T in steps of
+// 1/32 says how far down the kept set can reach; where that is 1024 tokens or
+// fewer, as a rule, they go to the first CTA of the row, which narrows by the logits'
+// order-preserving bits (count or mass against its target) and then by the index
+// (mass against u times the total) among them alone. Where it is more, all CTAs
+// narrow together, and the token is the first in index order whose running sum
+// passes.
 //
 // Sums are of integers, w in units of 2^-42: they are exact, so neither the
 // order of the atomics nor the split over threads changes a result.
@@ -32,8 +35,8 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr uint32_t kBins = kSampleThreads;  // a scan takes one bin for each thread
-constexpr uint32_t kFineBits = 8, kFineBins = 1u << kFineBits;
-constexpr uint32_t kListed = 512;           // tokens of one coarse bin that the first CTA can take by themselves
+constexpr uint32_t kBinBits = 10;
+constexpr uint32_t kListed = kSampleThreads;  // tokens that the first CTA takes by itself, one for each thread
 constexpr uint32_t kLimbBits = 14;          // 2^17 tokens of a slice times 2^14 stay below 2^32
 constexpr float kBinScale = 32.0f;      // coarse bins in a nat; the last bin takes all below e^-32, whose units are 0
 constexpr float kUnits = 4398046511104.0f;  // 2^42: 2^20 tokens of weight 1 stay below 2^63
@@ -101,10 +104,9 @@ __device__ __forceinline__ uint64_t warp_scan_u64(uint64_t v) {
   return v;
 }
 
-template <uint32_t BINS>
 struct Histogram {
-  uint64_t mass[BINS];
-  uint32_t count[BINS];
+  uint64_t mass[kBins];
+  uint32_t count[kBins];
 };
 
 // Where a prefix of the order ends: at the tokens whose key is `key`, with `count` tokens and `mass` above
@@ -117,16 +119,21 @@ struct Cut {
 
 struct SampleSmem {
   // The first CTA's are the row's.
-  Histogram<kBins> coarse;
-  Histogram<kFineBins> fine;
+  uint32_t coarse_count[kBins];
   union {
-    uint32_t limb[3][kBins];  // the slice's masses by bin, in limbs: 32-bit additions are native, 64-bit ones are not
+    uint64_t coarse_mass[kBins];
     struct {
       uint64_t units[kListed];
       uint32_t key[kListed];
+      uint32_t index[kListed];  // the top bit: less than min_p
     } list;
   };
+  union {
+    uint32_t limb[3][kBins];  // the slice's masses by bin, in limbs: 32-bit additions are native, 64-bit ones are not
+    Histogram fine;
+  };
   uint32_t listed;
+  uint32_t reach, reached;  // the last coarse bin that the kept set can touch, and the tokens down to it
   uint64_t sums[kSampleWarps];
   uint64_t scan[kSampleWarps];
   uint32_t scan_count[kSampleWarps];
@@ -139,51 +146,71 @@ struct SampleSmem {
   float values[];
 };
 
-template <uint32_t BINS>
-__device__ __forceinline__ void clear(Histogram<BINS>& h) {
-  if (threadIdx.x < BINS) {
-    h.mass[threadIdx.x] = 0;
-    h.count[threadIdx.x] = 0;
-  }
+__device__ __forceinline__ void clear(Histogram& h) {
+  h.mass[threadIdx.x] = 0;
+  h.count[threadIdx.x] = 0;
 }
 
-template <uint32_t BINS>
-__device__ __forceinline__ void add_to(Histogram<BINS>* h, uint32_t bin, uint32_t count, uint64_t mass) {
-  atomicAdd(&h->count[bin], count);
-  if (mass) atomicAdd(reinterpret_cast<unsigned long long*>(&h->mass[bin]), static_cast<unsigned long long>(mass));
+__device__ __forceinline__ void add_to(uint32_t* counts, uint64_t* masses, uint32_t bin, uint32_t count, uint64_t mass) {
+  atomicAdd(&counts[bin], count);
+  if (mass) atomicAdd(reinterpret_cast<unsigned long long*>(&masses[bin]), static_cast<unsigned long long>(mass));
 }
 
-// The bin of `h` (bin 0 on top) where what lies above it, added to `from`, reaches the target: `target` tokens, or
-// units if by_mass. All threads of the first CTA, one for each bin.
-template <uint32_t BINS>
-__device__ void find_bin(SampleSmem* s, const Histogram<BINS>& h, bool by_mass, uint64_t target, uint32_t from_count, uint64_t from_mass) {
+// Sums over the bins above (bins 0 .. threadIdx.x - 1) of a value for each thread of a CTA.
+template <typename V>
+__device__ V sum_above(SampleSmem* s, V v) {
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint64_t m = threadIdx.x < BINS ? h.mass[threadIdx.x] : 0;
-  const uint32_t n = threadIdx.x < BINS ? h.count[threadIdx.x] : 0;
-  uint64_t im = m;
-  uint32_t in = n;
+  V inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t um = __shfl_up_sync(0xffffffffu, im, o);
-    const uint32_t un = __shfl_up_sync(0xffffffffu, in, o);
-    if (lane >= static_cast<uint32_t>(o)) {
-      im += um;
-      in += un;
-    }
+    const V u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= static_cast<uint32_t>(o)) inc += u;
   }
-  if (lane == 31) {
-    s->scan[warp] = im;
-    s->scan_count[warp] = in;
-  }
+  if (lane == 31) s->scan[warp] = inc;
   __syncthreads();
-  const uint64_t wm = s->scan[lane];
-  const uint32_t wn = s->scan_count[lane];
-  const uint64_t bm = warp_sum_u64(lane < warp ? wm : 0);
-  const uint32_t bn = __reduce_add_sync(0xffffffffu, lane < warp ? wn : 0u);
-  const uint64_t above_mass = from_mass + bm + im - m;
-  const uint32_t above_count = from_count + bn + in - n;
+  V before = lane < warp ? static_cast<V>(s->scan[lane]) : V(0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  return before + inc - v;
+}
+
+// The bin (bin 0 on top) where what lies above it, added to `from`, reaches the target: `target` tokens, or
+// units if by_mass. All threads of a CTA, one for each bin; the answer is in s->cut after the next barrier.
+__device__ void find_bin(SampleSmem* s, const uint32_t* counts, const uint64_t* masses, bool by_mass, uint64_t target,
+                         uint32_t from_count, uint64_t from_mass) {
+  const uint64_t m = masses[threadIdx.x];
+  const uint32_t n = counts[threadIdx.x];
+  const uint64_t above_mass = from_mass + sum_above(s, m);
+  __syncthreads();
+  const uint32_t above_count = from_count + sum_above(s, n);
   const uint64_t above = by_mass ? above_mass : above_count, here = by_mass ? m : n;
   if (above < target && target <= above + here) s->cut = Cut{above_mass, m, above_count, n, threadIdx.x};
+}
+
+// Narrowing within one CTA: of the tokens that take part, one to a thread, with keys lo .. hi, the key at which
+// the falling order reaches the target, in s->cut.bin, and what lies above and at it. False if it is not reached.
+__device__ bool narrow(SampleSmem* s, bool part, uint32_t key, uint64_t units, uint32_t lo, uint32_t hi, bool by_mass, uint64_t target,
+                       Cut& cut) {
+  cut = Cut{0, 0, 0, 0, 0xFFFFFFFFu};
+  for (;;) {
+    clear(s->fine);
+    if (threadIdx.x == 0) s->cut.bin = 0xFFFFFFFFu;
+    __syncthreads();
+    const uint32_t bits = 32 - __clz((hi - lo) | 1u);
+    const uint32_t shift = bits > kBinBits ? bits - kBinBits : 0u;
+    if (part && key >= lo && key <= hi) add_to(s->fine.count, s->fine.mass, (hi - key) >> shift, 1, units);
+    __syncthreads();
+    find_bin(s, s->fine.count, s->fine.mass, by_mass, target, cut.count, cut.mass);
+    __syncthreads();
+    cut = s->cut;
+    if (cut.bin == 0xFFFFFFFFu) return false;
+    hi -= cut.bin << shift;
+    __syncthreads();  // (all have read the cut)
+    if (shift == 0) break;
+    lo = hi - min(hi - lo, (1u << shift) - 1u);
+  }
+  cut.bin = hi;
+  return true;
 }
 
 template <typename T, bool HELD>
@@ -253,10 +280,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
   if (lane == 0) s->sums[warp] = uint64_t(__float_as_uint(best)) << 32 | at;
-  clear(s->coarse);
-  clear(s->fine);
-#pragma unroll
-  for (int i = 0; i < 3; ++i) s->limb[i][threadIdx.x] = 0;
+  s->coarse_count[threadIdx.x] = 0;
   if (threadIdx.x == 0) s->total = 0, s->listed = 0;
   __syncthreads();
   better(__uint_as_float(static_cast<uint32_t>(s->sums[lane] >> 32)), static_cast<uint32_t>(s->sums[lane]));
@@ -279,31 +303,22 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     return;
   }
 
-  // All units, and the coarse histogram.
+  // All units, and how many tokens lie how far below the best.
   auto fall_of = [&](float x) { return x == best ? 0.0f : heat.fall(best, x); };
   auto coarse_bin = [&](float fall) { return static_cast<uint32_t>(fminf(fall * kBinScale, static_cast<float>(kBins - 1))); };
-  const bool cuts = by_count || by_mass;
+  const bool cuts = by_count || by_mass, any_cut = cuts || (!greedy && least > 0.0f);
   uint64_t run_sum = 0;
 #pragma unroll 4
   for (uint32_t i = i0; i < i1; i += 32) {
     const bool in = i + lane < i1;
     const float fall = in ? fall_of(value(i + lane)) : INFINITY;
-    const uint64_t u = units_of(weight_of(fall));
-    run_sum += u;
-    if (cuts) {
+    run_sum += units_of(weight_of(fall));
+    if (any_cut) {
       const uint32_t bin = coarse_bin(fall);
-      // The last bin's units are 0, and it can hold most of a row: one count for all its lanes.
+      // The last bin can hold most of a row: one count for all its lanes.
       const uint32_t last = __ballot_sync(0xffffffffu, in && bin == kBins - 1);
-      if (last && lane == 0) atomicAdd(&s->coarse.count[kBins - 1], static_cast<uint32_t>(__popc(last)));
-      if (in && bin != kBins - 1) {
-        constexpr uint32_t kLimb = (1u << kLimbBits) - 1u;
-        const uint32_t l0 = static_cast<uint32_t>(u) & kLimb, l1 = static_cast<uint32_t>(u >> kLimbBits) & kLimb;
-        const uint32_t l2 = static_cast<uint32_t>(u >> (2 * kLimbBits));
-        atomicAdd(&s->coarse.count[bin], 1u);
-        atomicAdd(&s->limb[0][bin], l0);
-        if (l1) atomicAdd(&s->limb[1][bin], l1);
-        if (l2) atomicAdd(&s->limb[2][bin], l2);
-      }
+      if (last && lane == 0) atomicAdd(&s->coarse_count[kBins - 1], static_cast<uint32_t>(__popc(last)));
+      if (in && bin != kBins - 1) atomicAdd(&s->coarse_count[bin], 1u);
     }
   }
   run_sum = warp_sum_u64(run_sum);
@@ -312,12 +327,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     atomicAdd(reinterpret_cast<unsigned long long*>(&s0->total), static_cast<unsigned long long>(run_sum));
   }
   __syncthreads();
-  if (cuts) {
-    const uint32_t n = s->coarse.count[threadIdx.x];
-    const uint64_t u = s->limb[0][threadIdx.x] + (uint64_t(s->limb[1][threadIdx.x]) << kLimbBits) +
-                       (uint64_t(s->limb[2][threadIdx.x]) << (2 * kLimbBits));
-    if (n) add_to(&s0->coarse, threadIdx.x, rank ? n : 0u, u);
-  }
+  if (any_cut && rank != 0 && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
   cluster.sync();
   const uint64_t all = s0->total;
   const float log_all = logf(static_cast<float>(all) / kUnits);
@@ -330,81 +340,181 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     return;
   }
 
-  // The key at which a prefix reaches the target. Every CTA comes here or none.
-  auto find_cut = [&](bool mass, uint64_t target, uint32_t& key, Cut& cut) {
-    if (rank == 0) find_bin(s, s->coarse, mass, target, 0, 0);
+  // The keys of coarse bins first .. last: their ends in logits, a little wider for their rounding.
+  auto keys_of = [&](uint32_t first, uint32_t last, uint32_t& lo, uint32_t& hi) {
+    const float slack = 4e-7f * (fabsf(best) + heat.heat * (last + 2) / kBinScale);
+    hi = order_key<T>(best - heat.heat * first / kBinScale + slack);
+    lo = last >= kBins - 1 ? 0u : order_key<T>(best - heat.heat * (last + 1) / kBinScale - slack);
+    if (!(best < INFINITY) || !(heat.heat < INFINITY) || !(hi >= lo)) lo = 0, hi = 0xFFFFFFFFu;
+  };
+
+  if (any_cut) {
+    // How far down the kept set can reach. top_p's bin is bounded by the least that the bins' tokens can weigh; where
+    // top_k cuts too, what top_k left has to be known first, and only top_k bounds.
+    if (rank == 0) {
+      const uint32_t n = s->coarse_count[threadIdx.x];
+      const uint32_t above = sum_above(s, n);
+      __syncthreads();
+      if (threadIdx.x == 0) s->reach = kBins - 1;
+      const float floor_weight = threadIdx.x == kBins - 1 ? 0.0f : weight_of((threadIdx.x + 1) / kBinScale) * 0.99999f;
+      const uint64_t floor_mass = units_of(floor_weight) * n;
+      const uint64_t floor_above = sum_above(s, floor_mass);
+      const uint64_t want = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(all)));
+      bool last = false;
+      if (by_count) last |= above < static_cast<uint32_t>(k_given) && static_cast<uint32_t>(k_given) <= above + n;
+      if (by_mass && !by_count) last |= floor_above < want && want <= floor_above + floor_mass;
+      if (!by_mass && least > 0.0f) last |= threadIdx.x == min(static_cast<uint32_t>(-logf(least) * kBinScale) + 1u, kBins - 1);
+      if (by_mass && !by_count && want == 0) last |= threadIdx.x == 0;
+      __syncthreads();
+      if (last) atomicMin(&s->reach, threadIdx.x);
+      __syncthreads();
+      if (threadIdx.x == s->reach) s->reached = above + n;
+    }
     cluster.sync();
-    cut = s0->cut;
-    const uint32_t bin = cut.bin;
-    // The bin's keys: its ends in logits, a little wider for their rounding.
-    const float slack = 4e-7f * (fabsf(best) + heat.heat * (bin + 2) / kBinScale);
-    uint32_t hi = order_key<T>(best - heat.heat * bin / kBinScale + slack);
-    uint32_t lo = bin == kBins - 1 ? 0u : order_key<T>(best - heat.heat * (bin + 1) / kBinScale - slack);
-    if (!(best < INFINITY) || !(hi >= lo)) lo = 0, hi = 0xFFFFFFFFu;
-    const bool by_list = cut.here <= kListed;
-    auto each_of_bin = [&](auto use) {  // the bin's tokens of this slice, those with keys lo .. hi
+    const uint32_t reach = s0->reach, reached = s0->reached;
+    if (reached <= kListed) {
+      // ---- few enough for the first CTA ----
+      uint32_t lo, hi;
+      keys_of(0, reach, lo, hi);
 #pragma unroll 4
       for (uint32_t i = i0; i < i1; i += 32) {
         const bool in = i + lane < i1;
         const float x = in ? value(i + lane) : 0.0f;
         const uint32_t k = order_key<T>(x);
-        bool mine = in && k <= hi && k >= lo;
+        bool mine = in && k >= lo;
         if (!__any_sync(0xffffffffu, mine)) continue;
         const float fall = fall_of(x);
-        mine = mine && coarse_bin(fall) == bin;
-        use(mine, k, units_of(weight_of(fall)));
-      }
-    };
-    if (by_list) {
-      each_of_bin([&](bool mine, uint32_t k, uint64_t u) {
+        mine = mine && coarse_bin(fall) <= reach;
         const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-        if (!votes) return;
+        if (!votes) continue;
         uint32_t at0 = 0;
         if (lane == 0) at0 = atomicAdd(&s0->listed, static_cast<uint32_t>(__popc(votes)));
         at0 = __shfl_sync(0xffffffffu, at0, 0) + __popc(votes & ((1u << lane) - 1u));
         if (mine && at0 < kListed) {
+          const float w = weight_of(fall);
           s0->list.key[at0] = k;
-          s0->list.units[at0] = u;
+          s0->list.index[at0] = (i + lane) | (w < least ? 0x80000000u : 0u);
+          s0->list.units[at0] = units_of(w);
         }
-      });
-      cluster.sync();
-    }
-    const bool have = by_list && rank == 0 && threadIdx.x < min(cut.here, s->listed);
-    const uint32_t my_key = have ? s->list.key[threadIdx.x] : 0u;
-    const uint64_t my_units = have ? s->list.units[threadIdx.x] : 0u;
-    while (!by_list || rank == 0) {
-      const uint32_t bits = 32 - __clz((hi - lo) | 1u);
-      const uint32_t shift = bits > kFineBits ? bits - kFineBits : 0u;
-      if (by_list) {
-        if (have && my_key <= hi && my_key >= lo) add_to(&s->fine, (hi - my_key) >> shift, 1, my_units);
-      } else {
-        each_of_bin([&](bool mine, uint32_t k, uint64_t u) {
-          if (mine) add_to(&s0->fine, (hi - k) >> shift, 1, u);
-        });
-        cluster.sync();
       }
+      cluster.sync();
+      if (rank != 0) return;  // nothing of this CTA is read from here on
+      bool kept = threadIdx.x < min(s->listed, kListed);
+      const uint32_t k = kept ? s->list.key[threadIdx.x] : 0u, index = kept ? s->list.index[threadIdx.x] : 0u;
+      const uint32_t place = ~index & 0x7FFFFFFFu;  // falling in the index
+      const uint64_t u = kept ? s->list.units[threadIdx.x] : 0;
+      const uint32_t place_lo = 0x7FFFFFFFu - (a.vocab - 1), place_hi = 0x7FFFFFFFu;
+      Cut cut = {};
+      // Keeps the tokens down to the cut, and `ties` of those at it, the lowest indices first.
+      auto keep_to = [&](uint32_t ties) {
+        const uint32_t key = cut.bin;
+        if (ties < cut.here) {
+          const bool tie = kept && k == key;
+          Cut at_cut;
+          const bool found = narrow(s, tie, place, u, place_lo, place_hi, false, ties, at_cut);
+          if (tie && found && place < at_cut.bin) kept = false;
+        }
+        kept = kept && k >= key;
+      };
+      uint64_t mass = all;
+      if (by_count) {
+        uint32_t bin_lo, bin_hi;
+        keys_of(0, reach, bin_lo, bin_hi);
+        if (narrow(s, kept, k, u, bin_lo, bin_hi, false, static_cast<uint32_t>(k_given), cut)) keep_to(static_cast<uint32_t>(k_given) - cut.count);
+        if (by_mass) {
+          const uint64_t above = sum_above(s, kept ? u : 0);
+          if (threadIdx.x == kSampleThreads - 1) s->slice_sum = above + (kept ? u : 0);
+          __syncthreads();
+          mass = s->slice_sum;
+          __syncthreads();
+        }
+      }
+      if (by_mass) {
+        uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
+        if (!(p_given > 0.0f) || target < 1) target = 1;
+        if (target > mass) target = mass;
+        if (narrow(s, kept, k, u, lo, hi, true, target, cut)) {
+          const uint64_t each = cut.here_mass / cut.here;
+          keep_to(static_cast<uint32_t>((target - cut.mass + each - 1) / each));
+        }
+      }
+      kept = kept && !(index & 0x80000000u);
+      const uint64_t above = sum_above(s, kept ? u : 0);
+      if (threadIdx.x == kSampleThreads - 1) s->slice_sum = above + (kept ? u : 0);
+      __syncthreads();
+      const uint64_t total = s->slice_sum;
+      const float draw = fminf(fmaxf(a.uniforms[r], 0.0f), 1.0f);
+      uint64_t goal = static_cast<uint64_t>(static_cast<double>(draw) * static_cast<double>(total));
+      if (goal >= total) goal = total - 1;
+      if (narrow(s, kept, place, u, place_lo, place_hi, true, goal + 1, cut) && kept && place == cut.bin) {
+        a.tokens[r] = index;
+        if (a.logprobs) a.logprobs[r] = -fall_of(key_value<T>(k)) - log_all;
+      }
+      return;
+    }
+  }
+
+  if (cuts) {
+    // ---- a large kept set: the masses of the coarse bins, then all CTAs narrow ----
+#pragma unroll
+    for (int i = 0; i < 3; ++i) s->limb[i][threadIdx.x] = 0;
+    s->coarse_mass[threadIdx.x] = 0;
+    cluster.sync();
+#pragma unroll 4
+    for (uint32_t i = i0; i < i1; i += 32) {
+      if (i + lane >= i1) continue;
+      const float fall = fall_of(value(i + lane));
+      const uint32_t bin = coarse_bin(fall);
+      if (bin == kBins - 1) continue;  // (its units are 0)
+      const uint64_t u = units_of(weight_of(fall));
+      constexpr uint32_t kLimb = (1u << kLimbBits) - 1u;
+      const uint32_t l0 = static_cast<uint32_t>(u) & kLimb, l1 = static_cast<uint32_t>(u >> kLimbBits) & kLimb;
+      const uint32_t l2 = static_cast<uint32_t>(u >> (2 * kLimbBits));
+      atomicAdd(&s->limb[0][bin], l0);
+      if (l1) atomicAdd(&s->limb[1][bin], l1);
+      if (l2) atomicAdd(&s->limb[2][bin], l2);
+    }
+    __syncthreads();
+    const uint64_t u = s->limb[0][threadIdx.x] + (uint64_t(s->limb[1][threadIdx.x]) << kLimbBits) +
+                       (uint64_t(s->limb[2][threadIdx.x]) << (2 * kLimbBits));
+    if (u) atomicAdd(reinterpret_cast<unsigned long long*>(&s0->coarse_mass[threadIdx.x]), static_cast<unsigned long long>(u));
+    __syncthreads();
+    clear(s->fine);
+    cluster.sync();
+  }
+
+  // The key at which a prefix reaches the target. Every CTA comes here or none.
+  auto find_cut = [&](bool mass, uint64_t target, uint32_t& key, Cut& cut) {
+    if (rank == 0) find_bin(s, s->coarse_count, s->coarse_mass, mass, target, 0, 0);
+    cluster.sync();
+    cut = s0->cut;
+    const uint32_t bin = cut.bin;
+    uint32_t lo, hi;
+    keys_of(bin, bin, lo, hi);
+    for (;;) {
+      const uint32_t bits = 32 - __clz((hi - lo) | 1u);
+      const uint32_t shift = bits > kBinBits ? bits - kBinBits : 0u;
+#pragma unroll 4
+      for (uint32_t i = i0; i < i1; i += 32) {
+        if (i + lane >= i1) continue;
+        const float x = value(i + lane);
+        const uint32_t k = order_key<T>(x);
+        if (k > hi || k < lo) continue;
+        const float fall = fall_of(x);
+        if (coarse_bin(fall) == bin) add_to(s0->fine.count, s0->fine.mass, (hi - k) >> shift, 1, units_of(weight_of(fall)));
+      }
+      cluster.sync();
       if (rank == 0) {
-        __syncthreads();
-        find_bin(s, s->fine, mass, target, cut.count, cut.mass);
+        find_bin(s, s->fine.count, s->fine.mass, mass, target, cut.count, cut.mass);
         __syncthreads();
         clear(s->fine);
-        if (threadIdx.x == 0) s->listed = 0;
-        __syncthreads();
       }
-      if (!by_list) cluster.sync();
+      cluster.sync();
       cut = s0->cut;
       hi -= cut.bin << shift;
       if (shift == 0) break;
       lo = hi - min(hi - lo, (1u << shift) - 1u);
-      if (!by_list) cluster.sync();  // (the first CTA does not write its cut again before all have read it)
-      if (by_list) __syncthreads();
-    }
-    if (by_list) {
-      __syncthreads();
-      if (rank == 0 && threadIdx.x == 0) s->cut.bin = hi;  // now the key
-      cluster.sync();
-      cut = s0->cut;
-      hi = cut.bin;
+      cluster.sync();  // (the first CTA does not write its cut again before all have read it)
     }
     key = hi;
   };

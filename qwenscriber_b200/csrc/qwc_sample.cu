@@ -6,7 +6,7 @@
 // kept set is one threshold logit and a number of tokens that equal it:
 // everything above, and the first of those at it. No sort: the threshold is
 // found by narrowing, ten bits at a time. A histogram of (m - x) / T in steps of
-// 1/32 says how far down the kept set can reach; where that is 1024 tokens or
+// 1/33 says how far down the kept set can reach; where that is 1024 tokens or
 // fewer, as a rule, they go to the first CTA of the row, which narrows by the logits'
 // order-preserving bits (count or mass against its target) and then by the index
 // (mass against u times the total) among them alone. Where it is more, all CTAs
@@ -37,8 +37,11 @@ constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr uint32_t kBins = kSampleThreads;  // a scan takes one bin for each thread
 constexpr uint32_t kBinBits = 10;
 constexpr uint32_t kListed = kSampleThreads;  // tokens that the first CTA takes by itself, one for each thread
+// Up to this many of them are compared pair by pair, each token by as many lanes as there are: two passes over
+// the list, where narrowing takes two or three histograms for each cut.
+constexpr uint32_t kPairs = 256;
 constexpr uint32_t kLimbBits = 14;          // 2^17 tokens of a slice times 2^14 stay below 2^32
-constexpr float kBinScale = 32.0f;      // coarse bins in a nat; the last bin takes all below e^-32, whose units are 0
+constexpr float kBinScale = 23.0f;      // coarse bins in a power of two; the last bin takes all below 2^-44, whose units are 0
 constexpr float kUnits = 4398046511104.0f;  // 2^42: 2^20 tokens of weight 1 stay below 2^63
 
 struct SampleArgs {
@@ -73,20 +76,14 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~(k | ((1u << kIdle) - 1u)));
 }
 
-// (best - x) / heat, correctly rounded save for the rarest cases: one step of Newton's on the product with
-// the reciprocal.
-struct Heat {
-  float heat, inverse;
-  __device__ __forceinline__ float fall(float best, float x) const {
-    const float d = best - x;
-    const float q = d * inverse;
-    const float r = fmaf(-q, heat, d);
-    const float f = fmaf(r, inverse, q);
-    return f == f ? f : q;  // (d infinite)
-  }
+// How far a logit lies below the best, at the row's temperature and in powers of two: t = (best - x) log2(e) / T,
+// so w = 2^-t. One rounding of t: a relative 2^-24 t of w, below 2e-6 for every w that counts. best - x is 0 for two
+// infinities; a temperature below 1e-37 counts as that.
+struct Fall {
+  float best, scale;
+  __device__ __forceinline__ float of(float x) const { return fmaxf(best - x, 0.0f) * scale; }
 };
-
-__device__ __forceinline__ float weight_of(float fall) { return expf(-fall); }
+__device__ __forceinline__ float weight_of(float t) { return ex2(-t); }
 __device__ __forceinline__ uint64_t units_of(float w) { return __float2ull_rn(w * kUnits); }
 
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
@@ -143,6 +140,7 @@ struct SampleSmem {
   float best;
   uint32_t best_at;
   Cut cut;
+  Cut answer;  // the first CTA's to the others
   float values[];
 };
 
@@ -175,11 +173,9 @@ __device__ V sum_above(SampleSmem* s, V v) {
 }
 
 // The bin (bin 0 on top) where what lies above it, added to `from`, reaches the target: `target` tokens, or
-// units if by_mass. All threads of a CTA, one for each bin; the answer is in s->cut after the next barrier.
-__device__ void find_bin(SampleSmem* s, const uint32_t* counts, const uint64_t* masses, bool by_mass, uint64_t target,
-                         uint32_t from_count, uint64_t from_mass) {
-  const uint64_t m = masses[threadIdx.x];
-  const uint32_t n = counts[threadIdx.x];
+// units if by_mass. All threads of a CTA, each with the n tokens and the mass m of its bin; the answer is in
+// s->cut after the next barrier.
+__device__ void find_bin(SampleSmem* s, uint32_t n, uint64_t m, bool by_mass, uint64_t target, uint32_t from_count, uint64_t from_mass) {
   const uint64_t above_mass = from_mass + sum_above(s, m);
   __syncthreads();
   const uint32_t above_count = from_count + sum_above(s, n);
@@ -188,24 +184,58 @@ __device__ void find_bin(SampleSmem* s, const uint32_t* counts, const uint64_t* 
 }
 
 // Narrowing within one CTA: of the tokens that take part, one to a thread, with keys lo .. hi, the key at which
-// the falling order reaches the target, in s->cut.bin, and what lies above and at it. False if it is not reached.
+// the falling order reaches the target, in cut.bin, and what lies above and at it. False if it is not reached.
+// Eight bits at a time, so that one warp can scan the bins, eight to a lane.
 __device__ bool narrow(SampleSmem* s, bool part, uint32_t key, uint64_t units, uint32_t lo, uint32_t hi, bool by_mass, uint64_t target,
-                       Cut& cut) {
-  cut = Cut{0, 0, 0, 0, 0xFFFFFFFFu};
+                       Cut& cut, uint32_t from_count = 0, uint64_t from_mass = 0) {
+  constexpr uint32_t kBits = 8;
+  const uint32_t lane = threadIdx.x % 32;
+  cut = Cut{from_mass, 0, from_count, 0, 0};
   for (;;) {
-    clear(s->fine);
-    if (threadIdx.x == 0) s->cut.bin = 0xFFFFFFFFu;
+    if (threadIdx.x < (1u << kBits)) {
+      s->fine.mass[threadIdx.x] = 0;
+      s->fine.count[threadIdx.x] = 0;
+    }
     __syncthreads();
     const uint32_t bits = 32 - __clz((hi - lo) | 1u);
-    const uint32_t shift = bits > kBinBits ? bits - kBinBits : 0u;
+    const uint32_t shift = bits > kBits ? bits - kBits : 0u;
     if (part && key >= lo && key <= hi) add_to(s->fine.count, s->fine.mass, (hi - key) >> shift, 1, units);
     __syncthreads();
-    find_bin(s, s->fine.count, s->fine.mass, by_mass, target, cut.count, cut.mass);
+    if (threadIdx.x < 32) {
+      uint64_t m[8], mass = 0;
+      uint32_t n[8], count = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        m[i] = s->fine.mass[8 * lane + i];
+        n[i] = s->fine.count[8 * lane + i];
+        mass += m[i];
+        count += n[i];
+      }
+      uint64_t above_mass = cut.mass + warp_scan_u64(mass) - mass;
+      uint32_t inc = count;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= static_cast<uint32_t>(o)) inc += v;
+      }
+      uint32_t above_count = cut.count + inc - count;
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint64_t above = by_mass ? above_mass : above_count, here = by_mass ? m[i] : n[i];
+        if (above < target && target <= above + here) {
+          s->cut = Cut{above_mass, m[i], above_count, n[i], 8 * lane + i};
+          found = true;
+        }
+        above_mass += m[i];
+        above_count += n[i];
+      }
+      if (!__any_sync(0xffffffffu, found) && lane == 0) s->cut.bin = 0xFFFFFFFFu;
+    }
     __syncthreads();
     cut = s->cut;
     if (cut.bin == 0xFFFFFFFFu) return false;
     hi -= cut.bin << shift;
-    __syncthreads();  // (all have read the cut)
     if (shift == 0) break;
     lo = hi - min(hi - lo, (1u << shift) - 1u);
   }
@@ -225,7 +255,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const float heat_given = a.temperature ? a.temperature[r] : 1.0f;
   const bool greedy = !(heat_given > 0.0f);
-  const Heat heat{greedy ? 1.0f : heat_given, 1.0f / (greedy ? 1.0f : heat_given)};
+  const float heat = greedy ? 1.0f : fmaxf(heat_given, 1e-37f);
   const int32_t k_given = a.top_k ? a.top_k[r] : 0;
   const float p_given = a.top_p ? a.top_p[r] : 1.0f;
   const float least = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
@@ -304,22 +334,31 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   }
 
   // All units, and how many tokens lie how far below the best.
-  auto fall_of = [&](float x) { return x == best ? 0.0f : heat.fall(best, x); };
-  auto coarse_bin = [&](float fall) { return static_cast<uint32_t>(fminf(fall * kBinScale, static_cast<float>(kBins - 1))); };
+  const Fall scaled{best, 1.4426950408889634f / heat};
+  auto fall_of = [&](float x) { return scaled.of(x); };
+  auto coarse_bin = [&](float t) { return static_cast<uint32_t>(fminf(t * kBinScale, static_cast<float>(kBins - 1))); };
   const bool cuts = by_count || by_mass, any_cut = cuts || (!greedy && least > 0.0f);
   uint64_t run_sum = 0;
-#pragma unroll 4
-  for (uint32_t i = i0; i < i1; i += 32) {
-    const bool in = i + lane < i1;
-    const float fall = in ? fall_of(value(i + lane)) : INFINITY;
-    run_sum += units_of(weight_of(fall));
+  auto count_in = [&](float t) {
     if (any_cut) {
-      const uint32_t bin = coarse_bin(fall);
+      const uint32_t bin = coarse_bin(t);
       // The last bin can hold most of a row: one count for all its lanes.
-      const uint32_t last = __ballot_sync(0xffffffffu, in && bin == kBins - 1);
+      const uint32_t last = __ballot_sync(0xffffffffu, bin == kBins - 1);
       if (last && lane == 0) atomicAdd(&s->coarse_count[kBins - 1], static_cast<uint32_t>(__popc(last)));
-      if (in && bin != kBins - 1) atomicAdd(&s->coarse_count[bin], 1u);
+      if (bin != kBins - 1) atomicAdd(&s->coarse_count[bin], 1u);
     }
+  };
+  const uint32_t whole = i0 + (i1 - i0) / 32 * 32;
+#pragma unroll 4
+  for (uint32_t i = i0; i < whole; i += 32) {
+    const float t = fall_of(value(i + lane));
+    run_sum += units_of(weight_of(t));
+    count_in(t);
+  }
+  if (whole + lane < i1) {
+    const float t = fall_of(value(whole + lane));
+    run_sum += units_of(weight_of(t));
+    if (any_cut) atomicAdd(&s->coarse_count[coarse_bin(t)], 1u);
   }
   run_sum = warp_sum_u64(run_sum);
   if (lane == 0) {
@@ -331,6 +370,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   cluster.sync();
   const uint64_t all = s0->total;
   const float log_all = logf(static_cast<float>(all) / kUnits);
+  auto log_of = [&](float x) { return (x == best ? 0.0f : (x - best) / heat) - log_all; };
   if (greedy) {
     if (rank == 0 && threadIdx.x == 0) {
       a.tokens[r] = at;
@@ -341,37 +381,45 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   }
 
   // The keys of coarse bins first .. last: their ends in logits, a little wider for their rounding.
+  const float step_heat = heat * 0.6931471805599453f;  // of a power of two, in logits
   auto keys_of = [&](uint32_t first, uint32_t last, uint32_t& lo, uint32_t& hi) {
-    const float slack = 4e-7f * (fabsf(best) + heat.heat * (last + 2) / kBinScale);
-    hi = order_key<T>(best - heat.heat * first / kBinScale + slack);
-    lo = last >= kBins - 1 ? 0u : order_key<T>(best - heat.heat * (last + 1) / kBinScale - slack);
-    if (!(best < INFINITY) || !(heat.heat < INFINITY) || !(hi >= lo)) lo = 0, hi = 0xFFFFFFFFu;
+    const float slack = 4e-7f * (fabsf(best) + step_heat * (last + 2) / kBinScale);
+    hi = order_key<T>(best - step_heat * first / kBinScale + slack);
+    lo = last >= kBins - 1 ? 0u : order_key<T>(best - step_heat * (last + 1) / kBinScale - slack);
+    if (!(best < INFINITY) || !(step_heat < INFINITY) || !(hi >= lo)) lo = 0, hi = 0xFFFFFFFFu;
   };
 
   if (any_cut) {
     // How far down the kept set can reach. top_p's bin is bounded by the least that the bins' tokens can weigh; where
     // top_k cuts too, what top_k left has to be known first, and only top_k bounds.
-    if (rank == 0) {
-      const uint32_t n = s->coarse_count[threadIdx.x];
+    // (Every CTA works it out from the first one's counts.)
+    uint32_t reach, reached;
+    {
+      const uint32_t n = s0->coarse_count[threadIdx.x];
       const uint32_t above = sum_above(s, n);
       __syncthreads();
       if (threadIdx.x == 0) s->reach = kBins - 1;
-      const float floor_weight = threadIdx.x == kBins - 1 ? 0.0f : weight_of((threadIdx.x + 1) / kBinScale) * 0.99999f;
-      const uint64_t floor_mass = units_of(floor_weight) * n;
-      const uint64_t floor_above = sum_above(s, floor_mass);
       const uint64_t want = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(all)));
+      uint64_t floor_mass = 0, floor_above = 0;
+      if (by_mass && !by_count) {
+        floor_mass = threadIdx.x == kBins - 1 ? 0 : units_of(weight_of((threadIdx.x + 1) / kBinScale) * 0.99999f) * n;
+        floor_above = sum_above(s, floor_mass);
+      } else {
+        __syncthreads();
+      }
       bool last = false;
       if (by_count) last |= above < static_cast<uint32_t>(k_given) && static_cast<uint32_t>(k_given) <= above + n;
       if (by_mass && !by_count) last |= floor_above < want && want <= floor_above + floor_mass;
-      if (!by_mass && least > 0.0f) last |= threadIdx.x == min(static_cast<uint32_t>(-logf(least) * kBinScale) + 1u, kBins - 1);
+      if (!by_mass && least > 0.0f) last |= threadIdx.x == min(static_cast<uint32_t>(fmaxf(-log2f(least), 0.0f) * kBinScale) + 1u, kBins - 1);
       if (by_mass && !by_count && want == 0) last |= threadIdx.x == 0;
       __syncthreads();
       if (last) atomicMin(&s->reach, threadIdx.x);
       __syncthreads();
-      if (threadIdx.x == s->reach) s->reached = above + n;
+      reach = s->reach;
+      if (threadIdx.x == reach) s->reached = above + n;
+      __syncthreads();
+      reached = s->reached;
     }
-    cluster.sync();
-    const uint32_t reach = s0->reach, reached = s0->reached;
     if (reached <= kListed) {
       // ---- few enough for the first CTA ----
       uint32_t lo, hi;
@@ -399,7 +447,72 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       }
       cluster.sync();
       if (rank != 0) return;  // nothing of this CTA is read from here on
-      bool kept = threadIdx.x < min(s->listed, kListed);
+      const uint32_t listed = min(s->listed, kListed);
+      const float draw = fminf(fmaxf(a.uniforms[r], 0.0f), 1.0f);
+      auto goal_of = [&](uint64_t total) {
+        const uint64_t goal = static_cast<uint64_t>(static_cast<double>(draw) * static_cast<double>(total));
+        return goal >= total ? total - 1 : goal;
+      };
+      auto target_of = [&](uint64_t mass) {  // top_p's
+        const uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
+        return !(p_given > 0.0f) || target < 1 ? uint64_t(1) : target > mass ? mass : target;
+      };
+      if (listed <= kPairs) {
+        // Lanes of a token: a power of two, at most a warp.
+        uint32_t lanes = 32;
+        while (lanes * listed > kSampleThreads) lanes /= 2;
+        const uint32_t me = threadIdx.x / lanes, part = threadIdx.x % lanes;
+        const bool in = me < listed;
+        const uint32_t k = in ? s->list.key[me] : 0u, index = in ? s->list.index[me] & 0x7FFFFFFFu : 0u;
+        const bool low = in && (s->list.index[me] & 0x80000000u);
+        const uint64_t u = in ? s->list.units[me] : 0;
+        uint32_t place = 0;
+        uint64_t above = 0;
+        if (in) {
+          for (uint32_t j = part; j < listed; j += lanes) {
+            const uint32_t kj = s->list.key[j];
+            if (kj > k || (kj == k && (s->list.index[j] & 0x7FFFFFFFu) < index)) {
+              ++place;
+              above += s->list.units[j];
+            }
+          }
+        }
+        for (uint32_t o = lanes / 2; o > 0; o /= 2) {
+          place += __shfl_xor_sync(0xffffffffu, place, o);
+          above += __shfl_xor_sync(0xffffffffu, above, o);
+        }
+        bool kept = in && !(by_count && place >= static_cast<uint32_t>(k_given));
+        uint64_t mass = all;
+        if (by_count) {
+          // The last token that top_k keeps has all of their mass behind it.
+          const uint32_t last = min(static_cast<uint32_t>(k_given), listed) - 1;
+          if (in && place == last && part == 0) s->slice_sum = above + u;
+          __syncthreads();
+          mass = s->slice_sum;
+        }
+        if (by_mass) kept = kept && above < target_of(mass);
+        kept = kept && !low;
+        __syncthreads();
+        if (in && part == 0 && !kept) s->list.units[me] = 0;
+        __syncthreads();
+        uint64_t before = 0, total = 0;
+        for (uint32_t j = part; j < listed; j += lanes) {
+          const uint64_t uj = s->list.units[j];
+          total += uj;
+          if ((s->list.index[j] & 0x7FFFFFFFu) < index) before += uj;
+        }
+        for (uint32_t o = lanes / 2; o > 0; o /= 2) {
+          before += __shfl_xor_sync(0xffffffffu, before, o);
+          total += __shfl_xor_sync(0xffffffffu, total, o);
+        }
+        const uint64_t goal = goal_of(total);
+        if (kept && part == 0 && before <= goal && goal < before + u) {
+          a.tokens[r] = index;
+          if (a.logprobs) a.logprobs[r] = log_of(key_value<T>(k));
+        }
+        return;
+      }
+      bool kept = threadIdx.x < listed;
       const uint32_t k = kept ? s->list.key[threadIdx.x] : 0u, index = kept ? s->list.index[threadIdx.x] : 0u;
       const uint32_t place = ~index & 0x7FFFFFFFu;  // falling in the index
       const uint64_t u = kept ? s->list.units[threadIdx.x] : 0;
@@ -430,9 +543,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         }
       }
       if (by_mass) {
-        uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
-        if (!(p_given > 0.0f) || target < 1) target = 1;
-        if (target > mass) target = mass;
+        const uint64_t target = target_of(mass);
         if (narrow(s, kept, k, u, lo, hi, true, target, cut)) {
           const uint64_t each = cut.here_mass / cut.here;
           keep_to(static_cast<uint32_t>((target - cut.mass + each - 1) / each));
@@ -442,20 +553,19 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       const uint64_t above = sum_above(s, kept ? u : 0);
       if (threadIdx.x == kSampleThreads - 1) s->slice_sum = above + (kept ? u : 0);
       __syncthreads();
-      const uint64_t total = s->slice_sum;
-      const float draw = fminf(fmaxf(a.uniforms[r], 0.0f), 1.0f);
-      uint64_t goal = static_cast<uint64_t>(static_cast<double>(draw) * static_cast<double>(total));
-      if (goal >= total) goal = total - 1;
+      const uint64_t goal = goal_of(s->slice_sum);
       if (narrow(s, kept, place, u, place_lo, place_hi, true, goal + 1, cut) && kept && place == cut.bin) {
         a.tokens[r] = index;
-        if (a.logprobs) a.logprobs[r] = -fall_of(key_value<T>(k)) - log_all;
+        if (a.logprobs) a.logprobs[r] = log_of(key_value<T>(k));
       }
       return;
     }
   }
 
+  uint32_t bin_count = 0;  // of coarse bin threadIdx.x, over the row
+  uint64_t bin_mass = 0;
   if (cuts) {
-    // ---- a large kept set: the masses of the coarse bins, then all CTAs narrow ----
+    // ---- a large kept set: the masses of the coarse bins, then the one that holds the cut ----
 #pragma unroll
     for (int i = 0; i < 3; ++i) s->limb[i][threadIdx.x] = 0;
     s->coarse_mass[threadIdx.x] = 0;
@@ -481,40 +591,83 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     __syncthreads();
     clear(s->fine);
     cluster.sync();
+    bin_count = s0->coarse_count[threadIdx.x];
+    bin_mass = s0->coarse_mass[threadIdx.x];
+    cluster.sync();  // (the list takes the masses' room)
   }
 
   // The key at which a prefix reaches the target. Every CTA comes here or none.
   auto find_cut = [&](bool mass, uint64_t target, uint32_t& key, Cut& cut) {
-    if (rank == 0) find_bin(s, s->coarse_count, s->coarse_mass, mass, target, 0, 0);
-    cluster.sync();
-    cut = s0->cut;
+    __syncthreads();
+    find_bin(s, bin_count, bin_mass, mass, target, 0, 0);
+    __syncthreads();
+    cut = s->cut;
     const uint32_t bin = cut.bin;
     uint32_t lo, hi;
     keys_of(bin, bin, lo, hi);
-    for (;;) {
-      const uint32_t bits = 32 - __clz((hi - lo) | 1u);
-      const uint32_t shift = bits > kBinBits ? bits - kBinBits : 0u;
+    const bool by_list = cut.here <= kListed;
+    auto each_of_bin = [&](auto use) {  // the bin's tokens of this slice, those with keys lo .. hi
 #pragma unroll 4
       for (uint32_t i = i0; i < i1; i += 32) {
-        if (i + lane >= i1) continue;
-        const float x = value(i + lane);
+        const bool in = i + lane < i1;
+        const float x = in ? value(i + lane) : 0.0f;
         const uint32_t k = order_key<T>(x);
-        if (k > hi || k < lo) continue;
+        bool mine = in && k <= hi && k >= lo;
+        if (!__any_sync(0xffffffffu, mine)) continue;
         const float fall = fall_of(x);
-        if (coarse_bin(fall) == bin) add_to(s0->fine.count, s0->fine.mass, (hi - k) >> shift, 1, units_of(weight_of(fall)));
+        mine = mine && coarse_bin(fall) == bin;
+        use(mine, k, units_of(weight_of(fall)));
       }
+    };
+    if (by_list) {
+      each_of_bin([&](bool mine, uint32_t k, uint64_t u) {
+        const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+        if (!votes) return;
+        uint32_t at0 = 0;
+        if (lane == 0) at0 = atomicAdd(&s0->listed, static_cast<uint32_t>(__popc(votes)));
+        at0 = __shfl_sync(0xffffffffu, at0, 0) + __popc(votes & ((1u << lane) - 1u));
+        if (mine && at0 < kListed) {
+          s0->list.key[at0] = k;
+          s0->list.units[at0] = u;
+        }
+      });
       cluster.sync();
       if (rank == 0) {
-        find_bin(s, s->fine.count, s->fine.mass, mass, target, cut.count, cut.mass);
+        const bool have = threadIdx.x < min(s->listed, kListed);
+        const uint32_t k = have ? s->list.key[threadIdx.x] : 0u;
+        const uint64_t u = have ? s->list.units[threadIdx.x] : 0;
+        Cut found;
+        narrow(s, have, k, u, lo, hi, mass, target, found, cut.count, cut.mass);
+        if (threadIdx.x == 0) {
+          s->answer = found;
+          s->listed = 0;
+        }
         __syncthreads();
-        clear(s->fine);
       }
       cluster.sync();
-      cut = s0->cut;
-      hi -= cut.bin << shift;
-      if (shift == 0) break;
-      lo = hi - min(hi - lo, (1u << shift) - 1u);
-      cluster.sync();  // (the first CTA does not write its cut again before all have read it)
+      cut = s0->answer;
+      hi = cut.bin;
+    } else {
+      for (;;) {
+        const uint32_t bits = 32 - __clz((hi - lo) | 1u);
+        const uint32_t shift = bits > kBinBits ? bits - kBinBits : 0u;
+        each_of_bin([&](bool mine, uint32_t k, uint64_t u) {
+          if (mine) add_to(s0->fine.count, s0->fine.mass, (hi - k) >> shift, 1, u);
+        });
+        cluster.sync();
+        if (rank == 0) {
+          find_bin(s, s->fine.count[threadIdx.x], s->fine.mass[threadIdx.x], mass, target, cut.count, cut.mass);
+          __syncthreads();
+          clear(s->fine);
+          if (threadIdx.x == 0) s->answer = s->cut;
+        }
+        cluster.sync();
+        cut = s0->answer;
+        hi -= cut.bin << shift;
+        cluster.sync();  // (the first CTA does not answer again before all have read it)
+        if (shift == 0) break;
+        lo = hi - min(hi - lo, (1u << shift) - 1u);
+      }
     }
     key = hi;
   };
@@ -530,7 +683,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     mass = cut.mass + cut.here_mass / cut.here * ties;
   }
   if (by_mass) {
-    if (by_count) cluster.sync();  // (all have read the first cut)
+    if (by_count) cluster.sync();  // (all have read the first answer)
     uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
     if (!(p_given > 0.0f) || target < 1) target = 1;
     if (target > mass) target = mass;
@@ -607,7 +760,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       if (past) {
         if (lane == static_cast<uint32_t>(__ffs(past)) - 1) {
           a.tokens[r] = i + lane;
-          if (a.logprobs) a.logprobs[r] = -fall_of(value(i + lane)) - log_all;
+          if (a.logprobs) a.logprobs[r] = log_of(value(i + lane));
         }
         break;
       }
@@ -619,9 +772,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
 
 template <typename T>
 int32_t sample_as(SampleArgs a, uint32_t rows, cudaStream_t stream) {
-  const uint32_t size = 8;
-  a.run = ((a.vocab + size * kSampleWarps - 1) / (size * kSampleWarps) + 31) / 32 * 32;
+  // CTAs to a row: as few as hold it in their shared memory, then twice as many while there are SMs for all rows, at
+  // most 8. One row of 151936: eight CTAs 17.6 us, four 23.5 (sixteen 17.6); 64 rows: four 67 us, eight 84 (more waves,
+  // each with a row's dozen exchanges), two 137 (slices that do not fit are read again and again).
   const uint32_t most = (227 * 1024 - 1024 - static_cast<uint32_t>(sizeof(SampleSmem))) / 4;
+  uint32_t size = 1;
+  while (size < 8 && (uint64_t(size) * most < a.vocab || rows * size * 2 <= 148)) size *= 2;
+  a.run = ((a.vocab + size * kSampleWarps - 1) / (size * kSampleWarps) + 31) / 32 * 32;
   a.held = a.run * kSampleWarps < most ? a.run * kSampleWarps : most;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * size);

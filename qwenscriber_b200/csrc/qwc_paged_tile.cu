@@ -77,6 +77,10 @@ struct TileConfig {
   static constexpr int CONVERT_REGS = 64;
   static_assert(4 * TILES * SOFTMAX_REGS + 2 * CONVERT_WARPS * CONVERT_REGS + LAUNCH_REGS <= WARPS * LAUNCH_REGS,
                 "a split cannot exceed the launch");
+  // The tensor cores cut off what an addition to an f32 sum leaves over, always towards zero: over n additions the
+  // output loses about n times 8e-9 of its size (2048 positions in two parts, 256 additions: 2e-6). f32 rows therefore
+  // start a new sum every FLUSH steps, and the sums are added in f32 in global memory.
+  static constexpr uint32_t FLUSH = SPLIT ? 8 : 1u << 31;
   // The weights' power of two, 2^(UP - vexp): weight times value scale below 2^15 (exact), value below 2^7 (scaled).
   static constexpr int UP = SCALED ? 14 : 21;
 };
@@ -444,8 +448,40 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       // Maxima and sums are those of scores in powers of two.
       float m = -INFINITY, l = 0.0f;
       uint32_t vexp = 0;
+      // f32: the sums so far, in units of the maximum flushed_m: [DIM / 4][HEIGHT] of four dims.
+      float4* const flushed = reinterpret_cast<float4*>(p.partials + (size_t(2) * gridDim.x * (DIM + 2) + size_t(blockIdx.x) * DIM) * HEIGHT);
+      float flushed_m = -INFINITY;
+      bool any_flushed = false;
       for (uint32_t j = j0; j < j1; ++j, ++it) {
         const uint32_t b = it & 3u;
+        if (SPLIT && j > j0 && (j - j0) % C::FLUSH == 0) {
+          ok = __all_sync(0xffffffffu, wait(&sm->pv_done[t], it - 1, 213));
+          if (!ok) break;
+          tc_fence_after();
+          // (m == -inf: this row has seen nothing, and its columns are sums of zeros.)
+          const float old = any_flushed && flushed_m != -INFINITY ? ex2(flushed_m - m) : 0.0f;
+          const float unit = pow2i(static_cast<int>(vexp) - C::UP);
+#pragma unroll 1
+          for (int i = 0; i < DIM; i += 32) {
+            float4 f[8];
+            if (any_flushed) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = flushed[size_t(i / 4 + e) * HEIGHT + tid];
+            }
+            float o[32];
+            tmem_ld32(taddr + kOutput + i, o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (!any_flushed) f[e] = make_float4(0, 0, 0, 0);
+              flushed[size_t(i / 4 + e) * HEIGHT + tid] =
+                  make_float4(fmaf(f[e].x, old, o[4 * e] * unit), fmaf(f[e].y, old, o[4 * e + 1] * unit),
+                              fmaf(f[e].z, old, o[4 * e + 2] * unit), fmaf(f[e].w, old, o[4 * e + 3] * unit));
+            }
+          }
+          tc_fence_before();
+          flushed_m = m;
+          any_flushed = true;
+        }
         ok = __all_sync(0xffffffffu, wait(&sm->ks_full[b], it >> 2, 210) && wait(&sm->s_full[it & 1u][t], it >> 1, 201) &&
                                             wait(&sm->vs_full[b], it >> 2, 211));
         if (!ok) break;
@@ -508,7 +544,8 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           vexp = top;
           grew = true;
         }
-        if (j > j0 && __any_sync(0xffffffffu, grew)) {
+        const bool fresh = (j - j0) % C::FLUSH == 0;  // nothing in the output's columns
+        if (!fresh && __any_sync(0xffffffffu, grew)) {
           // The last step's output must be complete. (The one before it is: its MMAs came before this step's scores.)
           ok = __all_sync(0xffffffffu, wait(&sm->pv_done[t], it - 1, 212));
           if (!ok) break;
@@ -608,14 +645,29 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         }
         __syncwarp();
       };
+      // 32 dims of the row's sum, in true units.
+      const float old = any_flushed && flushed_m != -INFINITY ? ex2(flushed_m - m) : 0.0f;
+      auto row_sum = [&](int i, float (&o)[32]) {
+        tmem_ld32(taddr + kOutput + i, o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * back;  // (nothing seen: the columns may hold anything)
+        if (SPLIT && any_flushed) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 f = flushed[size_t((i + e) / 4) * HEIGHT + tid];
+            o[e] = fmaf(f.x, old, o[e]), o[e + 1] = fmaf(f.y, old, o[e + 1]);
+            o[e + 2] = fmaf(f.z, old, o[e + 2]), o[e + 3] = fmaf(f.w, old, o[e + 3]);
+          }
+        }
+      };
       if (whole) {
-        const float inv = l == 0.0f ? 0.0f : back / l;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
         for (int i = 0; i < DIM; i += 32) {
           float o[32];
-          tmem_ld32(taddr + kOutput + i, o);
+          row_sum(i, o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : o[e] * inv;
+          for (int e = 0; e < 32; ++e) o[e] *= inv;
           put_row(i, o);
         }
         write_rows();
@@ -627,12 +679,10 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
 #pragma unroll 1
         for (int i = 0; i < DIM; i += 32) {
           float o[32];
-          tmem_ld32(taddr + kOutput + i, o);
+          row_sum(i, o);
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const float k = l == 0.0f ? 0.0f : 1.0f;  // (l == 0: nothing seen, and the columns may hold anything)
-            reinterpret_cast<float4*>(mine)[size_t((i + e) / 4) * HEIGHT + tid] =
-                k == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o[e] * back, o[e + 1] * back, o[e + 2] * back, o[e + 3] * back);
+            reinterpret_cast<float4*>(mine)[size_t((i + e) / 4) * HEIGHT + tid] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
         mine[size_t(DIM) * HEIGHT + tid] = m;
@@ -854,12 +904,12 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       for (int g = 0; g < G; ++g) {
         const uint64_t kd = k0 + (st * G + g) * kKvTile;
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
+        for (int q = PARTS - 1; q >= 0; --q) {  // lo before hi: while the sum is small, so is what an addition rounds off
           const uint64_t qd = q0 + ((t * PARTS + q) * G + g) * kQTile;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // 16 dims: 32 bytes of each row
             mma_ss(base + t * C::TMEM_TILE + (SCALED ? (n & 1u) * kStep : g * kStep), qd + 2 * kk, kd + 2 * kk, kIdescScores,
-                   (SCALED && g > 0) || q > 0 || kk > 0);
+                   (SCALED && g > 0) || q < PARTS - 1 || kk > 0);
           }
         }
       }
@@ -906,7 +956,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           ok = wait_all(&sm->p_full[it & 1u][t], it >> 1, 208);
           if (!ok) break;
           tc_fence_after();
-          output(t, it, j == j0);
+          output(t, it, (j - j0) % C::FLUSH == 0);
           mma_commit(&sm->pv_done[t]);
           if (!more) mma_commit(&sm->o_full[t]);
           if (t == TILES - 1) mma_commit(&sm->v_empty[it % STAGES]);
@@ -958,7 +1008,8 @@ TilePlan paged_tile_plan(const PagedArgs& a, uint32_t heads, uint32_t sms) {
   const uint64_t most = plan.tiles == 2 ? sms : 2 * sms;  // what is resident at once
   plan.too_long = steps / most >= 0x7FFFFFFFu;            // a stretch's steps are counted in 31 bits
   plan.grid = static_cast<uint32_t>(steps < most ? steps : most);
-  plan.partial_bytes = uint64_t(2) * plan.grid * (a.head_dim + 2) * height * 4;
+  // Two partial tiles a CTA, and its sums (f32 rows).
+  plan.partial_bytes = uint64_t(plan.grid) * (2 * (a.head_dim + 2) + a.head_dim) * height * 4;
   return plan;
 }
 

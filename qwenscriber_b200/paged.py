@@ -27,7 +27,13 @@ def refuse(name: str, call: str):
     raise QwcError(STATUS_CODE[name], call)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def current_stream(device: torch.device) -> int:
+    """torch's current stream of a device, as the C ABI takes it."""
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -60,6 +66,8 @@ class PagedCache:
         self.desc = PagedCacheDesc(k_scales.data_ptr(), k_codes.data_ptr(), v_scales.data_ptr(), v_codes.data_ptr(),
                                    self.pages, page_size, kv_heads, head_dim)
         self._ref = ctypes.addressof(self.desc)
+        self._index = self.device.index
+        self._key = (self.pages, page_size, kv_heads, head_dim)
 
     @classmethod
     def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda") -> "PagedCache":
@@ -101,10 +109,18 @@ def _rows(t: torch.Tensor, batch: PagedBatch, heads: int, dim: int, call: str) -
         refuse("shape_mismatch", call)
     if t.device != batch.device:
         refuse("invalid_argument", call)
-    stride = t.stride()
-    if (stride[2] != 1 and dim > 1) or (stride[1] != dim and heads > 1):
+    row, head, one = t.stride()
+    if (one != 1 and dim > 1) or (head != dim and heads > 1):
         refuse("invalid_argument", call)
-    return stride[0] if batch.tokens > 1 else max(stride[0], heads * dim)
+    return row if batch.tokens > 1 else max(row, heads * dim)
+
+
+def _table(t: torch.Tensor, shape: tuple, device: torch.device, call: str) -> None:
+    """f32 values of `shape` (rotation tables, norm weights)."""
+    if t.shape != shape:
+        refuse("shape_mismatch", call)
+    if t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+        refuse("invalid_argument", call)
 
 
 # Partial results of attention, one buffer for each (device, stream), zeroed when it is made and
@@ -112,19 +128,21 @@ def _rows(t: torch.Tensor, batch: PagedBatch, heads: int, dim: int, call: str) -
 _workspaces: dict = {}
 
 
-def _workspace(cache: PagedCache, batch: PagedBatch, fmt: int, heads: int, stream: int) -> torch.Tensor:
-    key = (cache.pages, cache.page_size, cache.kv_heads, cache.head_dim, fmt, heads)
+def _workspace(cache: PagedCache, batch: PagedBatch, fmt: int, heads: int, stream: int) -> tuple[int, int]:
+    """(address, bytes) of the stream's buffer, at least what this call needs."""
+    at = (cache._index, stream)
+    held = _workspaces.get(at)
+    key = (cache._key, fmt, heads)
     need = batch._workspace_bytes.get(key)
     if need is None:
         n = ctypes.c_uint64(0)
         check(lib().qwc_op_paged_attention_workspace(cache._ref, batch._ref, fmt, heads, ctypes.byref(n)),
               "qwc_op_paged_attention_workspace")
         need = batch._workspace_bytes[key] = n.value
-    at = (cache.device, stream)
-    held = _workspaces.get(at)
-    if held is None or held.numel() < need:
-        held = _workspaces[at] = torch.zeros(need, dtype=torch.uint8, device=cache.device)
-    return held
+    if held is None or held[1] < need:
+        buffer = torch.zeros(need, dtype=torch.uint8, device=cache.device)
+        held = _workspaces[at] = (buffer.data_ptr(), need, buffer)
+    return held[0], held[1]
 
 
 def append(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
@@ -134,25 +152,31 @@ def append(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, k: torch.Tenso
     for attention (`q_out`, a new tensor unless given; may be `q`)."""
     call = "qwc_op_paged_append"
     fmt = format_of(q, call)
-    if k.dtype != q.dtype or v.dtype != q.dtype or cache.device != batch.device or q.dim() != 3:
+    dtype, device = q.dtype, batch.device
+    if k.dtype != dtype or v.dtype != dtype or cache.device != device or q.dim() != 3:
         refuse("invalid_argument", call)
-    heads, dim = q.shape[1], cache.head_dim
+    heads, dim, kv_heads = q.shape[1], cache.head_dim, cache.kv_heads
+    q_stride, k_stride = _rows(q, batch, heads, dim, call), _rows(k, batch, kv_heads, dim, call)
+    v_stride = _rows(v, batch, kv_heads, dim, call)
     if q_out is None:
-        q_out = torch.empty(batch.tokens, heads, dim, dtype=q.dtype, device=q.device)
-    elif q_out.dtype != q.dtype:
+        q_out, out_stride = torch.empty((batch.tokens, heads, dim), dtype=dtype, device=device), heads * dim
+    elif q_out.dtype != dtype:
         refuse("invalid_argument", call)
-    strides = [_rows(t, batch, n, dim, call) for t, n in ((q, heads), (k, cache.kv_heads), (v, cache.kv_heads), (q_out, heads))]
-    for t, shape in ((cos, (cos.shape[0], dim // 2)), (sin, (cos.shape[0], dim // 2)), (q_norm, (dim,)), (k_norm, (dim,))):
-        if t is None:
-            continue
-        if t.shape != shape:
-            refuse("shape_mismatch", call)
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.device != batch.device:
-            refuse("invalid_argument", call)
-    check(lib().qwc_op_paged_append(
-        cache._ref, batch._ref, fmt, q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(), strides[2], heads,
+    else:
+        out_stride = _rows(q_out, batch, heads, dim, call)
+    rope_rows = cos.shape[0]
+    _table(cos, (rope_rows, dim // 2), device, call)
+    _table(sin, (rope_rows, dim // 2), device, call)
+    if q_norm is not None:
+        _table(q_norm, (dim,), device, call)
+    if k_norm is not None:
+        _table(k_norm, (dim,), device, call)
+    st = lib().qwc_op_paged_append(
+        cache._ref, batch._ref, fmt, q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, heads,
         None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps, cos.data_ptr(),
-        sin.data_ptr(), cos.shape[0], q_out.data_ptr(), strides[3], current_stream(cache.device)), call)
+        sin.data_ptr(), rope_rows, q_out.data_ptr(), out_stride, current_stream(device))
+    if st:
+        check(st, call)
     return q_out
 
 
@@ -163,15 +187,19 @@ def attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, out: torch.
     if cache.device != batch.device or q.dim() != 3:
         refuse("invalid_argument", call)
     heads, dim = q.shape[1], cache.head_dim
+    q_stride = _rows(q, batch, heads, dim, call)
     if out is None:
-        out = torch.empty(batch.tokens, heads, dim, dtype=q.dtype, device=q.device)
+        out, out_stride = torch.empty((batch.tokens, heads, dim), dtype=q.dtype, device=q.device), heads * dim
     elif out.dtype != q.dtype:
         refuse("invalid_argument", call)
-    q_stride, out_stride = _rows(q, batch, heads, dim, call), _rows(out, batch, heads, dim, call)
+    else:
+        out_stride = _rows(out, batch, heads, dim, call)
     stream = current_stream(cache.device)
-    work = _workspace(cache, batch, fmt, heads, stream)
-    check(lib().qwc_op_paged_attention(cache._ref, batch._ref, fmt, q.data_ptr(), q_stride, heads, out.data_ptr(),
-                                       out_stride, work.data_ptr(), work.numel(), stream), call)
+    work, size = _workspace(cache, batch, fmt, heads, stream)
+    st = lib().qwc_op_paged_attention(cache._ref, batch._ref, fmt, q.data_ptr(), q_stride, heads, out.data_ptr(), out_stride,
+                                      work, size, stream)
+    if st:
+        check(st, call)
     return out
 
 
@@ -179,13 +207,22 @@ def read(cache: PagedCache, batch: PagedBatch, dtype: torch.dtype = torch.float3
          v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached key and value rows of the batch's tokens as values, [tokens, kv_heads, head_dim]."""
     call = "qwc_op_paged_read"
-    shape = (batch.tokens, cache.kv_heads, cache.head_dim)
-    k_out = torch.empty(shape, dtype=dtype, device=cache.device) if k_out is None else k_out
-    v_out = torch.empty(shape, dtype=dtype, device=cache.device) if v_out is None else v_out
-    fmt = format_of(k_out, call)
-    if k_out.dtype != v_out.dtype or cache.device != batch.device:
+    tokens, kv_heads, dim, device = batch.tokens, cache.kv_heads, cache.head_dim, batch.device
+    if cache.device != device:
         refuse("invalid_argument", call)
-    check(lib().qwc_op_paged_read(cache._ref, batch._ref, fmt, k_out.data_ptr(), _rows(k_out, batch, *shape[1:], call),
-                                  v_out.data_ptr(), _rows(v_out, batch, *shape[1:], call),
-                                  current_stream(cache.device)), call)
+    if k_out is None:
+        k_out, k_stride = torch.empty((tokens, kv_heads, dim), dtype=dtype, device=device), kv_heads * dim
+    else:
+        k_stride = _rows(k_out, batch, kv_heads, dim, call)
+    if v_out is None:
+        v_out, v_stride = torch.empty((tokens, kv_heads, dim), dtype=dtype, device=device), kv_heads * dim
+    else:
+        v_stride = _rows(v_out, batch, kv_heads, dim, call)
+    fmt = format_of(k_out, call)
+    if k_out.dtype != v_out.dtype:
+        refuse("invalid_argument", call)
+    st = lib().qwc_op_paged_read(cache._ref, batch._ref, fmt, k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride,
+                                 current_stream(device))
+    if st:
+        check(st, call)
     return k_out, v_out

@@ -64,7 +64,7 @@ struct TileConfig {
   static constexpr int PARTS = SPLIT ? 2 : 1;
   static constexpr int SCORES = SCALED ? 1 : G;              // accumulators of 64 columns
   static constexpr int STAGES = TILES == 2 || !SPLIT ? 2 : 1;  // steps of converted keys and values
-  static constexpr int CONVERT_WARPS = 2 * TILES;            // for the keys, and as many for the values
+  static constexpr int CONVERT_WARPS = 4;                    // for the keys, and as many for the values
   static constexpr int WARPS = 4 * TILES + 2 * CONVERT_WARPS + 1;
   static constexpr int THREADS = 32 * WARPS;
   static constexpr uint32_t SCORE_COLS = SCALED ? 2 * kStep : G * kStep;  // scaled: two steps' scores in turn
@@ -72,9 +72,9 @@ struct TileConfig {
   static constexpr uint32_t TMEM_COLS = TMEM_TILE * TILES <= 128 ? 128 : TMEM_TILE * TILES <= 256 ? 256 : 512;
   // Registers a thread: at launch what fits (65,536 over the resident warps, by quarters of an SM), then the
   // softmax warps take what the convert warps give back.
-  static constexpr int LAUNCH_REGS = 96;
-  static constexpr int SOFTMAX_REGS = 128;
-  static constexpr int CONVERT_REGS = 64;
+  static constexpr int LAUNCH_REGS = TILES == 2 ? 96 : 72;
+  static constexpr int SOFTMAX_REGS = TILES == 2 ? 128 : 120;
+  static constexpr int CONVERT_REGS = TILES == 2 ? 64 : 48;
   static_assert(4 * TILES * SOFTMAX_REGS + 2 * CONVERT_WARPS * CONVERT_REGS + LAUNCH_REGS <= WARPS * LAUNCH_REGS,
                 "a split cannot exceed the launch");
   // The tensor cores cut off what an addition to an f32 sum leaves over, always towards zero: over n additions the

@@ -675,42 +675,48 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         // A partial: [DIM / 4][HEIGHT] of four dims, then maxima and sums. In the slots of stretch x: 2 x for the tile
         // that the stretch begins with, 2 x + 1 for the one that it ends with.
         auto slot = [&](uint32_t i) { return p.partials + size_t(i) * (DIM + 2) * HEIGHT; };
-        float* mine = slot(2 * blockIdx.x + (walk.first + static_cast<int32_t>(kTileCost) > 0 ? 1u : 0u));
-#pragma unroll 1
-        for (int i = 0; i < DIM; i += 32) {
-          float o[32];
-          row_sum(i, o);
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            reinterpret_cast<float4*>(mine)[size_t((i + e) / 4) * HEIGHT + tid] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-        }
-        mine[size_t(DIM) * HEIGHT + tid] = m;
-        mine[size_t(DIM + 1) * HEIGHT + tid] = l;
-        // The stretches that hold this tile: c0 .. c1 (stretch x starts at
-        // floor(x * total / grid)). Each warp joins its 32 rows by itself.
         const uint64_t seg0 = u0 + static_cast<int64_t>(walk.first) + kTileCost, seg1 = seg0 + walk.steps;
+        // The stretches that hold this tile: c0 .. c1 (stretch x starts at floor(x * total / grid)). Each warp joins its
+        // 32 rows by itself. One that finds all others done has no need to write its own part.
         const uint32_t c0 = static_cast<uint32_t>(((seg0 + 1) * grid - 1) / total);
         const uint32_t c1 = static_cast<uint32_t>((seg1 * grid - 1) / total);
-        __threadfence();
-        __syncwarp();
-        uint32_t last = 0;
-        if (lane == 0) {
-          uint32_t* counter = &p.counters[kAttnCounterStride * c0 + warp];
-          const uint32_t before = atomicAdd(counter, 1u);
-          last = before == c1 - c0;
-          if (last) *counter = 0;
+        uint32_t* counter = &p.counters[kAttnCounterStride * c0 + warp];
+        bool last = __shfl_sync(0xffffffffu, lane == 0 ? ld_acquire(counter) : 0u, 0) == c1 - c0;
+        if (!last) {
+          float* mine = slot(2 * blockIdx.x + (walk.first + static_cast<int32_t>(kTileCost) > 0 ? 1u : 0u));
+#pragma unroll 1
+          for (int i = 0; i < DIM; i += 32) {
+            float o[32];
+            row_sum(i, o);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              reinterpret_cast<float4*>(mine)[size_t((i + e) / 4) * HEIGHT + tid] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+          }
+          mine[size_t(DIM) * HEIGHT + tid] = m;
+          mine[size_t(DIM + 1) * HEIGHT + tid] = l;
+          __threadfence();
+          __syncwarp();
+          last = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(counter, 1u) : 0u, 0) == c1 - c0;
         }
-        last = __shfl_sync(0xffffffffu, last, 0);
         if (last) {
+          if (lane == 0) *counter = 0;
           __threadfence();
           const float* first = slot(2 * c0 + (seg0 > total * c0 / grid ? 1u : 0u));
           auto piece = [&](uint32_t x) -> const float* { return x == c0 ? first : slot(2 * x); };
           constexpr uint32_t kMax = DIM * HEIGHT, kSum = (DIM + 1) * HEIGHT;
-          float best = -INFINITY, sum = 0.0f;
-          for (uint32_t x = c0; x <= c1; ++x) best = fmaxf(best, __ldcg(piece(x) + kMax + tid));
+          // The pieces in order, this one's own from where it is: maxima, then the sum of the sums.
+          float best = m, sum = 0.0f;
+#pragma unroll 4
           for (uint32_t x = c0; x <= c1; ++x) {
-            sum = fmaf(__ldcg(piece(x) + kSum + tid), best == -INFINITY ? 1.0f : ex2(__ldcg(piece(x) + kMax + tid) - best), sum);
+            if (x != blockIdx.x) best = fmaxf(best, __ldcg(piece(x) + kMax + tid));
+          }
+          auto share_of = [&](float pm) { return best == -INFINITY ? 1.0f : ex2(pm - best); };
+#pragma unroll 4
+          for (uint32_t x = c0; x <= c1; ++x) {
+            const float pl = x == blockIdx.x ? l : __ldcg(piece(x) + kSum + tid);
+            const float pm = x == blockIdx.x ? m : __ldcg(piece(x) + kMax + tid);
+            sum = fmaf(pl, share_of(pm), sum);
           }
           const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
@@ -718,30 +724,24 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
             float o[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-            // Two pieces' loads in flight.
 #pragma unroll 1
-            for (uint32_t x0 = c0; x0 <= c1; x0 += 2) {
-              float4 v[2][8];
-              float f[2];
+            for (uint32_t x = c0; x <= c1; ++x) {
+              float v[32];
+              float pm = m;
+              if (x == blockIdx.x) {
+                row_sum(i, v);
+              } else {
+                const float* from = piece(x);
+                pm = __ldcg(from + kMax + tid);
 #pragma unroll
-              for (int w = 0; w < 2; ++w) {
-                const float* from = piece(min(x0 + w, c1));
-                f[w] = __ldcg(from + kMax + tid);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[w][e] = __ldcg(reinterpret_cast<const float4*>(from) + size_t(i / 4 + e) * HEIGHT + tid);
-              }
-#pragma unroll
-              for (int w = 0; w < 2; ++w) {
-                if (x0 + w > c1) break;
-                const float k = (best == -INFINITY ? 1.0f : ex2(f[w] - best)) * norm;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  o[4 * e] = fmaf(v[w][e].x, k, o[4 * e]);
-                  o[4 * e + 1] = fmaf(v[w][e].y, k, o[4 * e + 1]);
-                  o[4 * e + 2] = fmaf(v[w][e].z, k, o[4 * e + 2]);
-                  o[4 * e + 3] = fmaf(v[w][e].w, k, o[4 * e + 3]);
+                for (int e = 0; e < 32; e += 4) {
+                  const float4 f = __ldcg(reinterpret_cast<const float4*>(from) + size_t((i + e) / 4) * HEIGHT + tid);
+                  v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
                 }
               }
+              const float k = share_of(pm) * norm;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = fmaf(v[e], k, o[e]);
             }
             put_row(i, o);
           }

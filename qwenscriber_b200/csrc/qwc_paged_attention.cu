@@ -37,6 +37,11 @@ namespace {
 //
 // Both products have the cache on the 16-row side: with the query rows there instead, twice as many
 // MMAs and twice the output registers were spent on mostly empty rows (64 x 1 over 4096, f32: 95 us).
+//
+// 64 x 1 over up to 4096 (361 MB of cache), f32: 73 us, 4.9 TB/s; the copies and the conversions of codes share the
+// issue slots (53% taken), and two CTAs of eight warps leave them partly idle behind the chain of a block: scores,
+// maximum, exponential, transpose. 1 x 1 over 301: 9.7 us, of which the launch and the chain of dependent loads
+// (lengths, page table, codes, the joined pieces) are nearly all.
 
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = 32 * kFewWarps;
@@ -593,6 +598,8 @@ AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
   AttnPlan p = {};
   const uint64_t rows = uint64_t(a.max_query) * (heads / a.kv_heads);
   const uint64_t sms = 148;
+  // As many rows as the few-row kernel has columns for. 64 sequences of up to 4096 positions, 8 kv heads: f32, 8 rows,
+  // 150 us here and 396 on 128-row tiles; bf16, 16 rows, 212 and 242; 2 sequences up to 2047, f32, 8 rows, 19 and 55.
   p.few = rows <= (format == kFormatF32 ? 8u : 16u);
   if (!p.few) {
     p.tile = paged_tile_plan(a, heads, sms);
@@ -600,11 +607,16 @@ AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
     return p;
   }
   p.rows = static_cast<uint32_t>(rows);
+  // Heads to a CTA. More of them read wider rows and leave fewer warps' states to merge, but a sequence then lies in
+  // more stretches, each with more rows to join. 64 x 1 over 4096, f32: one head 82 us, two 74, four 73, eight 78;
+  // 64 x 4 over 4096 one 165, two 153, four 150; 8 x 1 over 4096 one 24, two 25, four 29; 2 x 4 over 2047 one 18,
+  // two 31, four 78. Two for a good number of short single tokens: 64 x 1 over 512 one 29, two 25; over 64 one 12, two
+  // 8; 16 x 1 over 4096 one 34.7, two 33.8; but 64 x 4 over 256 one 34, two 39.
   p.group = 1;
-  if (uint64_t(a.sequences) * a.kv_heads * a.max_context >= 8ull * 2 * sms * 512) {
-    for (uint32_t g = 2; g <= 4; ++g) {
-      if (a.kv_heads % g == 0) p.group = g;
-    }
+  const uint64_t pairs = uint64_t(a.sequences) * a.kv_heads;
+  const uint32_t most = pairs * a.max_context >= 8ull * 2 * sms * 512 ? 4 : pairs >= 128 && rows <= 2 ? 2 : 1;
+  for (uint32_t g = 2; g <= most; ++g) {
+    if (a.kv_heads % g == 0) p.group = g;
   }
   p.pb = kFewWarps / p.group;
   const uint64_t span = uint64_t(kFewBlock) * p.pb;

@@ -31,7 +31,14 @@
 //
 // Tensor memory: G x 64 columns of scores and DIM of output for a tile. With one
 // tile two CTAs share an SM, with two one CTA has it: either way one tile's
-// softmax covers the other's MMAs. Two tiles convert each step once for 256 rows.
+// softmax covers the other's MMAs. Two tiles convert each step once for 256 rows, so
+// they are taken where a kv head has more than 128: 4 x 1500 over 4096, bf16, one tile 218 us, two 148;
+// 2 x 391 over 2047, f32, one 69, two 66.
+//
+// What bounds it: the softmax and convert warps' instructions, not the tensor cores. 4 x 1500 over 4096, bf16:
+// 148 us, 520 TFLOP/s; 24 x 64 over 1237, bf16: 53 us, many tiles with a
+// few rows (down to one token's two) that cost as much as a full one, converting the cache; 2 x 391 over 2047, f32: 68 us, four times the scores' instructions of bf16 and four MMAs
+// for one.
 //
 // Work is dealt as in qwc_paged_attention.cu: the steps of all tiles stand in
 // one line, each CTA takes an equal stretch, a tile that is cut is joined by
@@ -52,7 +59,8 @@ constexpr uint32_t kRows = 128;   // rows of a tile
 constexpr uint32_t kStep = 64;    // positions of a step
 constexpr uint32_t kGrowth = 8;   // log2 of how far a maximum may run ahead of the one in use
 // What setting up and finishing a tile takes, in steps, when the work is dealt: these places of the line are
-// paid for but empty. Measured as COST_MEASURED.
+// paid for but empty. With 0, 1, 2, 3, 5 and 8 places: 4 x 1500 rows over 4096, bf16, 174, 164, 160, 154, 154 and 155 us;
+// 24 x 64 over 1237, bf16, 58, 57.5, 55.5, 56.5 (0 to 3); 2 x 391 over 2047, f32, 69.5, 66, -, 66, 68 and 71 us.
 constexpr uint32_t kTileCost = 3;
 
 template <typename T, int DIM_, int TILES_>
@@ -79,8 +87,10 @@ struct TileConfig {
                 "a split cannot exceed the launch");
   // The tensor cores cut off what an addition to an f32 sum leaves over, always towards zero: over n additions the
   // output loses about n times 8e-9 of its size (2048 positions in two parts, 256 additions: 2e-6). f32 rows therefore
-  // start a new sum every FLUSH steps, and the sums are added in f32 in global memory.
-  static constexpr uint32_t FLUSH = SPLIT ? 8 : 1u << 31;
+  // start a new sum every FLUSH steps, and the sums are added in f32 in global memory. Of 2 x 391 rows over 2047
+  // positions, f32: a sum over 2 steps 73 us, 4 steps 69, 8 steps 65; the largest error at length 2048 0.48e-6, 0.74e-6
+  // and 1.1e-6 of the output, where f32 arithmetic throughout has 0.9e-6.
+  static constexpr uint32_t FLUSH = SPLIT ? 4 : 1u << 31;
   // The weights' power of two, 2^(UP - vexp): weight times value scale below 2^15 (exact), value below 2^7 (scaled).
   static constexpr int UP = SCALED ? 14 : 21;
 };

@@ -146,6 +146,14 @@ def test_attention_over_long_contexts(gpu, cuda_lib, kind, query, context):
     check_attention(world, kind, 4, gpu)
 
 
+@pytest.mark.parametrize("kind,sequences,most", [("f32", 1000, 2), ("bf16", 600, 20), ("f32", 600, 20)])
+def test_attention_of_more_sequences_than_a_block_has_threads(gpu, cuda_lib, kind, sequences, most):
+    r = np.random.default_rng(sequences + most)
+    query = r.integers(0, most + 1, sequences)
+    world = World(query, query + r.integers(0, 100, sequences), 16, 1, 64, seed=sequences)
+    check_attention(world, kind, 2, gpu, seed=most)
+
+
 def test_attention_of_odd_head_shares(gpu, cuda_lib):
     for heads, kv_heads, dim in ((5, 5, 64), (9, 3, 128), (7, 1, 64), (40, 8, 128)):
         check_attention(World([3, 50, 1], [70, 50, 9], 16, kv_heads, dim, seed=heads), "f32", heads, gpu)

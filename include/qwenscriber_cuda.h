@@ -511,9 +511,10 @@ int32_t qwc_op_paged_append(const qwc_paged_cache* cache, const qwc_paged_batch*
  * the queries and weights (two parts, 22 bits, for f32 rows, one for 16-bit rows); for bf16 rows of a call with
  * more than 16 rows to a kv head, code times scale rounds to f16 first. Sums and the softmax are f32. A token that sees no position gives a row of zeros. q and out as in append.
  * `workspace` (16-byte aligned device memory of at least qwc_op_paged_attention_workspace bytes) holds
- * the partial results of contexts cut into pieces. It must be zero before its first use, is left ready for
- * the next call, and serves one stream at a time. Its first 32-bit word stays zero unless a wait inside the
- * kernel, bounded at 2 s, has run out: the call's rows are then undefined, and the workspace must be zeroed again. */
+ * the partial results of contexts cut into pieces. Its first QWC_PAGED_WORKSPACE_HEAD bytes must be zero before
+ * its first use; it is left ready for the next call, and serves one stream at a time. Its first 32-bit word stays zero unless a wait inside the
+ * kernel, bounded at 2 s, has run out: the call's rows are then undefined, and the head must be zeroed again. */
+#define QWC_PAGED_WORKSPACE_HEAD 33024u
 int32_t qwc_op_paged_attention(const qwc_paged_cache* cache, const qwc_paged_batch* batch, uint32_t format,
                                const void* q, uint64_t q_stride, uint32_t heads, void* out, uint64_t out_stride,
                                void* workspace, uint64_t workspace_bytes, void* stream);

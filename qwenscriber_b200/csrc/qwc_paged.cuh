@@ -154,6 +154,7 @@ constexpr uint32_t kMaxAttnCtas = 1024;
 constexpr uint32_t kAttnCounterStride = 8;  // a CTA's counters: one for each softmax warp
 constexpr uint32_t kAttnCounters = kAttnCounterStride * kMaxAttnCtas;
 constexpr uint64_t kAttnHeadBytes = 256 + kAttnCounters * 4;  // of the workspace: the error word, the counters
+static_assert(kAttnHeadBytes == QWC_PAGED_WORKSPACE_HEAD);
 
 // Many rows (qwc_paged_tile.cu): 128-row tiles that a CTA takes at once, its grid, its part of the workspace.
 struct TilePlan {

@@ -18,7 +18,8 @@ import ctypes
 import torch
 
 from .quant import GROUP
-from .runtime import FORMAT_BF16, FORMAT_F16, FORMAT_F32, STATUS_CODE, PagedBatchDesc, PagedCacheDesc, QwcError, check, lib
+from .runtime import (FORMAT_BF16, FORMAT_F16, FORMAT_F32, PAGED_WORKSPACE_HEAD, STATUS_CODE, PagedBatchDesc, PagedCacheDesc,
+                      QwcError, check, lib)
 
 FORMATS = {torch.float32: FORMAT_F32, torch.float16: FORMAT_F16, torch.bfloat16: FORMAT_BF16}
 
@@ -123,15 +124,17 @@ def _table(t: torch.Tensor, shape: tuple, device: torch.device, call: str) -> No
         refuse("invalid_argument", call)
 
 
-# Partial results of attention, one buffer for each (device, stream), zeroed when it is made and
-# kept at the largest size asked for.
+# Partial results of attention, one buffer for each (device, stream), kept at the largest size asked for.
 _workspaces: dict = {}
 
 
-def _workspace(cache: PagedCache, batch: PagedBatch, fmt: int, heads: int, stream: int) -> tuple[int, int]:
-    """(address, bytes) of the stream's buffer, at least what this call needs."""
-    at = (cache._index, stream)
-    held = _workspaces.get(at)
+def _new_workspace(need: int, device: torch.device) -> torch.Tensor:
+    buffer = torch.empty(need, dtype=torch.uint8, device=device)
+    buffer[:PAGED_WORKSPACE_HEAD].zero_()
+    return buffer
+
+
+def workspace_bytes(cache: PagedCache, batch: PagedBatch, heads: int, fmt: int) -> int:
     key = (cache._key, fmt, heads)
     need = batch._workspace_bytes.get(key)
     if need is None:
@@ -139,10 +142,44 @@ def _workspace(cache: PagedCache, batch: PagedBatch, fmt: int, heads: int, strea
         check(lib().qwc_op_paged_attention_workspace(cache._ref, batch._ref, fmt, heads, ctypes.byref(n)),
               "qwc_op_paged_attention_workspace")
         need = batch._workspace_bytes[key] = n.value
+    return need
+
+
+def workspace(cache: PagedCache, batch: PagedBatch, heads: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """A workspace for `attention` with this pool, batch and head count, to be used by one stream at a time."""
+    fmt = FORMATS.get(dtype)
+    if fmt is None:
+        refuse("unsupported", "qwc_op_paged_attention_workspace")
+    return _new_workspace(workspace_bytes(cache, batch, heads, fmt), cache.device)
+
+
+def _workspace(cache: PagedCache, need: int, stream: int) -> tuple[int, int]:
+    """(address, bytes) of the stream's buffer, at least what this call needs."""
+    if torch.cuda.is_current_stream_capturing():
+        # A graph may be replayed on any stream and outlive the stream's buffer: it gets one of its own, from the
+        # graph's pool, and zeroes its head in each replay.
+        buffer = _new_workspace(need, cache.device)
+        return buffer.data_ptr(), need
+    at = (cache._index, stream)
+    held = _workspaces.get(at)
     if held is None or held[1] < need:
-        buffer = torch.zeros(need, dtype=torch.uint8, device=cache.device)
+        buffer = _new_workspace(need, cache.device)
         held = _workspaces[at] = (buffer.data_ptr(), need, buffer)
     return held[0], held[1]
+
+
+def check_waits(workspace: torch.Tensor | None = None, device: torch.device | None = None) -> None:
+    """Raises `QwcError` if a bounded wait inside an attention kernel ran out (its rows are undefined then), and makes
+    the workspace ready again. Without a workspace, of the current stream's own. Waits for the stream."""
+    if workspace is None:
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        held = _workspaces.get((device.index, current_stream(device)))
+        if held is None:
+            return
+        workspace = held[2]
+    if int(workspace[:4].view(torch.int32)[0]):
+        workspace[:PAGED_WORKSPACE_HEAD].zero_()
+        refuse("invalid_state", "qwc_op_paged_attention")
 
 
 def append(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
@@ -180,8 +217,10 @@ def append(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, k: torch.Tenso
     return q_out
 
 
-def attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Causal attention of the batch's [tokens, heads, head_dim] queries over their sequences' pages."""
+def attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the batch's [tokens, heads, head_dim] queries over their sequences' pages. `workspace`: one
+    made by `workspace(...)`; without it, the current stream's own (in a graph under capture, the graph's own)."""
     call = "qwc_op_paged_attention"
     fmt = format_of(q, call)
     if cache.device != batch.device or q.dim() != 3:
@@ -195,7 +234,12 @@ def attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, out: torch.
     else:
         out_stride = _rows(out, batch, heads, dim, call)
     stream = current_stream(cache.device)
-    work, size = _workspace(cache, batch, fmt, heads, stream)
+    if workspace is None:
+        work, size = _workspace(cache, workspace_bytes(cache, batch, heads, fmt), stream)
+    elif workspace.dtype != torch.uint8 or workspace.device != cache.device or not workspace.is_contiguous():
+        refuse("invalid_argument", call)
+    else:
+        work, size = workspace.data_ptr(), workspace.numel()
     st = lib().qwc_op_paged_attention(cache._ref, batch._ref, fmt, q.data_ptr(), q_stride, heads, out.data_ptr(), out_stride,
                                       work, size, stream)
     if st:

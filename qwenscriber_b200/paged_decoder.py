@@ -183,6 +183,7 @@ class PagedDecoder:
             kinds = {k: torch.full((len(live),), v, dtype=torch.int32 if k == "top_k" else torch.float32, device=self.device)
                      for k, v in settings.items()}
             tokens, logprobs = (t.tolist() for t in sampling.sample(logits, u, **kinds))
+            paged.check_waits(device=self.device)
             for i, tok, lp in zip(live, tokens, logprobs):
                 out[i] = (out[i][0] + ([tok] if tok not in stop else []), out[i][1] + lp)
             going = [(i, tok) for i, tok in zip(live, tokens) if tok not in stop]

@@ -33,6 +33,7 @@ STATUS_CODE = {name: code for code, name in STATUS.items()}
 CACHE_F32, CACHE_Q8 = 0, 1
 FORMAT_F32, FORMAT_F16, FORMAT_BF16 = 0, 1, 2
 SAMPLE_MAX_VOCAB = 1048576  # QWC_SAMPLE_MAX_VOCAB
+PAGED_WORKSPACE_HEAD = 33024  # QWC_PAGED_WORKSPACE_HEAD
 OPTION_IGNORE_EOS, OPTION_KEEP_LOGITS, OPTION_STEP_CHUNK, OPTION_TRACE, OPTION_PREFILL_SERIAL = 1, 2, 3, 4, 5
 OPTION_EXACT, OPTION_WAIT_LIMIT_US, OPTION_TEST_STALL = 6, 7, 8
 FEATURE_MODEL, FEATURE_DECODE, FEATURE_STREAMS = 1 << 3, 1 << 4, 1 << 8

@@ -243,6 +243,56 @@ def test_attention_on_another_stream(gpu, cuda_lib):
         assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("query", [1, 40])
+def test_attention_in_a_graph(gpu, cuda_lib, query):
+    world = World([query, query], [500, 300], 16, 2, 128, seed=12)
+    cache, batch = world.device(gpu)
+    q = torch.randn(2 * query, 4, 128, device=gpu)
+    want = paged.attention(cache, batch, q)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = paged.attention(cache, batch, q)
+    with torch.cuda.stream(side):  # before the first replay: nothing that the capture made is used
+        early = paged.attention(cache, batch, q)
+    torch.cuda.synchronize()
+    assert torch.equal(early, want)
+    other = torch.cuda.Stream()
+    for _ in range(3):
+        got.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            graph.replay()
+        beside = paged.attention(cache, batch, q)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(beside, want)
+
+
+@pytest.mark.parametrize("query", [1, 40])
+def test_attention_with_a_workspace_of_the_callers(gpu, cuda_lib, query):
+    world = World([query, query], [500, 300], 16, 2, 128, seed=13)
+    cache, batch = world.device(gpu)
+    q = torch.randn(2 * query, 4, 128, device=gpu)
+    want = paged.attention(cache, batch, q)
+    work = paged.workspace(cache, batch, 4)
+    work[rt.PAGED_WORKSPACE_HEAD:] = 255  # only the head has to be zero
+    for _ in range(3):
+        assert torch.equal(paged.attention(cache, batch, q, workspace=work), want)
+    assert not work[:rt.PAGED_WORKSPACE_HEAD].any()
+    paged.check_waits(work)
+    paged.check_waits()
+    work[0] = 3
+    with pytest.raises(rt.QwcError) as e:
+        paged.check_waits(work)
+    assert e.value.name == "invalid_state"
+    paged.check_waits(work)
+    for bad, name in ((work[:-16], "limit_exceeded"), (work[1:], "invalid_argument"), (work.view(torch.int32), "invalid_argument"),
+                      (work.cpu(), "invalid_argument"), (torch.zeros(2 * work.numel(), dtype=torch.uint8, device=gpu)[::2], "invalid_argument")):
+        with pytest.raises(rt.QwcError) as e:
+            paged.attention(cache, batch, q, workspace=bad)
+        assert e.value.name == name
+
+
 def test_lengths_that_change_on_the_device(gpu, cuda_lib):
     # The bounds stay, the lengths do not: one batch object serves many steps, and replays in a graph.
     world = World([1, 1, 1], [300, 200, 100], 16, 2, 128, seed=11)

@@ -162,7 +162,7 @@ struct TilePlan {
   bool too_long;
   uint64_t partial_bytes;
 };
-TilePlan paged_tile_plan(const PagedArgs& a, uint32_t heads, uint32_t sms);
+TilePlan paged_tile_plan(const PagedArgs& a, uint32_t format, uint32_t heads, uint32_t sms);
 int32_t paged_tile_launch(const PagedArgs& a, const AttnArgs& p, uint32_t format, const TilePlan& plan, cudaStream_t stream);
 
 // ---- arithmetic of the attention kernels ----

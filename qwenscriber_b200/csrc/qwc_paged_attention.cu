@@ -602,7 +602,7 @@ AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
   // 150 us here and 396 on 128-row tiles; bf16, 16 rows, 212 and 242; 2 sequences up to 2047, f32, 8 rows, 19 and 55.
   p.few = rows <= (format == kFormatF32 ? 8u : 16u);
   if (!p.few) {
-    p.tile = paged_tile_plan(a, heads, sms);
+    p.tile = paged_tile_plan(a, format, heads, sms);
     p.partial_bytes = p.tile.partial_bytes;
     return p;
   }

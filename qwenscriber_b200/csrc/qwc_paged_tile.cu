@@ -36,9 +36,9 @@
 // 2 x 391 over 2047, f32, one 69, two 66.
 //
 // What bounds it: the softmax and convert warps' instructions, not the tensor cores. 4 x 1500 over 4096, bf16:
-// 148 us, 520 TFLOP/s; 24 x 64 over 1237, bf16: 53 us, many tiles with a
-// few rows (down to one token's two) that cost as much as a full one, converting the cache; 2 x 391 over 2047, f32: 68 us, four times the scores' instructions of bf16 and four MMAs
-// for one.
+// 148 us, 520 TFLOP/s; 24 x 64 over 1237, bf16: 53 us, many tiles with a few
+// rows (down to one token's two) that cost as much as a full one, converting the cache; 2 x 391 over 2047, f32: 68 us,
+// four times the scores' instructions of bf16 and four MMAs for one.
 //
 // Work is dealt as in qwc_paged_attention.cu: the steps of all tiles stand in
 // one line, each CTA takes an equal stretch, a tile that is cut is joined by
@@ -46,6 +46,7 @@
 
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "qwc_device.cuh"
@@ -62,6 +63,11 @@ constexpr uint32_t kGrowth = 8;   // log2 of how far a maximum may run ahead of 
 // paid for but empty. With 0, 1, 2, 3, 5 and 8 places: 4 x 1500 rows over 4096, bf16, 174, 164, 160, 154, 154 and 155 us;
 // 24 x 64 over 1237, bf16, 58, 57.5, 55.5, 56.5 (0 to 3); 2 x 391 over 2047, f32, 69.5, 66, -, 66, 68 and 71 us.
 constexpr uint32_t kTileCost = 3;
+// What joining one more piece of a cut tile takes, in steps. A stretch is no shorter than the square root of this times
+// the longest tile, where a tile's own steps and the joining of its pieces take equally long, unless a tile is shorter.
+// With 0, 0.3, 0.8, 2 and 4, bf16: 1 x 64 over 4096 84, 50, 44, 45 and 54 us; over 1237 47, 33, 30, 32, 37; 2 x 64 over 4096
+// 61, 54, 44, 46, 54; f32 (steps twice as long): 1 x 100 over 4096 69, 62, 65, 73, 93, 1 x 64 over 1237 52, 38, 40, 46, 54.
+constexpr double kJoinCost = 0.8, kJoinCostF32 = 0.4;
 
 template <typename T, int DIM_, int TILES_>
 struct TileConfig {
@@ -1008,16 +1014,20 @@ int32_t launch_tile_as(const PagedArgs& a, const AttnArgs& p, const TilePlan& pl
 
 }  // namespace
 
-TilePlan paged_tile_plan(const PagedArgs& a, uint32_t heads, uint32_t sms) {
+TilePlan paged_tile_plan(const PagedArgs& a, uint32_t format, uint32_t heads, uint32_t sms) {
   TilePlan plan;
   const uint64_t rows = uint64_t(a.max_query) * (heads / a.kv_heads);
   plan.tiles = rows > kRows ? 2 : 1;
   const uint64_t height = uint64_t(kRows) * plan.tiles;
-  const uint64_t steps = uint64_t(a.sequences) * a.kv_heads * ((rows + height - 1) / height) *
-                         (a.max_context ? (a.max_context + kStep - 1) / kStep : 1);
   const uint64_t most = plan.tiles == 2 ? sms : 2 * sms;  // what is resident at once
-  plan.too_long = steps / most >= 0x7FFFFFFFu;            // a stretch's steps are counted in 31 bits
-  plan.grid = static_cast<uint32_t>(steps < most ? steps : most);
+  const uint64_t length = (a.max_context ? (a.max_context + kStep - 1) / kStep : 1);
+  const uint64_t tiles = uint64_t(a.sequences) * a.kv_heads * ((rows + height - 1) / height), steps = tiles * length;
+  plan.too_long = steps / most >= 0x7FFFFFFFu;  // a stretch's steps are counted in 31 bits
+  const double join = format == kFormatF32 ? kJoinCostF32 : kJoinCost;
+  const double stretch = sqrt(1.0 + join * static_cast<double>(length));
+  uint64_t grid = static_cast<uint64_t>(static_cast<double>(steps) / stretch);
+  if (grid < tiles) grid = tiles;
+  plan.grid = static_cast<uint32_t>(grid < most ? grid : most);
   // Two partial tiles a CTA, and its sums (f32 rows).
   plan.partial_bytes = uint64_t(plan.grid) * (2 * (a.head_dim + 2) + a.head_dim) * height * 4;
   return plan;

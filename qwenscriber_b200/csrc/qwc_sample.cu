@@ -42,6 +42,7 @@ constexpr uint32_t kListed = kSampleThreads;  // tokens that the first CTA takes
 constexpr uint32_t kPairs = 256;
 constexpr uint32_t kLimbBits = 14;          // 2^17 tokens of a slice times 2^14 stay below 2^32
 constexpr float kBinScale = 23.0f;      // coarse bins in a power of two; the last bin takes all below 2^-44, whose units are 0
+constexpr uint32_t kNear = 16 * 23;  // coarse bins that are counted in the first pass
 constexpr float kUnits = 4398046511104.0f;  // 2^42: 2^20 tokens of weight 1 stay below 2^63
 
 struct SampleArgs {
@@ -78,7 +79,7 @@ __device__ __forceinline__ float key_value(uint32_t key) {
 
 // How far a logit lies below the best, at the row's temperature and in powers of two: t = (best - x) log2(e) / T,
 // so w = 2^-t. One rounding of t: a relative 2^-24 t of w, below 2e-6 for every w that counts. best - x is 0 for two
-// infinities; a temperature below 1e-37 counts as that.
+// infinities; a temperature below 1e-37 counts as that, one above 3e38 as that (0 times -inf is no weight).
 struct Fall {
   float best, scale;
   __device__ __forceinline__ float of(float x) const { return fmaxf(best - x, 0.0f) * scale; }
@@ -135,6 +136,7 @@ struct SampleSmem {
   uint64_t scan[kSampleWarps];
   uint32_t scan_count[kSampleWarps];
   uint64_t total;      // the row's (first CTA) sum of all units
+  uint64_t mass_above; // the row's (first CTA) sum of the units above the bins in question
   uint64_t slice_sum;  // this slice's sum of kept units
   uint32_t slice_ties;
   float best;
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const float heat_given = a.temperature ? a.temperature[r] : 1.0f;
   const bool greedy = !(heat_given > 0.0f);
-  const float heat = greedy ? 1.0f : fmaxf(heat_given, 1e-37f);
+  const float heat = greedy ? 1.0f : fminf(fmaxf(heat_given, 1e-37f), 3e38f);
   const int32_t k_given = a.top_k ? a.top_k[r] : 0;
   const float p_given = a.top_p ? a.top_p[r] : 1.0f;
   const float least = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
   if (lane == 0) s->sums[warp] = uint64_t(__float_as_uint(best)) << 32 | at;
   s->coarse_count[threadIdx.x] = 0;
-  if (threadIdx.x == 0) s->total = 0, s->listed = 0;
+  if (threadIdx.x == 0) s->total = 0, s->mass_above = 0, s->listed = 0;
   __syncthreads();
   better(__uint_as_float(static_cast<uint32_t>(s->sums[lane] >> 32)), static_cast<uint32_t>(s->sums[lane]));
 #pragma unroll
@@ -339,26 +341,21 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   auto coarse_bin = [&](float t) { return static_cast<uint32_t>(fminf(t * kBinScale, static_cast<float>(kBins - 1))); };
   const bool cuts = by_count || by_mass, any_cut = cuts || (!greedy && least > 0.0f);
   uint64_t run_sum = 0;
-  auto count_in = [&](float t) {
-    if (any_cut) {
-      const uint32_t bin = coarse_bin(t);
-      // The last bin can hold most of a row: one count for all its lanes.
-      const uint32_t last = __ballot_sync(0xffffffffu, bin == kBins - 1);
-      if (last && lane == 0) atomicAdd(&s->coarse_count[kBins - 1], static_cast<uint32_t>(__popc(last)));
-      if (bin != kBins - 1) atomicAdd(&s->coarse_count[bin], 1u);
-    }
-  };
+  // Most of a row lies far down, where a count is seldom asked for and costs a shared atomic: the bins of the first 16
+  // powers of two are counted here, the others only if the kept set reaches them.
   const uint32_t whole = i0 + (i1 - i0) / 32 * 32;
 #pragma unroll 4
   for (uint32_t i = i0; i < whole; i += 32) {
     const float t = fall_of(value(i + lane));
     run_sum += units_of(weight_of(t));
-    count_in(t);
+    const float place = t * kBinScale;
+    if (any_cut && place < kNear) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
   }
   if (whole + lane < i1) {
     const float t = fall_of(value(whole + lane));
     run_sum += units_of(weight_of(t));
-    if (any_cut) atomicAdd(&s->coarse_count[coarse_bin(t)], 1u);
+    const float place = t * kBinScale;
+    if (any_cut && place < kNear) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
   }
   run_sum = warp_sum_u64(run_sum);
   if (lane == 0) {
@@ -366,7 +363,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     atomicAdd(reinterpret_cast<unsigned long long*>(&s0->total), static_cast<unsigned long long>(run_sum));
   }
   __syncthreads();
-  if (any_cut && rank != 0 && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
+  if (any_cut && rank != 0 && threadIdx.x < kNear && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
   cluster.sync();
   const uint64_t all = s0->total;
   const float log_all = logf(static_cast<float>(all) / kUnits);
@@ -389,14 +386,42 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     if (!(best < INFINITY) || !(step_heat < INFINITY) || !(hi >= lo)) lo = 0, hi = 0xFFFFFFFFu;
   };
 
+  const float draw = fminf(fmaxf(a.uniforms[r], 0.0f), 1.0f);
+  auto goal_of = [&](uint64_t total) {
+    const uint64_t goal = static_cast<uint64_t>(static_cast<double>(draw) * static_cast<double>(total));
+    return goal >= total ? total - 1 : goal;
+  };
+  auto target_of = [&](uint64_t mass) {  // top_p's
+    const uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
+    return !(p_given > 0.0f) || target < 1 ? uint64_t(1) : target > mass ? mass : target;
+  };
+  // A token for the first CTA's list, of each lane that has one.
+  auto list_token = [&](bool mine, uint32_t k, uint32_t i, float w) {
+    const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+    if (!votes) return;
+    uint32_t at0 = 0;
+    if (lane == 0) at0 = atomicAdd(&s0->listed, static_cast<uint32_t>(__popc(votes)));
+    at0 = __shfl_sync(0xffffffffu, at0, 0) + __popc(votes & ((1u << lane) - 1u));
+    if (mine && at0 < kListed) {
+      s0->list.key[at0] = k;
+      s0->list.index[at0] = i | (w < least ? 0x80000000u : 0u);
+      s0->list.units[at0] = units_of(w);
+    }
+  };
+
+  // The kept set, once it is known: keys above `key`, and at it the first `ties` of the `here` tokens, or those up to index `tie_last`.
+  uint32_t key = 0, ties = 0xFFFFFFFFu, here = 0, tie_last = 0xFFFFFFFFu;
+  bool summed = false;  // the sums of the runs are those of the kept set
+
   if (any_cut) {
     // How far down the kept set can reach. top_p's bin is bounded by the least that the bins' tokens can weigh; where
     // top_k cuts too, what top_k left has to be known first, and only top_k bounds.
     // (Every CTA works it out from the first one's counts.)
-    uint32_t reach, reached;
-    {
-      const uint32_t n = s0->coarse_count[threadIdx.x];
-      const uint32_t above = sum_above(s, n);
+    uint32_t reach, reached, n, above;
+    uint32_t counted = kNear;
+    for (;; counted = kBins) {
+      n = threadIdx.x < counted ? s0->coarse_count[threadIdx.x] : 0u;
+      above = sum_above(s, n);
       __syncthreads();
       if (threadIdx.x == 0) s->reach = kBins - 1;
       const uint64_t want = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(all)));
@@ -413,12 +438,25 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       if (!by_mass && least > 0.0f) last |= threadIdx.x == min(static_cast<uint32_t>(fmaxf(-log2f(least), 0.0f) * kBinScale) + 1u, kBins - 1);
       if (by_mass && !by_count && want == 0) last |= threadIdx.x == 0;
       __syncthreads();
-      if (last) atomicMin(&s->reach, threadIdx.x);
+      if (last && threadIdx.x < counted) atomicMin(&s->reach, threadIdx.x);
       __syncthreads();
       reach = s->reach;
       if (threadIdx.x == reach) s->reached = above + n;
       __syncthreads();
       reached = s->reached;
+      if (reach < counted) break;
+      // The other bins' counts. (The last one can hold most of a row: one count for all its lanes.)
+#pragma unroll 4
+      for (uint32_t i = i0; i < i1; i += 32) {
+        const bool in = i + lane < i1;
+        const uint32_t bin = in ? coarse_bin(fall_of(value(i + lane))) : 0u;
+        const uint32_t end = __ballot_sync(0xffffffffu, bin == kBins - 1);
+        if (end && lane == 0) atomicAdd(&s->coarse_count[kBins - 1], static_cast<uint32_t>(__popc(end)));
+        if (bin >= kNear && bin != kBins - 1) atomicAdd(&s->coarse_count[bin], 1u);
+      }
+      __syncthreads();
+      if (rank != 0 && threadIdx.x >= kNear && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
+      cluster.sync();
     }
     if (reached <= kListed) {
       // ---- few enough for the first CTA ----
@@ -433,30 +471,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         if (!__any_sync(0xffffffffu, mine)) continue;
         const float fall = fall_of(x);
         mine = mine && coarse_bin(fall) <= reach;
-        const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-        if (!votes) continue;
-        uint32_t at0 = 0;
-        if (lane == 0) at0 = atomicAdd(&s0->listed, static_cast<uint32_t>(__popc(votes)));
-        at0 = __shfl_sync(0xffffffffu, at0, 0) + __popc(votes & ((1u << lane) - 1u));
-        if (mine && at0 < kListed) {
-          const float w = weight_of(fall);
-          s0->list.key[at0] = k;
-          s0->list.index[at0] = (i + lane) | (w < least ? 0x80000000u : 0u);
-          s0->list.units[at0] = units_of(w);
-        }
+        list_token(mine, k, i + lane, weight_of(fall));
       }
       cluster.sync();
       if (rank != 0) return;  // nothing of this CTA is read from here on
       const uint32_t listed = min(s->listed, kListed);
-      const float draw = fminf(fmaxf(a.uniforms[r], 0.0f), 1.0f);
-      auto goal_of = [&](uint64_t total) {
-        const uint64_t goal = static_cast<uint64_t>(static_cast<double>(draw) * static_cast<double>(total));
-        return goal >= total ? total - 1 : goal;
-      };
-      auto target_of = [&](uint64_t mass) {  // top_p's
-        const uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
-        return !(p_given > 0.0f) || target < 1 ? uint64_t(1) : target > mass ? mass : target;
-      };
       if (listed <= kPairs) {
         // Lanes of a token: a power of two, at most a warp.
         uint32_t lanes = 32;
@@ -560,11 +579,99 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       }
       return;
     }
+    if (by_mass && !by_count) {
+      // ---- top_p alone, many tokens: the few bins that can hold the cut ----
+      // The counts bound the mass above a bin from both sides, by what its tokens weigh at least and at most (a bin is 3%
+      // wide) and by the same of what lies below, taken from the total: near the end of the row, where top_p as a rule
+      // cuts, to a small part of a bin.
+      uint64_t n_least = n * units_of(weight_of((threadIdx.x + 1) / kBinScale) * 0.99999f);
+      uint64_t n_most = n * (units_of(weight_of(threadIdx.x / kBinScale) * 1.00001f) + 1);
+      if (threadIdx.x == kBins - 1) {  // (its units are 0; here: what was not counted)
+        n_least = 0;
+        n_most = counted == kBins ? 0 : (a.vocab - above) * (units_of(weight_of(kNear / kBinScale) * 1.00001f) + 1);
+      }
+      const uint64_t above_least = sum_above(s, n_least);
+      __syncthreads();
+      const uint64_t above_most = sum_above(s, n_most);
+      if (threadIdx.x == kBins - 1) {
+        s->cut.mass = above_least + n_least;
+        s->cut.here_mass = above_most + n_most;
+      }
+      if (threadIdx.x == 0) s->reach = 0, s->reached = kBins - 1;
+      __syncthreads();
+      const uint64_t target = target_of(all);
+      const uint64_t below_least = s->cut.mass - above_least, below_most = s->cut.here_mass - above_most;  // this bin and all below
+      const uint64_t at_most = min(above_most, all - below_least);
+      const uint64_t next_most = below_most - n_most;
+      const uint64_t next_least = max(above_least + n_least, next_most < all ? all - next_most : uint64_t(0));
+      if (at_most < target) atomicMax(&s->reach, threadIdx.x);
+      if (next_least >= target) atomicMin(&s->reached, threadIdx.x);
+      __syncthreads();
+      const uint32_t b0 = s->reach, b1 = s->reached;
+      if (threadIdx.x == b0) s->cut.count = above;
+      if (threadIdx.x == b1) s->cut.here = above + n;
+      __syncthreads();
+      const uint32_t over = s->cut.count, in_question = s->cut.here - over;
+      if (in_question <= kListed) {
+        // One pass: the exact mass above them, kept by run, and their tokens to the first CTA's list.
+        const float t0 = static_cast<float>(b0), t1 = static_cast<float>(b1 + 1);
+        uint64_t over_mass = 0, kept_mass = 0;
+#pragma unroll 4
+        for (uint32_t i = i0; i < i1; i += 32) {
+          const bool in = i + lane < i1;
+          const float x = in ? value(i + lane) : -INFINITY;
+          const float t = fall_of(x), w = weight_of(t), place = t * kBinScale;
+          if (place < t0) {
+            const uint64_t u = units_of(w);
+            over_mass += u;
+            if (least > 0.0f && w >= least) kept_mass += u;
+          }
+          list_token(in && place >= t0 && place < t1, order_key<T>(x), i + lane, w);
+        }
+        over_mass = warp_sum_u64(over_mass);
+        if (least > 0.0f) kept_mass = warp_sum_u64(kept_mass);
+        if (lane == 0) {
+          s->sums[warp] = least > 0.0f ? kept_mass : over_mass;
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s0->mass_above), static_cast<unsigned long long>(over_mass));
+        }
+        cluster.sync();
+        if (rank == 0) {
+          const bool have = threadIdx.x < min(s->listed, kListed);
+          const uint32_t k = have ? s->list.key[threadIdx.x] : 0u, flagged = have ? s->list.index[threadIdx.x] : 0u;
+          const uint32_t index = flagged & 0x7FFFFFFFu;
+          const uint64_t u = have ? s->list.units[threadIdx.x] : 0;
+          uint32_t lo, hi;
+          keys_of(b0, b1, lo, hi);
+          Cut cut;
+          narrow(s, have, k, u, lo, hi, true, target, cut, over, s->mass_above);
+          const uint64_t each = cut.here_mass / cut.here;
+          const uint32_t stay = static_cast<uint32_t>((target - cut.mass + each - 1) / each);
+          uint32_t last = 0xFFFFFFFFu;
+          if (stay < cut.here) {
+            Cut at_cut;
+            narrow(s, have && k == cut.bin, ~index & 0x7FFFFFFFu, u, 0x7FFFFFFFu - (a.vocab - 1), 0x7FFFFFFFu, false, stay, at_cut);
+            last = ~at_cut.bin & 0x7FFFFFFFu;
+          }
+          if (have && flagged == index && (k > cut.bin || (k == cut.bin && index <= last))) {
+            const uint32_t slice = index / (a.run * kSampleWarps);
+            atomicAdd(reinterpret_cast<unsigned long long*>(
+                          &cluster.map_shared_rank(s, slice)->sums[(index - slice * a.run * kSampleWarps) / a.run]),
+                      static_cast<unsigned long long>(u));
+          }
+          if (threadIdx.x == 0) s->answer = Cut{0, 0, last, 0, cut.bin};
+        }
+        cluster.sync();
+        key = s0->answer.bin;
+        tie_last = s0->answer.count;
+        run_sum = s->sums[warp];
+        summed = true;
+      }
+    }
   }
 
   uint32_t bin_count = 0;  // of coarse bin threadIdx.x, over the row
   uint64_t bin_mass = 0;
-  if (cuts) {
+  if (cuts && !summed) {
     // ---- a large kept set: the masses of the coarse bins, then the one that holds the cut ----
 #pragma unroll
     for (int i = 0; i < 3; ++i) s->limb[i][threadIdx.x] = 0;
@@ -672,21 +779,17 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     key = hi;
   };
 
-  // The kept set: keys above `cut`, and the first `ties` of the `here` at it.
-  uint32_t key = 0, ties = 0xFFFFFFFFu, here = 0;
   uint64_t mass = all;
-  if (by_count) {
+  if (by_count && !summed) {
     Cut cut;
     find_cut(false, static_cast<uint64_t>(k_given), key, cut);
     ties = static_cast<uint32_t>(k_given) - cut.count;
     here = cut.here;
     mass = cut.mass + cut.here_mass / cut.here * ties;
   }
-  if (by_mass) {
+  if (by_mass && !summed) {
     if (by_count) cluster.sync();  // (all have read the first answer)
-    uint64_t target = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(mass)));
-    if (!(p_given > 0.0f) || target < 1) target = 1;
-    if (target > mass) target = mass;
+    const uint64_t target = target_of(mass);
     Cut cut;
     find_cut(true, target, key, cut);
     const uint64_t each = cut.here_mass / cut.here;
@@ -715,7 +818,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     const bool in = i < i1;
     const float x = in ? value(i) : -INFINITY;
     const uint32_t k = order_key<T>(x);
-    bool keep = in && k >= key;
+    bool keep = in && (k > key || (k == key && i <= tie_last));
     if (rank_ties) {
       const bool tie = in && k == key;
       const uint32_t votes = __ballot_sync(0xffffffffu, tie);
@@ -729,7 +832,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   };
   // The sum of each run, then the walk of the one that holds the token.
   const bool every = !cuts && !(least > 0.0f);
-  if (!every) {
+  if (!every && !summed) {
     uint32_t tie_at = tie_base;
     run_sum = 0;
 #pragma unroll 4
@@ -748,9 +851,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   const uint64_t slice = lane < size ? cluster.map_shared_rank(s, lane)->slice_sum : 0;
   before += warp_sum_u64(lane < rank ? slice : 0);
   const uint64_t kept = warp_sum_u64(slice);
-  const float u = fminf(fmaxf(a.uniforms[r], 0.0f), 1.0f);
-  uint64_t goal = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(kept));
-  if (goal >= kept) goal = kept - 1;
+  const uint64_t goal = goal_of(kept);
   if (before <= goal && goal < before + run_sum) {
     uint64_t sum = before;
     uint32_t tie_at = tie_base;

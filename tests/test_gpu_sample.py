@@ -26,7 +26,7 @@ def allowed(x, heat, k, p, least, u):
         return {0}, np.full(len(x), -np.inf)
     greedy = not heat > 0
     with np.errstate(invalid="ignore"):
-        z = np.where(x == best, 0.0, (x - best) / (1.0 if greedy else heat))
+        z = np.where(x == best, 0.0, np.where(x == -np.inf, -np.inf, (x - best) / (1.0 if greedy else heat)))
     w = np.exp(z)
     logp = z - np.log(w.sum())
     if greedy:
@@ -96,6 +96,35 @@ def test_flat_rows_keep_the_lowest_indices(gpu, cuda_lib):
     assert np.array_equal(check(x, "bf16", 1.0, 0, 63.5 / n, 0.0, u, gpu), np.arange(64))
     assert np.array_equal(check(x, "f32", 1.0, 0, 1.0, 0.0, u, gpu), (u * n).astype(int))
     check(x, "f32", 0.0, 0, 1.0, 0.0, u, gpu)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [2500, 32003, 151936, 400001])
+@pytest.mark.parametrize("p", [0.05, 0.5, 0.9, 0.999, 0.9999999])
+def test_large_nuclei(gpu, cuda_lib, kind, vocab, p):
+    # Flat distributions: the kept set is a good part of the row, in f16 and bf16 with many ties at its end.
+    r = np.random.default_rng(vocab + int(1000 * p))
+    x = r.standard_normal((6, vocab)) * np.array([0.05, 0.5, 1.0, 1.0, 2.0, 3.0])[:, None]
+    check(x, kind, [1.0, 1.0, 0.8, 3.0, 1.0, 2.0], 0, p, [0.0, 0.0, 0.0, 0.01, 0.0, 0.001], r.random(6), gpu)
+
+
+@pytest.mark.parametrize("few", [1, 700, 1500])
+def test_two_values(gpu, cuda_lib, few):
+    # Two heaps of ties, the cut in either; numbers at both ends.
+    n = 20000
+    x = np.full((8, n), -1.0)
+    at = np.random.default_rng(few).permutation(n)[:few]
+    x[:, at] = 2.0
+    mass = few * np.exp(3.0)
+    ps = np.array([0.5 * mass, 0.999 * mass, mass + 0.5 * (n - few), mass + n - few - 1.5]) / (mass + n - few)
+    check(x, "f32", 1.0, 0, np.repeat(ps, 2), 0.0, np.tile([0.0, 0.99999], 4), gpu)
+
+
+def test_temperatures_without_bounds(gpu, cuda_lib):
+    x = np.random.default_rng(4).standard_normal((4, 3000))
+    x[:, ::3] = -np.inf
+    token = check(x, "f32", [1e38, 3e38, np.inf, np.inf], 0, [1.0, 0.5, 1.0, 0.5], 0.0, [0.3, 0.6, 0.9, 0.999], gpu)
+    assert np.all(token % 3 != 0)
 
 
 def test_zeros_of_both_signs_tie(gpu, cuda_lib):

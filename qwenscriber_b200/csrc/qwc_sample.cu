@@ -42,7 +42,7 @@ constexpr uint32_t kListed = kSampleThreads;  // tokens that the first CTA takes
 constexpr uint32_t kPairs = 256;
 constexpr uint32_t kLimbBits = 14;          // 2^17 tokens of a slice times 2^14 stay below 2^32
 constexpr float kBinScale = 23.0f;      // coarse bins in a power of two; the last bin takes all below 2^-44, whose units are 0
-constexpr uint32_t kNear = 16 * 23;  // coarse bins that are counted in the first pass
+constexpr float kNear = 12.0f;  // logits below the best whose coarse bins are counted in the first pass
 constexpr float kUnits = 4398046511104.0f;  // 2^42: 2^20 tokens of weight 1 stay below 2^63
 
 struct SampleArgs {
@@ -85,6 +85,7 @@ struct Fall {
   __device__ __forceinline__ float of(float x) const { return fmaxf(best - x, 0.0f) * scale; }
 };
 __device__ __forceinline__ float weight_of(float t) { return ex2(-t); }
+// (Moving the mantissa to its place by 64-bit shifts instead: 1 x 151936 17.0 us, this 15.9.)
 __device__ __forceinline__ uint64_t units_of(float w) { return __float2ull_rn(w * kUnits); }
 
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
@@ -136,9 +137,12 @@ struct SampleSmem {
   uint64_t scan[kSampleWarps];
   uint32_t scan_count[kSampleWarps];
   uint64_t total;      // the row's (first CTA) sum of all units
-  uint64_t mass_above; // the row's (first CTA) sum of the units above the bins in question
+  uint64_t mass_above; // the row's (first CTA) sum of the units above the bins in question; the units before the holder
   uint64_t slice_sum;  // this slice's sum of kept units
   uint32_t slice_ties;
+  uint32_t holder;  // the run that holds the token
+  uint32_t few, few_key[32];  // a bin's tokens
+  uint64_t few_units[32];
   float best;
   uint32_t best_at;
   Cut cut;
@@ -187,58 +191,60 @@ __device__ void find_bin(SampleSmem* s, uint32_t n, uint64_t m, bool by_mass, ui
 
 // Narrowing within one CTA: of the tokens that take part, one to a thread, with keys lo .. hi, the key at which
 // the falling order reaches the target, in cut.bin, and what lies above and at it. False if it is not reached.
-// Eight bits at a time, so that one warp can scan the bins, eight to a lane.
+// Ten bits at a time, until a warp can compare the tokens of a bin with one another.
 __device__ bool narrow(SampleSmem* s, bool part, uint32_t key, uint64_t units, uint32_t lo, uint32_t hi, bool by_mass, uint64_t target,
                        Cut& cut, uint32_t from_count = 0, uint64_t from_mass = 0) {
-  constexpr uint32_t kBits = 8;
   const uint32_t lane = threadIdx.x % 32;
   cut = Cut{from_mass, 0, from_count, 0, 0};
   for (;;) {
-    if (threadIdx.x < (1u << kBits)) {
-      s->fine.mass[threadIdx.x] = 0;
-      s->fine.count[threadIdx.x] = 0;
-    }
+    clear(s->fine);
     __syncthreads();
+    if (threadIdx.x == 0) {
+      s->cut.bin = 0xFFFFFFFFu;
+      s->few = 0;
+    }
     const uint32_t bits = 32 - __clz((hi - lo) | 1u);
-    const uint32_t shift = bits > kBits ? bits - kBits : 0u;
-    if (part && key >= lo && key <= hi) add_to(s->fine.count, s->fine.mass, (hi - key) >> shift, 1, units);
+    const uint32_t shift = bits > kBinBits ? bits - kBinBits : 0u;
+    const bool mine = part && key >= lo && key <= hi;
+    const uint32_t bin = (hi - key) >> shift;
+    if (mine) add_to(s->fine.count, s->fine.mass, bin, 1, units);
     __syncthreads();
-    if (threadIdx.x < 32) {
-      uint64_t m[8], mass = 0;
-      uint32_t n[8], count = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        m[i] = s->fine.mass[8 * lane + i];
-        n[i] = s->fine.count[8 * lane + i];
-        mass += m[i];
-        count += n[i];
-      }
-      uint64_t above_mass = cut.mass + warp_scan_u64(mass) - mass;
-      uint32_t inc = count;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= static_cast<uint32_t>(o)) inc += v;
-      }
-      uint32_t above_count = cut.count + inc - count;
-      bool found = false;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint64_t above = by_mass ? above_mass : above_count, here = by_mass ? m[i] : n[i];
-        if (above < target && target <= above + here) {
-          s->cut = Cut{above_mass, m[i], above_count, n[i], 8 * lane + i};
-          found = true;
-        }
-        above_mass += m[i];
-        above_count += n[i];
-      }
-      if (!__any_sync(0xffffffffu, found) && lane == 0) s->cut.bin = 0xFFFFFFFFu;
-    }
+    find_bin(s, s->fine.count[threadIdx.x], s->fine.mass[threadIdx.x], by_mass, target, cut.count, cut.mass);
     __syncthreads();
     cut = s->cut;
     if (cut.bin == 0xFFFFFFFFu) return false;
     hi -= cut.bin << shift;
     if (shift == 0) break;
+    if (cut.here <= 32) {
+      if (mine && bin == cut.bin) {
+        const uint32_t at = atomicAdd(&s->few, 1u);
+        s->few_key[at] = key;
+        s->few_units[at] = units;
+      }
+      __syncthreads();
+      if (threadIdx.x < 32) {
+        const bool in = lane < cut.here;
+        const uint32_t k = in ? s->few_key[lane] : 0u;
+        const uint64_t u = in ? s->few_units[lane] : 0;
+        uint32_t above = 0, here = 0;
+        uint64_t above_mass = 0, here_mass = 0;
+        for (uint32_t j = 0; j < cut.here; ++j) {
+          const uint32_t kj = __shfl_sync(0xffffffffu, k, j);
+          const uint64_t uj = __shfl_sync(0xffffffffu, u, j);
+          above += kj > k ? 1u : 0u;
+          above_mass += kj > k ? uj : 0;
+          here += kj == k ? 1u : 0u;
+          here_mass += kj == k ? uj : 0;
+        }
+        above += cut.count;
+        above_mass += cut.mass;
+        const uint64_t before = by_mass ? above_mass : above, at_it = by_mass ? here_mass : here;
+        if (in && before < target && target <= before + at_it) s->cut = Cut{above_mass, here_mass, above, here, k};
+      }
+      __syncthreads();
+      cut = s->cut;
+      return true;
+    }
     lo = hi - min(hi - lo, (1u << shift) - 1u);
   }
   cut.bin = hi;
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   for (int o = 16; o > 0; o >>= 1) better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, at, o));
   if (lane == 0) s->sums[warp] = uint64_t(__float_as_uint(best)) << 32 | at;
   s->coarse_count[threadIdx.x] = 0;
-  if (threadIdx.x == 0) s->total = 0, s->mass_above = 0, s->listed = 0;
+  if (threadIdx.x == 0) s->total = 0, s->mass_above = 0, s->listed = 0, s->holder = kSampleWarps;
   __syncthreads();
   better(__uint_as_float(static_cast<uint32_t>(s->sums[lane] >> 32)), static_cast<uint32_t>(s->sums[lane]));
 #pragma unroll
@@ -341,21 +347,23 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   auto coarse_bin = [&](float t) { return static_cast<uint32_t>(fminf(t * kBinScale, static_cast<float>(kBins - 1))); };
   const bool cuts = by_count || by_mass, any_cut = cuts || (!greedy && least > 0.0f);
   uint64_t run_sum = 0;
-  // Most of a row lies far down, where a count is seldom asked for and costs a shared atomic: the bins of the first 16
-  // powers of two are counted here, the others only if the kept set reaches them.
+  // Most of a row lies far down, where a count is seldom asked for and costs a shared atomic: the bins of the first
+  // kNear logits are counted here, the others only if the kept set reaches them, the last one never (it has the rest).
+  const uint32_t near = static_cast<uint32_t>(fminf(kNear * scaled.scale * kBinScale, static_cast<float>(kBins - 1)));
+  const float near_place = static_cast<float>(near);
   const uint32_t whole = i0 + (i1 - i0) / 32 * 32;
 #pragma unroll 4
   for (uint32_t i = i0; i < whole; i += 32) {
     const float t = fall_of(value(i + lane));
     run_sum += units_of(weight_of(t));
     const float place = t * kBinScale;
-    if (any_cut && place < kNear) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
+    if (any_cut && place < near_place) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
   }
   if (whole + lane < i1) {
     const float t = fall_of(value(whole + lane));
     run_sum += units_of(weight_of(t));
     const float place = t * kBinScale;
-    if (any_cut && place < kNear) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
+    if (any_cut && place < near_place) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
   }
   run_sum = warp_sum_u64(run_sum);
   if (lane == 0) {
@@ -363,7 +371,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     atomicAdd(reinterpret_cast<unsigned long long*>(&s0->total), static_cast<unsigned long long>(run_sum));
   }
   __syncthreads();
-  if (any_cut && rank != 0 && threadIdx.x < kNear && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
+  if (any_cut && rank != 0 && threadIdx.x < near && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
   cluster.sync();
   const uint64_t all = s0->total;
   const float log_all = logf(static_cast<float>(all) / kUnits);
@@ -412,16 +420,19 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   // The kept set, once it is known: keys above `key`, and at it the first `ties` of the `here` tokens, or those up to index `tie_last`.
   uint32_t key = 0, ties = 0xFFFFFFFFu, here = 0, tie_last = 0xFFFFFFFFu;
   bool summed = false;  // the sums of the runs are those of the kept set
+  uint32_t bin_count = 0;  // of coarse bin threadIdx.x, over the row, as far down as the kept set can reach
+  uint64_t bin_mass = 0;
 
   if (any_cut) {
     // How far down the kept set can reach. top_p's bin is bounded by the least that the bins' tokens can weigh; where
     // top_k cuts too, what top_k left has to be known first, and only top_k bounds.
     // (Every CTA works it out from the first one's counts.)
     uint32_t reach, reached, n, above;
-    uint32_t counted = kNear;
+    uint32_t counted = near == kBins - 1 ? kBins : near;
     for (;; counted = kBins) {
-      n = threadIdx.x < counted ? s0->coarse_count[threadIdx.x] : 0u;
+      n = threadIdx.x < min(counted, kBins - 1) ? s0->coarse_count[threadIdx.x] : 0u;
       above = sum_above(s, n);
+      if (counted == kBins && threadIdx.x == kBins - 1) n = a.vocab - above;
       __syncthreads();
       if (threadIdx.x == 0) s->reach = kBins - 1;
       const uint64_t want = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(all)));
@@ -444,20 +455,19 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       if (threadIdx.x == reach) s->reached = above + n;
       __syncthreads();
       reached = s->reached;
-      if (reach < counted) break;
-      // The other bins' counts. (The last one can hold most of a row: one count for all its lanes.)
+      // (top_p alone with many tokens: what follows needs every bin's count.)
+      if (counted == kBins || (reach < counted && (reached <= kListed || by_count || !by_mass))) break;
+      // The other bins' counts.
 #pragma unroll 4
       for (uint32_t i = i0; i < i1; i += 32) {
-        const bool in = i + lane < i1;
-        const uint32_t bin = in ? coarse_bin(fall_of(value(i + lane))) : 0u;
-        const uint32_t end = __ballot_sync(0xffffffffu, bin == kBins - 1);
-        if (end && lane == 0) atomicAdd(&s->coarse_count[kBins - 1], static_cast<uint32_t>(__popc(end)));
-        if (bin >= kNear && bin != kBins - 1) atomicAdd(&s->coarse_count[bin], 1u);
+        const uint32_t bin = i + lane < i1 ? coarse_bin(fall_of(value(i + lane))) : kBins - 1;
+        if (bin >= near && bin != kBins - 1) atomicAdd(&s->coarse_count[bin], 1u);
       }
       __syncthreads();
-      if (rank != 0 && threadIdx.x >= kNear && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
+      if (rank != 0 && threadIdx.x >= near && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
       cluster.sync();
     }
+    bin_count = n;
     if (reached <= kListed) {
       // ---- few enough for the first CTA ----
       uint32_t lo, hi;
@@ -586,16 +596,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       // cuts, to a small part of a bin.
       uint64_t n_least = n * units_of(weight_of((threadIdx.x + 1) / kBinScale) * 0.99999f);
       uint64_t n_most = n * (units_of(weight_of(threadIdx.x / kBinScale) * 1.00001f) + 1);
-      if (threadIdx.x == kBins - 1) {  // (its units are 0; here: what was not counted)
-        n_least = 0;
-        n_most = counted == kBins ? 0 : (a.vocab - above) * (units_of(weight_of(kNear / kBinScale) * 1.00001f) + 1);
-      }
+      if (threadIdx.x == kBins - 1) n_least = n_most = 0;  // (its units are 0)
       const uint64_t above_least = sum_above(s, n_least);
       __syncthreads();
       const uint64_t above_most = sum_above(s, n_most);
       if (threadIdx.x == kBins - 1) {
-        s->cut.mass = above_least + n_least;
-        s->cut.here_mass = above_most + n_most;
+        s->cut.mass = above_least;
+        s->cut.here_mass = above_most;
       }
       if (threadIdx.x == 0) s->reach = 0, s->reached = kBins - 1;
       __syncthreads();
@@ -669,8 +676,6 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     }
   }
 
-  uint32_t bin_count = 0;  // of coarse bin threadIdx.x, over the row
-  uint64_t bin_mass = 0;
   if (cuts && !summed) {
     // ---- a large kept set: the masses of the coarse bins, then the one that holds the cut ----
 #pragma unroll
@@ -698,7 +703,6 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     __syncthreads();
     clear(s->fine);
     cluster.sync();
-    bin_count = s0->coarse_count[threadIdx.x];
     bin_mass = s0->coarse_mass[threadIdx.x];
     cluster.sync();  // (the list takes the masses' room)
   }
@@ -852,20 +856,51 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   before += warp_sum_u64(lane < rank ? slice : 0);
   const uint64_t kept = warp_sum_u64(slice);
   const uint64_t goal = goal_of(kept);
+  auto answer_with = [&](uint32_t i) {
+    a.tokens[r] = i;
+    if (a.logprobs) a.logprobs[r] = log_of(value(i));
+  };
+  auto units_if_kept = [&](uint32_t i) -> uint64_t {
+    const float x = value(i);
+    const uint32_t k = order_key<T>(x);
+    if (!(k > key || (k == key && i <= tie_last))) return 0;
+    const float w = weight_of(fall_of(x));
+    return w >= least ? units_of(w) : 0;
+  };
   if (before <= goal && goal < before + run_sum) {
-    uint64_t sum = before;
-    uint32_t tie_at = tie_base;
-    for (uint32_t i = i0; i < i1; i += 32) {
-      const uint64_t inc = sum + warp_scan_u64(kept_units(i + lane, tie_at));
-      const uint32_t past = __ballot_sync(0xffffffffu, inc > goal);
-      if (past) {
-        if (lane == static_cast<uint32_t>(__ffs(past)) - 1) {
-          a.tokens[r] = i + lane;
-          if (a.logprobs) a.logprobs[r] = log_of(value(i + lane));
+    if (rank_ties) {
+      uint64_t sum = before;
+      uint32_t tie_at = tie_base;
+      for (uint32_t i = i0; i < i1; i += 32) {
+        const uint64_t inc = sum + warp_scan_u64(kept_units(i + lane, tie_at));
+        const uint32_t past = __ballot_sync(0xffffffffu, inc > goal);
+        if (past) {
+          if (lane == static_cast<uint32_t>(__ffs(past)) - 1) answer_with(i + lane);
+          break;
         }
-        break;
+        sum = __shfl_sync(0xffffffffu, inc, 31);
       }
-      sum = __shfl_sync(0xffffffffu, inc, 31);
+    } else if (lane == 0) {
+      s->holder = warp;
+      s->mass_above = before;
+    }
+  }
+  __syncthreads();
+  if (s->holder < kSampleWarps) {
+    // All warps walk the run that holds the token, 32 tokens of it to a warp at a time.
+    const uint32_t h0 = slice0 + s->holder * a.run, h1 = min(h0 + a.run, slice1);
+    uint64_t from = s->mass_above;
+    for (uint32_t h = h0; h < h1; h += 32 * kSampleWarps) {
+      const uint32_t i = h + threadIdx.x;
+      const uint64_t u = i < h1 ? units_if_kept(i) : 0, inc = warp_scan_u64(u);
+      if (lane == 31) s->scan[warp] = inc;
+      __syncthreads();
+      const uint64_t group = s->scan[lane];
+      const uint64_t mine = from + warp_sum_u64(lane < warp ? group : 0) + inc;
+      if (mine > goal && mine - u <= goal) answer_with(i);
+      from += warp_sum_u64(group);
+      if (from > goal) break;
+      __syncthreads();  // (before the next sums)
     }
   }
   cluster.sync();  // no CTA leaves while another reads its sums

@@ -5,13 +5,16 @@
 // top_k cuts it by count, top_p by the sum of w, min_p by w itself. So the
 // kept set is one threshold logit and a number of tokens that equal it:
 // everything above, and the first of those at it. No sort: the threshold is
-// found by narrowing, ten bits at a time. A histogram of (m - x) / T in steps of
-// 1/33 says how far down the kept set can reach; where that is 1024 tokens or
-// fewer, as a rule, they go to the first CTA of the row, which narrows by the logits'
-// order-preserving bits (count or mass against its target) and then by the index
-// (mass against u times the total) among them alone. Where it is more, all CTAs
-// narrow together, and the token is the first in index order whose running sum
-// passes.
+// found by narrowing. A histogram of (m - x) / T in steps of 1/23 of a power of two says how far down the kept set can
+// reach. Where that is 1024 tokens or fewer, as a rule, they go to the first CTA of the row, which compares them pair by
+// pair or narrows by the logits' order-preserving bits (count or mass against its target) and then by the index
+// (mass against u times the total) among them alone. top_p alone over more: the counts bound the mass above each bin
+// from both sides, and only the few bins that can hold the cut go there. What is left (top_k above 1024, heaps of ties)
+// is narrowed by all CTAs together. The token is the first in index order whose running sum passes.
+//
+// Bound by the chain of passes over the row's slices in shared memory (load and maximum 5.4 us, sums and histogram 6,
+// list 4, cut and token 2, of 64 x 151936) and the exchanges between them, not by HBM: 1 x 151936, f32, 16 us; 64 x 151936,
+// f32, 57 us, two waves of rows; 16 x 32003, bf16, 17 us.
 //
 // Sums are of integers, w in units of 2^-42: they are exact, so neither the
 // order of the atomics nor the split over threads changes a result.
@@ -37,12 +40,12 @@ constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr uint32_t kBins = kSampleThreads;  // a scan takes one bin for each thread
 constexpr uint32_t kBinBits = 10;
 constexpr uint32_t kListed = kSampleThreads;  // tokens that the first CTA takes by itself, one for each thread
-// Up to this many of them are compared pair by pair, each token by as many lanes as there are: two passes over
-// the list, where narrowing takes two or three histograms for each cut.
+// Up to this many of them are compared pair by pair, each token by as many lanes as there are: two passes over the
+// list, where narrowing takes a histogram and more for each cut. 1 x 151936 16 us, by narrowing 21; 16 x 32003 16 and 18.
+// (With 1024 in place of 256 64 x 151936 took 154 us for 67.)
 constexpr uint32_t kPairs = 256;
 constexpr uint32_t kLimbBits = 14;          // 2^17 tokens of a slice times 2^14 stay below 2^32
 constexpr float kBinScale = 23.0f;      // coarse bins in a power of two; the last bin takes all below 2^-44, whose units are 0
-constexpr float kNear = 12.0f;  // logits below the best whose coarse bins are counted in the first pass
 constexpr float kUnits = 4398046511104.0f;  // 2^42: 2^20 tokens of weight 1 stay below 2^63
 
 struct SampleArgs {
@@ -190,12 +193,12 @@ __device__ void find_bin(SampleSmem* s, uint32_t n, uint64_t m, bool by_mass, ui
 }
 
 // Narrowing within one CTA: of the tokens that take part, one to a thread, with keys lo .. hi, the key at which
-// the falling order reaches the target, in cut.bin, and what lies above and at it. False if it is not reached.
-// Ten bits at a time, until a warp can compare the tokens of a bin with one another.
-__device__ bool narrow(SampleSmem* s, bool part, uint32_t key, uint64_t units, uint32_t lo, uint32_t hi, bool by_mass, uint64_t target,
-                       Cut& cut, uint32_t from_count = 0, uint64_t from_mass = 0) {
+// the falling order reaches the target, in s->cut.bin, and what lies above and at it. False if it is not reached.
+// Ten bits at a time, until a warp can compare the tokens of a bin with one another. (One copy of its code: a row's
+// first call finds it in the instruction cache.)
+__device__ __noinline__ bool narrow(SampleSmem* s, bool part, uint32_t key, uint64_t units, uint32_t lo, uint32_t hi, bool by_mass,
+                                    uint64_t target, uint32_t from_count, uint64_t from_mass) {
   const uint32_t lane = threadIdx.x % 32;
-  cut = Cut{from_mass, 0, from_count, 0, 0};
   for (;;) {
     clear(s->fine);
     __syncthreads();
@@ -209,10 +212,12 @@ __device__ bool narrow(SampleSmem* s, bool part, uint32_t key, uint64_t units, u
     const uint32_t bin = (hi - key) >> shift;
     if (mine) add_to(s->fine.count, s->fine.mass, bin, 1, units);
     __syncthreads();
-    find_bin(s, s->fine.count[threadIdx.x], s->fine.mass[threadIdx.x], by_mass, target, cut.count, cut.mass);
+    find_bin(s, s->fine.count[threadIdx.x], s->fine.mass[threadIdx.x], by_mass, target, from_count, from_mass);
     __syncthreads();
-    cut = s->cut;
+    const Cut cut = s->cut;
     if (cut.bin == 0xFFFFFFFFu) return false;
+    from_count = cut.count;
+    from_mass = cut.mass;
     hi -= cut.bin << shift;
     if (shift == 0) break;
     if (cut.here <= 32) {
@@ -242,12 +247,13 @@ __device__ bool narrow(SampleSmem* s, bool part, uint32_t key, uint64_t units, u
         if (in && before < target && target <= before + at_it) s->cut = Cut{above_mass, here_mass, above, here, k};
       }
       __syncthreads();
-      cut = s->cut;
       return true;
     }
     lo = hi - min(hi - lo, (1u << shift) - 1u);
   }
-  cut.bin = hi;
+  __syncthreads();
+  if (threadIdx.x == 0) s->cut.bin = hi;
+  __syncthreads();
   return true;
 }
 
@@ -347,23 +353,21 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   auto coarse_bin = [&](float t) { return static_cast<uint32_t>(fminf(t * kBinScale, static_cast<float>(kBins - 1))); };
   const bool cuts = by_count || by_mass, any_cut = cuts || (!greedy && least > 0.0f);
   uint64_t run_sum = 0;
-  // Most of a row lies far down, where a count is seldom asked for and costs a shared atomic: the bins of the first
-  // kNear logits are counted here, the others only if the kept set reaches them, the last one never (it has the rest).
-  const uint32_t near = static_cast<uint32_t>(fminf(kNear * scaled.scale * kBinScale, static_cast<float>(kBins - 1)));
-  const float near_place = static_cast<float>(near);
+  // (The last bin, which can hold most of a row, is not counted: it has the rest.)
+  constexpr float kLastBin = static_cast<float>(kBins - 1);
   const uint32_t whole = i0 + (i1 - i0) / 32 * 32;
 #pragma unroll 4
   for (uint32_t i = i0; i < whole; i += 32) {
     const float t = fall_of(value(i + lane));
     run_sum += units_of(weight_of(t));
     const float place = t * kBinScale;
-    if (any_cut && place < near_place) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
+    if (any_cut && place < kLastBin) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
   }
   if (whole + lane < i1) {
     const float t = fall_of(value(whole + lane));
     run_sum += units_of(weight_of(t));
     const float place = t * kBinScale;
-    if (any_cut && place < near_place) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
+    if (any_cut && place < kLastBin) atomicAdd(&s->coarse_count[static_cast<uint32_t>(place)], 1u);
   }
   run_sum = warp_sum_u64(run_sum);
   if (lane == 0) {
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     atomicAdd(reinterpret_cast<unsigned long long*>(&s0->total), static_cast<unsigned long long>(run_sum));
   }
   __syncthreads();
-  if (any_cut && rank != 0 && threadIdx.x < near && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
+  if (any_cut && rank != 0 && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
   cluster.sync();
   const uint64_t all = s0->total;
   const float log_all = logf(static_cast<float>(all) / kUnits);
@@ -420,19 +424,18 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   // The kept set, once it is known: keys above `key`, and at it the first `ties` of the `here` tokens, or those up to index `tie_last`.
   uint32_t key = 0, ties = 0xFFFFFFFFu, here = 0, tie_last = 0xFFFFFFFFu;
   bool summed = false;  // the sums of the runs are those of the kept set
-  uint32_t bin_count = 0;  // of coarse bin threadIdx.x, over the row, as far down as the kept set can reach
+  uint32_t bin_count = 0;  // of coarse bin threadIdx.x, over the row
   uint64_t bin_mass = 0;
 
   if (any_cut) {
     // How far down the kept set can reach. top_p's bin is bounded by the least that the bins' tokens can weigh; where
     // top_k cuts too, what top_k left has to be known first, and only top_k bounds.
     // (Every CTA works it out from the first one's counts.)
-    uint32_t reach, reached, n, above;
-    uint32_t counted = near == kBins - 1 ? kBins : near;
-    for (;; counted = kBins) {
-      n = threadIdx.x < min(counted, kBins - 1) ? s0->coarse_count[threadIdx.x] : 0u;
-      above = sum_above(s, n);
-      if (counted == kBins && threadIdx.x == kBins - 1) n = a.vocab - above;
+    uint32_t reach, reached;
+    uint32_t n = s0->coarse_count[threadIdx.x];
+    const uint32_t above = sum_above(s, n);
+    if (threadIdx.x == kBins - 1) n = a.vocab - above;
+    {
       __syncthreads();
       if (threadIdx.x == 0) s->reach = kBins - 1;
       const uint64_t want = static_cast<uint64_t>(ceil(static_cast<double>(fmaxf(p_given, 0.0f)) * static_cast<double>(all)));
@@ -449,23 +452,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       if (!by_mass && least > 0.0f) last |= threadIdx.x == min(static_cast<uint32_t>(fmaxf(-log2f(least), 0.0f) * kBinScale) + 1u, kBins - 1);
       if (by_mass && !by_count && want == 0) last |= threadIdx.x == 0;
       __syncthreads();
-      if (last && threadIdx.x < counted) atomicMin(&s->reach, threadIdx.x);
+      if (last) atomicMin(&s->reach, threadIdx.x);
       __syncthreads();
       reach = s->reach;
       if (threadIdx.x == reach) s->reached = above + n;
       __syncthreads();
       reached = s->reached;
-      // (top_p alone with many tokens: what follows needs every bin's count.)
-      if (counted == kBins || (reach < counted && (reached <= kListed || by_count || !by_mass))) break;
-      // The other bins' counts.
-#pragma unroll 4
-      for (uint32_t i = i0; i < i1; i += 32) {
-        const uint32_t bin = i + lane < i1 ? coarse_bin(fall_of(value(i + lane))) : kBins - 1;
-        if (bin >= near && bin != kBins - 1) atomicAdd(&s->coarse_count[bin], 1u);
-      }
-      __syncthreads();
-      if (rank != 0 && threadIdx.x >= near && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
-      cluster.sync();
     }
     bin_count = n;
     if (reached <= kListed) {
@@ -552,9 +544,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         const uint32_t key = cut.bin;
         if (ties < cut.here) {
           const bool tie = kept && k == key;
-          Cut at_cut;
-          const bool found = narrow(s, tie, place, u, place_lo, place_hi, false, ties, at_cut);
-          if (tie && found && place < at_cut.bin) kept = false;
+          const bool found = narrow(s, tie, place, u, place_lo, place_hi, false, ties, 0, 0);
+          if (tie && found && place < s->cut.bin) kept = false;
         }
         kept = kept && k >= key;
       };
@@ -562,7 +553,10 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       if (by_count) {
         uint32_t bin_lo, bin_hi;
         keys_of(0, reach, bin_lo, bin_hi);
-        if (narrow(s, kept, k, u, bin_lo, bin_hi, false, static_cast<uint32_t>(k_given), cut)) keep_to(static_cast<uint32_t>(k_given) - cut.count);
+        if (narrow(s, kept, k, u, bin_lo, bin_hi, false, static_cast<uint32_t>(k_given), 0, 0)) {
+          cut = s->cut;
+          keep_to(static_cast<uint32_t>(k_given) - cut.count);
+        }
         if (by_mass) {
           const uint64_t above = sum_above(s, kept ? u : 0);
           if (threadIdx.x == kSampleThreads - 1) s->slice_sum = above + (kept ? u : 0);
@@ -573,7 +567,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       }
       if (by_mass) {
         const uint64_t target = target_of(mass);
-        if (narrow(s, kept, k, u, lo, hi, true, target, cut)) {
+        if (narrow(s, kept, k, u, lo, hi, true, target, 0, 0)) {
+          cut = s->cut;
           const uint64_t each = cut.here_mass / cut.here;
           keep_to(static_cast<uint32_t>((target - cut.mass + each - 1) / each));
         }
@@ -583,7 +578,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
       if (threadIdx.x == kSampleThreads - 1) s->slice_sum = above + (kept ? u : 0);
       __syncthreads();
       const uint64_t goal = goal_of(s->slice_sum);
-      if (narrow(s, kept, place, u, place_lo, place_hi, true, goal + 1, cut) && kept && place == cut.bin) {
+      if (narrow(s, kept, place, u, place_lo, place_hi, true, goal + 1, 0, 0) && kept && place == s->cut.bin) {
         a.tokens[r] = index;
         if (a.logprobs) a.logprobs[r] = log_of(key_value<T>(k));
       }
@@ -649,15 +644,14 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
           const uint64_t u = have ? s->list.units[threadIdx.x] : 0;
           uint32_t lo, hi;
           keys_of(b0, b1, lo, hi);
-          Cut cut;
-          narrow(s, have, k, u, lo, hi, true, target, cut, over, s->mass_above);
+          narrow(s, have, k, u, lo, hi, true, target, over, s->mass_above);
+          const Cut cut = s->cut;
           const uint64_t each = cut.here_mass / cut.here;
           const uint32_t stay = static_cast<uint32_t>((target - cut.mass + each - 1) / each);
           uint32_t last = 0xFFFFFFFFu;
           if (stay < cut.here) {
-            Cut at_cut;
-            narrow(s, have && k == cut.bin, ~index & 0x7FFFFFFFu, u, 0x7FFFFFFFu - (a.vocab - 1), 0x7FFFFFFFu, false, stay, at_cut);
-            last = ~at_cut.bin & 0x7FFFFFFFu;
+            narrow(s, have && k == cut.bin, ~index & 0x7FFFFFFFu, u, 0x7FFFFFFFu - (a.vocab - 1), 0x7FFFFFFFu, false, stay, 0, 0);
+            last = ~s->cut.bin & 0x7FFFFFFFu;
           }
           if (have && flagged == index && (k > cut.bin || (k == cut.bin && index <= last))) {
             const uint32_t slice = index / (a.run * kSampleWarps);
@@ -747,10 +741,9 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         const bool have = threadIdx.x < min(s->listed, kListed);
         const uint32_t k = have ? s->list.key[threadIdx.x] : 0u;
         const uint64_t u = have ? s->list.units[threadIdx.x] : 0;
-        Cut found;
-        narrow(s, have, k, u, lo, hi, mass, target, found, cut.count, cut.mass);
+        narrow(s, have, k, u, lo, hi, mass, target, cut.count, cut.mass);
         if (threadIdx.x == 0) {
-          s->answer = found;
+          s->answer = s->cut;
           s->listed = 0;
         }
         __syncthreads();
@@ -909,8 +902,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
 template <typename T>
 int32_t sample_as(SampleArgs a, uint32_t rows, cudaStream_t stream) {
   // CTAs to a row: as few as hold it in their shared memory, then twice as many while there are SMs for all rows, at
-  // most 8. One row of 151936: eight CTAs 17.6 us, four 23.5 (sixteen 17.6); 64 rows: four 67 us, eight 84 (more waves,
-  // each with a row's dozen exchanges), two 137 (slices that do not fit are read again and again).
+  // most 8. One row of 151936: eight CTAs 16 us, four 22 (sixteen as eight); 64 rows: four 62 us, eight 74 (more waves,
+  // each with a row's dozen exchanges), two 137 before later steps (slices that do not fit are read again and again).
   const uint32_t most = (227 * 1024 - 1024 - static_cast<uint32_t>(sizeof(SampleSmem))) / 4;
   uint32_t size = 1;
   while (size < 8 && (uint64_t(size) * most < a.vocab || rows * size * 2 <= 148)) size *= 2;

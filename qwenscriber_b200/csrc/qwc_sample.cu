@@ -380,11 +380,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   const uint64_t all = s0->total;
   const float log_all = logf(static_cast<float>(all) / kUnits);
   auto log_of = [&](float x) { return (x == best ? 0.0f : (x - best) / heat) - log_all; };
+  // The largest logit's token is the answer until another is found (each is written behind a barrier of the cluster):
+  // whatever the row holds, the outputs are written.
+  if (rank == 0 && threadIdx.x == 0) {
+    a.tokens[r] = at;
+    if (a.logprobs) a.logprobs[r] = -log_all;
+  }
   if (greedy) {
-    if (rank == 0 && threadIdx.x == 0) {
-      a.tokens[r] = at;
-      if (a.logprobs) a.logprobs[r] = -log_all;
-    }
     cluster.sync();
     return;
   }
@@ -742,6 +744,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         const uint32_t k = have ? s->list.key[threadIdx.x] : 0u;
         const uint64_t u = have ? s->list.units[threadIdx.x] : 0;
         narrow(s, have, k, u, lo, hi, mass, target, cut.count, cut.mass);
+        clear(s->fine);  // (the next cut may be narrowed by all CTAs, which add to it)
         if (threadIdx.x == 0) {
           s->answer = s->cut;
           s->listed = 0;

@@ -204,3 +204,48 @@ def test_refusals(gpu, cuda_lib):
     refused("invalid_argument", x, u, top_k=torch.zeros(2, device=gpu))
     refused("invalid_argument", x[:, :0], u)
     refused("limit_exceeded", torch.zeros(1, rt.SAMPLE_MAX_VOCAB + 1, device=gpu), u[:1])
+
+
+def check_counts_and_masses(x, kind, heat, k, p, least, gpu):
+    """One row of logits with several numbers, so that most of the kept set is walked."""
+    u = (np.arange(12) + 0.5) / 12
+    check(np.broadcast_to(x, (12, len(x))).copy(), kind, heat, k, p, least, u, gpu)
+
+
+def test_a_count_above_a_thousand_and_a_mass(gpu, cuda_lib):
+    # top_k's cut lies in a bin of few tokens or many, top_p's likewise: the two searches follow one another.
+    r = np.random.default_rng(21)
+    check_counts_and_masses(r.uniform(0, 0.055, 2100), "f32", 1.0, 2000, 0.5, 0.0, gpu)
+    check_counts_and_masses(r.standard_normal(5000), "f32", 20.0, 4900, 0.6, 0.0, gpu)
+    check_counts_and_masses(2.2 * r.standard_normal(151936), "f32", 10.0, 151000, 0.3, 0.0, gpu)
+    x = np.concatenate([r.uniform(0.032, 0.060, 1200), r.uniform(0, 0.028, 900)])
+    check_counts_and_masses(r.permutation(x), "f32", 1.0, 1900, 0.45, 0.0, gpu)
+    x = np.concatenate([[1.0], np.full(2000, 0.975), r.uniform(0.3685, 0.3965, 900), np.full(4000, -9.0)])
+    check_counts_and_masses(r.permutation(x), "f32", 1.0, 2500, 0.6, 0.0, gpu)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("at_mass", [300, 3000])
+@pytest.mark.parametrize("at_count", [300, 3000])
+@pytest.mark.parametrize("least", [0.0, 0.2])
+def test_ties_at_both_cuts(gpu, cuda_lib, kind, at_mass, at_count, least):
+    # Heaps of ties, small and large, the mass's cut inside the upper one and the count's inside the lower one.
+    r = np.random.default_rng(at_mass + 7 * at_count)
+    x = np.concatenate([2.0 + np.arange(1200) / 1200, np.full(at_mass, 1.5), 1.0 + np.arange(600) / 2400, np.full(at_count, 0.5),
+                        r.uniform(-4, -3, 5000)])
+    x = torch.as_tensor(x).to(TYPES[kind]).double().numpy()
+    k = 1200 + at_mass + 600 + at_count // 2
+    w = np.exp(x)
+    p = (w[:1200].sum() + w[1200:1200 + at_mass].sum() / 2) / w[:k].sum()
+    check_counts_and_masses(r.permutation(x), kind, 1.0, k, p, least, gpu)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [1100, 2100, 32003, 151936, 400001])
+def test_large_counts_with_masses(gpu, cuda_lib, kind, vocab):
+    r = np.random.default_rng(vocab)
+    rows = 16
+    x = r.standard_normal((rows, vocab)) * r.choice([0.02, 0.3, 1.0, 2.2], rows)[:, None]
+    k = np.exp(r.uniform(np.log(1025), np.log(vocab - 1), rows)).astype(int)
+    check(x, kind, r.choice([0.7, 1.0, 5.0, 20.0], rows), k, r.choice([0.05, 0.3, 0.6, 0.9, 0.999, 1.0], rows),
+          r.choice([0.0, 0.0, 0.001, 0.5], rows), r.random(rows), gpu)

@@ -46,7 +46,8 @@ constexpr uint32_t kListed = kSampleThreads;  // tokens that the first CTA takes
 constexpr uint32_t kPairs = 256;
 constexpr uint32_t kLimbBits = 14;          // 2^17 tokens of a slice times 2^14 stay below 2^32
 constexpr float kBinScale = 23.0f;      // coarse bins in a power of two; the last bin takes all below 2^-44, whose units are 0
-constexpr float kUnits = 4398046511104.0f;  // 2^42: 2^20 tokens of weight 1 stay below 2^63
+constexpr int kUnitBits = 42;               // a weight of 1 in units: 2^20 tokens of it stay below 2^63
+constexpr float kUnits = 4398046511104.0f;  // 2^42
 
 struct SampleArgs {
   const void* logits;
@@ -378,7 +379,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   if (any_cut && rank != 0 && s->coarse_count[threadIdx.x]) atomicAdd(&s0->coarse_count[threadIdx.x], s->coarse_count[threadIdx.x]);
   cluster.sync();
   const uint64_t all = s0->total;
-  const float log_all = logf(static_cast<float>(all) / kUnits);
+  // Of the sum 1 + rest, the largest token's unit taken off exactly: near 1 the logarithm keeps the bits of the rest.
+  const float log_all = log1pf(static_cast<float>(all - (uint64_t(1) << kUnitBits)) / kUnits);
   auto log_of = [&](float x) { return (x == best ? 0.0f : (x - best) / heat) - log_all; };
   // The largest logit's token is the answer until another is found (each is written behind a barrier of the cluster):
   // whatever the row holds, the outputs are written.

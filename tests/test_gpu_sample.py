@@ -249,3 +249,25 @@ def test_large_counts_with_masses(gpu, cuda_lib, kind, vocab):
     k = np.exp(r.uniform(np.log(1025), np.log(vocab - 1), rows)).astype(int)
     check(x, kind, r.choice([0.7, 1.0, 5.0, 20.0], rows), k, r.choice([0.05, 0.3, 0.6, 0.9, 0.999, 1.0], rows),
           r.choice([0.0, 0.0, 0.001, 0.5], rows), r.random(rows), gpu)
+
+
+@pytest.mark.parametrize("gap", [9.0, 14.0, 18.0, 20.0])
+@pytest.mark.parametrize("heat", [0.0, 0.7, 1.0])
+def test_log_probabilities_near_zero(gpu, cuda_lib, gap, heat):
+    # A token that is all but certain: its log-probability is -log1p of the others' weight. Each weight is off by the
+    # exponential's 2^-22 and by three roundings of its exponent (below 30: 30 * 3 * 2^-24), and by 2^-43 as an integer.
+    n = 40
+    r = np.random.default_rng(int(gap))
+    x = np.full((6, n), -np.inf)
+    x[:, 3] = 11.0
+    x[:, 7:7 + 6] = 11.0 - gap * (heat or 1.0) - np.arange(6) / 5 - r.random((6, 1))
+    x = torch.as_tensor(x).float()
+    temperature = torch.full((6,), heat, device=gpu)
+    token, logprob = sampling.sample(x.to(gpu), torch.full((6,), 0.5, device=gpu), temperature=temperature)
+    assert torch.all(token == 3)
+    z = (x.double() - x.double()[:, 3:4]) / (float(temperature[0]) or 1.0)
+    z[:, 3] = -np.inf
+    tail = z.exp().sum(-1)
+    want = -torch.log1p(tail)
+    bound = (2.0 ** -22 + 30 * 3 * 2.0 ** -24 + 2.0 ** -22) * want.abs() + 6 * 2.0 ** -43
+    assert torch.all((logprob.double().cpu() - want).abs() <= bound), (logprob, want)

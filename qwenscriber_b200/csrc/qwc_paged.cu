@@ -36,10 +36,11 @@ struct AppendArgs {
   float eps;
 };
 
-// 1 / sqrt(v): the hardware's estimate and one step of Newton's iteration.
+// 1 / sqrt(v): the hardware's estimate and one step of Newton's iteration, where that is of numbers (not of a sum that
+// overflowed, whose root's inverse is 0, nor of 0).
 __device__ __forceinline__ float inverse_root(float v) {
   const float r = rsqrtf(v);
-  return r == r && r < 1e30f ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
+  return r > 0.0f && r < 1e30f ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
 }
 
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {

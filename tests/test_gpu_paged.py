@@ -484,3 +484,23 @@ def test_refusals(gpu, cuda_lib):
     refused("unsupported", paged.attention, wrong, batch, torch.zeros(4, 4, 32, device=gpu))
     long = paged.PagedBatch(batch.query_starts, batch.context_lens, batch.page_table, tokens=4, max_query=3, max_context=16 * 50)
     refused("shape_mismatch", paged.attention, cache, long, q)
+
+
+def test_append_of_heads_whose_squares_overflow(gpu, cuda_lib):
+    # 128 squares of 1e19 and more pass f32: the norm's factor is 0 then, and so are the head's values, as in f32
+    # arithmetic throughout (x * (1 / sqrt(inf)) = 0). The other heads of the token keep theirs.
+    world = World([3], [3], 16, 2, 128, seed=14)
+    cache, batch = world.device(gpu)
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (torch.randn(3, n, 128, generator=g).to(gpu) for n in (4, 2, 2))
+    norms = dict(q_norm=torch.ones(128, device=gpu), k_norm=torch.ones(128, device=gpu))
+    tables = identity_tables(3, 128, gpu)
+    clean = paged.append(cache, batch, q, k, v, *tables, **norms)
+    clean_k = paged.read(cache, batch)[0]
+    q[1, 2] *= 1e20
+    k[2, 0, 5] = -3e19
+    got = paged.append(cache, batch, q, k, v, *tables, **norms)
+    got_k = paged.read(cache, batch)[0]
+    assert torch.all(got[1, 2] == 0) and torch.all(got_k[2, 0] == 0)
+    clean[1, 2], clean_k[2, 0] = 0, 0
+    assert torch.equal(got, clean) and torch.equal(got_k, clean_k)

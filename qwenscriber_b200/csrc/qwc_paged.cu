@@ -102,6 +102,9 @@ __device__ __forceinline__ void q8_codes(const uint64_t (&y)[V / 2], float store
 // blocks to an SM instead of 48 and five, 71 with two tokens to a block.
 constexpr uint32_t kAppendTokens = 4;
 
+// What a token that is not cached reads of the rotation (and does not use) where the tables have no row.
+__device__ __align__(16) const float kNoRotation[64] = {};
+
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreads, 5) paged_append_kernel(const PagedArgs a, const AppendArgs<T> p) {
   constexpr int V = Vec16<T>::kCount;
@@ -388,6 +391,12 @@ int32_t qwc_op_paged_append(const qwc_paged_cache* cache, const qwc_paged_batch*
   if ((st = paged_rows_check(k, k_stride, a.code_row, format)) != QWC_OK) return st;
   if ((st = paged_rows_check(v, v_stride, a.code_row, format)) != QWC_OK) return st;
   if ((st = paged_rows_check(q_out, q_out_stride, qw, format)) != QWC_OK) return st;
+  if (rope_rows == 0) {
+    void* none = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&none, kNoRotation);
+    if (e != cudaSuccess) return paged_status(e);
+    cos_table = sin_table = static_cast<const float*>(none);
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto run = format == kFormatF32 ? append_as<float> : format == kFormatF16 ? append_as<__half> : append_as<__nv_bfloat16>;
   return run(a, q, q_stride, k, k_stride, v, v_stride, heads, q_norm, k_norm, eps, cos_table, sin_table, rope_rows, q_out,

@@ -504,3 +504,19 @@ def test_append_of_heads_whose_squares_overflow(gpu, cuda_lib):
     assert torch.all(got[1, 2] == 0) and torch.all(got_k[2, 0] == 0)
     clean[1, 2], clean_k[2, 0] = 0, 0
     assert torch.equal(got, clean) and torch.equal(got_k, clean_k)
+
+
+def test_append_with_rotation_tables_of_no_rows(gpu, cuda_lib):
+    # rope_rows of 0 in the C call: every token lies past the tables, which are not read (the rows here are NaN).
+    world = World([2, 1], [20, 5], 16, 2, 64, seed=15)
+    cache, batch = world.device(gpu)
+    before = [t.clone() for t in (cache.k_scales, cache.k_codes, cache.v_scales, cache.v_codes)]
+    q, k, v = (torch.randn(3, n, 64, device=gpu) for n in (4, 2, 2))
+    out, nan = torch.full_like(q, 7.0), torch.full((1, 32), float("nan"), device=gpu)
+    st = rt.lib().qwc_op_paged_append(
+        cache._ref, batch._ref, rt.FORMAT_F32, q.data_ptr(), 256, k.data_ptr(), 128, v.data_ptr(), 128, 4, None, None, 1e-6,
+        nan.data_ptr(), nan.data_ptr(), 0, out.data_ptr(), 256, paged.current_stream(gpu))
+    torch.cuda.synchronize()
+    assert st == 0 and torch.all(out == 0)
+    for old, new in zip(before, (cache.k_scales, cache.k_codes, cache.v_scales, cache.v_codes)):
+        assert torch.equal(old.view(torch.uint8), new.view(torch.uint8))

@@ -482,13 +482,13 @@ typedef struct qwc_paged_cache {
 typedef struct qwc_paged_batch {
   const int32_t* query_starts; /* [sequences + 1], ascending, the last = tokens */
   const int32_t* context_lens; /* [sequences], this step's tokens included */
-  const int32_t* page_table;   /* [sequences][table_stride] */
+  const int32_t* page_table;   /* rows of table_entries, table_stride entries apart (0: one row for all sequences) */
   uint32_t sequences;
   uint32_t tokens;
   uint32_t table_stride;
   uint32_t max_query;
   uint32_t max_context;
-  uint32_t reserved;
+  uint32_t table_entries; /* entries of a row that may be read, enough for max_context; 0: table_stride */
 } qwc_paged_batch;
 
 /* QK-RMSNorm, rotary positions and the q8 append of a step's rows in one pass (what the decoder does

@@ -315,8 +315,9 @@ int32_t paged_args(const qwc_paged_cache* c, const qwc_paged_batch* b, PagedArgs
   }
   if (c->head_dim != 64 && c->head_dim != 128) return QWC_UNSUPPORTED;
   if (c->kv_heads == 0 || c->page_size == 0 || c->pages == 0) return QWC_SHAPE_MISMATCH;
-  // Every position of a sequence has an entry in its row of the table.
-  if (uint64_t(b->table_stride) * c->page_size < b->max_context) return QWC_SHAPE_MISMATCH;
+  // Every position of a sequence has an entry in its row of the table, whatever lies between two rows.
+  const uint32_t entries = b->table_entries ? b->table_entries : b->table_stride;
+  if (uint64_t(entries) * c->page_size < b->max_context) return QWC_SHAPE_MISMATCH;
   if (uint64_t(c->pages) * c->page_size > 0x7FFFFFFFu || b->max_context > 0x7FFFFFFFu || b->tokens > 0x7FFFFFFFu ||
       c->kv_heads > 1024 || b->sequences > kPagedMaxSequences) {
     return QWC_LIMIT_EXCEEDED;

@@ -97,9 +97,10 @@ class PagedBatch:
             refuse("invalid_argument", "PagedBatch")
         self.query_starts, self.context_lens, self.page_table = query_starts, context_lens, page_table
         self.device, self.tokens = query_starts.device, tokens
-        entries = page_table.stride(0) if n > 1 else page_table.shape[1]
+        # A view's rows may lie further apart than they are long (or be one row): the length bounds what is read.
+        entries = page_table.shape[1]
         self.desc = PagedBatchDesc(query_starts.data_ptr(), context_lens.data_ptr(), page_table.data_ptr(), n, tokens,
-                                   entries, max_query, max_context, 0)
+                                   page_table.stride(0) if n > 1 and entries else 0, max_query, max_context, entries)
         self._ref = ctypes.addressof(self.desc)
         self._workspace_bytes: dict = {}
 

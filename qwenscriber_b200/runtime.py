@@ -196,7 +196,7 @@ class PagedBatchDesc(ctypes.Structure):
     _fields_ = [
         ("query_starts", c_void_p), ("context_lens", c_void_p), ("page_table", c_void_p),
         ("sequences", c_uint32), ("tokens", c_uint32), ("table_stride", c_uint32), ("max_query", c_uint32),
-        ("max_context", c_uint32), ("reserved", c_uint32),
+        ("max_context", c_uint32), ("table_entries", c_uint32),
     ]
 
 

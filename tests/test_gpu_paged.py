@@ -520,3 +520,18 @@ def test_append_with_rotation_tables_of_no_rows(gpu, cuda_lib):
     assert st == 0 and torch.all(out == 0)
     for old, new in zip(before, (cache.k_scales, cache.k_codes, cache.v_scales, cache.v_codes)):
         assert torch.equal(old.view(torch.uint8), new.view(torch.uint8))
+
+
+@pytest.mark.parametrize("query", [1, 30])
+def test_tables_that_are_views(gpu, cuda_lib, query):
+    # Columns of a wider table, and one row for all sequences (a prefix that they share).
+    world = World([query, query, 2], [100, 70, 90], 16, 2, 128, seed=16)
+    world.table[1:] = world.table[0]
+    cache, batch = world.device(gpu)
+    q = torch.randn(world.tokens, 4, 128, device=gpu)
+    want, want_k = paged.attention(cache, batch, q), paged.read(cache, batch)[0]
+    wide = torch.full((3, 40), 2 ** 30, dtype=torch.int32, device=gpu)
+    wide[:, 11:11 + world.table.shape[1]] = batch.page_table
+    for table in (wide[:, 11:11 + world.table.shape[1]], batch.page_table[:1].expand(3, -1)):
+        b = paged.PagedBatch(batch.query_starts, batch.context_lens, table, tokens=world.tokens, max_query=max(query, 2), max_context=100)
+        assert torch.equal(paged.attention(cache, b, q), want) and torch.equal(paged.read(cache, b)[0], want_k)

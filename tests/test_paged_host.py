@@ -4,7 +4,9 @@ are made up, and no GPU is needed."""
 import ctypes
 
 import pytest
+import torch
 
+from qwenscriber_b200 import paged
 from qwenscriber_b200 import runtime as rt
 
 A = 1 << 20  # aligned to everything
@@ -116,3 +118,34 @@ def test_sample_arguments(cuda_lib, kw, status):
 
 def test_sample_of_no_rows(cuda_lib):
     assert rt.lib().qwc_op_sample(0, A, 100, 0, 100, None, None, None, None, A, A, None, None) == 0
+
+
+def host_batch(table, max_context):
+    n = table.shape[0]
+    ints = lambda a: torch.tensor(a, dtype=torch.int32)  # noqa: E731
+    return paged.PagedBatch(ints(range(n + 1)), ints([1] * n), table, tokens=n, max_query=1, max_context=max_context)
+
+
+@pytest.mark.parametrize("view,entries", [
+    (lambda t: t, 100), (lambda t: t[:, 96:], 4), (lambda t: t[:, 3:8], 5), (lambda t: t[:1, 90:], 10), (lambda t: t[:1, :7].expand(3, 7), 7),
+    (lambda t: t[1:2, 40:41].expand(3, 1), 1),
+])
+def test_a_table_is_as_long_as_its_columns(cuda_lib, view, entries):
+    # Not as its rows are apart: an entry past a view's columns is another sequence's, or past the storage.
+    table = view(torch.zeros(3, 100, dtype=torch.int32))
+    pool = paged.PagedCache.zeros(10, 16, 2, 128, device="cpu")
+    assert paged.workspace_bytes(pool, host_batch(table, 16 * entries), 4, 0) > 0
+    with pytest.raises(rt.QwcError) as e:
+        paged.workspace_bytes(pool, host_batch(table, 16 * entries + 1), 4, 0)
+    assert e.value.name == "shape_mismatch"
+
+
+@pytest.mark.parametrize("b,status", [
+    (dict(table_stride=100, max_context=81), SHAPE), (dict(table_stride=100, max_context=80), 0), (dict(table_stride=0, max_context=80), 0),
+    (dict(table_stride=3, max_context=81), SHAPE),
+])
+def test_entries_bound_the_context(cuda_lib, b, status):
+    n = ctypes.c_uint64(0)
+    d = batch(**b)
+    d.table_entries = 5
+    assert rt.lib().qwc_op_paged_attention_workspace(ctypes.addressof(cache()), ctypes.addressof(d), 0, 4, ctypes.byref(n)) == status

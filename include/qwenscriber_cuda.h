@@ -456,7 +456,9 @@ int32_t qwc_op_silu_mul(const float* gate, const float* up, uint32_t n, float* o
  * values apart): row `page * page_size + i` is position i of that page.
  * One step of a layer is append, then attention; `read` gives rows back as
  * values; `sample` ends the step where argmax does not. Formats of queries,
- * rows and logits: f32, f16 and bf16. */
+ * rows and logits: f32, f16 and bf16. A kernel is launched on the calling
+ * thread's current device, which has to be the one that holds the memory and
+ * the stream. */
 
 /* One layer's pool. `*_scales`: [pages * page_size][kv_heads * head_dim / 64] f16, 16-byte aligned;
  * `*_codes`: [pages * page_size][kv_heads * head_dim] u8, 16-byte aligned. */

@@ -2,8 +2,8 @@
 
 `PagedCache` names one layer's pool of pages, `PagedBatch` the tokens of one step; both hold
 torch tensors (device memory, nothing is computed by torch) and the descriptors that the C ABI
-takes, so a call is one ABI call on torch's current stream. A refused argument raises `QwcError`
-with the status, as everywhere in this package.
+takes, so a call is one ABI call on torch's current stream of the device that holds them. A refused argument
+raises `QwcError` with the status, as everywhere in this package.
 
     cache = PagedCache.zeros(pages=512, page_size=64, kv_heads=8, head_dim=128)     # one for each layer
     batch = PagedBatch(query_starts, context_lens, page_table, tokens=n, max_query=q, max_context=c)
@@ -36,6 +36,14 @@ def current_stream(device: torch.device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def elsewhere(device: torch.device, call: str):
+    """A kernel is launched on the current device: the context that makes `device` the current one, or None where it
+    is already. Memory that no GPU holds is refused."""
+    if device.type != "cuda":
+        refuse("invalid_argument", call)
+    return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def format_of(t: torch.Tensor, call: str) -> int:
@@ -189,6 +197,10 @@ def append(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, k: torch.Tenso
     """QK-RMSNorm, rotation and the q8 append of [tokens, heads, head_dim] rows; returns the queries
     for attention (`q_out`, a new tensor unless given; may be `q`)."""
     call = "qwc_op_paged_append"
+    away = elsewhere(cache.device, call)
+    if away is not None:
+        with away:
+            return append(cache, batch, q, k, v, cos, sin, q_norm=q_norm, k_norm=k_norm, eps=eps, q_out=q_out)
     fmt = format_of(q, call)
     dtype, device = q.dtype, batch.device
     if k.dtype != dtype or v.dtype != dtype or cache.device != device or q.dim() != 3:
@@ -223,6 +235,10 @@ def attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, out: torch.
     """Causal attention of the batch's [tokens, heads, head_dim] queries over their sequences' pages. `workspace`: one
     made by `workspace(...)`; without it, the current stream's own (in a graph under capture, the graph's own)."""
     call = "qwc_op_paged_attention"
+    away = elsewhere(cache.device, call)
+    if away is not None:
+        with away:
+            return attention(cache, batch, q, out, workspace)
     fmt = format_of(q, call)
     if cache.device != batch.device or q.dim() != 3:
         refuse("invalid_argument", call)
@@ -252,6 +268,10 @@ def read(cache: PagedCache, batch: PagedBatch, dtype: torch.dtype = torch.float3
          v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached key and value rows of the batch's tokens as values, [tokens, kv_heads, head_dim]."""
     call = "qwc_op_paged_read"
+    away = elsewhere(cache.device, call)
+    if away is not None:
+        with away:
+            return read(cache, batch, dtype, k_out, v_out)
     tokens, kv_heads, dim, device = batch.tokens, cache.kv_heads, cache.head_dim, batch.device
     if cache.device != device:
         refuse("invalid_argument", call)

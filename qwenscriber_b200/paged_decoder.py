@@ -14,6 +14,7 @@ its own slots and fused steps is `runtime.CudaModel`.
 
 from __future__ import annotations
 
+import contextlib
 import dataclasses
 
 import numpy as np
@@ -46,6 +47,8 @@ class PagedDecoder:
     def __init__(self, model: synthetic.Model, pages: int, page_size: int, device="cuda:0"):
         c = self.config = model.config
         self.device, self.page_size = torch.device(device), page_size
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.weights = {}
         for t in model.tensors:
             if t.kind < synthetic.EMBED:
@@ -101,7 +104,8 @@ class PagedDecoder:
     # ---- operators ----
 
     def _call(self, name: str, *args) -> None:
-        check(getattr(lib(), name)(*args, paged.current_stream(self.device)), name)
+        with paged.elsewhere(self.device, name) or contextlib.nullcontext():
+            check(getattr(lib(), name)(*args, paged.current_stream(self.device)), name)
 
     def _project(self, w: Matrix, x: torch.Tensor) -> torch.Tensor:
         out = torch.empty(x.shape[0], w.rows, dtype=torch.float32, device=self.device)

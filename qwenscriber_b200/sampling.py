@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import torch
 
-from .paged import current_stream, format_of, refuse
+from .paged import current_stream, elsewhere, format_of, refuse
 from .runtime import check, lib
 
 
@@ -15,6 +15,10 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: torch.T
     view of wider ones), from one number in [0, 1) for each row. Settings are one value for each row
     on the device (top_k int32, the others f32); None leaves a cut out, and the temperature 1."""
     call = "qwc_op_sample"
+    away = elsewhere(logits.device, call)
+    if away is not None:
+        with away:
+            return sample(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     fmt = format_of(logits, call)
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         refuse("invalid_argument", call)

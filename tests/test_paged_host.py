@@ -1,12 +1,13 @@
 """The paged operators' and the sampler's checks, which come before any CUDA call: the addresses here
 are made up, and no GPU is needed."""
 
+import contextlib
 import ctypes
 
 import pytest
 import torch
 
-from qwenscriber_b200 import paged
+from qwenscriber_b200 import paged, paged_decoder, sampling
 from qwenscriber_b200 import runtime as rt
 
 A = 1 << 20  # aligned to everything
@@ -149,3 +150,104 @@ def test_entries_bound_the_context(cuda_lib, b, status):
     d = batch(**b)
     d.table_entries = 5
     assert rt.lib().qwc_op_paged_attention_workspace(ctypes.addressof(cache()), ctypes.addressof(d), 0, 4, ctypes.byref(n)) == status
+
+
+class Stub:
+    """A tensor of a device that is not there."""
+
+    def __init__(self, *shape, dtype=torch.float32, device="cuda:1"):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype, torch.device(device)
+
+    dim = lambda self: len(self.shape)  # noqa: E731
+    numel = lambda self: self.shape.numel()  # noqa: E731
+    data_ptr = lambda self: A  # noqa: E731
+    is_contiguous = lambda self: True  # noqa: E731
+
+    def stride(self, i=None):
+        strides = [self.shape[j + 1:].numel() for j in range(self.dim())]
+        return strides if i is None else strides[i]
+
+
+def stub_calls(device):
+    """Each call of the package on tensors of `device`."""
+    t = lambda *shape, dtype=torch.float32: Stub(*shape, dtype=dtype, device=device)  # noqa: E731
+    planes = [t(160, 4, dtype=torch.float16), t(160, 256, dtype=torch.uint8)] * 2
+    pool = paged.PagedCache(*planes, page_size=16, kv_heads=2, head_dim=128)
+    i32 = torch.int32
+    b = paged.PagedBatch(t(3, dtype=i32), t(2, dtype=i32), t(2, 5, dtype=i32), tokens=2, max_query=1, max_context=80)
+    q, kv, table = t(2, 4, 128), t(2, 2, 128), t(100, 64)
+    return {
+        "append": lambda: paged.append(pool, b, q, kv, kv, table, table, q_out=q),
+        "attention": lambda: paged.attention(pool, b, q, q, t(1 << 30, dtype=torch.uint8)),
+        "read": lambda: paged.read(pool, b, torch.float32, kv, kv),
+        "sample": lambda: sampling.sample(t(2, 100), t(2)),
+    }
+
+
+CALLS = ["append", "attention", "read", "sample"]
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("current", [0, 1, 2])
+def test_launches_go_to_the_tensors_device(monkeypatch, name, current):
+    at, launched, entered = [current], [], []
+
+    class Current:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            entered.append(self.index)
+            self.before, at[0] = at[0], self.index
+
+        def __exit__(self, *a):
+            at[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: launched.append((name, at[0], a[-1])) or 0
+
+    calls = stub_calls("cuda:1")
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    monkeypatch.setattr(torch, "empty", lambda *shape, dtype, device: Stub(*shape, dtype=dtype, device=device))
+    for module in (paged, sampling):
+        monkeypatch.setattr(module, "lib", lambda: Lib())
+        monkeypatch.setattr(module, "current_stream", lambda device: 1000 + device.index)
+    calls[name]()
+    assert [c[1:] for c in launched] == [(1, 1001)]
+    assert entered == ([] if current == 1 else [1]) and at[0] == current
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_host_memory_is_refused(monkeypatch, name):
+    def launched():
+        raise AssertionError("a kernel was given host memory")
+
+    for module in (paged, sampling):
+        monkeypatch.setattr(module, "lib", launched)
+    with pytest.raises(rt.QwcError) as e:
+        stub_calls("cpu")[name]()
+    assert e.value.name == "invalid_argument"
+
+
+def test_an_operator_of_the_decoder_goes_to_its_device(monkeypatch):
+    at, launched = [0], []
+
+    @contextlib.contextmanager
+    def current(device):
+        before, at[0] = at[0], device.index
+        yield
+        at[0] = before
+
+    class Lib:
+        qwc_op_silu_mul = staticmethod(lambda *a: launched.append((at[0], a[-1])) or 0)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(torch.cuda, "device", current)
+    monkeypatch.setattr(paged_decoder, "lib", Lib)
+    monkeypatch.setattr(paged, "current_stream", lambda device: 1000 + device.index)
+    d = object.__new__(paged_decoder.PagedDecoder)
+    d.device = torch.device("cuda:1")
+    d._call("qwc_op_silu_mul", A, A, 4, A)
+    assert launched == [(1, 1001)] and at[0] == 0

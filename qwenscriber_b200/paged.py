@@ -162,19 +162,21 @@ def workspace(cache: PagedCache, batch: PagedBatch, heads: int, dtype: torch.dty
     return _new_workspace(workspace_bytes(cache, batch, heads, fmt), cache.device)
 
 
-def _workspace(cache: PagedCache, need: int, stream: int) -> tuple[int, int]:
-    """(address, bytes) of the stream's buffer, at least what this call needs."""
+def _workspace(cache: PagedCache, need: int, stream: int) -> tuple[int, int, torch.Tensor]:
+    """(address, bytes, tensor) of the stream's buffer, at least what this call needs. The caller holds the tensor until
+    its launch is enqueued: another thread on the stream may put a larger one in its place at any time. (After the launch
+    the order of the stream keeps it.)"""
     if torch.cuda.is_current_stream_capturing():
         # A graph may be replayed on any stream and outlive the stream's buffer: it gets one of its own, from the
         # graph's pool, and zeroes its head in each replay.
         buffer = _new_workspace(need, cache.device)
-        return buffer.data_ptr(), need
+        return buffer.data_ptr(), need, buffer
     at = (cache._index, stream)
     held = _workspaces.get(at)
     if held is None or held[1] < need:
         buffer = _new_workspace(need, cache.device)
         held = _workspaces[at] = (buffer.data_ptr(), need, buffer)
-    return held[0], held[1]
+    return held
 
 
 def check_waits(workspace: torch.Tensor | None = None, device: torch.device | None = None) -> None:
@@ -252,7 +254,7 @@ def attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, out: torch.
         out_stride = _rows(out, batch, heads, dim, call)
     stream = current_stream(cache.device)
     if workspace is None:
-        work, size = _workspace(cache, workspace_bytes(cache, batch, heads, fmt), stream)
+        work, size, held = _workspace(cache, workspace_bytes(cache, batch, heads, fmt), stream)  # noqa: F841 (held until the launch)
     elif workspace.dtype != torch.uint8 or workspace.device != cache.device or not workspace.is_contiguous():
         refuse("invalid_argument", call)
     else:

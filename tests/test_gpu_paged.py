@@ -12,6 +12,8 @@ mistake shows. Tolerances (derived here, before any run):
   |v|. 16-bit rows: the query is exact in one part, a weight rounds by 2^-11, and the output once to its type.
 """
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -535,3 +537,29 @@ def test_tables_that_are_views(gpu, cuda_lib, query):
     for table in (wide[:, 11:11 + world.table.shape[1]], batch.page_table[:1].expand(3, -1)):
         b = paged.PagedBatch(batch.query_starts, batch.context_lens, table, tokens=world.tokens, max_query=max(query, 2), max_context=100)
         assert torch.equal(paged.attention(cache, b, q), want) and torch.equal(paged.read(cache, b)[0], want_k)
+
+
+def test_threads_on_one_stream_with_growing_workspaces(gpu, cuda_lib):
+    worlds = [World([query] * n, [300] * n, 16, 2, 128, seed=20 + n) for query, n in ((1, 1), (40, 1), (1, 40), (40, 6))]
+    made = [(*w.device(gpu), torch.randn(w.tokens, 4, 128, device=gpu)) for w in worlds]
+    want = [paged.attention(*m) for m in made]
+    torch.cuda.synchronize()
+    key = (gpu.index, paged.current_stream(gpu))
+    wrong, start = [], threading.Barrier(4)
+
+    def work(i):
+        start.wait()
+        for n in range(60):
+            if i == 0:
+                paged._workspaces.pop(key, None)  # the next calls grow it again, from nothing
+            j = (n + i) % len(made)
+            if not torch.equal(paged.attention(*made[j]), want[j]):
+                wrong.append((i, n))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    paged.check_waits()

@@ -3,6 +3,9 @@ are made up, and no GPU is needed."""
 
 import contextlib
 import ctypes
+import gc
+import threading
+import weakref
 
 import pytest
 import torch
@@ -251,3 +254,43 @@ def test_an_operator_of_the_decoder_goes_to_its_device(monkeypatch):
     d.device = torch.device("cuda:1")
     d._call("qwc_op_silu_mul", A, A, 4, A)
     assert launched == [(1, 1001)] and at[0] == 0
+
+
+def test_a_workspace_lives_until_the_launch(cuda_lib, monkeypatch):
+    # Another thread on the stream puts a larger buffer in the place of the one that a call has looked up.
+    born, alive = [], []
+
+    def new(need, device):
+        buffer = torch.zeros(need, dtype=torch.uint8)
+        born.append((buffer.data_ptr(), weakref.ref(buffer)))
+        return buffer
+
+    class Lib:
+        @staticmethod
+        def qwc_op_paged_attention_workspace(cache, batch, fmt, heads, n):
+            return rt.lib().qwc_op_paged_attention_workspace(cache, batch, fmt, heads, n)
+
+        @staticmethod
+        def qwc_op_paged_attention(*a):
+            thread = threading.Thread(target=paged._workspace, args=(pool, a[9] + 4096, 1001))
+            thread.start()
+            thread.join()
+            gc.collect()
+            alive.extend(ref() is not None for address, ref in born if address == a[8])
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(paged, "current_stream", lambda device: 1000 + device.index)
+    monkeypatch.setattr(paged, "_new_workspace", new)
+    monkeypatch.setattr(paged, "_workspaces", {})
+    monkeypatch.setattr(paged, "lib", lambda: Lib)
+    t = lambda *shape, dtype=torch.float32: Stub(*shape, dtype=dtype)  # noqa: E731
+    pool = paged.PagedCache(*[t(160, 4, dtype=torch.float16), t(160, 256, dtype=torch.uint8)] * 2, page_size=16, kv_heads=2, head_dim=128)
+    b = paged.PagedBatch(t(3, dtype=torch.int32), t(2, dtype=torch.int32), t(2, 5, dtype=torch.int32), tokens=2, max_query=1, max_context=80)
+    q = t(2, 4, 128)
+    for _ in range(3):
+        paged.attention(pool, b, q, q)
+    assert len(alive) == 3 and all(alive)
+    gc.collect()
+    assert sum(ref() is not None for _, ref in born) == 1  # the stream keeps the largest alone

@@ -183,7 +183,8 @@ def check_waits(workspace: torch.Tensor | None = None, device: torch.device | No
     """Raises `QwcError` if a bounded wait inside an attention kernel ran out (its rows are undefined then), and makes
     the workspace ready again. Without a workspace, of the current stream's own. Waits for the stream."""
     if workspace is None:
-        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        if device is None or device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         held = _workspaces.get((device.index, current_stream(device)))
         if held is None:
             return

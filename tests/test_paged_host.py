@@ -294,3 +294,17 @@ def test_a_workspace_lives_until_the_launch(cuda_lib, monkeypatch):
     assert len(alive) == 3 and all(alive)
     gc.collect()
     assert sum(ref() is not None for _, ref in born) == 1  # the stream keeps the largest alone
+
+
+@pytest.mark.parametrize("device", [None, torch.device("cuda"), torch.device("cuda:1")])
+def test_a_wait_that_ran_out_is_found_by_any_name_of_the_device(monkeypatch, device):
+    buffer = torch.zeros(rt.PAGED_WORKSPACE_HEAD + 64, dtype=torch.uint8)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(paged, "current_stream", lambda d: 1000 + (1 if d.index is None else d.index))
+    monkeypatch.setattr(paged, "_workspaces", {(1, 1001): (buffer.data_ptr(), buffer.numel(), buffer)})
+    paged.check_waits(device=device)
+    buffer[0], buffer[400] = 3, 7
+    with pytest.raises(rt.QwcError) as e:
+        paged.check_waits(device=device)
+    assert e.value.name == "invalid_state" and not buffer.any()
+    paged.check_waits(device=device)

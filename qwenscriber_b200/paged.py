@@ -175,6 +175,8 @@ def _workspace(cache: PagedCache, need: int, stream: int) -> tuple[int, int, tor
     held = _workspaces.get(at)
     if held is None or held[1] < need:
         buffer = _new_workspace(need, cache.device)
+        if held is not None:
+            buffer[:4].copy_(held[2][:4])  # a wait that ran out is still to be told of
         held = _workspaces[at] = (buffer.data_ptr(), need, buffer)
     return held
 

@@ -308,3 +308,19 @@ def test_a_wait_that_ran_out_is_found_by_any_name_of_the_device(monkeypatch, dev
         paged.check_waits(device=device)
     assert e.value.name == "invalid_state" and not buffer.any()
     paged.check_waits(device=device)
+
+
+def test_a_larger_workspace_still_tells_of_a_wait_that_ran_out(monkeypatch):
+    pool = paged.PagedCache(*[Stub(160, 4, dtype=torch.float16), Stub(160, 256, dtype=torch.uint8)] * 2, page_size=16, kv_heads=2, head_dim=128)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(paged, "current_stream", lambda device: 1000 + device.index)
+    monkeypatch.setattr(paged, "_new_workspace", lambda need, device: torch.zeros(need, dtype=torch.uint8))
+    monkeypatch.setattr(paged, "_workspaces", {})
+    held = paged._workspace(pool, 40000, 1001)[2]
+    held[1] = 2  # the kernel's error word
+    assert paged._workspace(pool, 50000, 1001)[1] == 50000
+    with pytest.raises(rt.QwcError) as e:
+        paged.check_waits(device=torch.device("cuda:1"))
+    assert e.value.name == "invalid_state"
+    paged.check_waits(device=torch.device("cuda:1"))

@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from . import paged, quant, sampling, synthetic
-from .runtime import QwcError, STATUS_CODE, check, lib, rope_tables
+from .runtime import check, lib, rope_tables
 
 COLUMNS = 64  # rows of activations that one qwc_op_gemm_streams call takes
 
@@ -76,7 +76,10 @@ class PagedDecoder:
             if n == 0:
                 self.holders[i] = 1
                 return i
-        raise QwcError(STATUS_CODE["limit_exceeded"], "PagedDecoder: the pool has no free page")
+        self._no_page()
+
+    def _no_page(self):
+        paged.refuse("limit_exceeded", "PagedDecoder: the pool has no free page")
 
     def start(self) -> Sequence:
         return Sequence([])
@@ -89,6 +92,8 @@ class PagedDecoder:
     def fork(self, seq: Sequence) -> Sequence:
         """A sequence with the same positions: full pages shared, the one in use copied."""
         full = seq.length // self.page_size
+        if len(seq.pages) - full > self.holders.count(0):
+            self._no_page()
         for p in seq.pages[:full]:
             self.holders[p] += 1
         out = Sequence(seq.pages[:full], seq.length)
@@ -132,15 +137,44 @@ class PagedDecoder:
 
     def step(self, work: list[tuple[Sequence, np.ndarray, np.ndarray | None]]) -> torch.Tensor:
         """Runs each sequence's new tokens ids (where token_audio_pad stands, the next row of its audio rows)
-        and returns the logits after the last of each, [sequences, vocab]."""
+        and returns the logits after the last of each, [sequences, vocab]. Waits for the device. A step that is
+        refused, or fails, leaves every sequence as it was."""
+        if not work:
+            return torch.empty(0, self.config.vocab_size, dtype=torch.float32, device=self.device)
+        self._check(work)
+        before = [(seq, seq.length, len(seq.pages)) for seq, _, _ in work]
+        try:
+            for seq, ids, _ in work:
+                seq.length += len(ids)
+                while len(seq.pages) * self.page_size < seq.length:
+                    seq.pages.append(self._take())
+            logits = self._forward(work)
+            paged.check_waits(device=self.device)
+        except BaseException:
+            for seq, length, count in before:
+                for p in seq.pages[count:]:
+                    self.holders[p] -= 1
+                del seq.pages[count:]
+                seq.length = length
+            raise
+        return logits
+
+    def _check(self, work) -> None:
+        """Refuses a step before anything of it is done."""
+        c, call = self.config, "PagedDecoder.step"
+        pages = 0
+        for seq, ids, _ in work:
+            ids = np.asarray(ids)
+            if ids.size == 0 or seq.length + ids.size > c.max_positions:
+                paged.refuse("limit_exceeded", call)
+            pages += -(-(seq.length + ids.size) // self.page_size) - len(seq.pages)
+        if pages > self.holders.count(0):
+            self._no_page()
+
+    def _forward(self, work) -> torch.Tensor:
+        """The logits of a step whose sequences have their lengths and pages."""
         c = self.config
         lengths = [len(ids) for _, ids, _ in work]
-        for (seq, ids, _), n in zip(work, lengths):
-            if n == 0 or seq.length + n > c.max_positions:
-                raise QwcError(STATUS_CODE["limit_exceeded"], "PagedDecoder.step")
-            seq.length += n
-            while len(seq.pages) * self.page_size < seq.length:
-                seq.pages.append(self._take())
         table = np.zeros((len(work), max(len(s.pages) for s, _, _ in work)), np.int32)
         for row, (seq, _, _) in zip(table, work):
             row[:len(seq.pages)] = seq.pages
@@ -178,25 +212,27 @@ class PagedDecoder:
         once; `settings` are sampling.sample's, one value for all."""
         c = self.config
         stop = {c.token_eos_primary, c.token_eos_secondary, c.token_endoftext}
-        first = self.start()
-        logits = self.step([(first, prompt.tokens, prompt.audio)]).expand(count, -1).contiguous()
-        seqs = [first] + [self.fork(first) for _ in range(count - 1)]
+        seqs = [self.start()]
         out, live = [([], 0.0) for _ in range(count)], list(range(count))
-        for _ in range(max_tokens):
-            u = torch.rand(len(live), generator=generator).to(self.device)
-            kinds = {k: torch.full((len(live),), v, dtype=torch.int32 if k == "top_k" else torch.float32, device=self.device)
-                     for k, v in settings.items()}
-            tokens, logprobs = (t.tolist() for t in sampling.sample(logits, u, **kinds))
-            paged.check_waits(device=self.device)
-            for i, tok, lp in zip(live, tokens, logprobs):
-                out[i] = (out[i][0] + ([tok] if tok not in stop else []), out[i][1] + lp)
-            going = [(i, tok) for i, tok in zip(live, tokens) if tok not in stop]
-            live = [i for i, _ in going]
-            if not live:
-                break
-            logits = self.step([(seqs[i], np.asarray([tok]), None) for i, tok in going])
-        for s in seqs:
-            self.release(s)
+        try:
+            logits = self.step([(seqs[0], prompt.tokens, prompt.audio)]).expand(count, -1).contiguous()
+            for _ in range(count - 1):
+                seqs.append(self.fork(seqs[0]))
+            for _ in range(max_tokens):
+                u = torch.rand(len(live), generator=generator).to(self.device)
+                kinds = {k: torch.full((len(live),), v, dtype=torch.int32 if k == "top_k" else torch.float32, device=self.device)
+                         for k, v in settings.items()}
+                tokens, logprobs = (t.tolist() for t in sampling.sample(logits, u, **kinds))
+                for i, tok, lp in zip(live, tokens, logprobs):
+                    out[i] = (out[i][0] + ([tok] if tok not in stop else []), out[i][1] + lp)
+                going = [(i, tok) for i, tok in zip(live, tokens) if tok not in stop]
+                live = [i for i, _ in going]
+                if not live:
+                    break
+                logits = self.step([(seqs[i], np.asarray([tok]), None) for i, tok in going])
+        finally:
+            for s in seqs:
+                self.release(s)
         return out
 
 

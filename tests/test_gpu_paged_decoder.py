@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from qwenscriber_b200 import quant, synthetic
+from qwenscriber_b200 import paged, quant, synthetic
 from qwenscriber_b200 import runtime as rt
 from qwenscriber_b200.paged_decoder import PagedDecoder
 
@@ -77,3 +77,31 @@ def test_transcripts(gpu, cuda_lib):
     assert sampled == run(1, temperature=1.5, top_k=200)
     assert len({tuple(t) for t, _ in sampled}) > 1 and all(s < 0 for _, s in sampled)
     assert not any(d.holders)
+
+
+def test_a_step_after_a_refused_one_is_as_if_there_had_been_none(gpu, cuda_lib):
+    c = small_config(quant.Q8)
+    model = synthetic.make_model(c, quant.Q8, seed=6)
+    prompt = synthetic.make_prompt(c, 20, 6, seed=6)
+    d = PagedDecoder(model, pages=5, page_size=16, device="cuda")  # the current device
+    want = d.start()
+    d.step([(want, prompt.tokens, prompt.audio)])
+    want_logits = d.step([(want, [7, 8], None)])
+    d.release(want)
+    a, filler = d.start(), d.start()
+    d.step([(a, prompt.tokens, prompt.audio), (filler, np.arange(40), None)])
+    for work in ([(a, [7, 8], None), (filler, np.arange(30), None)], [(a, np.arange(40), None)]):
+        with pytest.raises(rt.QwcError) as e:
+            d.step(work)
+        assert e.value.name == "limit_exceeded" and a.length == 26 and filler.length == 40 and d.holders.count(0) == 0
+    d.release(filler)
+    # 28 positions in the same pages: the refused tokens have left nothing behind.
+    assert torch.equal(d.step([(a, [7, 8], None)]), want_logits)
+    # A wait that ran out in a step's attention is told of by the step.
+    stream = paged.current_stream(d.device)
+    paged._workspaces[d.device.index, stream][2][0] = 1
+    with pytest.raises(rt.QwcError) as e:
+        d.step([(a, [9], None)])
+    assert e.value.name == "invalid_state" and a.length == 28
+    d.step([(a, [9], None)])
+    assert a.length == 29

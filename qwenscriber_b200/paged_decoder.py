@@ -162,11 +162,19 @@ class PagedDecoder:
     def _check(self, work) -> None:
         """Refuses a step before anything of it is done."""
         c, call = self.config, "PagedDecoder.step"
+        if len({id(seq) for seq, _, _ in work}) < len(work):
+            paged.refuse("invalid_argument", call)
         pages = 0
-        for seq, ids, _ in work:
+        for seq, ids, audio in work:
             ids = np.asarray(ids)
+            if ids.ndim != 1:
+                paged.refuse("shape_mismatch", call)
             if ids.size == 0 or seq.length + ids.size > c.max_positions:
                 paged.refuse("limit_exceeded", call)
+            if ids.dtype.kind not in "iu" or ids.min() < 0 or ids.max() >= c.vocab_size:
+                paged.refuse("invalid_argument", call)  # (an embedding row that is not there is an assertion on the device)
+            if audio is not None and np.shape(audio) != (np.count_nonzero(ids == c.token_audio_pad), c.text_hidden_size):
+                paged.refuse("shape_mismatch", call)
             pages += -(-(seq.length + ids.size) // self.page_size) - len(seq.pages)
         if pages > self.holders.count(0):
             self._no_page()

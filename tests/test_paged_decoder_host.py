@@ -51,6 +51,13 @@ def test_a_refused_step_changes_nothing(decoder):
         ("limit_exceeded", [(a, tokens(30), None), (b, tokens(30), None)]),              # for both together
         ("limit_exceeded", [(a, tokens(1), None), (b, tokens(0), None)]),                # nothing to run
         ("limit_exceeded", [(a, tokens(1), None), (b, tokens(c.max_positions), None)]),  # too long
+        ("invalid_argument", [(a, tokens(1), None), (a, tokens(1), None)]),              # twice the same sequence
+        ("invalid_argument", [(a, tokens(1), None), (b, [c.vocab_size], None)]),         # rows that the embedding lacks
+        ("invalid_argument", [(a, tokens(1), None), (b, [3, -1], None)]),
+        ("invalid_argument", [(a, tokens(1), None), (b, [0.5], None)]),
+        ("shape_mismatch", [(a, tokens(1), None), (b, np.zeros((1, 2), np.int64), None)]),
+        ("shape_mismatch", [(a, [pad, 1], rows(2)), (b, [pad, pad], rows(1))]),          # another sequence's rows would be taken
+        ("shape_mismatch", [(a, tokens(1), None), (b, [pad], np.zeros((1, 3), np.float32))]),
     ):
         refused(name, d.step, work)
         assert state(d, a, b) == before, work

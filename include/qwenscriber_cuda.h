@@ -511,7 +511,8 @@ int32_t qwc_op_paged_append(const qwc_paged_cache* cache, const qwc_paged_batch*
  * (kernels.zig:697-767 for one token): query head h reads kv head h / (heads / kv_heads), scores are
  * scaled by 1 / sqrt(head_dim). Products enter the tensor cores as exact codes against f16 parts of
  * the queries and weights (two parts, 22 bits, for f32 rows, one for 16-bit rows); for bf16 rows of a call with
- * more than 16 rows to a kv head, code times scale rounds to f16 first. Sums and the softmax are f32. A token that sees no position gives a row of zeros. q and out as in append.
+ * more than 16 rows to a kv head, code times scale rounds to f16 first. Sums and the softmax are f32. A token that sees no position gives a row of zeros.
+ * A head's row that sees a position whose value scale is no number is NaN; rows that do not see it are not touched by it. q and out as in append.
  * `workspace` (16-byte aligned device memory of at least qwc_op_paged_attention_workspace bytes) holds
  * the partial results of contexts cut into pieces. Its first QWC_PAGED_WORKSPACE_HEAD bytes must be zero before
  * its first use; it is left ready for the next call, and serves one stream at a time. Its first 32-bit word stays zero unless a wait inside the

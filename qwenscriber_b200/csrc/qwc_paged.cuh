@@ -189,6 +189,11 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
 }
 __device__ __forceinline__ float2 f16x2_f32(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
+// A value scale that is no number (infinity, NaN) must not reach the rows that do not see its position: a weight of 0 times it
+// is NaN. It enters the products as some number, and the rows that do see it are made NaN by themselves. With
+// kOddStep added, a scale's exponent field is one more, that of one that is no number is 0, and its sign bit is set.
+constexpr uint32_t kOddStep = 0x04000400u, kOddBits = 0x80008000u;
+
 // The power of two that brings a row of queries near 1: their f16 parts then
 // hold 11 (or 22) bits of every value that matters beside the largest.
 __device__ __forceinline__ int row_exponent(float amax) {

@@ -87,6 +87,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
   constexpr int PARTS = SPLIT ? 2 : 1;    // columns of a query row
   constexpr int RPL = SPLIT ? 1 : 2;      // rows of a column tile whose scores a lane holds
   constexpr uint32_t kValueSwizzle = DIM == 128 ? 6u : 2u;  // chunks of the rows that a half warp reads at once: apart
+  constexpr bool kComparesFields = SPLIT && NCT == 2;
+  constexpr int kUp = kComparesFields ? 28 : 29;  // the weights' power of two, and 1 where the fields are one more
   constexpr int STATE = DIM + 4;          // a row's state in shared memory or a partial: output, maximum, sum
   extern __shared__ __align__(128) uint8_t few_smem[];
   FewTile<DIM>* ring = reinterpret_cast<FewTile<DIM>*>(few_smem);                                  // [warp][stage]
@@ -285,15 +287,25 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
         bool grew = false;
         float down = 1.0f;
         {
-          const uint32_t f = scale_next;
-          const uint32_t e = lane < 16 ? 0u : max((f >> 10) & 31u, (f >> 26) & 31u);
-          const uint32_t top = min(__reduce_max_sync(0xffffffffu, e), 30u);
+          const uint32_t f = scale_next, next = f + kOddStep;
+          const uint32_t odd = __shfl_xor_sync(0xffffffffu, next & kOddBits, 16);  // keys: of the position's values
+          // The fields without those of 31, which are no numbers: by comparing them for two column tiles of f32 rows, whose
+          // registers come out better that way (64 x 4 over 4096 146 us for 155), else by kOddStep (74.4 us for 76.2 of
+          // 64 x 1, f16).
+          uint32_t e;
+          if constexpr (kComparesFields) {
+            const uint32_t e0 = (f >> 10) & 31u, e1 = (f >> 26) & 31u;
+            e = lane < 16 ? 0u : max(e0 == 31u ? 0u : e0, e1 == 31u ? 0u : e1);
+          } else {
+            e = lane < 16 ? 0u : max((next >> 10) & 31u, (next >> 26) & 31u);
+          }
+          const uint32_t top = __reduce_max_sync(0xffffffffu, e);
           if (top > vexp) {
             down = pow2i(static_cast<int>(vexp) - static_cast<int>(top));
             vexp = top;
             grew = true;
           }
-          const float up = lane < 16 ? 1.0f : pow2i(28 - static_cast<int>(vexp));
+          const float up = lane >= 16 ? pow2i(kUp - static_cast<int>(vexp)) : odd ? __int_as_float(0x7FC00000) : 1.0f;  // (NaN: its scores)
           const float2 both = f16x2_f32(f);
           my_scales[lane] = make_float2(both.x * up, both.y * up);  // (the last block's reads lie before the loop's end)
         }
@@ -400,7 +412,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
           const float2 vs = my_scales[16 + r + 8 * hp];
 #pragma unroll
           for (int g = 0; g < G; ++g) {
-            const float v = g ? vs.y : vs.x;
+            const float v = fminf(g ? vs.y : vs.x, 32768.0f);  // (more is no number)
 #pragma unroll
             for (int ct = 0; ct < NCT; ++ct) {
               if constexpr (SPLIT) {
@@ -444,7 +456,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
       }
 
       // ---- this warp's state: lane (r, c) has dims 64 g + 8 r + 0..7 of its rows ----
-      const float back = pow2i(static_cast<int>(vexp) - 28);
+      const float back = pow2i(static_cast<int>(vexp) - kUp);
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) {
 #pragma unroll

@@ -111,6 +111,7 @@ struct __align__(1024) TileSmem {
   float ks[4][C::G][kStep];  // exact: the key scales
   float vs[4][C::G][kStep];  // and the value scales, times 2^(UP - vexp)
   uint64_t valid[4];         // one bit for each position that is cached
+  uint64_t odd[4];           // and for each whose values are no numbers
   uint32_t kexp[4], vexp[4];
   // Scores and weights by the step's parity: with scores a step ahead, a barrier of one phase could pass two
   // phases before a late warp looks.
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           tc_fence_after();
           // (m == -inf: this row has seen nothing, and its columns are sums of zeros.)
           const float old = any_flushed && flushed_m != -INFINITY ? ex2(flushed_m - m) : 0.0f;
-          const float unit = pow2i(static_cast<int>(vexp) - C::UP);
+          const float unit = pow2i(static_cast<int>(vexp) - (C::UP + 1));
 #pragma unroll 1
           for (int i = 0; i < DIM; i += 32) {
             float4 f[8];
@@ -619,6 +620,10 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
             if constexpr (SPLIT) tmem_st16(scol + 32 * (G + g) + i / 2, lo);
           }
         }
+        if (const uint64_t odd = sm->odd[b]) {  // (looked at here, where few registers are in use: 6 us of 190 beside the mask)
+          const uint64_t sees = limit < pos0 ? 0ull : limit - pos0 > 62 ? ~0ull : (2ull << (limit - pos0)) - 1;
+          if (odd & sees) l = __int_as_float(0x7FC00000);  // and so is all that it divides
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -630,7 +635,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
       ok = __all_sync(0xffffffffu, wait(&sm->o_full[t], seg, 202));
       if (!ok) break;
       tc_fence_after();
-      const float back = pow2i(static_cast<int>(vexp) - C::UP);
+      const float back = pow2i(static_cast<int>(vexp) - (C::UP + 1));
       const bool whole = j0 == 0 && j1 == walk.steps;
       // Finished rows go through shared memory (the tile's queries are done with) and leave a row at a time.
       constexpr int W = Vec16<T>::kCount;
@@ -838,12 +843,19 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         if (!ok) break;
         // Every warp finds the largest exponent for itself.
         int up = 0;
+        uint32_t odd[2] = {0, 0};
         if (VALUES || SCALED) {
+          // (Of the values, one more: the fields that kOddStep gives.)
           uint32_t e = 0;
 #pragma unroll
-          for (int n = 0; n < 2; ++n) e = max(e, max((scale_raw[n] >> 10) & 31u, (scale_raw[n] >> 26) & 31u));
-          top = max(top, min(__reduce_max_sync(0xffffffffu, e), 30u));
-          up = (VALUES ? C::UP : 14) - static_cast<int>(top);
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t f = VALUES ? scale_raw[n] + kOddStep : scale_raw[n];
+            if (VALUES) odd[n] = __ballot_sync(0xffffffffu, f & kOddBits);
+            e = max(e, max((f >> 10) & 31u, (f >> 26) & 31u));
+          }
+          e = __reduce_max_sync(0xffffffffu, e);
+          top = max(top, VALUES ? e : min(e, 30u));
+          up = (VALUES ? C::UP + 1 : 14) - static_cast<int>(top);
         }
         const float up2 = pow2i(up);
         // Chunk ch is dims 16 ch .. + 15: two 16-byte chunks of f16 in group ch / 4's tile.
@@ -861,7 +873,8 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
           }
           if constexpr (SCALED) {
             const uint32_t both = __shfl_sync(0xffffffffu, scale_raw[i * ROWS_PASS / 32], r % 32);
-            const float f = f16_bits_to_f32(ch >= 4 ? both >> 16 : both & 0xFFFFu) * up2;
+            float f = f16_bits_to_f32(ch >= 4 ? both >> 16 : both & 0xFFFFu) * up2;
+            if (VALUES) f = fminf(f, 1.0f);  // (more is no number)
             const uint32_t f2 = f16x2(f, f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(f2));
@@ -878,12 +891,14 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
             if (pos / (kStep / CW) != cw) continue;
             const float2 f = f16x2_f32(scale_raw[e]);
             float* dst = VALUES ? &sm->vs[b][0][pos] : &sm->ks[b][0][pos];
-            dst[0] = f.x * up2;
-            if constexpr (G == 2) dst[kStep] = f.y * up2;
+            // (Values' are below 128; more is no number.)
+            dst[0] = VALUES ? fminf(f.x * up2, 128.0f) : f.x * up2;
+            if constexpr (G == 2) dst[kStep] = VALUES ? fminf(f.y * up2, 128.0f) : f.y * up2;
           }
         }
         if (cw == 0 && lane == 0) {
           if constexpr (VALUES) {
+            sm->odd[b] = odd[0] | uint64_t(odd[1]) << 32;
             sm->vexp[b] = top;
           } else {
             sm->valid[b] = valid_bits[0] | uint64_t(valid_bits[1]) << 32;

@@ -563,3 +563,30 @@ def test_threads_on_one_stream_with_growing_workspaces(gpu, cuda_lib):
         t.join()
     assert not wrong
     paged.check_waits()
+
+
+def close_where_finite(got, ref, tol):
+    got = got.double().cpu().numpy()
+    numbers = np.isfinite(ref)
+    assert np.array_equal(np.isfinite(got), numbers), (np.argwhere(np.isfinite(got) != numbers)[:5], numbers.mean())
+    assert np.all(np.abs(got - ref)[numbers] <= tol[numbers]), float(np.abs(got - ref)[numbers].max())
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("query", [1, 2, 4, 8, 40, 300])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_attention_of_values_that_are_no_numbers(gpu, cuda_lib, kind, query, bad):
+    # Value scales of two positions: one among the new tokens, which the earlier of them do not see, and one in the middle of
+    # another sequence's context. The heads' rows that see one are no numbers, and nothing else is.
+    world = World([query, query], [query + 70, query + 70], 16, 2, 128, seed=17 + query)
+    vmax = np.abs(world.values("v", np.flatnonzero(world.held))).max()
+    for s, p, group in ((0, 70 + query // 2, 1), (1, 33, 2)):
+        world.scales["v"][world.rows(s, np.array([p])), group] = bad
+    cache, batch = world.device(gpu)
+    q = torch.randn(world.tokens, 4, 128, generator=torch.Generator().manual_seed(query)).to(TYPES[kind]).to(gpu)
+    with np.errstate(invalid="ignore"):
+        ref = world.attention(q.double().cpu().numpy())
+    assert not np.isfinite(ref[:, :2, 64:][query // 2:query]).any() and np.isfinite(ref[:query // 2]).all() and np.isfinite(ref[:query, 2:]).all()
+    ref[~np.isfinite(ref).all(-1)] = np.nan
+    tol = np.full(ref.shape, 4e-5 * vmax) if kind == "f32" else (4e-5 + 2.0 ** -10) * vmax + UNIT[kind] * np.abs(ref)
+    close_where_finite(paged.attention(cache, batch, q), ref, tol)

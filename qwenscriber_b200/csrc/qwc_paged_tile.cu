@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         const uint32_t scol = taddr + (SCALED ? (it & 1u) * kStep : 0u);
         uint64_t seen = sm->valid[b];
         const uint32_t top = sm->vexp[b];
-        const float step_factor = SCALED ? factor * pow2i(static_cast<int>(sm->kexp[b]) - 14) : factor;
+        const float step_factor = SCALED ? factor * pow2i(static_cast<int>(sm->kexp[b]) - 15) : factor;
         uint64_t x[kStep / 2];
 #pragma unroll
         for (int i = 0; i < static_cast<int>(kStep); i += 32 / C::SCORES) {
@@ -845,17 +845,16 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         int up = 0;
         uint32_t odd[2] = {0, 0};
         if (VALUES || SCALED) {
-          // (Of the values, one more: the fields that kOddStep gives.)
+          // (One more: the fields that kOddStep gives.)
           uint32_t e = 0;
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const uint32_t f = VALUES ? scale_raw[n] + kOddStep : scale_raw[n];
+            const uint32_t f = scale_raw[n] + kOddStep;
             if (VALUES) odd[n] = __ballot_sync(0xffffffffu, f & kOddBits);
             e = max(e, max((f >> 10) & 31u, (f >> 26) & 31u));
           }
-          e = __reduce_max_sync(0xffffffffu, e);
-          top = max(top, VALUES ? e : min(e, 30u));
-          up = (VALUES ? C::UP + 1 : 14) - static_cast<int>(top);
+          top = max(top, __reduce_max_sync(0xffffffffu, e));
+          up = (VALUES ? C::UP : 14) + 1 - static_cast<int>(top);
         }
         const float up2 = pow2i(up);
         // Chunk ch is dims 16 ch .. + 15: two 16-byte chunks of f16 in group ch / 4's tile.

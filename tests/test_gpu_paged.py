@@ -590,3 +590,23 @@ def test_attention_of_values_that_are_no_numbers(gpu, cuda_lib, kind, query, bad
     ref[~np.isfinite(ref).all(-1)] = np.nan
     tol = np.full(ref.shape, 4e-5 * vmax) if kind == "f32" else (4e-5 + 2.0 ** -10) * vmax + UNIT[kind] * np.abs(ref)
     close_where_finite(paged.attention(cache, batch, q), ref, tol)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("query", [2, 8, 40, 300])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_attention_beside_keys_that_are_no_numbers(gpu, cuda_lib, kind, query, bad):
+    # A key scale among the new tokens: the tokens before it keep their results.
+    world = World([query], [query + 70], 16, 2, 128, seed=18 + query)
+    vmax = np.abs(world.values("v", np.flatnonzero(world.held))).max()
+    p = 70 + query // 2
+    world.scales["k"][world.rows(0, np.array([p])), 1] = bad
+    cache, batch = world.device(gpu)
+    q = torch.randn(world.tokens, 4, 128, generator=torch.Generator().manual_seed(query)).to(TYPES[kind]).to(gpu)
+    with np.errstate(invalid="ignore"):
+        ref = world.attention(q.double().cpu().numpy())
+    got = paged.attention(cache, batch, q).double().cpu().numpy()
+    tol = np.full(ref.shape, 4e-5 * vmax) if kind == "f32" else (4e-5 + 2.0 ** -10) * vmax + UNIT[kind] * np.abs(ref)
+    free = np.zeros(ref.shape, bool)
+    free[:query // 2] = free[:, 2:] = True  # does not see it, or is another kv head's
+    assert np.all(np.abs(got - ref)[free] <= tol[free]), float(np.abs(got - ref)[free].max())

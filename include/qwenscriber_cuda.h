@@ -510,9 +510,13 @@ int32_t qwc_op_paged_append(const qwc_paged_cache* cache, const qwc_paged_batch*
 /* Causal attention of a step's tokens, one or many for each sequence, over the sequences' pages
  * (kernels.zig:697-767 for one token): query head h reads kv head h / (heads / kv_heads), scores are
  * scaled by 1 / sqrt(head_dim). Products enter the tensor cores as exact codes against f16 parts of
- * the queries and weights (two parts, 22 bits, for f32 rows, one for 16-bit rows); for bf16 rows of a call with
- * more than 16 rows to a kv head, code times scale rounds to f16 first. Sums and the softmax are f32. A token that sees no position gives a row of zeros.
- * A head's row that sees a position whose value scale is no number is NaN; rows that do not see it are not touched by it. q and out as in append.
+ * the queries and weights (two parts, 22 bits, for f32 rows, one for 16-bit rows); sums and the softmax are f32. A
+ * weight times a value scale is off by 2^-22 (or 2^-11) of itself, and by 2^-31 of the largest value scale of the
+ * context so far. For bf16 rows of a call with more than 16 rows to a kv head, code times scale rounds to f16
+ * first, in units of the largest key scale of 64 positions and of the largest value scale of the context so far: an
+ * element is off by 2^-11 of itself, and by 2^-17 of that scale.
+ * A token that sees no position gives a row of zeros. A head's row that sees a position whose value scale is no
+ * number is NaN; rows that do not see it keep their results. q and out as in append.
  * `workspace` (16-byte aligned device memory of at least qwc_op_paged_attention_workspace bytes) holds
  * the partial results of contexts cut into pieces. Its first QWC_PAGED_WORKSPACE_HEAD bytes must be zero before
  * its first use; it is left ready for the next call, and serves one stream at a time. Its first 32-bit word stays zero unless a wait inside the

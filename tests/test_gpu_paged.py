@@ -610,3 +610,27 @@ def test_attention_beside_keys_that_are_no_numbers(gpu, cuda_lib, kind, query, b
     free = np.zeros(ref.shape, bool)
     free[:query // 2] = free[:, 2:] = True  # does not see it, or is another kv head's
     assert np.all(np.abs(got - ref)[free] <= tol[free]), float(np.abs(got - ref)[free].max())
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("query", [2, 8, 40, 300])
+@pytest.mark.parametrize("plane", ["k", "v"])
+def test_attention_beside_a_position_of_another_size(gpu, cuda_lib, kind, query, plane):
+    # One position's keys or values are a thousand times the others', and a token before it does not see it: what it may cost
+    # them. A weight times a scale is off by 2^-31 of the largest value scale (times 128 codes); bf16 rows in tiles have keys
+    # and values off by 2^-17 of the largest scale (a score by that times the sum of its |q| / sqrt(d), a weight by e to it).
+    world = World([query], [query + 70], 16, 2, 128, seed=19 + query)
+    p, large = 70 + query // 2, 32.0
+    seen = np.abs(world.values("v", world.rows(0, np.arange(p)))).max()
+    world.scales[plane][world.rows(0, np.array([p]))] = large
+    cache, batch = world.device(gpu)
+    q = torch.randn(world.tokens, 4, 128, generator=torch.Generator().manual_seed(query)).to(TYPES[kind]).to(gpu)
+    ref = world.attention(q.double().cpu().numpy())[:query // 2]
+    got = paged.attention(cache, batch, q).double().cpu().numpy()[:query // 2]
+    tiles = kind == "bf16" and query * 2 > 16
+    if plane == "v":
+        rest = 2.0 ** -17 * large if tiles else 2.0 ** -24 * large
+    else:
+        rest = 2 * 2.0 ** -17 * large * float(q.abs().sum(-1).max()) / 128 ** 0.5 * seen if tiles else 0.0
+    tol = rest + (4e-5 * seen if kind == "f32" else (4e-5 + 2.0 ** -10) * seen + UNIT[kind] * np.abs(ref))
+    assert np.all(np.abs(got - ref) <= tol), (float(np.abs(got - ref).max()), seen)

@@ -723,6 +723,7 @@ __global__ void __launch_bounds__(TileConfig<T, DIM, TILES>::THREADS, TILES == 1
         if (last) {
           if (lane == 0) *counter = 0;
           __threadfence();
+          __syncwarp();  // what lane 0 has acquired, the others may read
           const float* first = slot(2 * c0 + (seg0 > total * c0 / grid ? 1u : 0u));
           auto piece = [&](uint32_t x) -> const float* { return x == c0 ? first : slot(2 * x); };
           constexpr uint32_t kMax = DIM * HEIGHT, kSum = (DIM + 1) * HEIGHT;

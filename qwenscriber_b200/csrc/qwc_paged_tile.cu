@@ -1037,12 +1037,12 @@ TilePlan paged_tile_plan(const PagedArgs& a, uint32_t format, uint32_t heads, ui
   const uint64_t most = plan.tiles == 2 ? sms : 2 * sms;  // what is resident at once
   const uint64_t length = (a.max_context ? (a.max_context + kStep - 1) / kStep : 1);
   const uint64_t tiles = uint64_t(a.sequences) * a.kv_heads * ((rows + height - 1) / height), steps = tiles * length;
-  plan.too_long = steps / most >= 0x7FFFFFFFu;  // a stretch's steps are counted in 31 bits
   const double join = format == kFormatF32 ? kJoinCostF32 : kJoinCost;
   const double stretch = sqrt(1.0 + join * static_cast<double>(length));
   uint64_t grid = static_cast<uint64_t>(static_cast<double>(steps) / stretch);
   if (grid < tiles) grid = tiles;
   plan.grid = static_cast<uint32_t>(grid < most ? grid : most);
+  plan.too_long = plan.grid && tiles * (length + kTileCost) / plan.grid >= 0x7FFFFFFFu;  // a stretch's places are counted in 31 bits
   // Two partial tiles a CTA, and its sums (f32 rows).
   plan.partial_bytes = uint64_t(plan.grid) * (2 * (a.head_dim + 2) + a.head_dim) * height * 4;
   return plan;

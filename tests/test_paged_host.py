@@ -324,3 +324,9 @@ def test_a_larger_workspace_still_tells_of_a_wait_that_ran_out(monkeypatch):
         paged.check_waits(device=torch.device("cuda:1"))
     assert e.value.name == "invalid_state"
     paged.check_waits(device=torch.device("cuda:1"))
+
+
+def test_stretches_of_more_places_than_are_counted_in_31_bits(cuda_lib):
+    # A tile of one step takes four places: 65535 sequences of 1024 kv heads and 1211 tiles each are 2.2e9 places to a CTA.
+    b = batch(sequences=65535, tokens=(1 << 31) - 1, max_query=310000, max_context=16, table_stride=1)
+    assert attention(cache(kv_heads=1024, head_dim=64), b, q_stride=1024 * 64, heads=1024, out_stride=1024 * 64) == LIMIT

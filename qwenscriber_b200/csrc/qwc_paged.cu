@@ -308,7 +308,7 @@ int32_t paged_rows_check(const void* p, uint64_t stride, uint64_t width, uint32_
 int32_t paged_args(const qwc_paged_cache* c, const qwc_paged_batch* b, PagedArgs* out) {
   if (!c || !b) return QWC_INVALID_ARGUMENT;
   if (!c->k_scales || !c->k_codes || !c->v_scales || !c->v_codes) return QWC_INVALID_ARGUMENT;
-  if (!b->query_starts || !b->context_lens || !b->page_table) return QWC_INVALID_ARGUMENT;
+  if (b->sequences && (!b->query_starts || !b->context_lens || !b->page_table)) return QWC_INVALID_ARGUMENT;
   if (!aligned(c->k_scales, 16) || !aligned(c->k_codes, 16) || !aligned(c->v_scales, 16) || !aligned(c->v_codes, 16) ||
       !aligned(b->query_starts, 4) || !aligned(b->context_lens, 4) || !aligned(b->page_table, 4)) {
     return QWC_INVALID_ARGUMENT;
@@ -317,7 +317,7 @@ int32_t paged_args(const qwc_paged_cache* c, const qwc_paged_batch* b, PagedArgs
   if (c->kv_heads == 0 || c->page_size == 0 || c->pages == 0) return QWC_SHAPE_MISMATCH;
   // Every position of a sequence has an entry in its row of the table, whatever lies between two rows.
   const uint32_t entries = b->table_entries ? b->table_entries : b->table_stride;
-  if (uint64_t(entries) * c->page_size < b->max_context) return QWC_SHAPE_MISMATCH;
+  if (b->sequences && uint64_t(entries) * c->page_size < b->max_context) return QWC_SHAPE_MISMATCH;
   if (uint64_t(c->pages) * c->page_size > 0x7FFFFFFFu || b->max_context > 0x7FFFFFFFu || b->tokens > 0x7FFFFFFFu ||
       c->kv_heads > 1024 || b->sequences > kPagedMaxSequences) {
     return QWC_LIMIT_EXCEEDED;

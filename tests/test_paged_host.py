@@ -330,3 +330,11 @@ def test_stretches_of_more_places_than_are_counted_in_31_bits(cuda_lib):
     # A tile of one step takes four places: 65535 sequences of 1024 kv heads and 1211 tiles each are 2.2e9 places to a CTA.
     b = batch(sequences=65535, tokens=(1 << 31) - 1, max_query=310000, max_context=16, table_stride=1)
     assert attention(cache(kv_heads=1024, head_dim=64), b, q_stride=1024 * 64, heads=1024, out_stride=1024 * 64) == LIMIT
+
+
+def test_a_batch_of_no_sequences(cuda_lib):
+    # Its arrays have no elements, so no addresses.
+    b = batch(sequences=0, tokens=0, query_starts=None, context_lens=None, page_table=None, table_stride=0)
+    for max_context in (0, 80):
+        b.max_context = max_context
+        assert attention(cache(), b) == 0 and append(cache(), b) == 0 and read(cache(), b) == 0

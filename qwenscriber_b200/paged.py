@@ -122,7 +122,7 @@ def _rows(t: torch.Tensor, batch: PagedBatch, heads: int, dim: int, call: str) -
     row, head, one = t.stride()
     if (one != 1 and dim > 1) or (head != dim and heads > 1):
         refuse("invalid_argument", call)
-    return row if batch.tokens > 1 else max(row, heads * dim)
+    return row if batch.tokens > 1 else heads * dim  # (nothing is a stride away from the only row)
 
 
 def _table(t: torch.Tensor, shape: tuple, device: torch.device, call: str) -> None:

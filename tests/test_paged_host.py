@@ -338,3 +338,14 @@ def test_a_batch_of_no_sequences(cuda_lib):
     for max_context in (0, 80):
         b.max_context = max_context
         assert attention(cache(), b) == 0 and append(cache(), b) == 0 and read(cache(), b) == 0
+
+
+def test_a_single_token_may_lie_in_a_row_of_any_width(monkeypatch):
+    # Nothing is a row's stride away from the only row.
+    class Row(Stub):
+        def stride(self, i=None):
+            strides = [1001, self.shape[2], 1]
+            return strides if i is None else strides[i]
+
+    b = paged.PagedBatch(Stub(2, dtype=torch.int32), Stub(1, dtype=torch.int32), Stub(1, 5, dtype=torch.int32), tokens=1, max_query=1, max_context=80)
+    assert paged._rows(Row(1, 4, 128), b, 4, 128, "test") == 512

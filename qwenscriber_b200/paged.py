@@ -38,12 +38,19 @@ def current_stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def elsewhere(device: torch.device, call: str):
-    """A kernel is launched on the current device: the context that makes `device` the current one, or None where it
-    is already. Memory that no GPU holds is refused."""
-    if device.type != "cuda":
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def elsewhere(index: int | None, call: str):
+    """A kernel is launched on the current device: the context that makes device `index` the current one, or None where it
+    is already. Memory that no GPU holds (no index) is refused."""
+    if index is None:
         refuse("invalid_argument", call)
-    return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return None if index == _current_device() else torch.cuda.device(index)
+
+
+def cuda_index(device: torch.device) -> int | None:
+    return device.index if device.type == "cuda" else None
 
 
 def format_of(t: torch.Tensor, call: str) -> int:
@@ -75,7 +82,7 @@ class PagedCache:
         self.desc = PagedCacheDesc(k_scales.data_ptr(), k_codes.data_ptr(), v_scales.data_ptr(), v_codes.data_ptr(),
                                    self.pages, page_size, kv_heads, head_dim)
         self._ref = ctypes.addressof(self.desc)
-        self._index = self.device.index
+        self._index = cuda_index(self.device)
         self._key = (self.pages, page_size, kv_heads, head_dim)
 
     @classmethod
@@ -202,7 +209,7 @@ def append(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, k: torch.Tenso
     """QK-RMSNorm, rotation and the q8 append of [tokens, heads, head_dim] rows; returns the queries
     for attention (`q_out`, a new tensor unless given; may be `q`)."""
     call = "qwc_op_paged_append"
-    away = elsewhere(cache.device, call)
+    away = elsewhere(cache._index, call)
     if away is not None:
         with away:
             return append(cache, batch, q, k, v, cos, sin, q_norm=q_norm, k_norm=k_norm, eps=eps, q_out=q_out)
@@ -240,7 +247,7 @@ def attention(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, out: torch.
     """Causal attention of the batch's [tokens, heads, head_dim] queries over their sequences' pages. `workspace`: one
     made by `workspace(...)`; without it, the current stream's own (in a graph under capture, the graph's own)."""
     call = "qwc_op_paged_attention"
-    away = elsewhere(cache.device, call)
+    away = elsewhere(cache._index, call)
     if away is not None:
         with away:
             return attention(cache, batch, q, out, workspace)
@@ -273,7 +280,7 @@ def read(cache: PagedCache, batch: PagedBatch, dtype: torch.dtype = torch.float3
          v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached key and value rows of the batch's tokens as values, [tokens, kv_heads, head_dim]."""
     call = "qwc_op_paged_read"
-    away = elsewhere(cache.device, call)
+    away = elsewhere(cache._index, call)
     if away is not None:
         with away:
             return read(cache, batch, dtype, k_out, v_out)

@@ -109,7 +109,7 @@ class PagedDecoder:
     # ---- operators ----
 
     def _call(self, name: str, *args) -> None:
-        with paged.elsewhere(self.device, name) or contextlib.nullcontext():
+        with paged.elsewhere(paged.cuda_index(self.device), name) or contextlib.nullcontext():
             check(getattr(lib(), name)(*args, paged.current_stream(self.device)), name)
 
     def _project(self, w: Matrix, x: torch.Tensor) -> torch.Tensor:

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import torch
 
-from .paged import current_stream, elsewhere, format_of, refuse
+from .paged import cuda_index, current_stream, elsewhere, format_of, refuse
 from .runtime import check, lib
 
 
@@ -14,8 +14,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: torch.T
     """(tokens int32 [rows], log-probabilities f32 [rows]) of [rows, vocab] logits (rows may be a
     view of wider ones), from one number in [0, 1) for each row. Settings are one value for each row
     on the device (top_k int32, the others f32); None leaves a cut out, and the temperature 1."""
-    call = "qwc_op_sample"
-    away = elsewhere(logits.device, call)
+    call, device = "qwc_op_sample", logits.device
+    away = elsewhere(cuda_index(device), call)
     if away is not None:
         with away:
             return sample(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
@@ -31,11 +31,11 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: torch.T
             continue
         if t.shape != (rows,):
             refuse("shape_mismatch", call)
-        if t.dtype != dtype or t.device != logits.device or not t.is_contiguous():
+        if t.dtype != dtype or t.device != device or not t.is_contiguous():
             refuse("invalid_argument", call)
         pointers.append(t.data_ptr())
-    tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    tokens = torch.empty(rows, dtype=torch.int32, device=device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
     check(lib().qwc_op_sample(fmt, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, *pointers,
-                              tokens.data_ptr(), logprobs.data_ptr(), current_stream(logits.device)), call)
+                              tokens.data_ptr(), logprobs.data_ptr(), current_stream(device)), call)
     return tokens, logprobs

@@ -197,7 +197,7 @@ def test_launches_go_to_the_tensors_device(monkeypatch, name, current):
 
     class Current:
         def __init__(self, device):
-            self.index = torch.device(device).index
+            self.index = device
 
         def __enter__(self):
             entered.append(self.index)
@@ -211,7 +211,7 @@ def test_launches_go_to_the_tensors_device(monkeypatch, name, current):
             return lambda *a: launched.append((name, at[0], a[-1])) or 0
 
     calls = stub_calls("cuda:1")
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(paged, "_current_device", lambda: at[0])
     monkeypatch.setattr(torch.cuda, "device", Current)
     monkeypatch.setattr(torch, "empty", lambda *shape, dtype, device: Stub(*shape, dtype=dtype, device=device))
     for module in (paged, sampling):
@@ -238,15 +238,15 @@ def test_an_operator_of_the_decoder_goes_to_its_device(monkeypatch):
     at, launched = [0], []
 
     @contextlib.contextmanager
-    def current(device):
-        before, at[0] = at[0], device.index
+    def current(index):
+        before, at[0] = at[0], index
         yield
         at[0] = before
 
     class Lib:
         qwc_op_silu_mul = staticmethod(lambda *a: launched.append((at[0], a[-1])) or 0)
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(paged, "_current_device", lambda: at[0])
     monkeypatch.setattr(torch.cuda, "device", current)
     monkeypatch.setattr(paged_decoder, "lib", Lib)
     monkeypatch.setattr(paged, "current_stream", lambda device: 1000 + device.index)
@@ -279,7 +279,7 @@ def test_a_workspace_lives_until_the_launch(cuda_lib, monkeypatch):
             alive.extend(ref() is not None for address, ref in born if address == a[8])
             return 0
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(paged, "_current_device", lambda: 1)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(paged, "current_stream", lambda device: 1000 + device.index)
     monkeypatch.setattr(paged, "_new_workspace", new)
@@ -312,7 +312,7 @@ def test_a_wait_that_ran_out_is_found_by_any_name_of_the_device(monkeypatch, dev
 
 def test_a_larger_workspace_still_tells_of_a_wait_that_ran_out(monkeypatch):
     pool = paged.PagedCache(*[Stub(160, 4, dtype=torch.float16), Stub(160, 256, dtype=torch.uint8)] * 2, page_size=16, kv_heads=2, head_dim=128)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(paged, "_current_device", lambda: 1)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(paged, "current_stream", lambda device: 1000 + device.index)
     monkeypatch.setattr(paged, "_new_workspace", lambda need, device: torch.zeros(need, dtype=torch.uint8))

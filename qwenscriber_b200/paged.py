@@ -115,7 +115,7 @@ class PagedBatch:
         # A view's rows may lie further apart than they are long (or be one row): the length bounds what is read.
         entries = page_table.shape[1]
         self.desc = PagedBatchDesc(query_starts.data_ptr(), context_lens.data_ptr(), page_table.data_ptr(), n, tokens,
-                                   page_table.stride(0) if n > 1 and entries else 0, max_query, max_context, entries)
+                                   page_table.stride(0) if n > 1 and entries else entries, max_query, max_context, entries)
         self._ref = ctypes.addressof(self.desc)
         self._workspace_bytes: dict = {}
 

@@ -501,7 +501,8 @@ typedef struct qwc_paged_batch {
  * out. cos / sin: [rope_rows][head_dim / 2] f32 (qwc_rope_tables). Row pointers and strides in bytes
  * are multiples of 16, the tables and norm weights 16-byte aligned (else QWC_INVALID_ARGUMENT).
  * A token whose position is not cached, or is rope_rows or more, is not written and its q_out
- * row is zero. */
+ * row is zero. A key or value that is NaN is stored as 0 and does not count towards its group's scale; an infinite one
+ * makes the scale infinite (both as in the reference's quantizer). */
 int32_t qwc_op_paged_append(const qwc_paged_cache* cache, const qwc_paged_batch* batch, uint32_t format, const void* q,
                             uint64_t q_stride, const void* k, uint64_t k_stride, const void* v, uint64_t v_stride,
                             uint32_t heads, const float* q_norm, const float* k_norm, float eps, const float* cos_table,
@@ -514,7 +515,8 @@ int32_t qwc_op_paged_append(const qwc_paged_cache* cache, const qwc_paged_batch*
  * weight times a value scale is off by 2^-22 (or 2^-11) of itself, and by 2^-31 of the largest value scale of the
  * context so far. For bf16 rows of a call with more than 16 rows to a kv head, code times scale rounds to f16
  * first, in units of the largest key scale of 64 positions and of the largest value scale of the context so far: an
- * element is off by 2^-11 of itself, and by 2^-17 of that scale.
+ * element is off by 2^-11 of itself, and by 2^-17 of that scale. (max_query decides for the whole call: a bf16 token
+ * beside another sequence's chunk may differ in its last bits from the same token in a call of single tokens.)
  * A token that sees no position gives a row of zeros. A head's row that sees a position whose value scale is no
  * number is NaN; rows that do not see it keep their results. q and out as in append.
  * `workspace` (16-byte aligned device memory of at least qwc_op_paged_attention_workspace bytes) holds

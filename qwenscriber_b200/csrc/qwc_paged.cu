@@ -98,8 +98,9 @@ __device__ __forceinline__ void q8_codes(const uint64_t (&y)[V / 2], float store
 // 16 bytes of a row (4 or 8 values); a group takes the same head of every token, so the loads of all of them are
 // in flight at once and what depends on the head alone is worked out once.
 //
-// 64 x 391 tokens at most, 14,135 in all (bf16, 16 + 2 x 8 heads of 128): 69 us, 2.9 TB/s. Bound by instructions, 212 for
-// a warp's 256 values, then by latency: 115 us with a division for each value, 79 with 78 registers and three
+// 64 x 391 tokens at most, 14,281 in all (bf16, 16 + 2 x 8 heads of 128): 69 us, 3.0 TB/s (f16 67, f32 90). 235 warp
+// instructions for 256 values, about a third of them the quantizer's, the others norms, rotation and maxima, take 70% of the
+// issue slots; the rest is latency: 115 us with a division for each value, 79 with 78 registers and three
 // blocks to an SM instead of 48 and five, 71 with two tokens to a block.
 constexpr uint32_t kAppendTokens = 4;
 

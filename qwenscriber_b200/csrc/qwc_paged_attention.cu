@@ -39,7 +39,7 @@ namespace {
 // MMAs and twice the output registers were spent on mostly empty rows (64 x 1 over 4096, f32: 95 us).
 //
 // 64 x 1 over up to 4096 (361 MB of cache), f32: 73 us, 4.9 TB/s; the copies and the conversions of codes share the
-// issue slots (53% taken), and two CTAs of eight warps leave them partly idle behind the chain of a block: scores,
+// issue slots (66% taken), and two CTAs of eight warps leave them partly idle behind the chain of a block: scores,
 // maximum, exponential, transpose. 1 x 1 over 301: 9.7 us, of which the launch and the chain of dependent loads
 // (lengths, page table, codes, the joined pieces) are nearly all.
 
@@ -611,7 +611,8 @@ AttnPlan attention_plan(const PagedArgs& a, uint32_t format, uint32_t heads) {
   const uint64_t rows = uint64_t(a.max_query) * (heads / a.kv_heads);
   const uint64_t sms = 148;
   // As many rows as the few-row kernel has columns for. 64 sequences of up to 4096 positions, 8 kv heads: f32, 8 rows,
-  // 150 us here and 396 on 128-row tiles; bf16, 16 rows, 212 and 242; 2 sequences up to 2047, f32, 8 rows, 19 and 55.
+  // 147 us here and 387 on 128-row tiles; bf16, 16 rows, 193 and 229; 2 sequences up to 2047, f32, 8 rows, 21 and 43;
+  // 64 of one token, f32, 75 and 418. (One kernel for the whole call: single tokens beside a chunk pay the latter.)
   p.few = rows <= (format == kFormatF32 ? 8u : 16u);
   if (!p.few) {
     p.tile = paged_tile_plan(a, format, heads, sms);

@@ -21,8 +21,11 @@
 // own weights, the softmax weight times the group's value scale. f32 queries and
 // weights enter as two f16 parts, hi and lo (22 bits), f16 rows as one.
 // bf16 rows (scaled): code times scale is rounded to f16 as it is converted, at a
-// power of two of the step. That adds a relative 2^-12 to each factor of a sum that
-// is rounded to 2^-9 in the end, and leaves the softmax threads a third of the work.
+// power of two of the step. That adds up to 2^-11 to each factor of a sum that is
+// rounded to 2^-9 in the end (4 x 1500 over 4096: 1.71e-3 from 64 bits, the rounding
+// alone 1.66e-3), and leaves the softmax threads a third of the work: f16 rows, which
+// keep codes exact, take 190 us there and bf16 148. A scale 2^14 below the largest of its
+// step (keys) or of the tile so far (values) loses bits.
 //
 // Each row of queries has its own power of two, so f16 holds its values whatever
 // their size; sums, maxima and the output are f32. The output is rescaled only when a
@@ -36,9 +39,10 @@
 // 2 x 391 over 2047, f32, one 69, two 66.
 //
 // What bounds it: the softmax and convert warps' instructions, not the tensor cores. 4 x 1500 over 4096, bf16:
-// 148 us, 520 TFLOP/s; 24 x 64 over 1237, bf16: 53 us, many tiles with a few
-// rows (down to one token's two) that cost as much as a full one, converting the cache; 2 x 391 over 2047, f32: 68 us,
-// four times the scores' instructions of bf16 and four MMAs for one.
+// 148 us, 520 TFLOP/s (f16 190, f32 366); 24 x 64 over 1237, bf16: 50 to 53 us, many tiles with few
+// rows (16 to 128) that cost as much as a full one, converting the cache; 2 x 391 over 2047, f32: 68 us,
+// four times the scores' instructions of bf16 and four MMAs for one. With 54% of the issue slots and 29% of the tensor
+// pipe in use neither is at its limit: much of it is the wait from scores to weights, one step of 64 positions at a time.
 //
 // Work is dealt as in qwc_paged_attention.cu: the steps of all tiles stand in
 // one line, each CTA takes an equal stretch, a tile that is cut is joined by

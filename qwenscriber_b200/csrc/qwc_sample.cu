@@ -14,7 +14,8 @@
 //
 // Bound by the chain of passes over the row's slices in shared memory (load and maximum 5.4 us, sums and histogram 6,
 // list 4, cut and token 2, of 64 x 151936) and the exchanges between them, not by HBM: 1 x 151936, f32, 16 us; 64 x 151936,
-// f32, 57 us, two waves of rows; 16 x 32003, bf16, 17 us.
+// f32, 49 to 67 us, two waves of rows; 16 x 32003, bf16, 18 to 28 us. Of 24 inputs each, three had a row with a large kept
+// set that takes longer: 25 to 27, 95 to 115 and 38 to 44 us.
 //
 // Sums are of integers, w in units of 2^-42: they are exact, so neither the
 // order of the atomics nor the split over threads changes a result.
@@ -41,8 +42,8 @@ constexpr uint32_t kBins = kSampleThreads;  // a scan takes one bin for each thr
 constexpr uint32_t kBinBits = 10;
 constexpr uint32_t kListed = kSampleThreads;  // tokens that the first CTA takes by itself, one for each thread
 // Up to this many of them are compared pair by pair, each token by as many lanes as there are: two passes over the
-// list, where narrowing takes a histogram and more for each cut. 1 x 151936 16 us, by narrowing 21; 16 x 32003 16 and 18.
-// (With 1024 in place of 256 64 x 151936 took 154 us for 67.)
+// list, where narrowing takes a histogram and more for each cut. 1 x 151936 16.5 us, by narrowing 23; 64 x 151936 55 and 59;
+// 16 x 32003 17.7 and 19.5. (With 1024 in place of 256: 64 x 151936 148 us, 16 x 32003 61.)
 constexpr uint32_t kPairs = 256;
 constexpr uint32_t kLimbBits = 14;          // 2^17 tokens of a slice times 2^14 stay below 2^32
 constexpr float kBinScale = 23.0f;      // coarse bins in a power of two; the last bin takes all below 2^-44, whose units are 0
@@ -907,8 +908,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
 template <typename T>
 int32_t sample_as(SampleArgs a, uint32_t rows, cudaStream_t stream) {
   // CTAs to a row: as few as hold it in their shared memory, then twice as many while there are SMs for all rows, at
-  // most 8. One row of 151936: eight CTAs 16 us, four 22 (sixteen as eight); 64 rows: four 62 us, eight 74 (more waves,
-  // each with a row's dozen exchanges), two 137 before later steps (slices that do not fit are read again and again).
+  // most 8. One row of 151936: eight CTAs 16.5 us, four 21, two 55 (sixteen as eight, on an earlier build); 64 rows: four 55 us,
+  // eight 69 (more waves, each with a row's dozen exchanges), two 105 (slices that do not fit are read again and again).
   const uint32_t most = (227 * 1024 - 1024 - static_cast<uint32_t>(sizeof(SampleSmem))) / 4;
   uint32_t size = 1;
   while (size < 8 && (uint64_t(size) * most < a.vocab || rows * size * 2 <= 148)) size *= 2;

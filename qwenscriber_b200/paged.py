@@ -190,7 +190,8 @@ def _workspace(cache: PagedCache, need: int, stream: int) -> tuple[int, int, tor
 
 def check_waits(workspace: torch.Tensor | None = None, device: torch.device | None = None) -> None:
     """Raises `QwcError` if a bounded wait inside an attention kernel ran out (its rows are undefined then), and makes
-    the workspace ready again. Without a workspace, of the current stream's own. Waits for the stream."""
+    the workspace ready again. Without a workspace, of the current stream's own. Waits for the stream. (The workspace that a
+    captured graph makes for itself is not kept and cannot be asked: capture with one of the caller's.)"""
     if workspace is None:
         if device is None or device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())

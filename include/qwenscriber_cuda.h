@@ -538,7 +538,7 @@ int32_t qwc_op_paged_read(const qwc_paged_cache* cache, const qwc_paged_batch* b
 /* One token of each row of logits, drawn with a given number uniforms[row] in [0, 1). With w = exp((x -
  * max) / temperature), the tokens in order of falling logit (ties: the lowest index first) are cut to the
  * first top_k (0: all), then to the first whose sum of w reaches top_p of what top_k left (1 or more: all;
- * the token that reaches it stays), then to those with w >= min_p (0: all); at least one stays. The token is
+ * the token that reaches it stays), then to those with w >= min_p (0: all; more than 1 counts as 1); at least one stays. The token is
  * the first, in index order, whose running sum of the kept w passes uniforms[row] of their total. A
  * temperature of 0 (or less, or NaN) takes the largest logit, as qwc_op_argmax. NaN logits count as -inf; a row
  * of nothing else gives token 0 and log-probability -inf. logprobs_out (may be NULL): the token's log-probability under
